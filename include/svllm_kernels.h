@@ -61,8 +61,9 @@ typedef enum svllm_status {
 } svllm_status;
 
 /* Bits of the device error word. */
-#define SVLLM_DEVERR_BAD_INDEX 1    /* an embedding id outside [0, vocab) (its row is zeroed) or a
-                                       KV slot past the cache (nothing written) */
+#define SVLLM_DEVERR_BAD_INDEX 1    /* an embedding id outside [0, vocab) (its row is zeroed), a KV
+                                       slot past the cache (nothing written), or an index of a
+                                       paged batch that its entry point documents */
 #define SVLLM_DEVERR_WAIT_TIMEOUT 2 /* a bulk copy did not land in time: the kernel stopped */
 
 /* Index dtype of positions / token ids. */
@@ -317,6 +318,120 @@ int svllm_lm_head_argmax_static_bf16(const void* hidden, int64_t num_rows, int64
                                      int64_t hidden_stride, const void* weight, int64_t vocab,
                                      int64_t weight_stride, int64_t* out_ids, void* logits,
                                      int64_t logits_stride, svllm_stream stream);
+
+/*
+ * Checking a tree of drafted tokens in one step (speculative decoding): four entry points around
+ * the forward of a step whose requests bring several tokens each. A request's tokens of the step
+ * are the nodes of a tree: node 0 is its last accepted token, every other node a drafted successor
+ * of its parent. parents[t] is the parent's index within the request, lower than the node's own,
+ * -1 for a root; parents == NULL everywhere stands for chains (node i hangs on node i - 1). Node
+ * i of a request with `context` cached tokens is written to the slot of row context + i, whatever
+ * its depth. query_start_loc: [num_seqs + 1] int32, starts at 0 and does not fall. New ops: the
+ * reference's AGENTS.md names the tensors (slot_mapping, block_tables, seq_lens, query_start_loc);
+ * it has no drafted tokens.
+ */
+
+/* Nodes of one request's tree: the widest tree_mask, path and walk the entry points take. */
+#define SVLLM_MAX_TREE_NODES 1024
+
+/*
+ * The paging of one step from request lengths. Per request s: context_lens[s] cached tokens,
+ * query_lens[s] tokens of this step (negative: the request has finished and gives its blocks
+ * back; 0: it sits the step out), blocks_owned[s] blocks in use at the front of its row of
+ * block_tables [num_seqs, max_blocks]. free_blocks [free_capacity] is a stack of block ids of
+ * which the first free_count[0] are free.
+ *   1. Finished requests, in order: their blocks go on the stack, behind the free ones.
+ *   2. need = max(0, ceil((context + query) / block_size) - owned), in the order of the requests:
+ *      a request whose need and all the needs before it fit the stack is served; one that needs no
+ *      block is always served. Block k of the step, counted over the requests, is
+ *      free_blocks[count - 1 - k]; it goes behind the request's owned blocks.
+ * Written: the new entries of block_tables and of free_blocks, nothing else of them (a second call
+ * with the same inputs writes the same); query_start_loc [num_seqs + 1]; seq_lens [num_seqs] =
+ * context + query, 0 for a finished request or one that was not served; blocks_owned_out and
+ * free_count_out (not the input arrays); and for the tokens t < num_tokens, slot_mapping (block *
+ * block_size + offset of row context + i), positions (context + depth in the tree; chains: context
+ * + i) and, with parents, tree_mask [num_tokens, ceil(max_query_len / 64)]: bit b of word w of a
+ * node is set where node 64 w + b is the node itself or one of its ancestors. A token of a request
+ * that was not served, and one behind the last request, has slot -1, position 0 and an empty mask.
+ * Not served, with SVLLM_DEVERR_BAD_INDEX: a negative context, blocks_owned outside [0,
+ * max_blocks], more rows than the table holds, tokens past num_tokens, more nodes than
+ * max_query_len (which only counts with parents; at most SVLLM_MAX_TREE_NODES). The same bit tells
+ * of a parent that does not come before its child (the node counts as a root), a free_count
+ * outside [0, free_capacity] (clamped), and blocks given back past free_capacity (dropped).
+ */
+int svllm_paged_plan(const int32_t* context_lens, const int32_t* query_lens, int64_t num_seqs,
+                     int32_t* block_tables, int64_t max_blocks, const int32_t* blocks_owned,
+                     int32_t* free_blocks, int64_t free_capacity, const int32_t* free_count,
+                     int64_t block_size, const int32_t* parents, int64_t max_query_len,
+                     int64_t num_tokens, int32_t* query_start_loc, int32_t* seq_lens,
+                     int64_t* slot_mapping, int64_t* positions, int64_t* tree_mask,
+                     int32_t* blocks_owned_out, int32_t* free_count_out, svllm_stream stream);
+
+/*
+ * Attention of every token of a step over a paged KV cache that already holds the step's own K and
+ * V (the rotary + cache-write entry points put them there). Token t, node i of request b with n
+ * tokens and context = seq_lens[b] - n, head h: out[t, h] = softmax_j(scale * q[t, h] . k_j) v_j
+ * over the rows j < context and those of the nodes j - context whose bit tree_mask[t] has; with
+ * tree_mask == NULL the nodes up to i (causal). Rows j as in svllm_paged_decode_attention_bf16,
+ * likewise the cache, q (q_token_stride) and the block tables. out: [num_tokens, num_heads,
+ * head_dim] contiguous. tree_mask: [num_tokens, mask_words] int64. A token that sees no row, every
+ * token of a request with seq_lens 0, and every row of out behind the last request is zero. A value
+ * that a token does not see never reaches its output, NaN and infinities included. bf16, fp32
+ * softmax and accumulation, the softmax numerators rounded to bf16 for the second product.
+ * head_dim 64 or 128, any number of query heads per KV head, 16-byte aligned out, q and caches, a
+ * q_token_stride of whole 16 bytes, else SVLLM_ERR_UNSUPPORTED. scale must be positive and finite.
+ * Zeros with SVLLM_DEVERR_BAD_INDEX: a request whose seq_lens is below its number of tokens or
+ * past its block table, or whose tree is wider than the mask; a query_start_loc that falls or ends
+ * past num_tokens. A table entry outside the cache raises the bit and reads block 0. workspace: at
+ * least svllm_tree_attention_workspace_bytes bytes of device memory, 16-byte aligned, any
+ * contents; calls that overlap on the GPU must not share it.
+ */
+int svllm_tree_attention_bf16(void* out, const void* q, int64_t q_token_stride,
+                              const void* k_cache, const void* v_cache, int64_t num_blocks,
+                              int64_t block_size, const int32_t* block_tables, int64_t max_blocks,
+                              const int32_t* seq_lens, const int32_t* query_start_loc,
+                              int64_t num_seqs, int64_t num_tokens, int64_t num_heads,
+                              int64_t num_kv_heads, int64_t head_dim, const int64_t* tree_mask,
+                              int64_t mask_words, float scale, void* workspace,
+                              int64_t workspace_bytes, svllm_stream stream);
+
+/* The workspace that svllm_tree_attention_bf16 needs on the current device, for any sizes with
+ * this head_dim. */
+int svllm_tree_attention_workspace_bytes(int64_t head_dim, int64_t* bytes);
+
+/*
+ * Greedy acceptance: from node 0, whose next token is targets[0], the walk goes to the first child
+ * of the current node whose id is the current node's target, until there is none. ids: [num_tokens]
+ * of id_type, the tokens the step was fed; targets: [num_tokens] int64, the model's next token
+ * after each node (svllm_argmax_* over its logits). Per request: path [num_seqs, max_query_len],
+ * the nodes walked, -1 behind them; tokens [num_seqs, max_query_len] int64, their targets, the
+ * tokens this step emits, -1 behind them; num_accepted, how many; context_lens_out = context_lens +
+ * num_accepted (may be context_lens itself). A request without tokens or with seq_lens 0 accepts
+ * none. More tokens than max_query_len or a query_start_loc that falls or ends past num_tokens:
+ * none, with SVLLM_DEVERR_BAD_INDEX. max_query_len is at most SVLLM_MAX_TREE_NODES.
+ */
+int svllm_tree_accept(const void* ids, int id_type, const int64_t* targets,
+                      const int32_t* parents, const int32_t* query_start_loc,
+                      const int32_t* seq_lens, const int32_t* context_lens, int64_t num_seqs,
+                      int64_t num_tokens, int64_t max_query_len, int32_t* path, int64_t* tokens,
+                      int32_t* num_accepted, int32_t* context_lens_out, svllm_stream stream);
+
+/*
+ * After svllm_tree_accept: moves the accepted nodes' rows to the front of the step's, in every
+ * cache: row slot_mapping[start + path[s][j]] to row slot_mapping[start + j] for 0 < j <
+ * num_accepted[s], start = query_start_loc[s]. k_caches, v_caches: HOST arrays of num_layers device
+ * pointers, each [num_slots, row_bytes] contiguous (row_bytes = num_kv_heads * head_dim * element
+ * size, a multiple of 16, 16-byte aligned, else SVLLM_ERR_UNSUPPORTED); the pointers are passed by
+ * value, so the arrays may be freed when the call returns. path: [num_seqs, max_query_len]. A row
+ * with a negative slot does not move. SVLLM_DEVERR_BAD_INDEX: a slot past num_slots (the row does
+ * not move), a path that does not rise or leaves the request (no row from there on moves), a count
+ * past the request's tokens (nothing of it moves). No two tokens of the step may share a slot.
+ */
+int svllm_tree_commit(void* const* k_caches, void* const* v_caches, int64_t num_layers,
+                      int64_t num_slots, int64_t row_bytes, const int32_t* path,
+                      const int32_t* num_accepted, const int64_t* slot_mapping,
+                      const int32_t* query_start_loc, int64_t num_seqs, int64_t num_tokens,
+                      int64_t max_query_len, svllm_stream stream);
 
 /*
  * Reads (and with reset != 0 clears) the library's own error word on `device`. Synchronises

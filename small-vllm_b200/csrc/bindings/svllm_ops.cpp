@@ -12,10 +12,13 @@
 #include "model/qwen3.h"
 #include "ops/add_rms_norm.h"
 #include "ops/embedding.h"
+#include "ops/paged_plan.h"
 #include "ops/rms_norm.h"
 #include "ops/rope.h"
 #include "ops/sampling.h"
 #include "ops/silu_and_mul.h"
+#include "ops/tree_accept.h"
+#include "ops/tree_attention.h"
 
 namespace py = pybind11;
 
@@ -67,6 +70,20 @@ PYBIND11_MODULE(svllm_ops, m) {
   m.def("argmax", &svllm::ops::argmax, py::arg("logits"));
   m.def("greedy_sample", &svllm::ops::greedy_sample, py::arg("hidden"),
         py::arg("lm_head_weight"));
+  m.def("paged_plan", &svllm::ops::paged_plan, py::arg("context_lens"), py::arg("query_lens"),
+        py::arg("block_tables"), py::arg("blocks_owned"), py::arg("free_blocks"),
+        py::arg("free_count"), py::arg("num_tokens"), py::arg("block_size"),
+        py::arg("parents") = std::nullopt, py::arg("max_query_len") = 1);
+  m.def("tree_attention", &svllm::ops::tree_attention, py::arg("q"), py::arg("k_cache"),
+        py::arg("v_cache"), py::arg("block_tables"), py::arg("seq_lens"),
+        py::arg("query_start_loc"), py::arg("tree_mask") = std::nullopt,
+        py::arg("scale") = std::nullopt);
+  m.def("tree_accept", &svllm::ops::tree_accept, py::arg("ids"), py::arg("targets"),
+        py::arg("parents"), py::arg("query_start_loc"), py::arg("seq_lens"),
+        py::arg("context_lens"), py::arg("max_query_len"));
+  m.def("tree_commit", &svllm::ops::tree_commit, py::arg("k_caches"), py::arg("v_caches"),
+        py::arg("path"), py::arg("num_accepted"), py::arg("slot_mapping"),
+        py::arg("query_start_loc"));
   m.def("read_device_error", &svllm::ops::read_device_error, py::arg("device_index"),
         py::arg("reset") = true);
 
@@ -119,6 +136,9 @@ PYBIND11_MODULE(svllm_ops, m) {
       .def("greedy", &Model::greedy, py::arg("hidden"))
       .def("decode", &Model::decode, py::arg("ids"), py::arg("positions"),
            py::arg("slot_mapping"), py::arg("block_tables"), py::arg("seq_lens"))
+      .def("verify", &Model::verify, py::arg("ids"), py::arg("positions"),
+           py::arg("slot_mapping"), py::arg("block_tables"), py::arg("seq_lens"),
+           py::arg("query_start_loc"), py::arg("tree_mask") = std::nullopt)
       .def_property_readonly("config", &Model::config)
       .def_property_readonly("block_size", &Model::block_size)
       .def_property_readonly("num_blocks", &Model::num_blocks)

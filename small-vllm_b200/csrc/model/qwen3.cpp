@@ -13,6 +13,7 @@
 #include "ops/rope.h"
 #include "ops/sampling.h"
 #include "ops/silu_and_mul.h"
+#include "ops/tree_attention.h"
 
 #include "svllm_kernels.h"
 
@@ -199,7 +200,13 @@ at::Tensor Model::forward(const at::Tensor& ids, const at::Tensor& positions,
   const int64_t Hq = config_.num_heads, Hk = config_.num_kv_heads, D = config_.head_dim;
   const double eps = config_.rms_norm_eps;
   const bool paged = paged_decode_ok(meta);
-  const AttentionPlan plan = paged ? AttentionPlan{} : plan_attention(T, meta);
+  const AttentionPlan plan = paged || meta.tree ? AttentionPlan{} : plan_attention(T, meta);
+  at::Tensor tables, lens, starts;
+  if (meta.tree) {
+    tables = meta.block_tables.to(at::kInt).contiguous();
+    lens = meta.seq_lens.to(at::kInt).contiguous();
+    starts = meta.query_start_loc.to(at::kInt).contiguous();
+  }
 
   at::Tensor hidden = ops::embedding(ids, embed_);
   at::Tensor residual;
@@ -223,8 +230,12 @@ at::Tensor Model::forward(const at::Tensor& ids, const at::Tensor& positions,
       ops::rope_cache(q, k, v, positions, meta.slot_mapping, k_cache_[l], v_cache_[l],
                       config_.rope_theta, config_.rope_scaling);
     }
-    const at::Tensor attn = paged ? paged_decode_attention(q, static_cast<int64_t>(l), meta)
-                                  : attention(q, static_cast<int64_t>(l), plan);
+    const at::Tensor attn =
+        meta.tree ? ops::tree_attention(q, k_cache_[l], v_cache_[l], tables, lens, starts,
+                                        meta.tree_mask, std::nullopt)
+                        .view({T, Hq * D})
+        : paged ? paged_decode_attention(q, static_cast<int64_t>(l), meta)
+                : attention(q, static_cast<int64_t>(l), plan);
     hidden = project(attn, layer.o_proj);
     ops::add_rms_norm(hidden, residual, layer.post_norm, eps);
     hidden = project(ops::silu_and_mul(project(hidden, layer.gate_up)), layer.down);
@@ -245,6 +256,16 @@ at::Tensor Model::decode(const at::Tensor& ids, const at::Tensor& positions,
   const at::Tensor qsl = at::arange(
       ids.size(0) + 1, at::TensorOptions().dtype(at::kInt).device(ids.device()));
   return greedy(forward(ids, positions, {slot_mapping, block_tables, seq_lens, qsl, true}));
+}
+
+at::Tensor Model::verify(const at::Tensor& ids, const at::Tensor& positions,
+                         const at::Tensor& slot_mapping, const at::Tensor& block_tables,
+                         const at::Tensor& seq_lens, const at::Tensor& query_start_loc,
+                         const std::optional<at::Tensor>& tree_mask) {
+  AttentionMetadata meta{slot_mapping, block_tables, seq_lens, query_start_loc};
+  meta.tree = true;
+  if (tree_mask.has_value()) meta.tree_mask = *tree_mask;
+  return greedy(forward(ids, positions, meta));
 }
 
 #ifdef SVLLM_CUDA

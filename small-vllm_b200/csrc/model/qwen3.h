@@ -10,13 +10,15 @@
 // add_rms_norm -> one gate_up GEMM -> silu_and_mul -> down GEMM. GEMMs are torch::linear
 // (cuBLAS on GPU, as the reference plans, docs/ROADMAP.md:16), except for batches of up to 16
 // token rows on CUDA, which take this library's decode-linear kernel. Attention: on CUDA
-// decode steps the paged decode-attention kernel reads the cache in place; otherwise (prefill,
-// mixed steps, CPU) a LibTorch composite over the gathered cache.
+// decode steps the paged decode-attention kernel reads the cache in place, steps that check drafted
+// tokens (Model::verify) take ops::tree_attention; otherwise (prefill, mixed steps, decode on the
+// CPU) a LibTorch composite over the gathered cache.
 
 #include <ATen/ATen.h>
 
 #include <cstdint>
 #include <memory>
+#include <optional>
 #include <string>
 #include <unordered_map>
 #include <vector>
@@ -40,6 +42,11 @@ struct AttentionMetadata {
   at::Tensor seq_lens;
   at::Tensor query_start_loc;
   bool decode = false;  // every request has one query token (query_start_loc = 0..S)
+  // Tokens of a request are nodes of a tree of drafted tokens: token i is written behind the
+  // context like any other, sits at its own `positions` entry and sees the context, itself and
+  // its ancestors (ops::tree_attention); tree_mask [T, W] int64, undefined for chains.
+  bool tree = false;
+  at::Tensor tree_mask = {};
 };
 
 // A decoder-only Qwen3 or Llama model. Weights are taken by their Hugging Face names; q/k/v and
@@ -69,6 +76,15 @@ class Model {
   at::Tensor decode(const at::Tensor& ids, const at::Tensor& positions,
                     const at::Tensor& slot_mapping, const at::Tensor& block_tables,
                     const at::Tensor& seq_lens);
+
+  // One verification step: every request feeds a tree (or chain) of drafted tokens, its nodes
+  // packed as ops::paged_plan lays them out (its slot_mapping, positions, seq_lens,
+  // query_start_loc and tree_mask). Returns the next token after every node, [T] int64: the
+  // targets of ops::tree_accept, which ops::tree_commit follows on k_cache() and v_cache().
+  at::Tensor verify(const at::Tensor& ids, const at::Tensor& positions,
+                    const at::Tensor& slot_mapping, const at::Tensor& block_tables,
+                    const at::Tensor& seq_lens, const at::Tensor& query_start_loc,
+                    const std::optional<at::Tensor>& tree_mask);
 
   const ModelConfig& config() const { return config_; }
   int64_t block_size() const { return block_size_; }

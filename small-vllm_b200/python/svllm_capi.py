@@ -70,6 +70,13 @@ SIGNATURES = {
     "svllm_paged_decode_attention_bf16": [_P, _P, _I64, _P, _P, _I64, _I64, _P, _I64, _P, _I64,
                                           _I64, _I64, _I64, _I64, ctypes.c_float, _P],
     "svllm_decode_linear_bf16": [_P, _I64, _P, _I64, _I64, _I64, _P, _I64, _I64, _P],
+    "svllm_paged_plan": [_P, _P, _I64, _P, _I64, _P, _P, _I64, _P, _I64, _P, _I64, _I64, _P, _P,
+                         _P, _P, _P, _P, _P, _P],
+    "svllm_tree_attention_bf16": [_P, _P, _I64, _P, _P, _I64, _I64, _P, _I64, _P, _P, _I64, _I64,
+                                  _I64, _I64, _I64, _P, _I64, _F, _P, _I64, _P],
+    "svllm_tree_attention_workspace_bytes": [_I64, _P],
+    "svllm_tree_accept": [_P, _I, _P, _P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _P, _P, _P],
+    "svllm_tree_commit": [_P, _P, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _P],
     "svllm_read_device_error": [_I, _I, _P],
 }
 
@@ -264,6 +271,71 @@ def decode_linear(out, x, weight, stream=None) -> None:
     check(lib().svllm_decode_linear_bf16(
         out.data_ptr(), out.stride(0), x.data_ptr(), rows, in_features, x_stride,
         weight.data_ptr(), out_features, weight_stride, _stream(stream)), "decode_linear")
+
+
+def _ptr(t) -> int | None:
+    return t.data_ptr() if t is not None else None
+
+
+def paged_plan(context_lens, query_lens, block_tables, blocks_owned, free_blocks, free_count,
+               block_size: int, parents, max_query_len: int, num_tokens: int, query_start_loc,
+               seq_lens, slot_mapping, positions, tree_mask, blocks_owned_out, free_count_out,
+               stream=None) -> None:
+    """The paging of one step; the outputs from query_start_loc on, block_tables and free_blocks
+    are written. parents and tree_mask are None for chains."""
+    check(lib().svllm_paged_plan(
+        context_lens.data_ptr(), query_lens.data_ptr(), context_lens.numel(),
+        block_tables.data_ptr(), block_tables.shape[1], blocks_owned.data_ptr(),
+        free_blocks.data_ptr(), free_blocks.numel(), free_count.data_ptr(), block_size,
+        _ptr(parents), max_query_len, num_tokens, query_start_loc.data_ptr(),
+        seq_lens.data_ptr(), slot_mapping.data_ptr(), positions.data_ptr(), _ptr(tree_mask),
+        blocks_owned_out.data_ptr(), free_count_out.data_ptr(), _stream(stream)), "paged_plan")
+
+
+def tree_attention_workspace_bytes(head_dim: int) -> int:
+    size = _I64(0)
+    check(lib().svllm_tree_attention_workspace_bytes(head_dim, ctypes.byref(size)),
+          "tree_attention_workspace_bytes")
+    return size.value
+
+
+def tree_attention(out, q, k_cache, v_cache, block_tables, seq_lens, query_start_loc, tree_mask,
+                   scale: float, workspace, stream=None) -> None:
+    """out [T, Hq, D] = attention of q [T, Hq, D] over the paged caches; workspace: uint8 tensor
+    of tree_attention_workspace_bytes(D); tree_mask: int64 [T, W] or None (causal)."""
+    num_tokens, num_heads, head_dim = q.shape
+    num_blocks, block_size, num_kv_heads, _ = k_cache.shape
+    check(lib().svllm_tree_attention_bf16(
+        out.data_ptr(), q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(),
+        num_blocks, block_size, block_tables.data_ptr(), block_tables.shape[1],
+        seq_lens.data_ptr(), query_start_loc.data_ptr(), seq_lens.numel(), num_tokens, num_heads,
+        num_kv_heads, head_dim, _ptr(tree_mask),
+        tree_mask.shape[1] if tree_mask is not None else 0, scale, workspace.data_ptr(),
+        workspace.numel(), _stream(stream)), "tree_attention")
+
+
+def tree_accept(ids, targets, parents, query_start_loc, seq_lens, context_lens, path, tokens,
+                num_accepted, context_lens_out, stream=None) -> None:
+    """Greedy acceptance into path, tokens [S, max_query_len] and the counts."""
+    check(lib().svllm_tree_accept(
+        ids.data_ptr(), _index_type(ids), targets.data_ptr(), _ptr(parents),
+        query_start_loc.data_ptr(), seq_lens.data_ptr(), context_lens.data_ptr(),
+        seq_lens.numel(), ids.numel(), path.shape[1], path.data_ptr(), tokens.data_ptr(),
+        num_accepted.data_ptr(), context_lens_out.data_ptr(), _stream(stream)), "tree_accept")
+
+
+def tree_commit(k_caches, v_caches, path, num_accepted, slot_mapping, query_start_loc,
+                stream=None) -> None:
+    """Moves the accepted rows in every cache of the two lists."""
+    first = k_caches[0]
+    row = first.shape[-1] * first.shape[-2]
+    k = (_P * len(k_caches))(*[c.data_ptr() for c in k_caches])
+    v = (_P * len(v_caches))(*[c.data_ptr() for c in v_caches])
+    check(lib().svllm_tree_commit(
+        ctypes.cast(k, _P), ctypes.cast(v, _P), len(k_caches), first.numel() // row,
+        row * first.element_size(), path.data_ptr(), num_accepted.data_ptr(),
+        slot_mapping.data_ptr(), query_start_loc.data_ptr(), num_accepted.numel(),
+        slot_mapping.numel(), path.shape[1], _stream(stream)), "tree_commit")
 
 
 def read_device_error(device: int = 0, reset: bool = True) -> int:
