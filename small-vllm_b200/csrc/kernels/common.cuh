@@ -149,6 +149,34 @@ __device__ __forceinline__ uint64_t f32x2_mul(uint64_t a, uint64_t b) {
   return d;
 }
 
+// 2^x (the ex2 instruction; 2^-inf = 0).
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// j / d for 0 <= j < 2^31 by a precomputed reciprocal and a shift (Granlund and Montgomery,
+// "Division by invariant integers using multiplication", 1994): shift = ceil(log2 d), magic =
+// floor(2^32 (2^shift - d) / d) + 1.
+struct Divider {
+  uint32_t magic;
+  int shift;
+  __device__ __forceinline__ int divide(int j) const {
+    return static_cast<int>((__umulhi(static_cast<uint32_t>(j), magic) +
+                             static_cast<uint32_t>(j)) >> shift);
+  }
+};
+
+inline Divider make_divider(int64_t d) {
+  Divider r{};
+  while ((int64_t{1} << r.shift) < d) ++r.shift;
+  r.magic = static_cast<uint32_t>(
+      ((uint64_t{1} << 32) * ((uint64_t{1} << r.shift) - static_cast<uint64_t>(d))) /
+          static_cast<uint64_t>(d) + 1);
+  return r;
+}
+
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) {
   return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
 }

@@ -44,20 +44,12 @@ struct AttnArgs {
   int64_t num_blocks;
   int max_blocks;
   int block_size;
-  uint32_t page_magic;       // j / block_size = (umulhi(j, page_magic) + j) >> page_shift
-  int page_shift;
+  Divider page;              // by the block size
   int num_kv_heads;
   int splits;
   float scale_log2;          // scale * log2(e): scores are kept in the base-2 exponent domain
   int* err;
 };
-
-// 2^x (the ex2 instruction; 2^-inf = 0).
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // The warp's 8x8 bf16 matrix (lane l holds row l / 4, columns 2 (l % 4) and 2 (l % 4) + 1)
 // transposed, in the same layout.
@@ -68,13 +60,10 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 }
 
 // Byte offset of cache row j of a request (its page looked up in the block table) from the
-// start of the cache. Division by the block size: multiply by a precomputed reciprocal and
-// shift (Granlund and Montgomery, "Division by invariant integers using multiplication", 1994,
-// exact for j < 2^31).
+// start of the cache.
 __device__ __forceinline__ int64_t cache_row_offset(const AttnArgs& a, const int32_t* table,
                                                     int j, int64_t row_bytes) {
-  const int page = static_cast<int>((__umulhi(static_cast<uint32_t>(j), a.page_magic) +
-                                     static_cast<uint32_t>(j)) >> a.page_shift);
+  const int page = a.page.divide(j);
   int blk = __ldg(table + page);
   if (static_cast<uint64_t>(blk) >= static_cast<uint64_t>(a.num_blocks)) {
     raise_error(a.err, kErrBadIndex);  // an entry outside the cache: read block 0
@@ -422,14 +411,7 @@ extern "C" int svllm_paged_decode_attention_bf16(
   a.num_blocks = num_blocks;
   a.max_blocks = static_cast<int>(max_blocks);
   a.block_size = static_cast<int>(block_size);
-  // the reciprocal of the block size for the page lookup: shift = ceil(log2 block_size),
-  // magic = floor(2^32 (2^shift - block_size) / block_size) + 1
-  int shift = 0;
-  while ((int64_t{1} << shift) < block_size) ++shift;
-  a.page_shift = shift;
-  a.page_magic = static_cast<uint32_t>(
-      ((uint64_t{1} << 32) * ((uint64_t{1} << shift) - static_cast<uint64_t>(block_size))) /
-          static_cast<uint64_t>(block_size) + 1);
+  a.page = make_divider(block_size);
   a.num_kv_heads = static_cast<int>(num_kv_heads);
   a.scale_log2 = static_cast<float>(static_cast<double>(scale) / std::log(2.0));
   a.err = err;

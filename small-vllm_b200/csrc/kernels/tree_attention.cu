@@ -4,8 +4,30 @@
 //   o[t, h] = sum_j p_j v_j,  p = softmax_j(scale * q[t, h] . k_j),
 //   j < context, or j = context + node with the node's bit in tree_mask[t]
 //
-// One warp per (token, head): each lane scores one of 32 cache rows, then every row's value is
-// added by all lanes, 16 bytes or less of it each.
+// The query heads of a KV head share its cached rows, so a request's n tokens make n * G query
+// rows per KV head (G = heads / KV heads), and the cache is read once per 128 or 256 of them. At
+// R rows a cached row of D elements costs 4 R D operations and 4 D bytes: up to the R of a few
+// hundred where the tensor pipe becomes the bound (1616 TFLOP/s against 6.55 TB/s: 247), the
+// stream over K and V is what bounds this kernel.
+//
+// Work: rows come in M tiles of 128 (row = node * G + head), cached rows in tiles of 128. An item
+// is either two M tiles of one (request, KV head), which share every K and V tile, or, for a last
+// odd M tile, that tile of two neighbouring KV heads. Items times their key tiles form one line of
+// steps; each CTA (one per SM) computes the line's length from the request lengths and takes an
+// equal share, so ragged batches and single long requests fill the GPU alike and the host needs no
+// lengths. An item cut by a share's border leaves unnormalised partial sums in the workspace, which
+// a second small kernel joins.
+//
+// In a CTA: 4 producer warps gather K and V rows through the block table with cp.async into
+// 128-byte-swizzled tiles (any block size: a page may end anywhere in a tile); one thread issues
+// tcgen05.mma: S = Q K^T into TMEM, then O += P V with P read from TMEM and V as the N-major
+// operand, alternating between two accumulators so that the tensor pipe works on one M tile while
+// the other's softmax runs; two groups of 4 warps do the softmax, one thread per row, and write P
+// (bf16, as the second product takes it) over S. The running maximum is a reference that moves
+// only when a row exceeds it by 2^8, so O in TMEM is seldom rescaled; the sums are fp32 and the
+// result does not depend on the reference. Masked scores are replaced after the product, and
+// non-finite values of V in the tiles that hold tree nodes (0 * NaN would reach rows that do not
+// see them) are taken out on the way in and added again, for the rows that see them, at the end.
 #include <cuda_runtime.h>
 
 #include <cmath>
@@ -13,9 +35,44 @@
 
 #include "common.cuh"
 #include "host_common.h"
+#include "umma.cuh"
 
 namespace svllm::k {
 namespace {
+
+constexpr int kTile = 128;            // query rows per M tile, cached rows per key tile
+constexpr int kSoftmaxWarps = 8;      // two groups of 4: accumulators 0 and 1
+constexpr int kProducerWarps = 4;
+constexpr int kMmaWarp = kSoftmaxWarps + kProducerWarps;
+constexpr int kThreads = (kMmaWarp + 1) * kWarpSize;
+constexpr int kHalfBytes = kTile * 128;  // 128 rows of one 128-byte swizzle atom
+constexpr uint32_t kTmemColumns = 512;
+constexpr uint32_t kScores = 0;       // TMEM columns: S (and P) of accumulator w at 128 w,
+constexpr uint32_t kOutput = 256;     // O at 256 + 128 w
+constexpr float kRescaleAbove = 8.0f;  // in powers of two
+constexpr int kJoinThreads = 128;
+constexpr int kJoinRows = 32;
+
+template <int D>
+struct Shape {
+  static constexpr int kHalves = D / 64;
+  static constexpr int kTileBytes = kHalves * kHalfBytes;
+  static constexpr int kStagesK = D == 128 ? 3 : 6;
+  static constexpr int kStagesV = D == 128 ? 2 : 4;
+  static constexpr int kPending = D == 128 ? 4 : 7;  // cp.async groups in flight, at most 7
+  static constexpr size_t kSmem = 1024 + static_cast<size_t>(kTileBytes) *
+                                             (2 + kStagesK + kStagesV);
+  // partial sums of one accumulator: O as [D / 4][128 rows][4], then the rows' maxima and sums
+  static constexpr int kPartFloats = (D + 2) * kTile;
+};
+
+// A segment whose item is cut: what the join needs to know of it.
+struct Cut {
+  int flags;                       // 0: none, else kCut and the ends that are cut
+  int token0;                      // the request's first token
+  int kv_head[2], row0[2], rows[2];  // per accumulator; rows 0: unused
+};
+constexpr int kCut = 1, kCutFront = 2, kCutBack = 4;
 
 struct TreeAttnArgs {
   void* out;                       // [num_tokens, num_heads, head_dim] bf16, contiguous
@@ -26,113 +83,836 @@ struct TreeAttnArgs {
   const int32_t* seq_lens;         // [num_seqs]
   const int32_t* query_start_loc;  // [num_seqs + 1]
   const int64_t* tree_mask;        // [num_tokens, mask_words] or null: causal
+  float* parts;                    // [CTAs][2][2] partial sums
+  Cut* cuts;                       // [CTAs][2]
   int64_t q_stride;
   int64_t num_blocks;
   int64_t num_tokens;
   int64_t num_seqs;
   int max_blocks;
   int block_size;
-  int num_heads;
+  Divider page;                    // by the block size
+  int group;                       // query heads per KV head
   int num_kv_heads;
   int mask_words;
-  float scale_log2;
+  float scale_log2;                // scale * log2(e): scores are kept in powers of two
   int* err;
 };
 
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
+// One request's share of the line. Valid lengths only: anything else has no items.
+struct Request {
+  int start, nodes, context, length;  // first token, tokens, earlier rows, all rows
+  int steps;                          // key tiles
+  int pairs;                          // items of two M tiles per KV head
+  int odd;                            // 1: a last single M tile, in items of two KV heads
+  bool bad;                           // lengths out of range
+};
+
+__device__ __forceinline__ Request load_request(const TreeAttnArgs& a, int64_t s) {
+  Request r{};
+  const int64_t begin = a.query_start_loc[s], end = a.query_start_loc[s + 1];
+  const int64_t length = a.seq_lens[s];
+  if (begin < 0 || end < begin || end > a.num_tokens) {
+    r.bad = true;
+    return r;
+  }
+  r.start = static_cast<int>(begin);
+  r.nodes = static_cast<int>(end - begin);
+  if (length == 0) return r;
+  if (length < r.nodes || length > static_cast<int64_t>(a.max_blocks) * a.block_size ||
+      (a.tree_mask != nullptr && r.nodes > 64 * a.mask_words)) {
+    r.bad = true;
+    return r;
+  }
+  r.length = static_cast<int>(length);
+  r.context = r.length - r.nodes;
+  if (r.nodes > 0) {
+    const int tiles = (r.nodes * a.group + kTile - 1) / kTile;
+    r.steps = (r.length + kTile - 1) / kTile;
+    r.pairs = tiles / 2;
+    r.odd = tiles & 1;
+  }
+  return r;
+}
+
+// Steps of the line, weighted: a step over two KV heads loads twice what the others load.
+__device__ __forceinline__ int64_t request_cost(const TreeAttnArgs& a, const Request& r) {
+  return static_cast<int64_t>(a.num_kv_heads) * r.steps * (r.pairs + r.odd);
+}
+
+// A place on the line: request, item of the request, step of the item.
+struct Place {
+  int64_t s;
+  int item, step;
+};
+
+__device__ __forceinline__ Place locate(const TreeAttnArgs& a, int64_t s, const Request& r,
+                                        int64_t at) {
+  const int64_t shared = static_cast<int64_t>(a.num_kv_heads) * r.pairs * r.steps;
+  Place p{s, 0, 0};
+  if (at < shared) {
+    p.item = static_cast<int>(at / r.steps);
+    p.step = static_cast<int>(at % r.steps);
+    return p;
+  }
+  at -= shared;
+  const int pair = static_cast<int>(at / (2 * r.steps));
+  const int64_t rest = at - static_cast<int64_t>(pair) * 2 * r.steps;
+  const bool two = 2 * pair + 1 < a.num_kv_heads;
+  p.item = a.num_kv_heads * r.pairs + pair;
+  p.step = static_cast<int>(two ? (rest + 1) / 2 : rest);
+  if (p.step == r.steps) {  // rounded up to the item's end
+    ++p.item;
+    p.step = 0;
+  }
+  return p;
+}
+
+// A run of steps of one item.
+struct Segment {
+  int64_t s;
+  Request r;
+  bool shared;                   // both accumulators take the same K and V
+  int active;                    // accumulators in use, 1 or 2
+  int kv_head[2], row0[2], rows[2];
+  int step0, step1;
+  bool front, back;              // cut there
+};
+
+// The next segment of [at, end); false when there is none.
+__device__ __forceinline__ bool next_segment(const TreeAttnArgs& a, Place& at, const Place& end,
+                                             Segment& g) {
+  while (at.s < a.num_seqs &&
+         (at.s < end.s || (at.s == end.s && (at.item < end.item ||
+                                             (at.item == end.item && at.step < end.step))))) {
+    g.r = load_request(a, at.s);
+    const int shared_items = a.num_kv_heads * g.r.pairs;
+    const int items = g.r.steps == 0 ? 0
+                                     : shared_items + g.r.odd * ((a.num_kv_heads + 1) / 2);
+    if (at.item >= items) {
+      at = Place{at.s + 1, 0, 0};
+      continue;
+    }
+    const int all_rows = g.r.nodes * a.group;
+    g.s = at.s;
+    g.shared = at.item < shared_items;
+    if (g.shared) {
+      g.active = 2;
+      g.kv_head[0] = g.kv_head[1] = at.item / g.r.pairs;
+      g.row0[0] = (at.item % g.r.pairs) * 2 * kTile;
+      g.row0[1] = g.row0[0] + kTile;
+      g.rows[0] = kTile;
+      g.rows[1] = min(kTile, all_rows - g.row0[1]);
+    } else {
+      const int pair = at.item - shared_items;
+      g.kv_head[0] = 2 * pair;
+      g.kv_head[1] = 2 * pair + 1;
+      g.active = g.kv_head[1] < a.num_kv_heads ? 2 : 1;
+      g.row0[0] = g.row0[1] = g.r.pairs * 2 * kTile;
+      g.rows[0] = all_rows - g.row0[0];
+      g.rows[1] = g.active == 2 ? g.rows[0] : 0;
+    }
+    g.step0 = at.step;
+    g.step1 = at.s == end.s && at.item == end.item ? end.step : g.r.steps;
+    g.front = g.step0 > 0;
+    g.back = g.step1 < g.r.steps;
+    at = Place{at.s, at.item + 1, 0};
+    return true;
+  }
+  return false;
+}
+
+// Barriers and flags of one CTA.
+constexpr int kMaxStagesK = 6, kMaxStagesV = 4;
+constexpr int kFullK = 0, kFullV = kFullK + kMaxStagesK, kFullQ = kFullV + kMaxStagesV;
+constexpr int kEmptyK = kFullQ + 1, kEmptyV = kEmptyK + kMaxStagesK;
+constexpr int kEmptyQ = kEmptyV + kMaxStagesV;
+constexpr int kScoresDone = kEmptyQ + 1, kWeightsDone = kScoresDone + 2;
+constexpr int kOutputDone = kWeightsDone + 2, kDrain = kOutputDone + 2, kBarriers = kDrain + 1;
+
+struct Sync {
+  uint64_t bar[kBarriers];
+  uint32_t tmem_base;
+  int abort;
+  int odd_values[2][4];  // per accumulator and segment modulo 4: V held something not finite
+  int64_t sums[kMmaWarp + 1];
+  Place place[2];        // this CTA's share
+};
+
+// A ring of tiles: the slot in use and the parity of its current round.
+struct Ring {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void advance(int stages) {
+    if (++slot == stages) {
+      slot = 0;
+      phase ^= 1;
+    }
+  }
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(take ? 16 : 0)
+               : "memory");
+}
+
+__device__ __forceinline__ void cp_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Zeroes the non-finite halves of a word of two bf16; true if there were any.
+__device__ __forceinline__ bool drop_odd(uint32_t& w) {
+  const bool lo = (w & 0x7f80u) == 0x7f80u, hi = (w & 0x7f800000u) == 0x7f800000u;
+  if (lo) w &= 0xffff0000u;
+  if (hi) w &= 0x0000ffffu;
+  return lo || hi;
+}
+
+// The four producer warps: each gathers 32 of a tile's 128 rows. A thread signals a tile's barrier
+// when its own copies have landed and are visible to the tensor cores' proxy; up to kPending tiles
+// are in flight. Where the next slot is still in use it signals everything first and then waits, so
+// no consumer waits for a signal that waits for it.
+template <int D>
+struct Producer {
+  using S = Shape<D>;
+  static constexpr int kLanes = D / 8;                // lanes per row: 16 bytes each
+  static constexpr int kRowsAtOnce = kWarpSize / kLanes;
+
+  const TreeAttnArgs& a;
+  Sync& sy;
+  uint8_t* ring_k;
+  uint8_t* ring_v;
+  uint8_t* q_tiles;
+  int warp, lane;      // warp 0..3
+  Ring k{}, v{};
+  uint64_t pending = 0;  // barrier indices, oldest in the low byte
+  int count = 0;
+
+  __device__ void signal_oldest() {
+    fence_proxy_async_smem();
+    mbar_arrive(&sy.bar[pending & 0xff]);
+    pending >>= 8;
+    --count;
+  }
+  __device__ void flush() {
+    cp_async_wait<0>();
+    while (count > 0) signal_oldest();
+  }
+  __device__ bool acquire(int bar, uint32_t parity) {
+    bool free = mbar_test(&sy.bar[bar], parity);
+    if (!__all_sync(0xffffffffu, free)) {
+      flush();
+      free = wait_phase(&sy.bar[bar], parity, &sy.abort, a.err);
+      return __all_sync(0xffffffffu, free);
+    }
+    return true;
+  }
+  __device__ void issued(int bar) {
+    cp_async_commit();
+    pending |= static_cast<uint64_t>(bar) << (8 * count);
+    if (++count > S::kPending) {
+      cp_async_wait<S::kPending>();
+      signal_oldest();
+    }
+  }
+
+  // Element offset of KV head 0 of this lane's row of key tile `step`, -1 past the request's end.
+  __device__ int64_t row_offset(const Segment& g, int step) const {
+    const int j = step * kTile + warp * kWarpSize + lane;
+    if (step >= g.step1 || j >= g.r.length) return -1;
+    const int page = a.page.divide(j);
+    int64_t block = a.block_tables[g.s * a.max_blocks + page];
+    if (block < 0 || block >= a.num_blocks) {  // outside the cache: block 0 is read
+      raise_error(a.err, kErrBadIndex);
+      block = 0;
+    }
+    return (block * a.block_size + (j - page * a.block_size)) * a.num_kv_heads * D;
+  }
+
+  __device__ __forceinline__ uint32_t tile_place(uint32_t base, int row) const {
+    const int c = lane % kLanes;
+    return base + (c / 8) * kHalfBytes + row * 128 + (((c % 8) ^ (row & 7)) << 4);
+  }
+
+  // Rows of `src` at `offset` (one per lane, elements, -1 = zeros) into a tile.
+  __device__ void gather(uint8_t* tile, const void* src, int64_t offset, int64_t column) {
+    const uint32_t base = smem_addr(tile);
+    const auto* p = static_cast<const __nv_bfloat16*>(src) + column + (lane % kLanes) * 8;
+#pragma unroll 4
+    for (int i = 0; i < kWarpSize / kRowsAtOnce; ++i) {
+      const int row = i * kRowsAtOnce + lane / kLanes;
+      const int64_t off = __shfl_sync(0xffffffffu, offset, row);
+      cp_async16(tile_place(base, warp * kWarpSize + row), p + (off < 0 ? 0 : off), off >= 0);
+    }
+  }
+
+  // The same for a V tile that holds tree nodes: through registers, values that are not finite
+  // left out; true if there were any.
+  __device__ bool gather_checked(uint8_t* tile, const void* src, int64_t offset, int64_t column) {
+    const uint32_t base = smem_addr(tile);
+    const auto* p = static_cast<const __nv_bfloat16*>(src) + column + (lane % kLanes) * 8;
+    bool odd = false;
+#pragma unroll 8
+    for (int i = 0; i < kWarpSize / kRowsAtOnce; ++i) {
+      const int row = i * kRowsAtOnce + lane / kLanes;
+      const int64_t off = __shfl_sync(0xffffffffu, offset, row);
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (off >= 0) w = ld_global_nc_v4(p + off);
+      odd |= drop_odd(w.x) | drop_odd(w.y) | drop_odd(w.z) | drop_odd(w.w);
+      asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(
+                       tile_place(base, warp * kWarpSize + row)),
+                   "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
+                   : "memory");
+    }
+    return odd;
+  }
+
+  __device__ bool load_k(const Segment& g, int w, int64_t offset) {
+    if (!acquire(kEmptyK + k.slot, k.phase ^ 1)) return false;
+    gather(ring_k + k.slot * S::kTileBytes, a.k_cache, offset,
+           static_cast<int64_t>(g.kv_head[w]) * D);
+    issued(kFullK + k.slot);
+    k.advance(S::kStagesK);
+    return true;
+  }
+  __device__ bool load_v(const Segment& g, int w, int64_t offset, int step, int index) {
+    if (!acquire(kEmptyV + v.slot, v.phase ^ 1)) return false;
+    uint8_t* tile = ring_v + v.slot * S::kTileBytes;
+    const int64_t column = static_cast<int64_t>(g.kv_head[w]) * D;
+    if ((step + 1) * kTile > g.r.context) {
+      if (gather_checked(tile, a.v_cache, offset, column)) {
+        sy.odd_values[w][index & 3] = 1;
+        if (g.shared) sy.odd_values[1][index & 3] = 1;
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&sy.bar[kFullV + v.slot]);
+    } else {
+      gather(tile, a.v_cache, offset, column);
+      issued(kFullV + v.slot);
+    }
+    v.advance(S::kStagesV);
+    return true;
+  }
+
+  __device__ void run(Place at, const Place end) {
+    Segment g;
+    bool ok = true;
+    for (int index = 0; ok && next_segment(a, at, end, g); ++index) {
+      int64_t now = row_offset(g, g.step0);
+      // the query rows of both accumulators
+      ok = acquire(kEmptyQ, (index & 1) ^ 1);
+      if (!ok) break;
+      for (int w = 0; w < g.active; ++w) {
+        const int r = warp * kWarpSize + lane;
+        const int row = g.row0[w] + r;
+        const int64_t off =
+            r < g.rows[w] ? (g.r.start + row / a.group) * a.q_stride +
+                                (static_cast<int64_t>(g.kv_head[w]) * a.group + row % a.group) * D
+                          : -1;
+        gather(q_tiles + w * S::kTileBytes, a.q, off, 0);
+      }
+      issued(kFullQ);
+      // in the order in which the tensor cores take them
+      int64_t before = -1;
+      for (int step = g.step0; ok && step <= g.step1; ++step) {
+        const int64_t next = row_offset(g, step + 1);
+        for (int w = 0; ok && w < (g.shared ? 1 : g.active); ++w) {
+          if (step > g.step0) ok = load_v(g, w, before, step - 1, index);
+          if (ok && step < g.step1) ok = load_k(g, w, now);
+        }
+        before = now;
+        now = next;
+      }
+    }
+    flush();  // also after an abort: no copy of this CTA is in flight when it exits
+  }
+};
+
+// The thread that issues the matrix products.
+template <int D>
+__device__ void issue_products(const TreeAttnArgs& a, Sync& sy, const uint8_t* q_tiles,
+                               const uint8_t* ring_k, const uint8_t* ring_v, Place at,
+                               const Place end) {
+  using S = Shape<D>;
+  constexpr uint32_t kIdescS = idesc_bf16(kTile, kTile);
+  constexpr uint32_t kIdescO = idesc_bf16(kTile, D) | kIdescBMajorN;
+  Ring k, v;
+  uint32_t weights_phase[2] = {0, 0};
+  bool ok = true;
+  const auto wait = [&](int bar, uint32_t parity) {
+    ok = wait_phase(&sy.bar[bar], parity, &sy.abort, a.err);
+    tc_fence_after();
+    return ok;
+  };
+  Segment g;
+  for (int index = 0; ok && next_segment(a, at, end, g); ++index) {
+    const auto scores = [&](int w, bool last) {
+      const bool first_use = !g.shared || w == 0, last_use = !g.shared || w == 1;
+      if (first_use && !wait(kFullK + k.slot, k.phase)) return;
+      const uint8_t* qt = q_tiles + w * S::kTileBytes;
+      const uint8_t* kt = ring_k + k.slot * S::kTileBytes;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const int at_bytes = (kk / 4) * kHalfBytes + (kk % 4) * 32;
+        umma_bf16(sy.tmem_base + kScores + w * kTile, smem_desc_k_sw128(qt + at_bytes),
+                  smem_desc_k_sw128(kt + at_bytes), kIdescS, kk != 0);
+      }
+      umma_commit(&sy.bar[kScoresDone + w]);
+      if (last_use) {
+        umma_commit(&sy.bar[kEmptyK + k.slot]);
+        k.advance(S::kStagesK);
+      }
+      if (last && w == g.active - 1) umma_commit(&sy.bar[kEmptyQ]);
+    };
+    if (!wait(kFullQ, index & 1)) break;
+    for (int w = 0; ok && w < g.active; ++w) scores(w, g.step0 + 1 == g.step1);
+    for (int step = g.step0; ok && step < g.step1; ++step) {
+      for (int w = 0; ok && w < g.active; ++w) {
+        if (!wait(kWeightsDone + w, weights_phase[w])) break;
+        weights_phase[w] ^= 1;
+        const bool first_use = !g.shared || w == 0, last_use = !g.shared || w == 1;
+        if (first_use && !wait(kFullV + v.slot, v.phase)) break;
+        const uint8_t* vt = ring_v + v.slot * S::kTileBytes;
+#pragma unroll
+        for (int kk = 0; kk < kTile / 16; ++kk) {
+          umma_bf16_ts(sy.tmem_base + kOutput + w * kTile,
+                       sy.tmem_base + kScores + w * kTile + kk * 8,
+                       smem_desc_mn_sw128(vt + kk * 2048, kHalfBytes), kIdescO,
+                       step > g.step0 || kk != 0);
+        }
+        if (last_use) {
+          umma_commit(&sy.bar[kEmptyV + v.slot]);
+          v.advance(S::kStagesV);
+        }
+        if (step + 1 == g.step1) {
+          umma_commit(&sy.bar[kOutputDone + w]);
+        } else {
+          // the next scores may overwrite these weights: products complete in order
+          scores(w, step + 2 == g.step1);
+        }
+      }
+    }
+  }
+  // every product this thread issued has completed before the TMEM is freed
+  umma_commit(&sy.bar[kDrain]);
+  mbar_wait_bounded(&sy.bar[kDrain], 0);
+}
+
+// Which of the 32 cached rows from j on a node sees, as bits.
+__device__ __forceinline__ uint32_t visible32(const TreeAttnArgs& a, const Request& r,
+                                              const int64_t* mask, int node, int j) {
+  const int rel = j - r.context;  // node index of row j
+  const int limit = a.tree_mask == nullptr ? min(r.nodes, node + 1) : r.nodes;
+  uint32_t bits = ~0u;
+  if (rel + 32 > 0 && mask != nullptr) {
+    // 32 bits of the mask from bit `rel` on, ones for the context before it
+    const int lo = rel >> 6;
+    const uint64_t w0 = lo >= 0 && lo < a.mask_words ? static_cast<uint64_t>(mask[lo])
+                        : lo < 0                     ? ~uint64_t{0}
+                                                     : 0;
+    const uint64_t w1 = lo + 1 < a.mask_words ? static_cast<uint64_t>(mask[lo + 1]) : 0;
+    const int sh = rel & 63;
+    bits = static_cast<uint32_t>(sh == 0 ? w0 : (w0 >> sh) | (w1 << (64 - sh)));
+  }
+  const int left = limit - rel;  // rows from j on before the end
+  return left >= 32 ? bits : left <= 0 ? 0u : bits & ((1u << left) - 1);
+}
+
+// Softmax and epilogue of accumulator w; this thread owns row `row` of the tile.
+template <int D>
+__device__ void softmax(const TreeAttnArgs& a, Sync& sy, int w, Place at, const Place end) {
+  using S = Shape<D>;
+  const int quarter = (threadIdx.x / kWarpSize) % 4;
+  const int row = quarter * kWarpSize + threadIdx.x % kWarpSize;
+  const uint32_t lanes = static_cast<uint32_t>(quarter * kWarpSize) << 16;
+  const uint32_t scores = sy.tmem_base + kScores + w * kTile + lanes;
+  const uint32_t output = sy.tmem_base + kOutput + w * kTile + lanes;
+  const float kInf = __builtin_huge_valf();
+  uint32_t scores_phase = 0, output_phase = 0;
+  Segment g;
+  for (int index = 0; next_segment(a, at, end, g); ++index) {
+    if (threadIdx.x % (4 * kWarpSize) == 0) sy.odd_values[w][(index + 2) & 3] = 0;
+    if (w >= g.active) continue;
+    const bool any = quarter * kWarpSize < g.rows[w];  // the warp holds rows of the request
+    const int at_row = g.row0[w] + (row < g.rows[w] ? row : 0);
+    const int node = at_row / a.group;
+    const int64_t token = g.r.start + node;
+    const int64_t* mask =
+        a.tree_mask == nullptr ? nullptr : a.tree_mask + token * a.mask_words;
+    float ref = -kInf, sum = 0.0f;
+    for (int step = g.step0; step < g.step1; ++step) {
+      // the warp leaves together: the TMEM loads below are collective
+      if (!__all_sync(0xffffffffu, wait_phase(&sy.bar[kScoresDone + w], scores_phase, &sy.abort,
+                                              a.err))) {
+        return;
+      }
+      scores_phase ^= 1;
+      tc_fence_after();
+      if (any) {
+        const bool masked = (step + 1) * kTile > g.r.context;
+        uint32_t see[4] = {~0u, ~0u, ~0u, ~0u};
+        if (masked) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            see[c] = visible32(a, g.r, mask, node, step * kTile + 32 * c);
+          }
+        }
+        float top = -kInf;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t x[32];
+          tmem_load32(scores + 32 * c, x);
+          tmem_wait_load();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float f = __uint_as_float(x[i]);
+            top = fmaxf(top, !masked || (see[c] >> i) & 1 ? f : -kInf);
+          }
+        }
+        top *= a.scale_log2;
+        if (ref == -kInf || top > ref + kRescaleAbove) {
+          // a first reference, or one that rose: O so far is in units of 2^ref
+        } else {
+          top = ref;
+        }
+        const bool moved = top != ref;
+        if (step > g.step0 && __any_sync(0xffffffffu, moved)) {
+          const float f = moved ? exp2_approx(ref - top) : 1.0f;
+          sum *= f;
+#pragma unroll 1
+          for (int c = 0; c < D; c += 16) {
+            uint32_t o[16];
+            tmem_load16(output + c, o);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_store16(output + c, o);
+          }
+        }
+        ref = top;
+        const float base = ref == -kInf ? 0.0f : ref;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t x[32], p[16];
+          tmem_load32(scores + 32 * c, x);
+          tmem_wait_load();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float e = exp2_approx(fmaf(__uint_as_float(x[i]), a.scale_log2, -base));
+            const float f = !masked || (see[c] >> i) & 1 ? e : 0.0f;
+            sum += f;
+            x[i] = __float_as_uint(f);
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            p[i] = pack_bf16x2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
+          }
+          tmem_store16(scores + 16 * c, p);  // over scores that have been read
+        }
+        tmem_wait_store();
+      }
+      tc_fence_before();
+      mbar_arrive(&sy.bar[kWeightsDone + w]);
+    }
+
+    if (!__all_sync(0xffffffffu, wait_phase(&sy.bar[kOutputDone + w], output_phase, &sy.abort,
+                                            a.err))) {
+      return;
+    }
+    output_phase ^= 1;
+    tc_fence_after();
+    const bool cut = g.front || g.back;
+    // a CTA has at most two cut segments: its first and its last
+    const int slot = index == 0 ? 0 : 1;
+    float* part = a.parts + ((static_cast<int64_t>(blockIdx.x) * 2 + slot) * 2 + w) *
+                                S::kPartFloats;
+    if (cut && threadIdx.x % (4 * kWarpSize) == 0 && w == 0) {
+      Cut& c = a.cuts[blockIdx.x * 2 + slot];
+      c.flags = kCut | (g.front ? kCutFront : 0) | (g.back ? kCutBack : 0);
+      c.token0 = g.r.start;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        c.kv_head[x] = g.kv_head[x];
+        c.row0[x] = g.row0[x];
+        c.rows[x] = g.rows[x];
+      }
+    }
+    if (any) {
+      const bool odd = static_cast<volatile int*>(sy.odd_values[w])[index & 3] != 0;
+      const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+      __nv_bfloat16* out =
+          static_cast<__nv_bfloat16*>(a.out) +
+          ((token * a.num_kv_heads + g.kv_head[w]) * a.group + at_row % a.group) * D;
+#pragma unroll 1
+      for (int c = 0; c < D; c += 16) {
+        uint32_t x[16];
+        tmem_load16(output + c, x);
+        float o[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = __uint_as_float(x[i]);
+        if (odd && row < g.rows[w]) {
+          // V values that are not finite, of the rows this node sees: the weights are positive
+          const int first = max(g.step0, g.r.context / kTile) * kTile;
+          const int last = min(g.step1 * kTile, g.r.length);
+          for (int j = first; j < last; ++j) {
+            if (!(visible32(a, g.r, mask, node, j) & 1)) continue;
+            const int page = a.page.divide(j);
+            int64_t block = a.block_tables[g.s * a.max_blocks + page];
+            if (block < 0 || block >= a.num_blocks) block = 0;
+            const auto* v = static_cast<const uint16_t*>(a.v_cache) +
+                            ((block * a.block_size + (j - page * a.block_size)) *
+                                 a.num_kv_heads + g.kv_head[w]) * D + c;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const uint32_t bits = static_cast<uint32_t>(v[i]) << 16;
+              if ((bits & 0x7f800000u) == 0x7f800000u) o[i] += __uint_as_float(bits);
+            }
+          }
+        }
+        if (cut) {
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            *reinterpret_cast<float4*>(part + (((c + i) / 4) * kTile + row) * 4) =
+                make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          }
+        } else if (row < g.rows[w]) {
+          // a sum of zero: the node saw no row
+          float f[8];
+#pragma unroll
+          for (int i = 0; i < 16; i += 8) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = sum == 0.0f ? 0.0f : o[i + e] * inverse;
+            st_global_v4(out + c + i, pack<Bf16>(f));
+          }
+        }
+      }
+      if (cut) {
+        part[D * kTile + row] = ref;
+        part[(D + 1) * kTile + row] = sum;
+      }
+    }
+  }
 }
 
 template <int D>
-__global__ void __launch_bounds__(128) tree_attention_simple_kernel(const TreeAttnArgs a) {
+__global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const TreeAttnArgs a) {
+  using S = Shape<D>;
   grid_dependency_sync();
-  constexpr int kPer = D / kWarpSize;  // output elements per lane
-  const int lane = threadIdx.x % kWarpSize;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWarpSize;
-  const int64_t t = unit / a.num_heads;
-  const int h = static_cast<int>(unit % a.num_heads);
-  if (t >= a.num_tokens) return;
-  const int kh = h / (a.num_heads / a.num_kv_heads);
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ Sync sy;
+  uint8_t* q_tiles = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+  uint8_t* ring_k = q_tiles + 2 * S::kTileBytes;
+  uint8_t* ring_v = ring_k + S::kStagesK * S::kTileBytes;
+  const int tid = threadIdx.x;
+  const int warp = tid / kWarpSize, lane = tid % kWarpSize;
 
-  int64_t b = 0;  // the request: the first whose end lies beyond t
-  while (b < a.num_seqs && a.query_start_loc[b + 1] <= t) ++b;
-  int64_t context = 0, seq = 0, node = 0;
-  if (b < a.num_seqs) {
-    const int64_t start = a.query_start_loc[b];
-    const int64_t n = a.query_start_loc[b + 1] - start;
-    seq = a.seq_lens[b];
-    context = seq - n;
-    node = t - start;
-    if (seq != 0 && (context < 0 || seq > static_cast<int64_t>(a.max_blocks) * a.block_size ||
-                     (a.tree_mask != nullptr && n > 64 * a.mask_words))) {
-      raise_error(a.err, kErrBadIndex);
-      seq = 0;
+  if (tid == 0) {
+    for (int i = 0; i < kBarriers; ++i) {
+      const bool full = i < kEmptyK;
+      const bool weights = i == kWeightsDone || i == kWeightsDone + 1;
+      mbar_init(&sy.bar[i], full ? kProducerWarps * kWarpSize : weights ? 4 * kWarpSize : 1);
     }
+    fence_mbar_init();
+    sy.abort = 0;
+    for (int i = 0; i < 8; ++i) sy.odd_values[i / 4][i % 4] = 0;
+    sy.place[0] = sy.place[1] = Place{a.num_seqs, 0, 0};
+    a.cuts[blockIdx.x * 2].flags = 0;
+    a.cuts[blockIdx.x * 2 + 1].flags = 0;
   }
-  float q[D];
-  const __nv_bfloat16* qp =
-      static_cast<const __nv_bfloat16*>(a.q) + t * a.q_stride + static_cast<int64_t>(h) * D;
-  for (int d = 0; d < D; ++d) q[d] = __bfloat162float(qp[d]);
-  float m = -__builtin_huge_valf(), l = 0.0f, acc[kPer] = {};
-  const int32_t* table = a.block_tables + b * a.max_blocks;
-  for (int64_t j0 = 0; j0 < seq; j0 += kWarpSize) {
-    const int64_t j = j0 + lane;
-    bool sees = j < context;
-    if (!sees && j < seq) {
-      const int64_t x = j - context;
-      sees = a.tree_mask == nullptr
-                 ? x <= node
-                 : (static_cast<uint64_t>(a.tree_mask[t * a.mask_words + x / 64]) >> (x % 64)) & 1;
+  if (warp == kMmaWarp) tmem_alloc(&sy.tmem_base, kTmemColumns);
+
+  // this CTA's share of the line: its length, then the requests that hold the share's two ends
+  int64_t cost = 0;
+  for (int64_t s = tid; s < a.num_seqs; s += kThreads) cost += request_cost(a, load_request(a, s));
+#pragma unroll
+  for (int off = 16; off > 0; off /= 2) cost += __shfl_xor_sync(0xffffffffu, cost, off);
+  if (lane == 0) sy.sums[warp] = cost;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  int64_t total = 0;
+#pragma unroll
+  for (int i = 0; i <= kMmaWarp; ++i) total += sy.sums[i];
+  // at least two steps each: a shorter share costs more in the join than it saves
+  int64_t share = (total + gridDim.x - 1) / gridDim.x;
+  if (share < 2) share = 2;
+  const int64_t ends[2] = {blockIdx.x * share, (blockIdx.x + 1) * share};
+  int64_t before = 0;
+  for (int64_t base = 0; base < a.num_seqs; base += kThreads) {
+    Request r{};
+    if (base + tid < a.num_seqs) r = load_request(a, base + tid);
+    const int64_t own = request_cost(a, r);
+    int64_t upto = own;
+#pragma unroll
+    for (int off = 1; off < kWarpSize; off *= 2) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, upto, off);
+      if (lane >= off) upto += up;
     }
-    int64_t row = 0;
-    float s = -__builtin_huge_valf();
-    if (sees) {
-      int64_t blk = table[j / a.block_size];
-      if (blk < 0 || blk >= a.num_blocks) {
-        raise_error(a.err, kErrBadIndex);
-        blk = 0;
+    __syncthreads();  // sy.sums has been read
+    if (lane == kWarpSize - 1) sy.sums[warp] = upto;
+    __syncthreads();
+    int64_t chunk = 0;
+#pragma unroll
+    for (int i = 0; i <= kMmaWarp; ++i) {
+      if (i < warp) upto += sy.sums[i];
+      chunk += sy.sums[i];
+    }
+    upto += before;
+    before += chunk;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      if (ends[e] >= upto - own && ends[e] < upto) {
+        sy.place[e] = locate(a, base + tid, r, ends[e] - (upto - own));
       }
-      row = ((blk * a.block_size + j % a.block_size) * a.num_kv_heads + kh) * D;
-      const __nv_bfloat16* kp = static_cast<const __nv_bfloat16*>(a.k_cache) + row;
-      s = 0.0f;
-      for (int d = 0; d < D; ++d) s = fmaf(q[d], __bfloat162float(kp[d]), s);
-      s *= a.scale_log2;
-    }
-    float mx = s;
-    for (int off = 16; off > 0; off /= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-    mx = fmaxf(m, mx);
-    const float base = mx == -__builtin_huge_valf() ? 0.0f : mx;
-    const float al = exp2_approx(m - base);
-    const float p = sees ? exp2_approx(s - base) : 0.0f;
-    l = l * al + p;
-    for (int e = 0; e < kPer; ++e) acc[e] *= al;
-    m = mx;
-    unsigned live = __ballot_sync(0xffffffffu, sees);
-    while (live != 0) {
-      const int src = __ffs(static_cast<int>(live)) - 1;
-      live &= live - 1;
-      const float pj = __shfl_sync(0xffffffffu, p, src);
-      const int64_t rj = __shfl_sync(0xffffffffu, row, src);
-      const __nv_bfloat16* vp = static_cast<const __nv_bfloat16*>(a.v_cache) + rj + lane * kPer;
-      for (int e = 0; e < kPer; ++e) acc[e] = fmaf(pj, __bfloat162float(vp[e]), acc[e]);
     }
   }
-  for (int off = 16; off > 0; off /= 2) l += __shfl_xor_sync(0xffffffffu, l, off);
-  __nv_bfloat16* out =
-      static_cast<__nv_bfloat16*>(a.out) + (t * a.num_heads + h) * D + lane * kPer;
-  // a sum of zero: the token saw no row (a NaN sum stays NaN)
-  for (int e = 0; e < kPer; ++e) out[e] = __float2bfloat16_rn(l == 0.0f ? 0.0f : acc[e] / l);
+  __syncthreads();
+  const Place at = sy.place[0], end = sy.place[1];
+
+  if (warp == kMmaWarp) {
+    if (lane == 0) issue_products<D>(a, sy, q_tiles, ring_k, ring_v, at, end);
+  } else if (warp >= kSoftmaxWarps) {
+    Producer<D> p{a, sy, ring_k, ring_v, q_tiles, warp - kSoftmaxWarps, lane};
+    p.run(at, end);
+  } else {
+    softmax<D>(a, sy, warp / 4, at, end);
+  }
+
+  // rows that no item covers are zero: requests that were not served, and what lies behind the last
+  const int64_t row_vecs = static_cast<int64_t>(a.num_kv_heads) * a.group * D / 8;
+  uint4* out = static_cast<uint4*>(a.out);
+  for (int64_t s = blockIdx.x; s < a.num_seqs; s += gridDim.x) {
+    const Request r = load_request(a, s);
+    if (r.bad && tid == 0) raise_error(a.err, kErrBadIndex);
+    if (r.steps > 0) continue;
+    for (int64_t i = tid; i < r.nodes * row_vecs; i += kThreads) {
+      st_global_v4(out + r.start * row_vecs + i, make_uint4(0, 0, 0, 0));
+    }
+  }
+  int64_t tail = a.query_start_loc[a.num_seqs];
+  if (tail < 0) tail = 0;
+  for (int64_t t = tail + blockIdx.x; t < a.num_tokens; t += gridDim.x) {
+    for (int64_t i = tid; i < row_vecs; i += kThreads) {
+      st_global_v4(out + t * row_vecs + i, make_uint4(0, 0, 0, 0));
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kMmaWarp) tmem_dealloc(sy.tmem_base, kTmemColumns);
+}
+
+// Joins the segments of each cut item: block (b, y) looks at the border before CTA b, and the
+// first border inside an item does the item, 32 rows of one accumulator per y. With m and l the
+// maxima and sums of the segments, M the largest m: o = sum 2^(m - M) O / sum 2^(m - M) l.
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads) tree_attention_join_kernel(const TreeAttnArgs a,
+                                                                           int ctas) {
+  grid_dependency_sync();
+  using S = Shape<D>;
+  const int border = blockIdx.x + 1;
+  if (!(a.cuts[border * 2].flags & kCutFront)) return;
+  // the segment before the border: the previous CTA's second cut one, else its first
+  const int first = (border - 1) * 2 + (a.cuts[(border - 1) * 2 + 1].flags != 0 ? 1 : 0);
+  const Cut c = a.cuts[first];
+  if (c.flags & kCutFront) return;  // not the item's first border
+  int last = border;
+  while (last + 1 < ctas && (a.cuts[last * 2].flags & kCutBack)) ++last;
+
+  constexpr int kPer = D / 4 / (kJoinThreads / kJoinRows);  // 16-byte pieces of a row per thread
+  const int w = blockIdx.y / (kTile / kJoinRows);
+  const int row = (blockIdx.y % (kTile / kJoinRows)) * kJoinRows + threadIdx.x % kJoinRows;
+  if (row >= c.rows[w]) return;
+  const int piece = threadIdx.x / kJoinRows * kPer;
+  const auto part = [&](int i) {  // segment i of the item
+    const int64_t slot = i == 0 ? first : (border - 1 + i) * 2;
+    return a.parts + (slot * 2 + w) * S::kPartFloats;
+  };
+  const int n = last - border + 2;
+  const float kInf = __builtin_huge_valf();
+  float top = -kInf;
+  for (int i = 0; i < n; ++i) top = fmaxf(top, part(i)[D * kTile + row]);
+  const float base = top == -kInf ? 0.0f : top;
+  float sum = 0.0f;
+  float4 o[kPer];
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) o[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 2
+  for (int i = 0; i < n; ++i) {
+    const float* p = part(i);
+    const float l = p[(D + 1) * kTile + row];
+    const float f = exp2_approx(p[D * kTile + row] - base);
+    const bool any = l != 0.0f;  // a segment of which the node sees nothing has no part
+    sum += any ? f * l : 0.0f;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const float4 x = *reinterpret_cast<const float4*>(p + ((piece + e) * kTile + row) * 4);
+      o[e].x += any ? f * x.x : 0.0f;
+      o[e].y += any ? f * x.y : 0.0f;
+      o[e].z += any ? f * x.z : 0.0f;
+      o[e].w += any ? f * x.w : 0.0f;
+    }
+  }
+  const int at_row = c.row0[w] + row;
+  const int64_t token = c.token0 + at_row / a.group;
+  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) +
+                       ((token * a.num_kv_heads + c.kv_head[w]) * a.group + at_row % a.group) * D +
+                       piece * 4;
+  const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+  for (int e = 0; e < kPer; e += 2) {
+    const float f[8] = {o[e].x,     o[e].y,     o[e].z,     o[e].w,
+                        o[e + 1].x, o[e + 1].y, o[e + 1].z, o[e + 1].w};
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = sum == 0.0f ? 0.0f : f[i] * inverse;
+    st_global_v4(out + e * 4, pack<Bf16>(y));
+  }
+}
+
+// Workspace: the partial sums of every CTA, then its cuts.
+template <int D>
+int64_t workspace_bytes(int ctas) {
+  return static_cast<int64_t>(ctas) *
+         (4 * Shape<D>::kPartFloats * 4 + 2 * static_cast<int64_t>(sizeof(Cut)));
+}
+
+template <int D>
+int launch_tree_attention(TreeAttnArgs& a, void* workspace, int device, cudaStream_t stream) {
+  const int ctas = sm_count(device);
+  a.parts = static_cast<float*>(workspace);
+  a.cuts = reinterpret_cast<Cut*>(a.parts + static_cast<int64_t>(ctas) * 4 *
+                                                Shape<D>::kPartFloats);
+  // raises the kernel's shared-memory limit on its first use
+  if (blocks_per_sm(reinterpret_cast<const void*>(tree_attention_kernel<D>), kThreads,
+                    Shape<D>::kSmem, device) < 1) {
+    return SVLLM_ERR_CUDA;
+  }
+  // not scheduled early behind the previous kernel: a CTA takes nearly all of an SM
+  const int status = launch_serialized(tree_attention_kernel<D>, dim3(ctas), dim3(kThreads),
+                                       Shape<D>::kSmem, stream, 1u, a);
+  if (status != SVLLM_OK || ctas < 2) return status;
+  return launch(tree_attention_join_kernel<D>, dim3(ctas - 1, 2 * kTile / kJoinRows),
+                dim3(kJoinThreads), 0, stream, 1u, a, ctas);
 }
 
 }  // namespace
 }  // namespace svllm::k
 
 extern "C" int svllm_tree_attention_workspace_bytes(int64_t head_dim, int64_t* bytes) {
+  using namespace svllm::k;
   if (bytes == nullptr || head_dim <= 0) return SVLLM_ERR_INVALID_ARGUMENT;
   if (head_dim != 64 && head_dim != 128) return SVLLM_ERR_UNSUPPORTED;
-  *bytes = 0;
+  int device;
+  if (current_device(&device) != SVLLM_OK) return SVLLM_ERR_CUDA;
+  const int ctas = sm_count(device);
+  *bytes = head_dim == 128 ? workspace_bytes<128>(ctas) : workspace_bytes<64>(ctas);
   return SVLLM_OK;
 }
 
@@ -141,7 +921,7 @@ extern "C" int svllm_tree_attention_bf16(
     int64_t num_blocks, int64_t block_size, const int32_t* block_tables, int64_t max_blocks,
     const int32_t* seq_lens, const int32_t* query_start_loc, int64_t num_seqs, int64_t num_tokens,
     int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, const int64_t* tree_mask,
-    int64_t mask_words, float scale, void* workspace, int64_t workspace_bytes,
+    int64_t mask_words, float scale, void* workspace, int64_t workspace_size,
     svllm_stream stream) {
   using namespace svllm::k;
   if (num_seqs < 0 || num_tokens < 0 || num_heads <= 0 || num_kv_heads <= 0 ||
@@ -166,8 +946,12 @@ extern "C" int svllm_tree_attention_bf16(
       (tree_mask != nullptr && mask_words > SVLLM_MAX_TREE_NODES / 64)) {
     return SVLLM_ERR_TOO_LARGE;
   }
-  (void)workspace;
-  (void)workspace_bytes;
+  int64_t needed = 0;
+  const int sized = svllm_tree_attention_workspace_bytes(head_dim, &needed);
+  if (sized != SVLLM_OK) return sized;
+  if (workspace == nullptr || workspace_size < needed || !aligned16(workspace)) {
+    return SVLLM_ERR_INVALID_ARGUMENT;
+  }
   int device;
   if (current_device(&device) != SVLLM_OK) return SVLLM_ERR_CUDA;
   int* err = library_error_word(device);
@@ -187,13 +971,13 @@ extern "C" int svllm_tree_attention_bf16(
   a.num_seqs = num_seqs;
   a.max_blocks = static_cast<int>(max_blocks);
   a.block_size = static_cast<int>(block_size);
-  a.num_heads = static_cast<int>(num_heads);
+  a.page = make_divider(block_size);
+  a.group = static_cast<int>(num_heads / num_kv_heads);
   a.num_kv_heads = static_cast<int>(num_kv_heads);
   a.mask_words = static_cast<int>(mask_words);
   a.scale_log2 = static_cast<float>(static_cast<double>(scale) / std::log(2.0));
   a.err = err;
-  const dim3 grid(static_cast<unsigned>((num_tokens * num_heads + 3) / 4));
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return head_dim == 128 ? launch(tree_attention_simple_kernel<128>, grid, dim3(128), 0, s, 1u, a)
-                         : launch(tree_attention_simple_kernel<64>, grid, dim3(128), 0, s, 1u, a);
+  return head_dim == 128 ? launch_tree_attention<128>(a, workspace, device, s)
+                         : launch_tree_attention<64>(a, workspace, device, s);
 }

@@ -1,4 +1,5 @@
-// tcgen05 and TMA building blocks of the tensor-core GEMM (the fused LM head + greedy sampling):
+// tcgen05 and TMA building blocks of the tensor-core kernels (the LM head fused with greedy
+// sampling, tree attention):
 // bulk tensor copies into shared memory, TMEM allocation, tcgen05.mma with shared-memory
 // descriptors, commits to mbarriers, TMEM loads, bounded mbarrier waits, and the host-side
 // tensor maps they read through.
@@ -58,6 +59,18 @@ __device__ __forceinline__ void umma_bf16(uint32_t d_tmem, uint64_t a_desc, uint
       : "memory");
 }
 
+// The same with A in TMEM (lane = row, two bf16 of consecutive K per 32-bit column) and B as the
+// instruction descriptor says.
+__device__ __forceinline__ void umma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+                                             uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 // Arrives on `bar` once every tcgen05 operation this thread issued before it has completed.
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
@@ -77,6 +90,41 @@ __device__ __forceinline__ void tmem_load16(uint32_t taddr, uint32_t (&v)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+__device__ __forceinline__ void tmem_wait_load() {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void tmem_wait_store() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// 32 consecutive 32-bit TMEM columns of this thread's lane; valid after tmem_wait_load.
+__device__ __forceinline__ void tmem_load32(uint32_t taddr, uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+      "%30, %31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+        "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]),
+        "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]),
+        "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(taddr)
+      : "memory");
+}
+
+// 16 registers to 16 consecutive 32-bit TMEM columns of this thread's lane; done after
+// tmem_wait_store.
+__device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+      "r"(v[15])
+      : "memory");
+}
+
 // Shared-memory matrix descriptor of a K-major tile written by TMA with the 128-byte swizzle:
 // rows of 128 bytes, 8-row groups 1024 bytes apart (stride byte offset), 1024-byte aligned.
 __device__ __forceinline__ uint64_t smem_desc_k_sw128(const void* tile) {
@@ -88,6 +136,22 @@ __device__ __forceinline__ uint64_t smem_desc_k_sw128(const void* tile) {
   d |= 2ull << 61;                            // SWIZZLE_128B
   return d;
 }
+
+// Descriptor of an N-major B tile (rows of K, 64 elements of N = 128 swizzled bytes each): 8-row
+// groups 1024 bytes apart (stride byte offset), blocks of 64 N elements `block_bytes` apart
+// (leading byte offset), 1024-byte aligned.
+__device__ __forceinline__ uint64_t smem_desc_mn_sw128(const void* tile, uint32_t block_bytes) {
+  const uint64_t addr = smem_addr(tile);
+  uint64_t d = (addr >> 4) & 0x3FFFull;
+  d |= static_cast<uint64_t>((block_bytes >> 4) & 0x3FFF) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= 1ull << 46;
+  d |= 2ull << 61;
+  return d;
+}
+
+// Set in an instruction descriptor: B is N-major.
+constexpr uint32_t kIdescBMajorN = 1u << 16;
 
 // Instruction descriptor: bf16 A and B, fp32 D, both K-major, M x N.
 __host__ __device__ constexpr uint32_t idesc_bf16(int m, int n) {
