@@ -59,7 +59,6 @@ struct Shape {
   static constexpr int kTileBytes = kHalves * kHalfBytes;
   static constexpr int kStagesK = D == 128 ? 3 : 6;
   static constexpr int kStagesV = D == 128 ? 2 : 4;
-  static constexpr int kPending = D == 128 ? 4 : 7;  // cp.async groups in flight, at most 7
   static constexpr size_t kSmem = 1024 + static_cast<size_t>(kTileBytes) *
                                              (2 + kStagesK + kStagesV);
   // partial sums of one accumulator: O as [D / 4][128 rows][4], then the rows' maxima and sums
@@ -257,13 +256,14 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool t
                : "memory");
 }
 
-__device__ __forceinline__ void cp_async_commit() {
-  asm volatile("cp.async.commit_group;" ::: "memory");
+// Arrives on `bar` (one of its counted arrivals) once this thread's copies so far have landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar))
+               : "memory");
 }
 
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+__device__ __forceinline__ void cp_async_wait_all() {
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // Zeroes the non-finite halves of a word of two bf16; true if there were any.
@@ -274,10 +274,9 @@ __device__ __forceinline__ bool drop_odd(uint32_t& w) {
   return lo || hi;
 }
 
-// The four producer warps: each gathers 32 of a tile's 128 rows. A thread signals a tile's barrier
-// when its own copies have landed and are visible to the tensor cores' proxy; up to kPending tiles
-// are in flight. Where the next slot is still in use it signals everything first and then waits, so
-// no consumer waits for a signal that waits for it.
+// The four producer warps: each gathers 32 of a tile's 128 rows. The copies signal the tile's
+// barrier themselves as they land (the thread that issues the products orders them before the
+// tensor cores' reads), so the producers run ahead as far as the rings have room.
 template <int D>
 struct Producer {
   using S = Shape<D>;
@@ -291,35 +290,9 @@ struct Producer {
   uint8_t* q_tiles;
   int warp, lane;      // warp 0..3
   Ring k{}, v{};
-  uint64_t pending = 0;  // barrier indices, oldest in the low byte
-  int count = 0;
 
-  __device__ void signal_oldest() {
-    fence_proxy_async_smem();
-    mbar_arrive(&sy.bar[pending & 0xff]);
-    pending >>= 8;
-    --count;
-  }
-  __device__ void flush() {
-    cp_async_wait<0>();
-    while (count > 0) signal_oldest();
-  }
   __device__ bool acquire(int bar, uint32_t parity) {
-    bool free = mbar_test(&sy.bar[bar], parity);
-    if (!__all_sync(0xffffffffu, free)) {
-      flush();
-      free = wait_phase(&sy.bar[bar], parity, &sy.abort, a.err);
-      return __all_sync(0xffffffffu, free);
-    }
-    return true;
-  }
-  __device__ void issued(int bar) {
-    cp_async_commit();
-    pending |= static_cast<uint64_t>(bar) << (8 * count);
-    if (++count > S::kPending) {
-      cp_async_wait<S::kPending>();
-      signal_oldest();
-    }
+    return __all_sync(0xffffffffu, wait_phase(&sy.bar[bar], parity, &sy.abort, a.err));
   }
 
   // Element offset of KV head 0 of this lane's row of key tile `step`, -1 past the request's end.
@@ -377,7 +350,7 @@ struct Producer {
     if (!acquire(kEmptyK + k.slot, k.phase ^ 1)) return false;
     gather(ring_k + k.slot * S::kTileBytes, a.k_cache, offset,
            static_cast<int64_t>(g.kv_head[w]) * D);
-    issued(kFullK + k.slot);
+    cp_async_arrive(&sy.bar[kFullK + k.slot]);
     k.advance(S::kStagesK);
     return true;
   }
@@ -394,7 +367,7 @@ struct Producer {
       mbar_arrive(&sy.bar[kFullV + v.slot]);
     } else {
       gather(tile, a.v_cache, offset, column);
-      issued(kFullV + v.slot);
+      cp_async_arrive(&sy.bar[kFullV + v.slot]);
     }
     v.advance(S::kStagesV);
     return true;
@@ -417,7 +390,7 @@ struct Producer {
                           : -1;
         gather(q_tiles + w * S::kTileBytes, a.q, off, 0);
       }
-      issued(kFullQ);
+      cp_async_arrive(&sy.bar[kFullQ]);
       // in the order in which the tensor cores take them
       int64_t before = -1;
       for (int step = g.step0; ok && step <= g.step1; ++step) {
@@ -430,7 +403,7 @@ struct Producer {
         now = next;
       }
     }
-    flush();  // also after an abort: no copy of this CTA is in flight when it exits
+    cp_async_wait_all();  // also after an abort: no copy is in flight when the CTA exits
   }
 };
 
@@ -450,11 +423,17 @@ __device__ void issue_products(const TreeAttnArgs& a, Sync& sy, const uint8_t* q
     tc_fence_after();
     return ok;
   };
+  // a tile: the producers' writes, made through the generic proxy, before the tensor cores' reads
+  const auto wait_tile = [&](int bar, uint32_t parity) {
+    wait(bar, parity);
+    fence_proxy_async_smem();
+    return ok;
+  };
   Segment g;
   for (int index = 0; ok && next_segment(a, at, end, g); ++index) {
     const auto scores = [&](int w, bool last) {
       const bool first_use = !g.shared || w == 0, last_use = !g.shared || w == 1;
-      if (first_use && !wait(kFullK + k.slot, k.phase)) return;
+      if (first_use && !wait_tile(kFullK + k.slot, k.phase)) return;
       const uint8_t* qt = q_tiles + w * S::kTileBytes;
       const uint8_t* kt = ring_k + k.slot * S::kTileBytes;
 #pragma unroll
@@ -470,14 +449,14 @@ __device__ void issue_products(const TreeAttnArgs& a, Sync& sy, const uint8_t* q
       }
       if (last && w == g.active - 1) umma_commit(&sy.bar[kEmptyQ]);
     };
-    if (!wait(kFullQ, index & 1)) break;
+    if (!wait_tile(kFullQ, index & 1)) break;
     for (int w = 0; ok && w < g.active; ++w) scores(w, g.step0 + 1 == g.step1);
     for (int step = g.step0; ok && step < g.step1; ++step) {
       for (int w = 0; ok && w < g.active; ++w) {
         if (!wait(kWeightsDone + w, weights_phase[w])) break;
         weights_phase[w] ^= 1;
         const bool first_use = !g.shared || w == 0, last_use = !g.shared || w == 1;
-        if (first_use && !wait(kFullV + v.slot, v.phase)) break;
+        if (first_use && !wait_tile(kFullV + v.slot, v.phase)) break;
         const uint8_t* vt = ring_v + v.slot * S::kTileBytes;
 #pragma unroll
         for (int kk = 0; kk < kTile / 16; ++kk) {
