@@ -44,14 +44,17 @@ constexpr int kTile = 128;            // query rows per M tile, cached rows per 
 constexpr int kSoftmaxWarps = 8;      // two groups of 4: accumulators 0 and 1
 constexpr int kProducerWarps = 4;
 constexpr int kMmaWarp = kSoftmaxWarps + kProducerWarps;
-constexpr int kThreads = (kMmaWarp + 1) * kWarpSize;
+constexpr int kThreads = 16 * kWarpSize;  // the last three warps only fill the register groups
+// Registers per thread after the split of the launch's 512 x 128: the softmax warps hold a row of
+// scores each, 8 x 32 x 192 + 8 x 32 x 64 = 65536.
+constexpr int kSoftmaxRegisters = 192, kOtherRegisters = 64;
 constexpr int kHalfBytes = kTile * 128;  // 128 rows of one 128-byte swizzle atom
 constexpr uint32_t kTmemColumns = 512;
 constexpr uint32_t kScores = 0;       // TMEM columns: S (and P) of accumulator w at 128 w,
 constexpr uint32_t kOutput = 256;     // O at 256 + 128 w
 constexpr float kRescaleAbove = 8.0f;  // in powers of two
-constexpr int kJoinThreads = 128;
-constexpr int kJoinRows = 32;
+constexpr int kJoinRows = 8;
+constexpr int kMaxCtas = 256;         // one per SM; the join lists their borders
 
 template <int D>
 struct Shape {
@@ -234,7 +237,7 @@ struct Sync {
   uint32_t tmem_base;
   int abort;
   int odd_values[2][4];  // per accumulator and segment modulo 4: V held something not finite
-  int64_t sums[kMmaWarp + 1];
+  int64_t sums[kThreads / kWarpSize];
   Place place[2];        // this CTA's share
 };
 
@@ -289,112 +292,125 @@ struct Producer {
   uint8_t* ring_v;
   uint8_t* q_tiles;
   int warp, lane;      // warp 0..3
+  uint32_t row_bytes;  // of a cached row, all KV heads
   Ring k{}, v{};
 
-  __device__ bool acquire(int bar, uint32_t parity) {
+  __device__ __forceinline__ bool acquire(int bar, uint32_t parity) {
     return __all_sync(0xffffffffu, wait_phase(&sy.bar[bar], parity, &sy.abort, a.err));
   }
 
-  // Element offset of KV head 0 of this lane's row of key tile `step`, -1 past the request's end.
-  __device__ int64_t row_offset(const Segment& g, int step) const {
+  // The cache slot of this lane's row of key tile `step`, -1 past the request's end. A slot fits
+  // 31 bits: 2^31 rows of 64 bf16 would be 256 GB.
+  __device__ __forceinline__ int cache_slot(const Segment& g, int step) const {
     const int j = step * kTile + warp * kWarpSize + lane;
     if (step >= g.step1 || j >= g.r.length) return -1;
     const int page = a.page.divide(j);
-    int64_t block = a.block_tables[g.s * a.max_blocks + page];
-    if (block < 0 || block >= a.num_blocks) {  // outside the cache: block 0 is read
-      raise_error(a.err, kErrBadIndex);
+    int block = a.block_tables[g.s * a.max_blocks + page];
+    if (static_cast<uint64_t>(block) >= static_cast<uint64_t>(a.num_blocks)) {
+      raise_error(a.err, kErrBadIndex);  // outside the cache: block 0 is read
       block = 0;
     }
-    return (block * a.block_size + (j - page * a.block_size)) * a.num_kv_heads * D;
+    return block * a.block_size + (j - page * a.block_size);
   }
 
-  __device__ __forceinline__ uint32_t tile_place(uint32_t base, int row) const {
+  // Where this lane's 16 bytes of its row in round i go: round i brings rows i * kRowsAtOnce ..
+  // of the warp's 32, lane / kLanes of them this lane's. The swizzle depends on the row modulo 8.
+  __device__ __forceinline__ uint32_t tile_place(uint32_t base, int i) const {
     const int c = lane % kLanes;
-    return base + (c / 8) * kHalfBytes + row * 128 + (((c % 8) ^ (row & 7)) << 4);
+    const int row = i * kRowsAtOnce + lane / kLanes;
+    return base + (c / 8) * kHalfBytes + (warp * kWarpSize + row) * 128 +
+           (((c % 8) ^ (row & 7)) << 4);
   }
 
-  // Rows of `src` at `offset` (one per lane, elements, -1 = zeros) into a tile.
-  __device__ void gather(uint8_t* tile, const void* src, int64_t offset, int64_t column) {
+  // The rows `slot` (one per lane, -1 = zeros) of `src`, `stride` bytes apart, into a tile.
+  __device__ __forceinline__ void gather(uint8_t* tile, const uint8_t* src, int slot,
+                                         uint32_t stride) {
     const uint32_t base = smem_addr(tile);
-    const auto* p = static_cast<const __nv_bfloat16*>(src) + column + (lane % kLanes) * 8;
-#pragma unroll 4
+    src += (lane % kLanes) * 16;
+#pragma unroll
     for (int i = 0; i < kWarpSize / kRowsAtOnce; ++i) {
-      const int row = i * kRowsAtOnce + lane / kLanes;
-      const int64_t off = __shfl_sync(0xffffffffu, offset, row);
-      cp_async16(tile_place(base, warp * kWarpSize + row), p + (off < 0 ? 0 : off), off >= 0);
+      const int row = __shfl_sync(0xffffffffu, slot, i * kRowsAtOnce + lane / kLanes);
+      cp_async16(tile_place(base, i), src + static_cast<uint64_t>(max(row, 0)) * stride, row >= 0);
     }
   }
 
   // The same for a V tile that holds tree nodes: through registers, values that are not finite
   // left out; true if there were any.
-  __device__ bool gather_checked(uint8_t* tile, const void* src, int64_t offset, int64_t column) {
+  __device__ __forceinline__ bool gather_checked(uint8_t* tile, const uint8_t* src, int slot,
+                                              uint32_t stride) {
     const uint32_t base = smem_addr(tile);
-    const auto* p = static_cast<const __nv_bfloat16*>(src) + column + (lane % kLanes) * 8;
+    src += (lane % kLanes) * 16;
     bool odd = false;
-#pragma unroll 8
+#pragma unroll 4
     for (int i = 0; i < kWarpSize / kRowsAtOnce; ++i) {
-      const int row = i * kRowsAtOnce + lane / kLanes;
-      const int64_t off = __shfl_sync(0xffffffffu, offset, row);
+      const int row = __shfl_sync(0xffffffffu, slot, i * kRowsAtOnce + lane / kLanes);
       uint4 w = make_uint4(0, 0, 0, 0);
-      if (off >= 0) w = ld_global_nc_v4(p + off);
+      if (row >= 0) w = ld_global_nc_v4(src + static_cast<uint64_t>(row) * stride);
       odd |= drop_odd(w.x) | drop_odd(w.y) | drop_odd(w.z) | drop_odd(w.w);
-      asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(
-                       tile_place(base, warp * kWarpSize + row)),
+      asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(tile_place(base, i)),
                    "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
                    : "memory");
     }
     return odd;
   }
 
-  __device__ bool load_k(const Segment& g, int w, int64_t offset) {
+  __device__ __forceinline__ bool load_k(const Segment& g, int w, int slot) {
     if (!acquire(kEmptyK + k.slot, k.phase ^ 1)) return false;
-    gather(ring_k + k.slot * S::kTileBytes, a.k_cache, offset,
-           static_cast<int64_t>(g.kv_head[w]) * D);
+    gather(ring_k + k.slot * S::kTileBytes,
+           static_cast<const uint8_t*>(a.k_cache) + g.kv_head[w] * D * 2, slot, row_bytes);
     cp_async_arrive(&sy.bar[kFullK + k.slot]);
     k.advance(S::kStagesK);
     return true;
   }
-  __device__ bool load_v(const Segment& g, int w, int64_t offset, int step, int index) {
+  __device__ __forceinline__ bool load_v(const Segment& g, int w, int slot, int step, int index) {
     if (!acquire(kEmptyV + v.slot, v.phase ^ 1)) return false;
     uint8_t* tile = ring_v + v.slot * S::kTileBytes;
-    const int64_t column = static_cast<int64_t>(g.kv_head[w]) * D;
+    const uint8_t* src = static_cast<const uint8_t*>(a.v_cache) + g.kv_head[w] * D * 2;
     if ((step + 1) * kTile > g.r.context) {
-      if (gather_checked(tile, a.v_cache, offset, column)) {
+      if (gather_checked(tile, src, slot, row_bytes)) {
         sy.odd_values[w][index & 3] = 1;
         if (g.shared) sy.odd_values[1][index & 3] = 1;
       }
       fence_proxy_async_smem();
       mbar_arrive(&sy.bar[kFullV + v.slot]);
     } else {
-      gather(tile, a.v_cache, offset, column);
+      gather(tile, src, slot, row_bytes);
       cp_async_arrive(&sy.bar[kFullV + v.slot]);
     }
     v.advance(S::kStagesV);
     return true;
   }
 
-  __device__ void run(Place at, const Place end) {
+  // The query rows of accumulator w: row = node * group + head of the KV head.
+  __device__ __forceinline__ void load_q(const Segment& g, int w) {
+    const int r = warp * kWarpSize + lane;
+    const int row = g.row0[w] + r;
+    const int64_t offset =
+        r < g.rows[w] ? (g.r.start + row / a.group) * a.q_stride +
+                            (static_cast<int64_t>(g.kv_head[w]) * a.group + row % a.group) * D
+                      : -1;
+    const uint32_t base = smem_addr(q_tiles + w * S::kTileBytes);
+    const auto* src = static_cast<const __nv_bfloat16*>(a.q) + (lane % kLanes) * 8;
+#pragma unroll 4
+    for (int i = 0; i < kWarpSize / kRowsAtOnce; ++i) {
+      const int64_t at = __shfl_sync(0xffffffffu, offset, i * kRowsAtOnce + lane / kLanes);
+      cp_async16(tile_place(base, i), src + (at < 0 ? 0 : at), at >= 0);
+    }
+  }
+
+  __device__ __forceinline__ void run(Place at, const Place end) {
     Segment g;
     bool ok = true;
     for (int index = 0; ok && next_segment(a, at, end, g); ++index) {
-      int64_t now = row_offset(g, g.step0);
-      // the query rows of both accumulators
+      int now = cache_slot(g, g.step0);
       ok = acquire(kEmptyQ, (index & 1) ^ 1);
       if (!ok) break;
-      for (int w = 0; w < g.active; ++w) {
-        const int r = warp * kWarpSize + lane;
-        const int row = g.row0[w] + r;
-        const int64_t off =
-            r < g.rows[w] ? (g.r.start + row / a.group) * a.q_stride +
-                                (static_cast<int64_t>(g.kv_head[w]) * a.group + row % a.group) * D
-                          : -1;
-        gather(q_tiles + w * S::kTileBytes, a.q, off, 0);
-      }
+      for (int w = 0; w < g.active; ++w) load_q(g, w);
       cp_async_arrive(&sy.bar[kFullQ]);
       // in the order in which the tensor cores take them
-      int64_t before = -1;
+      int before = -1;
       for (int step = g.step0; ok && step <= g.step1; ++step) {
-        const int64_t next = row_offset(g, step + 1);
+        const int next = cache_slot(g, step + 1);
         for (int w = 0; ok && w < (g.shared ? 1 : g.active); ++w) {
           if (step > g.step0) ok = load_v(g, w, before, step - 1, index);
           if (ok && step < g.step1) ok = load_k(g, w, now);
@@ -409,7 +425,7 @@ struct Producer {
 
 // The thread that issues the matrix products.
 template <int D>
-__device__ void issue_products(const TreeAttnArgs& a, Sync& sy, const uint8_t* q_tiles,
+__device__ __forceinline__ void issue_products(const TreeAttnArgs& a, Sync& sy, const uint8_t* q_tiles,
                                const uint8_t* ring_k, const uint8_t* ring_v, Place at,
                                const Place end) {
   using S = Shape<D>;
@@ -505,7 +521,7 @@ __device__ __forceinline__ uint32_t visible32(const TreeAttnArgs& a, const Reque
 
 // Softmax and epilogue of accumulator w; this thread owns row `row` of the tile.
 template <int D>
-__device__ void softmax(const TreeAttnArgs& a, Sync& sy, int w, Place at, const Place end) {
+__device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w, Place at, const Place end) {
   using S = Shape<D>;
   const int quarter = (threadIdx.x / kWarpSize) % 4;
   const int row = quarter * kWarpSize + threadIdx.x % kWarpSize;
@@ -535,31 +551,34 @@ __device__ void softmax(const TreeAttnArgs& a, Sync& sy, int w, Place at, const 
       tc_fence_after();
       if (any) {
         const bool masked = (step + 1) * kTile > g.r.context;
-        uint32_t see[4] = {~0u, ~0u, ~0u, ~0u};
+        uint32_t x[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_load32(scores + 32 * c, x[c]);
+        tmem_wait_load();
         if (masked) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            see[c] = visible32(a, g.r, mask, node, step * kTile + 32 * c);
+            const uint32_t see = visible32(a, g.r, mask, node, step * kTile + 32 * c);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              if (!((see >> i) & 1)) x[c][i] = __float_as_uint(-kInf);
+            }
           }
         }
-        float top = -kInf;
+        float tops[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          uint32_t x[32];
-          tmem_load32(scores + 32 * c, x);
-          tmem_wait_load();
+          tops[c] = __uint_as_float(x[c][0]);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float f = __uint_as_float(x[i]);
-            top = fmaxf(top, !masked || (see[c] >> i) & 1 ? f : -kInf);
+          for (int i = 1; i + 1 < 32; i += 2) {  // one three-operand maximum each
+            tops[c] = fmaxf(fmaxf(tops[c], __uint_as_float(x[c][i])),
+                            __uint_as_float(x[c][i + 1]));
           }
+          tops[c] = fmaxf(tops[c], __uint_as_float(x[c][31]));
         }
-        top *= a.scale_log2;
-        if (ref == -kInf || top > ref + kRescaleAbove) {
-          // a first reference, or one that rose: O so far is in units of 2^ref
-        } else {
-          top = ref;
-        }
+        // the reference moves when it is the first or is exceeded by 2^8
+        float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * a.scale_log2;
+        if (ref != -kInf && !(top > ref + kRescaleAbove)) top = ref;
         const bool moved = top != ref;
         if (step > g.step0 && __any_sync(0xffffffffu, moved)) {
           const float f = moved ? exp2_approx(ref - top) : 1.0f;
@@ -575,24 +594,29 @@ __device__ void softmax(const TreeAttnArgs& a, Sync& sy, int w, Place at, const 
         }
         ref = top;
         const float base = ref == -kInf ? 0.0f : ref;
+        const uint64_t scale2 = f32x2(a.scale_log2, a.scale_log2), base2 = f32x2(-base, -base);
+        uint64_t sum2[2] = {f32x2(sum, 0.0f), f32x2(0.0f, 0.0f)};
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          uint32_t x[32], p[16];
-          tmem_load32(scores + 32 * c, x);
-          tmem_wait_load();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float e = exp2_approx(fmaf(__uint_as_float(x[i]), a.scale_log2, -base));
-            const float f = !masked || (see[c] >> i) & 1 ? e : 0.0f;
-            sum += f;
-            x[i] = __float_as_uint(f);
-          }
+          uint32_t p[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            p[i] = pack_bf16x2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
+            float lo, hi;
+            f32x2_split(f32x2_fma(f32x2(__uint_as_float(x[c][2 * i]),
+                                        __uint_as_float(x[c][2 * i + 1])),
+                                  scale2, base2),
+                        lo, hi);
+            lo = exp2_approx(lo);
+            hi = exp2_approx(hi);
+            sum2[i % 2] = f32x2_add(sum2[i % 2], f32x2(lo, hi));
+            p[i] = pack_bf16x2(lo, hi);
           }
-          tmem_store16(scores + 16 * c, p);  // over scores that have been read
+          tmem_store16(scores + 16 * c, p);  // over the scores, which have all been read
         }
+        float s0, s1, s2, s3;
+        f32x2_split(sum2[0], s0, s1);
+        f32x2_split(sum2[1], s2, s3);
+        sum = (s0 + s1) + (s2 + s3);
         tmem_wait_store();
       }
       tc_fence_before();
@@ -706,8 +730,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const TreeA
   if (warp == kMmaWarp) tmem_alloc(&sy.tmem_base, kTmemColumns);
 
   // this CTA's share of the line: its length, then the requests that hold the share's two ends
-  int64_t cost = 0;
-  for (int64_t s = tid; s < a.num_seqs; s += kThreads) cost += request_cost(a, load_request(a, s));
+  Request r{};
+  if (tid < a.num_seqs) r = load_request(a, tid);
+  int64_t cost = request_cost(a, r);
+  for (int64_t s = tid + kThreads; s < a.num_seqs; s += kThreads) {
+    cost += request_cost(a, load_request(a, s));
+  }
 #pragma unroll
   for (int off = 16; off > 0; off /= 2) cost += __shfl_xor_sync(0xffffffffu, cost, off);
   if (lane == 0) sy.sums[warp] = cost;
@@ -716,15 +744,17 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const TreeA
   tc_fence_after();
   int64_t total = 0;
 #pragma unroll
-  for (int i = 0; i <= kMmaWarp; ++i) total += sy.sums[i];
+  for (int i = 0; i < kThreads / kWarpSize; ++i) total += sy.sums[i];
   // at least two steps each: a shorter share costs more in the join than it saves
   int64_t share = (total + gridDim.x - 1) / gridDim.x;
   if (share < 2) share = 2;
   const int64_t ends[2] = {blockIdx.x * share, (blockIdx.x + 1) * share};
   int64_t before = 0;
   for (int64_t base = 0; base < a.num_seqs; base += kThreads) {
-    Request r{};
-    if (base + tid < a.num_seqs) r = load_request(a, base + tid);
+    if (base > 0) {
+      r = Request{};
+      if (base + tid < a.num_seqs) r = load_request(a, base + tid);
+    }
     const int64_t own = request_cost(a, r);
     int64_t upto = own;
 #pragma unroll
@@ -737,7 +767,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const TreeA
     __syncthreads();
     int64_t chunk = 0;
 #pragma unroll
-    for (int i = 0; i <= kMmaWarp; ++i) {
+    for (int i = 0; i < kThreads / kWarpSize; ++i) {
       if (i < warp) upto += sy.sums[i];
       chunk += sy.sums[i];
     }
@@ -753,13 +783,18 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const TreeA
   __syncthreads();
   const Place at = sy.place[0], end = sy.place[1];
 
-  if (warp == kMmaWarp) {
-    if (lane == 0) issue_products<D>(a, sy, q_tiles, ring_k, ring_v, at, end);
-  } else if (warp >= kSoftmaxWarps) {
-    Producer<D> p{a, sy, ring_k, ring_v, q_tiles, warp - kSoftmaxWarps, lane};
-    p.run(at, end);
-  } else {
+  if (warp < kSoftmaxWarps) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
     softmax<D>(a, sy, warp / 4, at, end);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
+    if (warp < kMmaWarp) {
+      Producer<D> p{a,    sy,   ring_k, ring_v, q_tiles, warp - kSoftmaxWarps,
+                    lane, static_cast<uint32_t>(a.num_kv_heads) * D * 2};
+      p.run(at, end);
+    } else if (warp == kMmaWarp && lane == 0) {
+      issue_products<D>(a, sy, q_tiles, ring_k, ring_v, at, end);
+    }
   }
 
   // rows that no item covers are zero: requests that were not served, and what lies behind the last
@@ -787,72 +822,93 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const TreeA
   if (warp == kMmaWarp) tmem_dealloc(sy.tmem_base, kTmemColumns);
 }
 
-// Joins the segments of each cut item: block (b, y) looks at the border before CTA b, and the
-// first border inside an item does the item, 32 rows of one accumulator per y. With m and l the
-// maxima and sums of the segments, M the largest m: o = sum 2^(m - M) O / sum 2^(m - M) l.
+// Joins the segments of each cut item. A border between two CTAs' shares that lies inside an item
+// is the item's if it is the first of those; each block lists these borders (one thread per border)
+// and takes every gridDim-th unit of 8 rows of one accumulator, a thread 16 bytes of a row. With m
+// and l the maxima and sums of the segments, M the largest m:
+//   o = sum 2^(m - M) O / sum 2^(m - M) l.
 template <int D>
-__global__ void __launch_bounds__(kJoinThreads) tree_attention_join_kernel(const TreeAttnArgs a,
-                                                                           int ctas) {
+__global__ void __launch_bounds__(kJoinRows * D / 4) tree_attention_join_kernel(
+    const TreeAttnArgs a, int ctas) {
   grid_dependency_sync();
   using S = Shape<D>;
-  const int border = blockIdx.x + 1;
-  if (!(a.cuts[border * 2].flags & kCutFront)) return;
-  // the segment before the border: the previous CTA's second cut one, else its first
-  const int first = (border - 1) * 2 + (a.cuts[(border - 1) * 2 + 1].flags != 0 ? 1 : 0);
-  const Cut c = a.cuts[first];
-  if (c.flags & kCutFront) return;  // not the item's first border
-  int last = border;
-  while (last + 1 < ctas && (a.cuts[last * 2].flags & kCutBack)) ++last;
-
-  constexpr int kPer = D / 4 / (kJoinThreads / kJoinRows);  // 16-byte pieces of a row per thread
-  const int w = blockIdx.y / (kTile / kJoinRows);
-  const int row = (blockIdx.y % (kTile / kJoinRows)) * kJoinRows + threadIdx.x % kJoinRows;
-  if (row >= c.rows[w]) return;
-  const int piece = threadIdx.x / kJoinRows * kPer;
-  const auto part = [&](int i) {  // segment i of the item
-    const int64_t slot = i == 0 ? first : (border - 1 + i) * 2;
-    return a.parts + (slot * 2 + w) * S::kPartFloats;
-  };
-  const int n = last - border + 2;
-  const float kInf = __builtin_huge_valf();
-  float top = -kInf;
-  for (int i = 0; i < n; ++i) top = fmaxf(top, part(i)[D * kTile + row]);
-  const float base = top == -kInf ? 0.0f : top;
-  float sum = 0.0f;
-  float4 o[kPer];
-#pragma unroll
-  for (int e = 0; e < kPer; ++e) o[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 2
-  for (int i = 0; i < n; ++i) {
-    const float* p = part(i);
-    const float l = p[(D + 1) * kTile + row];
-    const float f = exp2_approx(p[D * kTile + row] - base);
-    const bool any = l != 0.0f;  // a segment of which the node sees nothing has no part
-    sum += any ? f * l : 0.0f;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      const float4 x = *reinterpret_cast<const float4*>(p + ((piece + e) * kTile + row) * 4);
-      o[e].x += any ? f * x.x : 0.0f;
-      o[e].y += any ? f * x.y : 0.0f;
-      o[e].z += any ? f * x.z : 0.0f;
-      o[e].w += any ? f * x.w : 0.0f;
+  constexpr int kBlock = kJoinRows * D / 4;
+  constexpr int kUnits = 2 * kTile / kJoinRows;  // per item
+  __shared__ int borders[kMaxCtas];
+  __shared__ int warp_counts[kBlock / kWarpSize];
+  const int tid = threadIdx.x, lane = tid % kWarpSize;
+  int items = 0;
+  for (int b0 = 1; b0 < ctas; b0 += kBlock) {
+    const int b = b0 + tid;
+    bool own = false;
+    if (b < ctas && (a.cuts[b * 2].flags & kCutFront)) {
+      // the segment before the border: the previous CTA's second cut one, else its first
+      own = a.cuts[b * 2 - 1].flags != 0 || !(a.cuts[b * 2 - 2].flags & kCutFront);
     }
+    const unsigned owners = __ballot_sync(0xffffffffu, own);
+    if (lane == 0) warp_counts[tid / kWarpSize] = __popc(owners);
+    __syncthreads();
+    int at = items + __popc(owners & ((1u << lane) - 1));
+    for (int i = 0; i < kBlock / kWarpSize; ++i) {
+      if (i < tid / kWarpSize) at += warp_counts[i];
+      items += warp_counts[i];
+    }
+    if (own) borders[at] = b;
+    __syncthreads();
   }
-  const int at_row = c.row0[w] + row;
-  const int64_t token = c.token0 + at_row / a.group;
-  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) +
-                       ((token * a.num_kv_heads + c.kv_head[w]) * a.group + at_row % a.group) * D +
-                       piece * 4;
-  const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-  for (int e = 0; e < kPer; e += 2) {
-    const float f[8] = {o[e].x,     o[e].y,     o[e].z,     o[e].w,
-                        o[e + 1].x, o[e + 1].y, o[e + 1].z, o[e + 1].w};
-    float y[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = sum == 0.0f ? 0.0f : f[i] * inverse;
-    st_global_v4(out + e * 4, pack<Bf16>(y));
+
+  const float kInf = __builtin_huge_valf();
+  for (int unit = blockIdx.x; unit < items * kUnits; unit += gridDim.x) {
+    const int border = borders[unit / kUnits];
+    const int first = border * 2 - (a.cuts[border * 2 - 1].flags != 0 ? 1 : 2);
+    const int w = unit % kUnits / (kUnits / 2);
+    const int row = unit % (kUnits / 2) * kJoinRows + tid % kJoinRows;
+    const Cut& c = a.cuts[first];
+    if (unit % (kUnits / 2) * kJoinRows >= c.rows[w]) continue;
+    int last = border;
+    while (last + 1 < ctas && (a.cuts[last * 2].flags & kCutBack)) ++last;
+    const int piece = tid / kJoinRows;
+    const auto part = [&](int i) {  // segment i of the item
+      const int64_t slot = i == 0 ? first : (border - 1 + i) * 2;
+      return a.parts + (slot * 2 + w) * S::kPartFloats;
+    };
+    const int n = last - border + 2;
+    float top = -kInf;
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) top = fmaxf(top, part(i)[D * kTile + row]);
+    const float base = top == -kInf ? 0.0f : top;
+    float sum = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+      const float* p = part(i);
+      const float l = p[(D + 1) * kTile + row];
+      const float f = exp2_approx(p[D * kTile + row] - base);
+      const float4 x = *reinterpret_cast<const float4*>(p + (piece * kTile + row) * 4);
+      if (l != 0.0f) {  // a segment of which the node sees nothing has no part
+        sum = fmaf(f, l, sum);
+        o.x = fmaf(f, x.x, o.x);
+        o.y = fmaf(f, x.y, o.y);
+        o.z = fmaf(f, x.z, o.z);
+        o.w = fmaf(f, x.w, o.w);
+      }
+    }
+    if (row >= c.rows[w]) continue;
+    const int at_row = c.row0[w] + row;
+    const int64_t token = c.token0 + at_row / a.group;
+    auto* out = static_cast<__nv_bfloat16*>(a.out) +
+                ((token * a.num_kv_heads + c.kv_head[w]) * a.group + at_row % a.group) * D +
+                piece * 4;
+    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (sum == 0.0f) o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(o.x * inverse, o.y * inverse),
+                                                pack_bf16x2(o.z * inverse, o.w * inverse));
   }
+}
+
+inline int attention_ctas(int device) {
+  const int sms = sm_count(device);
+  return sms < kMaxCtas ? sms : kMaxCtas;
 }
 
 // Workspace: the partial sums of every CTA, then its cuts.
@@ -864,7 +920,7 @@ int64_t workspace_bytes(int ctas) {
 
 template <int D>
 int launch_tree_attention(TreeAttnArgs& a, void* workspace, int device, cudaStream_t stream) {
-  const int ctas = sm_count(device);
+  const int ctas = attention_ctas(device);
   a.parts = static_cast<float*>(workspace);
   a.cuts = reinterpret_cast<Cut*>(a.parts + static_cast<int64_t>(ctas) * 4 *
                                                 Shape<D>::kPartFloats);
@@ -877,8 +933,8 @@ int launch_tree_attention(TreeAttnArgs& a, void* workspace, int device, cudaStre
   const int status = launch_serialized(tree_attention_kernel<D>, dim3(ctas), dim3(kThreads),
                                        Shape<D>::kSmem, stream, 1u, a);
   if (status != SVLLM_OK || ctas < 2) return status;
-  return launch(tree_attention_join_kernel<D>, dim3(ctas - 1, 2 * kTile / kJoinRows),
-                dim3(kJoinThreads), 0, stream, 1u, a, ctas);
+  return launch(tree_attention_join_kernel<D>, dim3(4 * ctas), dim3(kJoinRows * D / 4), 0, stream,
+                1u, a, ctas);
 }
 
 }  // namespace
@@ -890,7 +946,7 @@ extern "C" int svllm_tree_attention_workspace_bytes(int64_t head_dim, int64_t* b
   if (head_dim != 64 && head_dim != 128) return SVLLM_ERR_UNSUPPORTED;
   int device;
   if (current_device(&device) != SVLLM_OK) return SVLLM_ERR_CUDA;
-  const int ctas = sm_count(device);
+  const int ctas = attention_ctas(device);
   *bytes = head_dim == 128 ? workspace_bytes<128>(ctas) : workspace_bytes<64>(ctas);
   return SVLLM_OK;
 }
