@@ -18,16 +18,16 @@
 // lengths. An item cut by a share's border leaves unnormalised partial sums in the workspace, which
 // a second small kernel joins.
 //
-// In a CTA: 4 producer warps gather K and V rows through the block table with cp.async into
-// 128-byte-swizzled tiles (any block size: a page may end anywhere in a tile); one thread issues
-// tcgen05.mma: S = Q K^T into TMEM, then O += P V with P read from TMEM and V as the N-major
-// operand, alternating between two accumulators so that the tensor pipe works on one M tile while
-// the other's softmax runs; two groups of 4 warps do the softmax, one thread per row, and write P
-// (bf16, as the second product takes it) over S. The running maximum is a reference that moves
-// only when a row exceeds it by 2^8, so O in TMEM is seldom rescaled; the sums are fp32 and the
-// result does not depend on the reference. Masked scores are replaced after the product, and
-// non-finite values of V in the tiles that hold tree nodes (0 * NaN would reach rows that do not
-// see them) are taken out on the way in and added again, for the rows that see them, at the end.
+// In a CTA: two warps bring K and V rows through the block table with TMA into 128-byte-swizzled
+// tiles (any block size: a page may end anywhere in a tile); one thread issues tcgen05.mma: S = Q K^T into TMEM, then O += P V with P read from TMEM and V as
+// the N-major operand, alternating between two accumulators so that the tensor pipe works on one M
+// tile while the other's softmax runs; two groups of 4 warps do the softmax, one thread per row,
+// and write P (bf16, as the second product takes it) over S. The running maximum is a reference
+// that moves only when a row exceeds it by 2^8, so O in TMEM is seldom rescaled; the sums are fp32
+// and the result does not depend on the reference. Masked scores are replaced after the product.
+// Four helper warps bring the query rows and, since 0 * NaN would reach rows that do not see it,
+// zero the values of V that are not finite in the tiles that hold tree nodes; they are added
+// again, for the rows that see them, at the end.
 #include <cuda_runtime.h>
 
 #include <cmath>
@@ -42,9 +42,10 @@ namespace {
 
 constexpr int kTile = 128;            // query rows per M tile, cached rows per key tile
 constexpr int kSoftmaxWarps = 8;      // two groups of 4: accumulators 0 and 1
-constexpr int kProducerWarps = 4;
-constexpr int kMmaWarp = kSoftmaxWarps + kProducerWarps;
-constexpr int kThreads = 16 * kWarpSize;  // the last three warps only fill the register groups
+constexpr int kHelperWarps = 4;       // query rows and the check of V
+constexpr int kMmaWarp = kSoftmaxWarps + kHelperWarps;
+constexpr int kLoadWarp = kMmaWarp + 1;  // K, and the next one V
+constexpr int kThreads = 16 * kWarpSize;  // the last warp only fills the register groups
 // Registers per thread after the split of the launch's 512 x 128: the softmax warps hold a row of
 // scores each, 8 x 32 x 192 + 8 x 32 x 64 = 65536.
 constexpr int kSoftmaxRegisters = 192, kOtherRegisters = 64;
@@ -96,6 +97,8 @@ struct TreeAttnArgs {
   Divider page;                    // by the block size
   int group;                       // query heads per KV head
   int num_kv_heads;
+  int cache_slots;
+  int box_rows;                    // rows of a TMA box; 1: four rows gathered per instruction
   int mask_words;
   float scale_log2;                // scale * log2(e): scores are kept in powers of two
   int* err;
@@ -227,7 +230,11 @@ __device__ __forceinline__ bool next_segment(const TreeAttnArgs& a, Place& at, c
 // Barriers and flags of one CTA.
 constexpr int kMaxStagesK = 6, kMaxStagesV = 4;
 constexpr int kFullK = 0, kFullV = kFullK + kMaxStagesK, kFullQ = kFullV + kMaxStagesV;
-constexpr int kEmptyK = kFullQ + 1, kEmptyV = kEmptyK + kMaxStagesK;
+// A V tile with tree nodes lands on its own barrier, for the helpers, which signal when it is
+// checked; kFullV stands for the others. (A slot's parity counts the uses of one barrier, so every
+// waiter of a barrier has to see all of them.)
+constexpr int kCheckedV = kFullQ + 1, kLandedV = kCheckedV + kMaxStagesV;
+constexpr int kEmptyK = kLandedV + kMaxStagesV, kEmptyV = kEmptyK + kMaxStagesK;
 constexpr int kEmptyQ = kEmptyV + kMaxStagesV;
 constexpr int kScoresDone = kEmptyQ + 1, kWeightsDone = kScoresDone + 2;
 constexpr int kOutputDone = kWeightsDone + 2, kDrain = kOutputDone + 2, kBarriers = kDrain + 1;
@@ -277,33 +284,30 @@ __device__ __forceinline__ bool drop_odd(uint32_t& w) {
   return lo || hi;
 }
 
-// The four producer warps: each gathers 32 of a tile's 128 rows. The copies signal the tile's
-// barrier themselves as they land (the thread that issues the products orders them before the
-// tensor cores' reads), so the producers run ahead as far as the rings have room.
-template <int D>
-struct Producer {
-  using S = Shape<D>;
-  static constexpr int kLanes = D / 8;                // lanes per row: 16 bytes each
-  static constexpr int kRowsAtOnce = kWarpSize / kLanes;
+// The V tiles of these steps hold tree nodes.
+__device__ __forceinline__ bool has_nodes(const Segment& g, int step) {
+  return (step + 1) * kTile > g.r.context;
+}
 
+// One of the two warps that bring K and V: the tiles of one of them, in the order in which the
+// tensor cores take them. Where the block size allows, a TMA box is a run of 8 to 128 rows that no
+// page border can fall into, gcd(block_size, 128); otherwise one instruction gathers 4 rows.
+template <int D>
+struct Loader {
+  using S = Shape<D>;
   const TreeAttnArgs& a;
   Sync& sy;
-  uint8_t* ring_k;
-  uint8_t* ring_v;
-  uint8_t* q_tiles;
-  int warp, lane;      // warp 0..3
-  uint32_t row_bytes;  // of a cached row, all KV heads
-  Ring k{}, v{};
+  const CUtensorMap* map;
+  uint8_t* ring;
+  bool values;           // V, else K
+  int lane;
+  Ring at{};
+  uint64_t used = 0, parity = 0;  // barriers signalled so far, and the parity of their next use
 
-  __device__ __forceinline__ bool acquire(int bar, uint32_t parity) {
-    return __all_sync(0xffffffffu, wait_phase(&sy.bar[bar], parity, &sy.abort, a.err));
-  }
-
-  // The cache slot of this lane's row of key tile `step`, -1 past the request's end. A slot fits
-  // 31 bits: 2^31 rows of 64 bf16 would be 256 GB.
-  __device__ __forceinline__ int cache_slot(const Segment& g, int step) const {
-    const int j = step * kTile + warp * kWarpSize + lane;
-    if (step >= g.step1 || j >= g.r.length) return -1;
+  // The cache slot of row j of the request; past its end a slot past the cache, which reads as
+  // zeros.
+  __device__ __forceinline__ int cache_slot(const Segment& g, int j) const {
+    if (j >= g.r.length) return a.cache_slots;
     const int page = a.page.divide(j);
     int block = a.block_tables[g.s * a.max_blocks + page];
     if (static_cast<uint64_t>(block) >= static_cast<uint64_t>(a.num_blocks)) {
@@ -313,115 +317,156 @@ struct Producer {
     return block * a.block_size + (j - page * a.block_size);
   }
 
-  // Where this lane's 16 bytes of its row in round i go: round i brings rows i * kRowsAtOnce ..
-  // of the warp's 32, lane / kLanes of them this lane's. The swizzle depends on the row modulo 8.
-  __device__ __forceinline__ uint32_t tile_place(uint32_t base, int i) const {
-    const int c = lane % kLanes;
-    const int row = i * kRowsAtOnce + lane / kLanes;
-    return base + (c / 8) * kHalfBytes + (warp * kWarpSize + row) * 128 +
-           (((c % 8) ^ (row & 7)) << 4);
-  }
-
-  // The rows `slot` (one per lane, -1 = zeros) of `src`, `stride` bytes apart, into a tile.
-  __device__ __forceinline__ void gather(uint8_t* tile, const uint8_t* src, int slot,
-                                         uint32_t stride) {
-    const uint32_t base = smem_addr(tile);
-    src += (lane % kLanes) * 16;
-#pragma unroll
-    for (int i = 0; i < kWarpSize / kRowsAtOnce; ++i) {
-      const int row = __shfl_sync(0xffffffffu, slot, i * kRowsAtOnce + lane / kLanes);
-      cp_async16(tile_place(base, i), src + static_cast<uint64_t>(max(row, 0)) * stride, row >= 0);
-    }
-  }
-
-  // The same for a V tile that holds tree nodes: through registers, values that are not finite
-  // left out; true if there were any.
-  __device__ __forceinline__ bool gather_checked(uint8_t* tile, const uint8_t* src, int slot,
-                                              uint32_t stride) {
-    const uint32_t base = smem_addr(tile);
-    src += (lane % kLanes) * 16;
-    bool odd = false;
-#pragma unroll 4
-    for (int i = 0; i < kWarpSize / kRowsAtOnce; ++i) {
-      const int row = __shfl_sync(0xffffffffu, slot, i * kRowsAtOnce + lane / kLanes);
-      uint4 w = make_uint4(0, 0, 0, 0);
-      if (row >= 0) w = ld_global_nc_v4(src + static_cast<uint64_t>(row) * stride);
-      odd |= drop_odd(w.x) | drop_odd(w.y) | drop_odd(w.z) | drop_odd(w.w);
-      asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(tile_place(base, i)),
-                   "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
-                   : "memory");
-    }
-    return odd;
-  }
-
-  __device__ __forceinline__ bool load_k(const Segment& g, int w, int slot) {
-    if (!acquire(kEmptyK + k.slot, k.phase ^ 1)) return false;
-    gather(ring_k + k.slot * S::kTileBytes,
-           static_cast<const uint8_t*>(a.k_cache) + g.kv_head[w] * D * 2, slot, row_bytes);
-    cp_async_arrive(&sy.bar[kFullK + k.slot]);
-    k.advance(S::kStagesK);
-    return true;
-  }
-  __device__ __forceinline__ bool load_v(const Segment& g, int w, int slot, int step, int index) {
-    if (!acquire(kEmptyV + v.slot, v.phase ^ 1)) return false;
-    uint8_t* tile = ring_v + v.slot * S::kTileBytes;
-    const uint8_t* src = static_cast<const uint8_t*>(a.v_cache) + g.kv_head[w] * D * 2;
-    if ((step + 1) * kTile > g.r.context) {
-      if (gather_checked(tile, src, slot, row_bytes)) {
-        sy.odd_values[w][index & 3] = 1;
-        if (g.shared) sy.odd_values[1][index & 3] = 1;
-      }
-      fence_proxy_async_smem();
-      mbar_arrive(&sy.bar[kFullV + v.slot]);
+  // This lane's rows of key tile `step`: the first of box `lane`, or four rows from 4 * lane on.
+  __device__ __forceinline__ void find_rows(const Segment& g, int step, int (&rows)[4]) const {
+    if (step >= g.step1) return;
+    if (a.box_rows > 1) {
+      const int j = lane * a.box_rows;
+      if (j < kTile) rows[0] = cache_slot(g, step * kTile + j);
     } else {
-      gather(tile, src, slot, row_bytes);
-      cp_async_arrive(&sy.bar[kFullV + v.slot]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) rows[i] = cache_slot(g, step * kTile + 4 * lane + i);
     }
-    v.advance(S::kStagesV);
+  }
+
+  __device__ __forceinline__ bool load(int bar, const int (&rows)[4], int kv_head) {
+    const int empty = values ? kEmptyV : kEmptyK;
+    if (!__all_sync(0xffffffffu, wait_phase(&sy.bar[empty + at.slot], at.phase ^ 1, &sy.abort,
+                                            a.err))) {
+      return false;
+    }
+    if (lane == 0) mbar_arrive_expect_tx(&sy.bar[bar], S::kTileBytes);
+    __syncwarp();
+    const uint32_t dst = smem_addr(ring + at.slot * S::kTileBytes);
+    const int column = kv_head * D;
+    if (a.box_rows > 1) {
+      const int boxes = kTile / a.box_rows;
+      const uint32_t box_bytes = a.box_rows * 128;
+      for (int i = 0; i < boxes; ++i) {
+        const int row = __shfl_sync(0xffffffffu, rows[0], i);
+        if (lane == 0) {
+#pragma unroll
+          for (int h = 0; h < S::kHalves; ++h) {
+            tma_load_2d(dst + h * kHalfBytes + i * box_bytes, map, column + h * kTmaBoxCols, row,
+                        &sy.bar[bar]);
+          }
+        }
+      }
+    } else {
+#pragma unroll 4
+      for (int i = 0; i < kTile / 4; ++i) {
+        int32_t y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = __shfl_sync(0xffffffffu, rows[e], i);
+        if (lane == 0) {
+#pragma unroll
+          for (int h = 0; h < S::kHalves; ++h) {
+            tma_gather4(dst + h * kHalfBytes + i * 512, map, column + h * kTmaBoxCols, y,
+                        &sy.bar[bar]);
+          }
+        }
+      }
+    }
+    used |= uint64_t{1} << bar;
+    parity ^= uint64_t{1} << bar;
+    at.advance(values ? S::kStagesV : S::kStagesK);
     return true;
   }
 
-  // The query rows of accumulator w: row = node * group + head of the KV head.
-  __device__ __forceinline__ void load_q(const Segment& g, int w) {
-    const int r = warp * kWarpSize + lane;
-    const int row = g.row0[w] + r;
-    const int64_t offset =
-        r < g.rows[w] ? (g.r.start + row / a.group) * a.q_stride +
-                            (static_cast<int64_t>(g.kv_head[w]) * a.group + row % a.group) * D
-                      : -1;
-    const uint32_t base = smem_addr(q_tiles + w * S::kTileBytes);
-    const auto* src = static_cast<const __nv_bfloat16*>(a.q) + (lane % kLanes) * 8;
-#pragma unroll 4
-    for (int i = 0; i < kWarpSize / kRowsAtOnce; ++i) {
-      const int64_t at = __shfl_sync(0xffffffffu, offset, i * kRowsAtOnce + lane / kLanes);
-      cp_async16(tile_place(base, i), src + (at < 0 ? 0 : at), at >= 0);
-    }
-  }
-
-  __device__ __forceinline__ void run(Place at, const Place end) {
+  __device__ __forceinline__ void run(Place place, const Place end) {
     Segment g;
     bool ok = true;
-    for (int index = 0; ok && next_segment(a, at, end, g); ++index) {
-      int now = cache_slot(g, g.step0);
-      ok = acquire(kEmptyQ, (index & 1) ^ 1);
-      if (!ok) break;
-      for (int w = 0; w < g.active; ++w) load_q(g, w);
-      cp_async_arrive(&sy.bar[kFullQ]);
-      // in the order in which the tensor cores take them
-      int before = -1;
-      for (int step = g.step0; ok && step <= g.step1; ++step) {
-        const int next = cache_slot(g, step + 1);
-        for (int w = 0; ok && w < (g.shared ? 1 : g.active); ++w) {
-          if (step > g.step0) ok = load_v(g, w, before, step - 1, index);
-          if (ok && step < g.step1) ok = load_k(g, w, now);
-        }
-        before = now;
-        now = next;
+    while (ok && next_segment(a, place, end, g)) {
+      int now[4], next[4];
+      find_rows(g, g.step0, now);
+      for (int step = g.step0; ok && step < g.step1; ++step) {
+        find_rows(g, step + 1, next);
+        const int full = !values ? kFullK : has_nodes(g, step) ? kLandedV : kFullV;
+        ok = load(full + at.slot, now, g.kv_head[0]);
+        if (ok && !g.shared && g.active == 2) ok = load(full + at.slot, now, g.kv_head[1]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) now[i] = next[i];
       }
     }
-    cp_async_wait_all();  // also after an abort: no copy is in flight when the CTA exits
+    // every copy has landed before the CTA exits: the last use of each barrier
+    for (int bar = 0; bar < kEmptyK; ++bar) {
+      if ((used >> bar) & 1) mbar_wait_bounded(&sy.bar[bar], ((parity >> bar) & 1) ^ 1);
+    }
   }
 };
+static_assert(kEmptyK <= 64, "one bit per barrier that a copy may signal");
+
+// The four helper warps: the query rows of each segment, and the V tiles that hold tree nodes,
+// whose values that are not finite are zeroed before the tensor cores see them.
+template <int D>
+__device__ __forceinline__ void help(const TreeAttnArgs& a, Sync& sy, uint8_t* q_tiles,
+                                     uint8_t* ring_v, int warp, int lane, Place at,
+                                     const Place end) {
+  using S = Shape<D>;
+  constexpr int kLanes = D / 8;  // lanes per query row: 16 bytes each
+  constexpr int kRowsAtOnce = kWarpSize / kLanes;
+  const auto wait = [&](int bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, wait_phase(&sy.bar[bar], parity, &sy.abort, a.err));
+  };
+  Ring v;
+  uint32_t landed = 0;  // parity of the next use of each V slot's barrier
+  Segment g;
+  bool ok = true;
+  for (int index = 0; ok && next_segment(a, at, end, g); ++index) {
+    ok = wait(kEmptyQ, (index & 1) ^ 1);
+    if (!ok) break;
+    for (int w = 0; w < g.active; ++w) {
+      // row = node * group + head of the KV head
+      const int r = warp * kWarpSize + lane;
+      const int row = g.row0[w] + r;
+      const int64_t offset =
+          r < g.rows[w] ? (g.r.start + row / a.group) * a.q_stride +
+                              (static_cast<int64_t>(g.kv_head[w]) * a.group + row % a.group) * D
+                        : -1;
+      const uint32_t base = smem_addr(q_tiles + w * S::kTileBytes);
+      const int c = lane % kLanes;
+      const auto* src = static_cast<const __nv_bfloat16*>(a.q) + c * 8;
+#pragma unroll 4
+      for (int i = 0; i < kWarpSize / kRowsAtOnce; ++i) {
+        const int x = i * kRowsAtOnce + lane / kLanes;
+        const int64_t from = __shfl_sync(0xffffffffu, offset, x);
+        cp_async16(base + (c / 8) * kHalfBytes + (warp * kWarpSize + x) * 128 +
+                       (((c % 8) ^ (x & 7)) << 4),
+                   src + (from < 0 ? 0 : from), from >= 0);
+      }
+    }
+    cp_async_arrive(&sy.bar[kFullQ]);
+    for (int step = g.step0; ok && step < g.step1; ++step) {
+      for (int w = 0; ok && w < (g.shared ? 1 : g.active); ++w) {
+        if (has_nodes(g, step)) {
+          ok = wait(kLandedV + v.slot, (landed >> v.slot) & 1);
+          if (!ok) break;
+          landed ^= 1u << v.slot;
+          auto* tile = reinterpret_cast<uint4*>(ring_v + v.slot * S::kTileBytes);
+          bool odd = false;
+#pragma unroll 4
+          for (int i = warp * kWarpSize + lane; i < S::kTileBytes / 16; i += 4 * kWarpSize) {
+            uint4 x = tile[i];
+            if (step * kTile + i * 16 % kHalfBytes / 128 >= g.r.length) {
+              tile[i] = make_uint4(0, 0, 0, 0);  // behind the request's end, whatever it holds
+            } else if (drop_odd(x.x) | drop_odd(x.y) | drop_odd(x.z) | drop_odd(x.w)) {
+              tile[i] = x;
+              odd = true;
+            }
+          }
+          if (odd) {
+            sy.odd_values[w][index & 3] = 1;
+            if (g.shared) sy.odd_values[1][index & 3] = 1;
+          }
+          fence_proxy_async_smem();
+          mbar_arrive(&sy.bar[kCheckedV + v.slot]);
+        }
+        v.advance(S::kStagesV);
+      }
+    }
+  }
+  cp_async_wait_all();  // also after an abort: no copy is in flight when the CTA exits
+}
 
 // The thread that issues the matrix products.
 template <int D>
@@ -439,17 +484,12 @@ __device__ __forceinline__ void issue_products(const TreeAttnArgs& a, Sync& sy, 
     tc_fence_after();
     return ok;
   };
-  // a tile: the producers' writes, made through the generic proxy, before the tensor cores' reads
-  const auto wait_tile = [&](int bar, uint32_t parity) {
-    wait(bar, parity);
-    fence_proxy_async_smem();
-    return ok;
-  };
+  uint32_t full_v = 0, checked_v = 0;  // parity of the next use of each V slot's barriers
   Segment g;
   for (int index = 0; ok && next_segment(a, at, end, g); ++index) {
     const auto scores = [&](int w, bool last) {
       const bool first_use = !g.shared || w == 0, last_use = !g.shared || w == 1;
-      if (first_use && !wait_tile(kFullK + k.slot, k.phase)) return;
+      if (first_use && !wait(kFullK + k.slot, k.phase)) return;
       const uint8_t* qt = q_tiles + w * S::kTileBytes;
       const uint8_t* kt = ring_k + k.slot * S::kTileBytes;
 #pragma unroll
@@ -465,14 +505,20 @@ __device__ __forceinline__ void issue_products(const TreeAttnArgs& a, Sync& sy, 
       }
       if (last && w == g.active - 1) umma_commit(&sy.bar[kEmptyQ]);
     };
-    if (!wait_tile(kFullQ, index & 1)) break;
+    if (!wait(kFullQ, index & 1)) break;
+    fence_proxy_async_smem();  // the helpers' copies, before the tensor cores' reads
     for (int w = 0; ok && w < g.active; ++w) scores(w, g.step0 + 1 == g.step1);
     for (int step = g.step0; ok && step < g.step1; ++step) {
       for (int w = 0; ok && w < g.active; ++w) {
         if (!wait(kWeightsDone + w, weights_phase[w])) break;
         weights_phase[w] ^= 1;
         const bool first_use = !g.shared || w == 0, last_use = !g.shared || w == 1;
-        if (first_use && !wait_tile(kFullV + v.slot, v.phase)) break;
+        if (first_use) {
+          const bool nodes = has_nodes(g, step);
+          uint32_t& parity = nodes ? checked_v : full_v;
+          if (!wait((nodes ? kCheckedV : kFullV) + v.slot, (parity >> v.slot) & 1)) break;
+          parity ^= 1u << v.slot;
+        }
         const uint8_t* vt = ring_v + v.slot * S::kTileBytes;
 #pragma unroll
         for (int kk = 0; kk < kTile / 16; ++kk) {
@@ -703,7 +749,9 @@ __device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w, 
 }
 
 template <int D>
-__global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const TreeAttnArgs a) {
+__global__ void __launch_bounds__(kThreads, 1)
+    tree_attention_kernel(const __grid_constant__ CUtensorMap map_k,
+                          const __grid_constant__ CUtensorMap map_v, const TreeAttnArgs a) {
   using S = Shape<D>;
   grid_dependency_sync();
   extern __shared__ uint8_t smem_raw[];
@@ -716,9 +764,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const TreeA
 
   if (tid == 0) {
     for (int i = 0; i < kBarriers; ++i) {
-      const bool full = i < kEmptyK;
+      const bool helpers = i >= kFullQ && i < kLandedV;
       const bool weights = i == kWeightsDone || i == kWeightsDone + 1;
-      mbar_init(&sy.bar[i], full ? kProducerWarps * kWarpSize : weights ? 4 * kWarpSize : 1);
+      mbar_init(&sy.bar[i], helpers || weights ? 4 * kWarpSize : 1);
     }
     fence_mbar_init();
     sy.abort = 0;
@@ -789,9 +837,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_attention_kernel(const TreeA
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
     if (warp < kMmaWarp) {
-      Producer<D> p{a,    sy,   ring_k, ring_v, q_tiles, warp - kSoftmaxWarps,
-                    lane, static_cast<uint32_t>(a.num_kv_heads) * D * 2};
-      p.run(at, end);
+      help<D>(a, sy, q_tiles, ring_v, warp - kSoftmaxWarps, lane, at, end);
+    } else if (warp == kLoadWarp || warp == kLoadWarp + 1) {
+      const bool values = warp > kLoadWarp;
+      Loader<D> l{a, sy, values ? &map_v : &map_k, values ? ring_v : ring_k, values, lane};
+      l.run(at, end);
     } else if (warp == kMmaWarp && lane == 0) {
       issue_products<D>(a, sy, q_tiles, ring_k, ring_v, at, end);
     }
@@ -924,6 +974,12 @@ int launch_tree_attention(TreeAttnArgs& a, void* workspace, int device, cudaStre
   a.parts = static_cast<float*>(workspace);
   a.cuts = reinterpret_cast<Cut*>(a.parts + static_cast<int64_t>(ctas) * 4 *
                                                 Shape<D>::kPartFloats);
+  CUtensorMap map_k, map_v;
+  const int64_t cols = static_cast<int64_t>(a.num_kv_heads) * D;
+  if (!make_map(&map_k, a.k_cache, a.cache_slots, cols, cols, a.box_rows) ||
+      !make_map(&map_v, a.v_cache, a.cache_slots, cols, cols, a.box_rows)) {
+    return SVLLM_ERR_CUDA;
+  }
   // raises the kernel's shared-memory limit on its first use
   if (blocks_per_sm(reinterpret_cast<const void*>(tree_attention_kernel<D>), kThreads,
                     Shape<D>::kSmem, device) < 1) {
@@ -931,7 +987,7 @@ int launch_tree_attention(TreeAttnArgs& a, void* workspace, int device, cudaStre
   }
   // not scheduled early behind the previous kernel: a CTA takes nearly all of an SM
   const int status = launch_serialized(tree_attention_kernel<D>, dim3(ctas), dim3(kThreads),
-                                       Shape<D>::kSmem, stream, 1u, a);
+                                       Shape<D>::kSmem, stream, 1u, map_k, map_v, a);
   if (status != SVLLM_OK || ctas < 2) return status;
   return launch(tree_attention_join_kernel<D>, dim3(4 * ctas), dim3(kJoinRows * D / 4), 0, stream,
                 1u, a, ctas);
@@ -978,6 +1034,8 @@ extern "C" int svllm_tree_attention_bf16(
   constexpr int64_t kMax = int64_t{1} << 31;
   if (num_seqs >= kMax || num_tokens * num_heads >= kMax || max_blocks >= kMax ||
       block_size >= (int64_t{1} << 20) || max_blocks * block_size >= kMax ||
+      num_blocks >= kMax || num_kv_heads >= (int64_t{1} << 20) ||
+      num_blocks * block_size >= kMax ||
       (tree_mask != nullptr && mask_words > SVLLM_MAX_TREE_NODES / 64)) {
     return SVLLM_ERR_TOO_LARGE;
   }
@@ -1009,6 +1067,10 @@ extern "C" int svllm_tree_attention_bf16(
   a.page = make_divider(block_size);
   a.group = static_cast<int>(num_heads / num_kv_heads);
   a.num_kv_heads = static_cast<int>(num_kv_heads);
+  a.cache_slots = static_cast<int>(num_blocks * block_size);
+  a.box_rows = 128;
+  while (block_size % a.box_rows != 0) a.box_rows /= 2;
+  if (a.box_rows < 8) a.box_rows = 1;
   a.mask_words = static_cast<int>(mask_words);
   a.scale_log2 = static_cast<float>(static_cast<double>(scale) / std::log(2.0));
   a.err = err;

@@ -18,12 +18,29 @@ namespace svllm::k {
 // Columns of one TMA box: 64 bf16 = 128 bytes, one 128-byte swizzle atom.
 constexpr int kTmaBoxCols = 64;
 
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int32_t x,
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int32_t x,
                                             int32_t y, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_addr(dst)),
+      " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_addr(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int32_t x,
+                                            int32_t y, uint64_t* bar) {
+  tma_load_2d(smem_addr(dst), map, x, y, bar);
+}
+
+// Rows y[0..3] of a 2-D map whose box is one row: kTmaBoxCols columns from x, 128 bytes each, into
+// four consecutive rows of a 128-byte-swizzled tile. A row past the tensor's end reads as zeros.
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, int32_t x,
+                                            const int32_t (&y)[4], uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y[0]), "r"(y[1]), "r"(y[2]), "r"(y[3]),
+      "r"(smem_addr(bar))
       : "memory");
 }
 
