@@ -55,6 +55,7 @@ constexpr uint32_t kScores = 0;       // TMEM columns: S (and P) of accumulator 
 constexpr uint32_t kOutput = 256;     // O at 256 + 128 w
 constexpr float kRescaleAbove = 8.0f;  // in powers of two
 constexpr int kJoinRows = 8;
+constexpr int kJoinBatch = 4;         // segments whose loads are in flight together
 constexpr int kMaxCtas = 256;         // one per SM; the join lists their borders
 
 template <int D>
@@ -335,7 +336,7 @@ struct Loader {
                                             a.err))) {
       return false;
     }
-    if (lane == 0) mbar_arrive_expect_tx(&sy.bar[bar], S::kTileBytes);
+    if (elect_one()) mbar_arrive_expect_tx(&sy.bar[bar], S::kTileBytes);
     __syncwarp();
     const uint32_t dst = smem_addr(ring + at.slot * S::kTileBytes);
     const int column = kv_head * D;
@@ -344,7 +345,7 @@ struct Loader {
       const uint32_t box_bytes = a.box_rows * 128;
       for (int i = 0; i < boxes; ++i) {
         const int row = __shfl_sync(0xffffffffu, rows[0], i);
-        if (lane == 0) {
+        if (elect_one()) {
 #pragma unroll
           for (int h = 0; h < S::kHalves; ++h) {
             tma_load_2d(dst + h * kHalfBytes + i * box_bytes, map, column + h * kTmaBoxCols, row,
@@ -358,7 +359,7 @@ struct Loader {
         int32_t y[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] = __shfl_sync(0xffffffffu, rows[e], i);
-        if (lane == 0) {
+        if (elect_one()) {
 #pragma unroll
           for (int h = 0; h < S::kHalves; ++h) {
             tma_gather4(dst + h * kHalfBytes + i * 512, map, column + h * kTmaBoxCols, y,
@@ -468,7 +469,7 @@ __device__ __forceinline__ void help(const TreeAttnArgs& a, Sync& sy, uint8_t* q
   cp_async_wait_all();  // also after an abort: no copy is in flight when the CTA exits
 }
 
-// The thread that issues the matrix products.
+// The warp that issues the matrix products, one lane of it each of them.
 template <int D>
 __device__ __forceinline__ void issue_products(const TreeAttnArgs& a, Sync& sy, const uint8_t* q_tiles,
                                const uint8_t* ring_k, const uint8_t* ring_v, Place at,
@@ -476,11 +477,16 @@ __device__ __forceinline__ void issue_products(const TreeAttnArgs& a, Sync& sy, 
   using S = Shape<D>;
   constexpr uint32_t kIdescS = idesc_bf16(kTile, kTile);
   constexpr uint32_t kIdescO = idesc_bf16(kTile, D) | kIdescBMajorN;
+  // descriptors of the first tile of each kind; a tile further on, the start address moves
+  constexpr uint64_t kTileStep = S::kTileBytes >> 4;
+  const uint64_t q_desc = smem_desc_k_sw128(q_tiles), k_desc = smem_desc_k_sw128(ring_k);
+  const uint64_t v_desc = smem_desc_mn_sw128(ring_v, kHalfBytes);
+  const uint32_t tmem = sy.tmem_base;
   Ring k, v;
-  uint32_t weights_phase[2] = {0, 0};
+  uint32_t weights_phase = 0;  // one bit per accumulator
   bool ok = true;
   const auto wait = [&](int bar, uint32_t parity) {
-    ok = wait_phase(&sy.bar[bar], parity, &sy.abort, a.err);
+    ok = __all_sync(0xffffffffu, wait_phase(&sy.bar[bar], parity, &sy.abort, a.err));
     tc_fence_after();
     return ok;
   };
@@ -490,28 +496,27 @@ __device__ __forceinline__ void issue_products(const TreeAttnArgs& a, Sync& sy, 
     const auto scores = [&](int w, bool last) {
       const bool first_use = !g.shared || w == 0, last_use = !g.shared || w == 1;
       if (first_use && !wait(kFullK + k.slot, k.phase)) return;
-      const uint8_t* qt = q_tiles + w * S::kTileBytes;
-      const uint8_t* kt = ring_k + k.slot * S::kTileBytes;
+      if (elect_one()) {
+        const uint64_t qd = q_desc + w * kTileStep;
+        const uint64_t kd = k_desc + k.slot * kTileStep;
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        const int at_bytes = (kk / 4) * kHalfBytes + (kk % 4) * 32;
-        umma_bf16(sy.tmem_base + kScores + w * kTile, smem_desc_k_sw128(qt + at_bytes),
-                  smem_desc_k_sw128(kt + at_bytes), kIdescS, kk != 0);
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint64_t step = ((kk / 4) * kHalfBytes + (kk % 4) * 32) >> 4;
+          umma_bf16(tmem + kScores + w * kTile, qd + step, kd + step, kIdescS, kk != 0);
+        }
+        umma_commit(&sy.bar[kScoresDone + w]);
+        if (last_use) umma_commit(&sy.bar[kEmptyK + k.slot]);
+        if (last && w == g.active - 1) umma_commit(&sy.bar[kEmptyQ]);
       }
-      umma_commit(&sy.bar[kScoresDone + w]);
-      if (last_use) {
-        umma_commit(&sy.bar[kEmptyK + k.slot]);
-        k.advance(S::kStagesK);
-      }
-      if (last && w == g.active - 1) umma_commit(&sy.bar[kEmptyQ]);
+      if (last_use) k.advance(S::kStagesK);
     };
     if (!wait(kFullQ, index & 1)) break;
     fence_proxy_async_smem();  // the helpers' copies, before the tensor cores' reads
     for (int w = 0; ok && w < g.active; ++w) scores(w, g.step0 + 1 == g.step1);
     for (int step = g.step0; ok && step < g.step1; ++step) {
       for (int w = 0; ok && w < g.active; ++w) {
-        if (!wait(kWeightsDone + w, weights_phase[w])) break;
-        weights_phase[w] ^= 1;
+        if (!wait(kWeightsDone + w, (weights_phase >> w) & 1)) break;
+        weights_phase ^= 1u << w;
         const bool first_use = !g.shared || w == 0, last_use = !g.shared || w == 1;
         if (first_use) {
           const bool nodes = has_nodes(g, step);
@@ -519,29 +524,25 @@ __device__ __forceinline__ void issue_products(const TreeAttnArgs& a, Sync& sy, 
           if (!wait((nodes ? kCheckedV : kFullV) + v.slot, (parity >> v.slot) & 1)) break;
           parity ^= 1u << v.slot;
         }
-        const uint8_t* vt = ring_v + v.slot * S::kTileBytes;
+        if (elect_one()) {
+          const uint64_t vd = v_desc + v.slot * kTileStep;
+          const uint32_t first = step > g.step0;
 #pragma unroll
-        for (int kk = 0; kk < kTile / 16; ++kk) {
-          umma_bf16_ts(sy.tmem_base + kOutput + w * kTile,
-                       sy.tmem_base + kScores + w * kTile + kk * 8,
-                       smem_desc_mn_sw128(vt + kk * 2048, kHalfBytes), kIdescO,
-                       step > g.step0 || kk != 0);
+          for (int kk = 0; kk < kTile / 16; ++kk) {
+            umma_bf16_ts(tmem + kOutput + w * kTile, tmem + kScores + w * kTile + kk * 8,
+                         vd + ((kk * 2048) >> 4), kIdescO, kk != 0 ? 1u : first);
+          }
+          if (last_use) umma_commit(&sy.bar[kEmptyV + v.slot]);
+          if (step + 1 == g.step1) umma_commit(&sy.bar[kOutputDone + w]);
         }
-        if (last_use) {
-          umma_commit(&sy.bar[kEmptyV + v.slot]);
-          v.advance(S::kStagesV);
-        }
-        if (step + 1 == g.step1) {
-          umma_commit(&sy.bar[kOutputDone + w]);
-        } else {
-          // the next scores may overwrite these weights: products complete in order
-          scores(w, step + 2 == g.step1);
-        }
+        if (last_use) v.advance(S::kStagesV);
+        // the next scores may overwrite these weights: products complete in order
+        if (step + 1 < g.step1) scores(w, step + 2 == g.step1);
       }
     }
   }
   // every product this thread issued has completed before the TMEM is freed
-  umma_commit(&sy.bar[kDrain]);
+  if (elect_one()) umma_commit(&sy.bar[kDrain]);
   mbar_wait_bounded(&sy.bar[kDrain], 0);
 }
 
@@ -842,7 +843,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool values = warp > kLoadWarp;
       Loader<D> l{a, sy, values ? &map_v : &map_k, values ? ring_v : ring_k, values, lane};
       l.run(at, end);
-    } else if (warp == kMmaWarp && lane == 0) {
+    } else if (warp == kMmaWarp) {
       issue_products<D>(a, sy, q_tiles, ring_k, ring_v, at, end);
     }
   }
@@ -872,6 +873,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kMmaWarp) tmem_dealloc(sy.tmem_base, kTmemColumns);
 }
 
+__device__ __forceinline__ float ld_global_f32(const float* p) {
+  float v;
+  asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+
+__device__ __forceinline__ float4 ld_global_f32x4(const float* p) {
+  float4 v;
+  asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "l"(p));
+  return v;
+}
+
 // Joins the segments of each cut item. A border between two CTAs' shares that lies inside an item
 // is the item's if it is the first of those; each block lists these borders (one thread per border)
 // and takes every gridDim-th unit of 8 rows of one accumulator, a thread 16 bytes of a row. With m
@@ -884,17 +899,23 @@ __global__ void __launch_bounds__(kJoinRows * D / 4) tree_attention_join_kernel(
   using S = Shape<D>;
   constexpr int kBlock = kJoinRows * D / 4;
   constexpr int kUnits = 2 * kTile / kJoinRows;  // per item
-  __shared__ int borders[kMaxCtas];
+  __shared__ int borders[kMaxCtas], lasts[kMaxCtas];
+  __shared__ uint8_t inside[kMaxCtas + 1];  // the border lies inside an item; 2: as its first
   __shared__ int warp_counts[kBlock / kWarpSize];
   const int tid = threadIdx.x, lane = tid % kWarpSize;
-  int items = 0;
-  for (int b0 = 1; b0 < ctas; b0 += kBlock) {
-    const int b = b0 + tid;
-    bool own = false;
-    if (b < ctas && (a.cuts[b * 2].flags & kCutFront)) {
+  for (int b = tid; b <= ctas; b += kBlock) {
+    uint8_t kind = 0;
+    if (b > 0 && b < ctas && (a.cuts[b * 2].flags & kCutFront)) {
       // the segment before the border: the previous CTA's second cut one, else its first
-      own = a.cuts[b * 2 - 1].flags != 0 || !(a.cuts[b * 2 - 2].flags & kCutFront);
+      kind = a.cuts[b * 2 - 1].flags != 0 || !(a.cuts[b * 2 - 2].flags & kCutFront) ? 2 : 1;
     }
+    inside[b] = kind;
+  }
+  __syncthreads();
+  int items = 0;
+  for (int b0 = 0; b0 < ctas; b0 += kBlock) {
+    const int b = b0 + tid;
+    const bool own = b < ctas && inside[b] == 2;
     const unsigned owners = __ballot_sync(0xffffffffu, own);
     if (lane == 0) warp_counts[tid / kWarpSize] = __popc(owners);
     __syncthreads();
@@ -903,7 +924,12 @@ __global__ void __launch_bounds__(kJoinRows * D / 4) tree_attention_join_kernel(
       if (i < tid / kWarpSize) at += warp_counts[i];
       items += warp_counts[i];
     }
-    if (own) borders[at] = b;
+    if (own) {
+      int last = b;
+      while (inside[last + 1] == 1) ++last;
+      borders[at] = b;
+      lasts[at] = last;
+    }
     __syncthreads();
   }
 
@@ -915,33 +941,46 @@ __global__ void __launch_bounds__(kJoinRows * D / 4) tree_attention_join_kernel(
     const int row = unit % (kUnits / 2) * kJoinRows + tid % kJoinRows;
     const Cut& c = a.cuts[first];
     if (unit % (kUnits / 2) * kJoinRows >= c.rows[w]) continue;
-    int last = border;
-    while (last + 1 < ctas && (a.cuts[last * 2].flags & kCutBack)) ++last;
+    const int last = lasts[unit / kUnits];
     const int piece = tid / kJoinRows;
     const auto part = [&](int i) {  // segment i of the item
       const int64_t slot = i == 0 ? first : (border - 1 + i) * 2;
       return a.parts + (slot * 2 + w) * S::kPartFloats;
     };
     const int n = last - border + 2;
-    float top = -kInf;
-#pragma unroll 8
-    for (int i = 0; i < n; ++i) top = fmaxf(top, part(i)[D * kTile + row]);
-    const float base = top == -kInf ? 0.0f : top;
-    float sum = 0.0f;
+    // four segments at a time, all their loads before any use
+    float top = -kInf, sum = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-    for (int i = 0; i < n; ++i) {
-      const float* p = part(i);
-      const float l = p[(D + 1) * kTile + row];
-      const float f = exp2_approx(p[D * kTile + row] - base);
-      const float4 x = *reinterpret_cast<const float4*>(p + (piece * kTile + row) * 4);
-      if (l != 0.0f) {  // a segment of which the node sees nothing has no part
-        sum = fmaf(f, l, sum);
-        o.x = fmaf(f, x.x, o.x);
-        o.y = fmaf(f, x.y, o.y);
-        o.z = fmaf(f, x.z, o.z);
-        o.w = fmaf(f, x.w, o.w);
+    for (int i0 = 0; i0 < n; i0 += kJoinBatch) {
+      float m[kJoinBatch], l[kJoinBatch];
+      float4 x[kJoinBatch];
+#pragma unroll
+      for (int e = 0; e < kJoinBatch; ++e) {
+        const float* p = part(min(i0 + e, n - 1));
+        m[e] = ld_global_f32(p + D * kTile + row);
+        l[e] = ld_global_f32(p + (D + 1) * kTile + row);
+        x[e] = ld_global_f32x4(p + (piece * kTile + row) * 4);
       }
+      float up = top;
+#pragma unroll
+      for (int e = 0; e < kJoinBatch; ++e) up = fmaxf(up, m[e]);
+      const float base = up == -kInf ? 0.0f : up;
+      const float f0 = exp2_approx(top - base);
+      sum *= f0;
+      o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
+#pragma unroll
+      for (int e = 0; e < kJoinBatch; ++e) {
+        // a segment of which the node sees nothing has no part
+        if (i0 + e < n && l[e] != 0.0f) {
+          const float f = exp2_approx(m[e] - base);
+          sum = fmaf(f, l[e], sum);
+          o.x = fmaf(f, x[e].x, o.x);
+          o.y = fmaf(f, x[e].y, o.y);
+          o.z = fmaf(f, x[e].z, o.z);
+          o.w = fmaf(f, x[e].w, o.w);
+        }
+      }
+      top = up;
     }
     if (row >= c.rows[w]) continue;
     const int at_row = c.row0[w] + row;

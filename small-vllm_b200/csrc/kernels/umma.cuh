@@ -18,6 +18,20 @@ namespace svllm::k {
 // Columns of one TMA box: 64 bf16 = 128 bytes, one 128-byte swizzle atom.
 constexpr int kTmaBoxCols = 64;
 
+// True in one lane of the converged warp, the same one every time. Instructions that one thread
+// issues (TMA, tcgen05.mma, commit) take their operands from uniform registers: under this predicate
+// the compiler keeps them there, while under `lane == 0` it moves each of them for every
+// instruction.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(yes));
+  return yes != 0;
+}
+
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int32_t x,
                                             int32_t y, uint64_t* bar) {
   asm volatile(
