@@ -18,14 +18,14 @@
 // lengths. An item cut by a share's border leaves unnormalised partial sums in the workspace, which
 // a second small kernel joins.
 //
-// In a CTA: two warps bring K and V rows through the block table with TMA into 128-byte-swizzled
+// In a CTA: four warps bring K and V rows through the block table with TMA into 128-byte-swizzled
 // tiles (any block size: a page may end anywhere in a tile); one thread issues tcgen05.mma: S = Q K^T into TMEM, then O += P V with P read from TMEM and V as
 // the N-major operand, alternating between two accumulators so that the tensor pipe works on one M
 // tile while the other's softmax runs; two groups of 4 warps do the softmax, one thread per row,
 // and write P (bf16, as the second product takes it) over S. The running maximum is a reference
 // that moves only when a row exceeds it by 2^8, so O in TMEM is seldom rescaled; the sums are fp32
 // and the result does not depend on the reference. Masked scores are replaced after the product.
-// Four helper warps bring the query rows and, since 0 * NaN would reach rows that do not see it,
+// Two helper warps bring the query rows and, since 0 * NaN would reach rows that do not see it,
 // zero the values of V that are not finite in the tiles that hold tree nodes; they are added
 // again, for the rows that see them, at the end.
 #include <cuda_runtime.h>
@@ -42,10 +42,13 @@ namespace {
 
 constexpr int kTile = 128;            // query rows per M tile, cached rows per key tile
 constexpr int kSoftmaxWarps = 8;      // two groups of 4: accumulators 0 and 1
-constexpr int kHelperWarps = 4;       // query rows and the check of V
-constexpr int kMmaWarp = kSoftmaxWarps + kHelperWarps;
-constexpr int kLoadWarp = kMmaWarp + 1;  // K, and the next one V
-constexpr int kThreads = 16 * kWarpSize;  // the last warp only fills the register groups
+constexpr int kHelperWarps = 2;       // query rows and the check of V
+constexpr int kLoaderWarps = 4;       // K and V
+constexpr int kLoadWarp = kSoftmaxWarps + kHelperWarps;
+constexpr int kMmaWarp = kLoadWarp + kLoaderWarps;
+constexpr int kPlanWarp = kMmaWarp + 1;  // lists the CTA's segments, zeroes rows without an item
+constexpr int kThreads = (kPlanWarp + 1) * kWarpSize;
+constexpr int kWarps = kThreads / kWarpSize;
 // Registers per thread after the split of the launch's 512 x 128: the softmax warps hold a row of
 // scores each, 8 x 32 x 192 + 8 x 32 x 64 = 65536.
 constexpr int kSoftmaxRegisters = 192, kOtherRegisters = 64;
@@ -62,10 +65,8 @@ template <int D>
 struct Shape {
   static constexpr int kHalves = D / 64;
   static constexpr int kTileBytes = kHalves * kHalfBytes;
-  static constexpr int kStagesK = D == 128 ? 3 : 6;
-  static constexpr int kStagesV = D == 128 ? 2 : 4;
-  static constexpr size_t kSmem = 1024 + static_cast<size_t>(kTileBytes) *
-                                             (2 + kStagesK + kStagesV);
+  static constexpr int kStages = D == 128 ? 5 : 10;
+  static constexpr size_t kSmem = 1024 + static_cast<size_t>(kTileBytes) * (2 + kStages);
   // partial sums of one accumulator: O as [D / 4][128 rows][4], then the rows' maxima and sums
   static constexpr int kPartFloats = (D + 2) * kTile;
 };
@@ -91,12 +92,15 @@ struct TreeAttnArgs {
   Cut* cuts;                       // [CTAs][2]
   int64_t q_stride;
   int64_t num_blocks;
-  int64_t num_tokens;
-  int64_t num_seqs;
+  int num_tokens;
+  int num_seqs;
   int max_blocks;
+  int max_length;                  // rows that a block table holds
+  int max_nodes;                   // nodes that the mask's words hold
   int block_size;
   Divider page;                    // by the block size
   int group;                       // query heads per KV head
+  Divider by_group;
   int num_kv_heads;
   int cache_slots;
   int box_rows;                    // rows of a TMA box; 1: four rows gathered per instruction
@@ -114,27 +118,26 @@ struct Request {
   bool bad;                           // lengths out of range
 };
 
-__device__ __forceinline__ Request load_request(const TreeAttnArgs& a, int64_t s) {
+__device__ __forceinline__ Request load_request(const TreeAttnArgs& a, int s) {
   Request r{};
-  const int64_t begin = a.query_start_loc[s], end = a.query_start_loc[s + 1];
-  const int64_t length = a.seq_lens[s];
+  const int begin = a.query_start_loc[s], end = a.query_start_loc[s + 1];
+  const int length = a.seq_lens[s];
   if (begin < 0 || end < begin || end > a.num_tokens) {
     r.bad = true;
     return r;
   }
-  r.start = static_cast<int>(begin);
-  r.nodes = static_cast<int>(end - begin);
+  r.start = begin;
+  r.nodes = end - begin;
   if (length == 0) return r;
-  if (length < r.nodes || length > static_cast<int64_t>(a.max_blocks) * a.block_size ||
-      (a.tree_mask != nullptr && r.nodes > 64 * a.mask_words)) {
+  if (length < r.nodes || length > a.max_length || r.nodes > a.max_nodes) {
     r.bad = true;
     return r;
   }
-  r.length = static_cast<int>(length);
-  r.context = r.length - r.nodes;
+  r.length = length;
+  r.context = length - r.nodes;
   if (r.nodes > 0) {
     const int tiles = (r.nodes * a.group + kTile - 1) / kTile;
-    r.steps = (r.length + kTile - 1) / kTile;
+    r.steps = (length + kTile - 1) / kTile;
     r.pairs = tiles / 2;
     r.odd = tiles & 1;
   }
@@ -148,21 +151,25 @@ __device__ __forceinline__ int64_t request_cost(const TreeAttnArgs& a, const Req
 
 // A place on the line: request, item of the request, step of the item.
 struct Place {
-  int64_t s;
-  int item, step;
+  int s, item, step;
 };
 
-__device__ __forceinline__ Place locate(const TreeAttnArgs& a, int64_t s, const Request& r,
+__device__ __forceinline__ int64_t quotient(int64_t n, int d) {
+  return n >> 31 == 0 ? static_cast<uint32_t>(n) / static_cast<uint32_t>(d) : n / d;
+}
+
+
+__device__ __forceinline__ Place locate(const TreeAttnArgs& a, int s, const Request& r,
                                         int64_t at) {
   const int64_t shared = static_cast<int64_t>(a.num_kv_heads) * r.pairs * r.steps;
   Place p{s, 0, 0};
   if (at < shared) {
-    p.item = static_cast<int>(at / r.steps);
-    p.step = static_cast<int>(at % r.steps);
+    p.item = static_cast<int>(quotient(at, r.steps));
+    p.step = static_cast<int>(at - static_cast<int64_t>(p.item) * r.steps);
     return p;
   }
   at -= shared;
-  const int pair = static_cast<int>(at / (2 * r.steps));
+  const int pair = static_cast<int>(quotient(at, 2 * r.steps));
   const int64_t rest = at - static_cast<int64_t>(pair) * 2 * r.steps;
   const bool two = 2 * pair + 1 < a.num_kv_heads;
   p.item = a.num_kv_heads * r.pairs + pair;
@@ -174,80 +181,171 @@ __device__ __forceinline__ Place locate(const TreeAttnArgs& a, int64_t s, const 
   return p;
 }
 
-// A run of steps of one item.
+// A run of steps of one item. The plan warp lists a CTA's segments in a ring; the other warps copy
+// one at a time.
 struct Segment {
-  int64_t s;
-  Request r;
-  bool shared;                   // both accumulators take the same K and V
-  int active;                    // accumulators in use, 1 or 2
+  int s, start, nodes, context, length;  // the request
+  int shared;                    // both accumulators take the same K and V
+  int active;                    // accumulators in use, 1 or 2; 0: the end of the list
   int kv_head[2], row0[2], rows[2];
   int step0, step1;
-  bool front, back;              // cut there
+  int front, back;               // cut there
 };
 
-// The next segment of [at, end); false when there is none.
-__device__ __forceinline__ bool next_segment(const TreeAttnArgs& a, Place& at, const Place& end,
-                                             Segment& g) {
-  while (at.s < a.num_seqs &&
-         (at.s < end.s || (at.s == end.s && (at.item < end.item ||
-                                             (at.item == end.item && at.step < end.step))))) {
-    g.r = load_request(a, at.s);
-    const int shared_items = a.num_kv_heads * g.r.pairs;
-    const int items = g.r.steps == 0 ? 0
-                                     : shared_items + g.r.odd * ((a.num_kv_heads + 1) / 2);
-    if (at.item >= items) {
-      at = Place{at.s + 1, 0, 0};
-      continue;
-    }
-    const int all_rows = g.r.nodes * a.group;
-    g.s = at.s;
-    g.shared = at.item < shared_items;
-    if (g.shared) {
-      g.active = 2;
-      g.kv_head[0] = g.kv_head[1] = at.item / g.r.pairs;
-      g.row0[0] = (at.item % g.r.pairs) * 2 * kTile;
-      g.row0[1] = g.row0[0] + kTile;
-      g.rows[0] = kTile;
-      g.rows[1] = min(kTile, all_rows - g.row0[1]);
-    } else {
-      const int pair = at.item - shared_items;
-      g.kv_head[0] = 2 * pair;
-      g.kv_head[1] = 2 * pair + 1;
-      g.active = g.kv_head[1] < a.num_kv_heads ? 2 : 1;
-      g.row0[0] = g.row0[1] = g.r.pairs * 2 * kTile;
-      g.rows[0] = all_rows - g.row0[0];
-      g.rows[1] = g.active == 2 ? g.rows[0] : 0;
-    }
-    g.step0 = at.step;
-    g.step1 = at.s == end.s && at.item == end.item ? end.step : g.r.steps;
-    g.front = g.step0 > 0;
-    g.back = g.step1 < g.r.steps;
-    at = Place{at.s, at.item + 1, 0};
-    return true;
-  }
-  return false;
-}
-
-// Barriers and flags of one CTA.
-constexpr int kMaxStagesK = 6, kMaxStagesV = 4;
-constexpr int kFullK = 0, kFullV = kFullK + kMaxStagesK, kFullQ = kFullV + kMaxStagesV;
-// A V tile with tree nodes lands on its own barrier, for the helpers, which signal when it is
-// checked; kFullV stands for the others. (A slot's parity counts the uses of one barrier, so every
-// waiter of a barrier has to see all of them.)
-constexpr int kCheckedV = kFullQ + 1, kLandedV = kCheckedV + kMaxStagesV;
-constexpr int kEmptyK = kLandedV + kMaxStagesV, kEmptyV = kEmptyK + kMaxStagesK;
-constexpr int kEmptyQ = kEmptyV + kMaxStagesV;
+// Barriers and flags of one CTA. A V tile with tree nodes lands on its own barrier, for the helpers,
+// which signal when it is checked; kFull stands for all other tiles. (A slot's parity counts the
+// uses of one barrier, so every waiter of a barrier has to see all of them.)
+constexpr int kMaxStages = 10;
+constexpr int kSegments = 4;    // of the list's ring
+constexpr int kFull = 0, kLanded = kFull + kMaxStages;
+constexpr int kChecked = kLanded + kMaxStages, kFullQ = kChecked + kMaxStages;
+constexpr int kEmpty = kFullQ + 1, kEmptyQ = kEmpty + kMaxStages;
 constexpr int kScoresDone = kEmptyQ + 1, kWeightsDone = kScoresDone + 2;
-constexpr int kOutputDone = kWeightsDone + 2, kDrain = kOutputDone + 2, kBarriers = kDrain + 1;
+constexpr int kOutputDone = kWeightsDone + 2, kDrain = kOutputDone + 2;
+constexpr int kListed = kDrain + 1, kRead = kListed + kSegments, kBarriers = kRead + kSegments;
+
+__device__ __forceinline__ int arrivals(int bar) {
+  if (bar < kChecked) return kLoaderWarps;
+  if (bar < kEmpty) return kHelperWarps * kWarpSize;
+  if (bar >= kRead) return kPlanWarp;  // every other warp
+  return bar == kWeightsDone || bar == kWeightsDone + 1 ? 4 * kWarpSize : 1;
+}
 
 struct Sync {
   uint64_t bar[kBarriers];
   uint32_t tmem_base;
   int abort;
   int odd_values[2][4];  // per accumulator and segment modulo 4: V held something not finite
-  int64_t sums[kThreads / kWarpSize];
-  Place place[2];        // this CTA's share
+  int64_t costs[kWarps];  // of the warps' shares of the requests
+  Segment list[kSegments];
 };
+
+// The plan warp: this CTA's share of the line, as segments. `chunk` requests make a warp's share
+// of the costs.
+__device__ __forceinline__ void plan(const TreeAttnArgs& a, Sync& sy, int chunk, int lane) {
+  int64_t upto = lane < kWarps ? sy.costs[lane] : 0;
+#pragma unroll
+  for (int off = 1; off < kWarpSize; off *= 2) {
+    const int64_t up = __shfl_up_sync(0xffffffffu, upto, off);
+    if (lane >= off) upto += up;
+  }
+  const int64_t total = __shfl_sync(0xffffffffu, upto, kWarpSize - 1);
+  // at least two steps each: a shorter share costs more in the join than it saves
+  int64_t share = quotient(total + gridDim.x - 1, gridDim.x);
+  if (share < 2) share = 2;
+  Place places[2];
+#pragma unroll 1
+  for (int e = 0; e < 2; ++e) {
+    const int64_t border = (blockIdx.x + e) * share;
+    Place p{a.num_seqs, 0, 0};
+    if (border < total) {
+      // the warp's share of the requests that holds it, then the request
+      const int c = __ffs(static_cast<int>(__ballot_sync(0xffffffffu, border < upto))) - 1;
+      int64_t before = c > 0 ? __shfl_sync(0xffffffffu, upto, c - 1) : 0;
+#pragma unroll 1
+      for (int s0 = c * chunk;; s0 += kWarpSize) {
+        Request r{};
+        if (s0 + lane < min(a.num_seqs, (c + 1) * chunk)) r = load_request(a, s0 + lane);
+        const int64_t own = request_cost(a, r);
+        int64_t sum = own;
+#pragma unroll
+        for (int off = 1; off < kWarpSize; off *= 2) {
+          const int64_t up = __shfl_up_sync(0xffffffffu, sum, off);
+          if (lane >= off) sum += up;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, border < before + sum);
+        if (past != 0) {
+          const int owner = __ffs(static_cast<int>(past)) - 1;
+          if (lane == owner) p = locate(a, s0 + lane, r, border - (before + sum - own));
+          p.s = __shfl_sync(0xffffffffu, p.s, owner);
+          p.item = __shfl_sync(0xffffffffu, p.item, owner);
+          p.step = __shfl_sync(0xffffffffu, p.step, owner);
+          break;
+        }
+        before += __shfl_sync(0xffffffffu, sum, kWarpSize - 1);
+      }
+    }
+    places[e] = p;
+  }
+  Place at = places[0];
+  const Place end = places[1];
+  Request r{};
+  int loaded = -1;
+  const auto list = [&](int index, const Segment& g) {
+    const int slot = index % kSegments;
+    if (!__all_sync(0xffffffffu, wait_phase(&sy.bar[kRead + slot], (index / kSegments & 1) ^ 1,
+                                            &sy.abort, a.err))) {
+      return false;
+    }
+    if (lane == 0) {
+      sy.list[slot] = g;
+      mbar_arrive(&sy.bar[kListed + slot]);
+    }
+    return true;
+  };
+  int index = 0;
+#pragma unroll 1
+  while (at.s < a.num_seqs &&
+         (at.s < end.s || (at.s == end.s && (at.item < end.item ||
+                                             (at.item == end.item && at.step < end.step))))) {
+    if (at.s != loaded) {
+      r = load_request(a, at.s);
+      loaded = at.s;
+    }
+    const int shared_items = a.num_kv_heads * r.pairs;
+    const int items = r.steps == 0 ? 0 : shared_items + r.odd * ((a.num_kv_heads + 1) / 2);
+    if (at.item >= items) {
+      at = Place{at.s + 1, 0, 0};
+      continue;
+    }
+    Segment g;
+    g.s = at.s;
+    g.start = r.start;
+    g.nodes = r.nodes;
+    g.context = r.context;
+    g.length = r.length;
+    g.shared = at.item < shared_items;
+    const int all_rows = r.nodes * a.group;
+    if (g.shared) {
+      g.active = 2;
+      g.kv_head[0] = g.kv_head[1] = at.item / r.pairs;
+      g.row0[0] = (at.item - g.kv_head[0] * r.pairs) * 2 * kTile;
+      g.row0[1] = g.row0[0] + kTile;
+      g.rows[0] = kTile;
+      g.rows[1] = min(kTile, all_rows - g.row0[1]);
+    } else {
+      g.kv_head[0] = 2 * (at.item - shared_items);
+      g.kv_head[1] = g.kv_head[0] + 1;
+      g.active = g.kv_head[1] < a.num_kv_heads ? 2 : 1;
+      g.row0[0] = g.row0[1] = r.pairs * 2 * kTile;
+      g.rows[0] = all_rows - g.row0[0];
+      g.rows[1] = g.active == 2 ? g.rows[0] : 0;
+    }
+    g.step0 = at.step;
+    g.step1 = at.s == end.s && at.item == end.item ? end.step : r.steps;
+    g.front = g.step0 > 0;
+    g.back = g.step1 < r.steps;
+    if (!list(index, g)) return;
+    ++index;
+    at = Place{at.s, at.item + 1, 0};
+  }
+  Segment none{};
+  list(index, none);
+}
+
+// The list's segment `index`, for a warp that reads them all in order; false at its end.
+__device__ __forceinline__ bool next_segment(const TreeAttnArgs& a, Sync& sy, int index,
+                                             Segment& g) {
+  const int slot = index % kSegments;
+  if (!__all_sync(0xffffffffu, wait_phase(&sy.bar[kListed + slot], index / kSegments & 1,
+                                          &sy.abort, a.err))) {
+    return false;
+  }
+  g = sy.list[slot];
+  __syncwarp();
+  if (threadIdx.x % kWarpSize == 0) mbar_arrive(&sy.bar[kRead + slot]);
+  return g.active > 0;
+}
 
 // A ring of tiles: the slot in use and the parity of its current round.
 struct Ring {
@@ -287,30 +385,31 @@ __device__ __forceinline__ bool drop_odd(uint32_t& w) {
 
 // The V tiles of these steps hold tree nodes.
 __device__ __forceinline__ bool has_nodes(const Segment& g, int step) {
-  return (step + 1) * kTile > g.r.context;
+  return (step + 1) * kTile > g.context;
 }
 
-// One of the two warps that bring K and V: the tiles of one of them, in the order in which the
-// tensor cores take them. Where the block size allows, a TMA box is a run of 8 to 128 rows that no
-// page border can fall into, gcd(block_size, 128); otherwise one instruction gathers 4 rows.
+// One of the warps that bring K and V, tile after tile in the order in which the tensor cores take
+// them: every kLoaderWarps-th TMA instruction of each tile (one costs its issuer some 100 cycles, a
+// tile of 16-row pages has 16). Where the block size allows, a TMA box is a run of 8 to 128 rows
+// that no page border can fall into, gcd(block_size, 128); otherwise an instruction gathers 4 rows.
 template <int D>
 struct Loader {
   using S = Shape<D>;
   const TreeAttnArgs& a;
   Sync& sy;
-  const CUtensorMap* map;
+  const CUtensorMap& map_k;
+  const CUtensorMap& map_v;
   uint8_t* ring;
-  bool values;           // V, else K
-  int lane;
+  int part, lane;        // part 0 .. kLoaderWarps - 1 of every tile
   Ring at{};
   uint64_t used = 0, parity = 0;  // barriers signalled so far, and the parity of their next use
 
   // The cache slot of row j of the request; past its end a slot past the cache, which reads as
   // zeros.
   __device__ __forceinline__ int cache_slot(const Segment& g, int j) const {
-    if (j >= g.r.length) return a.cache_slots;
+    if (j >= g.length) return a.cache_slots;
     const int page = a.page.divide(j);
-    int block = a.block_tables[g.s * a.max_blocks + page];
+    int block = a.block_tables[static_cast<int64_t>(g.s) * a.max_blocks + page];
     if (static_cast<uint64_t>(block) >= static_cast<uint64_t>(a.num_blocks)) {
       raise_error(a.err, kErrBadIndex);  // outside the cache: block 0 is read
       block = 0;
@@ -330,139 +429,169 @@ struct Loader {
     }
   }
 
-  __device__ __forceinline__ bool load(int bar, const int (&rows)[4], int kv_head) {
-    const int empty = values ? kEmptyV : kEmptyK;
-    if (!__all_sync(0xffffffffu, wait_phase(&sy.bar[empty + at.slot], at.phase ^ 1, &sy.abort,
+  // This warp's part of one tile into the ring's next slot.
+  __device__ __forceinline__ bool load(const CUtensorMap* map, int full, const int (&rows)[4],
+                                       int kv_head) {
+    if (!__all_sync(0xffffffffu, wait_phase(&sy.bar[kEmpty + at.slot], at.phase ^ 1, &sy.abort,
                                             a.err))) {
       return false;
     }
-    if (elect_one()) mbar_arrive_expect_tx(&sy.bar[bar], S::kTileBytes);
-    __syncwarp();
+    // boxes (or groups of 4 rows) part, part + kLoaderWarps, ..., both halves of a row together
+    const int rows_each = a.box_rows > 1 ? a.box_rows : 4;
+    const int count = kTile / rows_each;
+    const int mine = (count - part + kLoaderWarps - 1) / kLoaderWarps;
+    uint64_t* bar = &sy.bar[full + at.slot];
     const uint32_t dst = smem_addr(ring + at.slot * S::kTileBytes);
     const int column = kv_head * D;
+    if (elect_one()) mbar_arrive_expect_tx(bar, mine * rows_each * 128 * S::kHalves);
+    __syncwarp();
     if (a.box_rows > 1) {
-      const int boxes = kTile / a.box_rows;
-      const uint32_t box_bytes = a.box_rows * 128;
-      for (int i = 0; i < boxes; ++i) {
+#pragma unroll 1
+      for (int i = part; i < count; i += kLoaderWarps) {
         const int row = __shfl_sync(0xffffffffu, rows[0], i);
         if (elect_one()) {
 #pragma unroll
           for (int h = 0; h < S::kHalves; ++h) {
-            tma_load_2d(dst + h * kHalfBytes + i * box_bytes, map, column + h * kTmaBoxCols, row,
-                        &sy.bar[bar]);
+            tma_load_2d(dst + h * kHalfBytes + i * rows_each * 128, map,
+                        column + h * kTmaBoxCols, row, bar);
           }
         }
       }
     } else {
-#pragma unroll 4
-      for (int i = 0; i < kTile / 4; ++i) {
+#pragma unroll 1
+      for (int i = part; i < kTile / 4; i += kLoaderWarps) {
         int32_t y[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] = __shfl_sync(0xffffffffu, rows[e], i);
         if (elect_one()) {
 #pragma unroll
           for (int h = 0; h < S::kHalves; ++h) {
-            tma_gather4(dst + h * kHalfBytes + i * 512, map, column + h * kTmaBoxCols, y,
-                        &sy.bar[bar]);
+            tma_gather4(dst + h * kHalfBytes + i * 512, map, column + h * kTmaBoxCols, y, bar);
           }
         }
       }
     }
-    used |= uint64_t{1} << bar;
-    parity ^= uint64_t{1} << bar;
-    at.advance(values ? S::kStagesV : S::kStagesK);
+    used |= uint64_t{1} << (full + at.slot);
+    parity ^= uint64_t{1} << (full + at.slot);
+    at.advance(S::kStages);
     return true;
   }
 
-  __device__ __forceinline__ void run(Place place, const Place end) {
+  __device__ __forceinline__ void run() {
     Segment g;
     bool ok = true;
-    while (ok && next_segment(a, place, end, g)) {
-      int now[4], next[4];
-      find_rows(g, g.step0, now);
-      for (int step = g.step0; ok && step < g.step1; ++step) {
+#pragma unroll 1
+    for (int index = 0; ok && next_segment(a, sy, index, g); ++index) {
+      const int heads = g.shared ? 1 : g.active;
+      int before[4] = {}, now[4] = {}, next[4] = {};
+#pragma unroll 1
+      for (int step = g.step0 - 1; ok && step <= g.step1; ++step) {
         find_rows(g, step + 1, next);
-        const int full = !values ? kFullK : has_nodes(g, step) ? kLandedV : kFullV;
-        ok = load(full + at.slot, now, g.kv_head[0]);
-        if (ok && !g.shared && g.active == 2) ok = load(full + at.slot, now, g.kv_head[1]);
+        // V of the step before, then K, head by head
+#pragma unroll 1
+        for (int i = 0; ok && step >= g.step0 && i < 2 * heads; ++i) {
+          const bool values = i % 2 == 0;
+          if (values ? step == g.step0 : step == g.step1) continue;
+          int rows[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) now[i] = next[i];
+          for (int e = 0; e < 4; ++e) rows[e] = values ? before[e] : now[e];
+          ok = load(values ? &map_v : &map_k,
+                    values && has_nodes(g, step - 1) ? kLanded : kFull, rows,
+                    i < 2 ? g.kv_head[0] : g.kv_head[1]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          before[e] = now[e];
+          now[e] = next[e];
+        }
       }
     }
     // every copy has landed before the CTA exits: the last use of each barrier
-    for (int bar = 0; bar < kEmptyK; ++bar) {
+#pragma unroll 1
+    for (int bar = 0; bar < kChecked; ++bar) {
       if ((used >> bar) & 1) mbar_wait_bounded(&sy.bar[bar], ((parity >> bar) & 1) ^ 1);
     }
   }
 };
-static_assert(kEmptyK <= 64, "one bit per barrier that a copy may signal");
+static_assert(kChecked <= 64, "one bit per barrier that a copy may signal");
 
-// The four helper warps: the query rows of each segment, and the V tiles that hold tree nodes,
+// The helper warps: the query rows of each segment, and the V tiles that hold tree nodes,
 // whose values that are not finite are zeroed before the tensor cores see them.
 template <int D>
 __device__ __forceinline__ void help(const TreeAttnArgs& a, Sync& sy, uint8_t* q_tiles,
-                                     uint8_t* ring_v, int warp, int lane, Place at,
-                                     const Place end) {
+                                     uint8_t* ring, int warp, int lane) {
   using S = Shape<D>;
   constexpr int kLanes = D / 8;  // lanes per query row: 16 bytes each
   constexpr int kRowsAtOnce = kWarpSize / kLanes;
   const auto wait = [&](int bar, uint32_t parity) {
     return __all_sync(0xffffffffu, wait_phase(&sy.bar[bar], parity, &sy.abort, a.err));
   };
-  Ring v;
-  uint32_t landed = 0;  // parity of the next use of each V slot's barrier
+  Ring ring_at;
+  uint32_t landed = 0;  // parity of the next use of each slot's barrier
   Segment g;
   bool ok = true;
-  for (int index = 0; ok && next_segment(a, at, end, g); ++index) {
+#pragma unroll 1
+  for (int index = 0; ok && next_segment(a, sy, index, g); ++index) {
     ok = wait(kEmptyQ, (index & 1) ^ 1);
     if (!ok) break;
+#pragma unroll 1
     for (int w = 0; w < g.active; ++w) {
-      // row = node * group + head of the KV head
-      const int r = warp * kWarpSize + lane;
-      const int row = g.row0[w] + r;
-      const int64_t offset =
-          r < g.rows[w] ? (g.r.start + row / a.group) * a.q_stride +
-                              (static_cast<int64_t>(g.kv_head[w]) * a.group + row % a.group) * D
-                        : -1;
-      const uint32_t base = smem_addr(q_tiles + w * S::kTileBytes);
-      const int c = lane % kLanes;
-      const auto* src = static_cast<const __nv_bfloat16*>(a.q) + c * 8;
+#pragma unroll 1
+      for (int r0 = warp * kWarpSize; r0 < kTile; r0 += kHelperWarps * kWarpSize) {
+        // row = node * group + head of the KV head
+        const int row = g.row0[w] + r0 + lane;
+        const int node = a.by_group.divide(row);
+        const int64_t offset =
+            r0 + lane < g.rows[w]
+                ? (g.start + node) * a.q_stride +
+                      (static_cast<int64_t>(g.kv_head[w] - node) * a.group + row) * D
+                : -1;
+        const int c = lane % kLanes;
+        const uint32_t base = smem_addr(q_tiles + w * S::kTileBytes) + (c / 8) * kHalfBytes;
+        const auto* src = static_cast<const __nv_bfloat16*>(a.q) + c * 8;
 #pragma unroll 4
-      for (int i = 0; i < kWarpSize / kRowsAtOnce; ++i) {
-        const int x = i * kRowsAtOnce + lane / kLanes;
-        const int64_t from = __shfl_sync(0xffffffffu, offset, x);
-        cp_async16(base + (c / 8) * kHalfBytes + (warp * kWarpSize + x) * 128 +
-                       (((c % 8) ^ (x & 7)) << 4),
-                   src + (from < 0 ? 0 : from), from >= 0);
+        for (int i = 0; i < kWarpSize / kRowsAtOnce; ++i) {
+          const int x = i * kRowsAtOnce + lane / kLanes;
+          const int64_t from = __shfl_sync(0xffffffffu, offset, x);
+          cp_async16(base + (r0 + x) * 128 + (((c % 8) ^ (x & 7)) << 4),
+                     src + (from < 0 ? 0 : from), from >= 0);
+        }
       }
     }
     cp_async_arrive(&sy.bar[kFullQ]);
-    for (int step = g.step0; ok && step < g.step1; ++step) {
+#pragma unroll 1
+    for (int step = g.step0; ok && step <= g.step1; ++step) {
+#pragma unroll 1
       for (int w = 0; ok && w < (g.shared ? 1 : g.active); ++w) {
-        if (has_nodes(g, step)) {
-          ok = wait(kLandedV + v.slot, (landed >> v.slot) & 1);
-          if (!ok) break;
-          landed ^= 1u << v.slot;
-          auto* tile = reinterpret_cast<uint4*>(ring_v + v.slot * S::kTileBytes);
-          bool odd = false;
+        if (step > g.step0) {
+          if (has_nodes(g, step - 1)) {
+            ok = wait(kLanded + ring_at.slot, (landed >> ring_at.slot) & 1);
+            if (!ok) break;
+            landed ^= 1u << ring_at.slot;
+            auto* tile = reinterpret_cast<uint4*>(ring + ring_at.slot * S::kTileBytes);
+            const int end_row = g.length - (step - 1) * kTile;
+            bool odd = false;
 #pragma unroll 4
-          for (int i = warp * kWarpSize + lane; i < S::kTileBytes / 16; i += 4 * kWarpSize) {
-            uint4 x = tile[i];
-            if (step * kTile + i * 16 % kHalfBytes / 128 >= g.r.length) {
-              tile[i] = make_uint4(0, 0, 0, 0);  // behind the request's end, whatever it holds
-            } else if (drop_odd(x.x) | drop_odd(x.y) | drop_odd(x.z) | drop_odd(x.w)) {
-              tile[i] = x;
-              odd = true;
+            for (int i = warp * kWarpSize + lane; i < S::kTileBytes / 16;
+                 i += kHelperWarps * kWarpSize) {
+              uint4 x = tile[i];
+              if (i * 16 % kHalfBytes / 128 >= end_row) {
+                tile[i] = make_uint4(0, 0, 0, 0);  // behind the request's end, whatever it holds
+              } else if (drop_odd(x.x) | drop_odd(x.y) | drop_odd(x.z) | drop_odd(x.w)) {
+                tile[i] = x;
+                odd = true;
+              }
             }
+            if (odd) {
+              sy.odd_values[w][index & 3] = 1;
+              if (g.shared) sy.odd_values[1][index & 3] = 1;
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&sy.bar[kChecked + ring_at.slot]);
           }
-          if (odd) {
-            sy.odd_values[w][index & 3] = 1;
-            if (g.shared) sy.odd_values[1][index & 3] = 1;
-          }
-          fence_proxy_async_smem();
-          mbar_arrive(&sy.bar[kCheckedV + v.slot]);
+          ring_at.advance(S::kStages);
         }
-        v.advance(S::kStagesV);
+        if (step < g.step1) ring_at.advance(S::kStages);  // a K tile
       }
     }
   }
@@ -471,73 +600,77 @@ __device__ __forceinline__ void help(const TreeAttnArgs& a, Sync& sy, uint8_t* q
 
 // The warp that issues the matrix products, one lane of it each of them.
 template <int D>
-__device__ __forceinline__ void issue_products(const TreeAttnArgs& a, Sync& sy, const uint8_t* q_tiles,
-                               const uint8_t* ring_k, const uint8_t* ring_v, Place at,
-                               const Place end) {
+__device__ __forceinline__ void issue_products(const TreeAttnArgs& a, Sync& sy,
+                                               const uint8_t* q_tiles, const uint8_t* ring) {
   using S = Shape<D>;
   constexpr uint32_t kIdescS = idesc_bf16(kTile, kTile);
   constexpr uint32_t kIdescO = idesc_bf16(kTile, D) | kIdescBMajorN;
   // descriptors of the first tile of each kind; a tile further on, the start address moves
   constexpr uint64_t kTileStep = S::kTileBytes >> 4;
-  const uint64_t q_desc = smem_desc_k_sw128(q_tiles), k_desc = smem_desc_k_sw128(ring_k);
-  const uint64_t v_desc = smem_desc_mn_sw128(ring_v, kHalfBytes);
+  const uint64_t q_desc = smem_desc_k_sw128(q_tiles), k_desc = smem_desc_k_sw128(ring);
+  const uint64_t v_desc = smem_desc_mn_sw128(ring, kHalfBytes);
   const uint32_t tmem = sy.tmem_base;
-  Ring k, v;
-  uint32_t weights_phase = 0;  // one bit per accumulator
+  Ring ring_at;
+  int k_slot = 0, v_slot = 0;           // the tiles in use
+  uint32_t full = 0, checked = 0;       // parity of the next use of each slot's barriers
+  uint32_t weights_phase = 0;           // one bit per accumulator
   bool ok = true;
   const auto wait = [&](int bar, uint32_t parity) {
     ok = __all_sync(0xffffffffu, wait_phase(&sy.bar[bar], parity, &sy.abort, a.err));
     tc_fence_after();
     return ok;
   };
-  uint32_t full_v = 0, checked_v = 0;  // parity of the next use of each V slot's barriers
+  // the ring's next tile
+  const auto take = [&](bool nodes, int& slot) {
+    slot = ring_at.slot;
+    uint32_t& parity = nodes ? checked : full;
+    if (!wait((nodes ? kChecked : kFull) + slot, (parity >> slot) & 1)) return false;
+    parity ^= 1u << slot;
+    ring_at.advance(S::kStages);
+    return true;
+  };
   Segment g;
-  for (int index = 0; ok && next_segment(a, at, end, g); ++index) {
-    const auto scores = [&](int w, bool last) {
-      const bool first_use = !g.shared || w == 0, last_use = !g.shared || w == 1;
-      if (first_use && !wait(kFullK + k.slot, k.phase)) return;
-      if (elect_one()) {
-        const uint64_t qd = q_desc + w * kTileStep;
-        const uint64_t kd = k_desc + k.slot * kTileStep;
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint64_t step = ((kk / 4) * kHalfBytes + (kk % 4) * 32) >> 4;
-          umma_bf16(tmem + kScores + w * kTile, qd + step, kd + step, kIdescS, kk != 0);
-        }
-        umma_commit(&sy.bar[kScoresDone + w]);
-        if (last_use) umma_commit(&sy.bar[kEmptyK + k.slot]);
-        if (last && w == g.active - 1) umma_commit(&sy.bar[kEmptyQ]);
-      }
-      if (last_use) k.advance(S::kStagesK);
-    };
+#pragma unroll 1
+  for (int index = 0; ok && next_segment(a, sy, index, g); ++index) {
     if (!wait(kFullQ, index & 1)) break;
     fence_proxy_async_smem();  // the helpers' copies, before the tensor cores' reads
-    for (int w = 0; ok && w < g.active; ++w) scores(w, g.step0 + 1 == g.step1);
-    for (int step = g.step0; ok && step < g.step1; ++step) {
+#pragma unroll 1
+    for (int step = g.step0 - 1; ok && step < g.step1; ++step) {
+#pragma unroll 1
       for (int w = 0; ok && w < g.active; ++w) {
-        if (!wait(kWeightsDone + w, (weights_phase >> w) & 1)) break;
-        weights_phase ^= 1u << w;
         const bool first_use = !g.shared || w == 0, last_use = !g.shared || w == 1;
-        if (first_use) {
-          const bool nodes = has_nodes(g, step);
-          uint32_t& parity = nodes ? checked_v : full_v;
-          if (!wait((nodes ? kCheckedV : kFullV) + v.slot, (parity >> v.slot) & 1)) break;
-          parity ^= 1u << v.slot;
-        }
-        if (elect_one()) {
-          const uint64_t vd = v_desc + v.slot * kTileStep;
-          const uint32_t first = step > g.step0;
+        if (step >= g.step0) {
+          if (!wait(kWeightsDone + w, (weights_phase >> w) & 1)) break;
+          weights_phase ^= 1u << w;
+          if (first_use && !take(has_nodes(g, step), v_slot)) break;
+          if (elect_one()) {
+            const uint64_t vd = v_desc + v_slot * kTileStep;
+            const uint32_t first = step > g.step0;
 #pragma unroll
-          for (int kk = 0; kk < kTile / 16; ++kk) {
-            umma_bf16_ts(tmem + kOutput + w * kTile, tmem + kScores + w * kTile + kk * 8,
-                         vd + ((kk * 2048) >> 4), kIdescO, kk != 0 ? 1u : first);
+            for (int kk = 0; kk < kTile / 16; ++kk) {
+              umma_bf16_ts(tmem + kOutput + w * kTile, tmem + kScores + w * kTile + kk * 8,
+                           vd + ((kk * 2048) >> 4), kIdescO, kk != 0 ? 1u : first);
+            }
+            if (last_use) umma_commit(&sy.bar[kEmpty + v_slot]);
+            if (step + 1 == g.step1) umma_commit(&sy.bar[kOutputDone + w]);
           }
-          if (last_use) umma_commit(&sy.bar[kEmptyV + v.slot]);
-          if (step + 1 == g.step1) umma_commit(&sy.bar[kOutputDone + w]);
         }
-        if (last_use) v.advance(S::kStagesV);
-        // the next scores may overwrite these weights: products complete in order
-        if (step + 1 < g.step1) scores(w, step + 2 == g.step1);
+        if (step + 1 < g.step1) {
+          // the next step's scores; they may overwrite these weights: products complete in order
+          if (first_use && !take(false, k_slot)) break;
+          if (elect_one()) {
+            const uint64_t qd = q_desc + w * kTileStep;
+            const uint64_t kd = k_desc + k_slot * kTileStep;
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint64_t step_k = ((kk / 4) * kHalfBytes + (kk % 4) * 32) >> 4;
+              umma_bf16(tmem + kScores + w * kTile, qd + step_k, kd + step_k, kIdescS, kk != 0);
+            }
+            umma_commit(&sy.bar[kScoresDone + w]);
+            if (last_use) umma_commit(&sy.bar[kEmpty + k_slot]);
+            if (step + 2 == g.step1 && w == g.active - 1) umma_commit(&sy.bar[kEmptyQ]);
+          }
+        }
       }
     }
   }
@@ -546,29 +679,43 @@ __device__ __forceinline__ void issue_products(const TreeAttnArgs& a, Sync& sy, 
   mbar_wait_bounded(&sy.bar[kDrain], 0);
 }
 
-// Which of the 32 cached rows from j on a node sees, as bits.
-__device__ __forceinline__ uint32_t visible32(const TreeAttnArgs& a, const Request& r,
-                                              const int64_t* mask, int node, int j) {
-  const int rel = j - r.context;  // node index of row j
-  const int limit = a.tree_mask == nullptr ? min(r.nodes, node + 1) : r.nodes;
-  uint32_t bits = ~0u;
-  if (rel + 32 > 0 && mask != nullptr) {
-    // 32 bits of the mask from bit `rel` on, ones for the context before it
-    const int lo = rel >> 6;
-    const uint64_t w0 = lo >= 0 && lo < a.mask_words ? static_cast<uint64_t>(mask[lo])
-                        : lo < 0                     ? ~uint64_t{0}
-                                                     : 0;
-    const uint64_t w1 = lo + 1 < a.mask_words ? static_cast<uint64_t>(mask[lo + 1]) : 0;
-    const int sh = rel & 63;
-    bits = static_cast<uint32_t>(sh == 0 ? w0 : (w0 >> sh) | (w1 << (64 - sh)));
+// Whether a node sees its request's row j.
+__device__ __forceinline__ bool sees(const Segment& g, const int64_t* mask, int node, int j) {
+  const int rel = j - g.context;
+  if (rel < 0 || mask == nullptr) return rel <= node;
+  return (static_cast<uint64_t>(mask[rel >> 6]) >> (rel & 63)) & 1;
+}
+
+// Which of the 128 cached rows from j on a node sees, as bits.
+__device__ __forceinline__ void visible(const TreeAttnArgs& a, const Segment& g,
+                                        const int64_t* mask, int node, int j,
+                                        uint64_t (&bits)[2]) {
+  const int rel = j - g.context;  // node index of row j
+  const int limit = mask == nullptr ? min(g.nodes, node + 1) : g.nodes;
+  bits[0] = bits[1] = ~uint64_t{0};
+  if (rel + kTile > 0 && mask != nullptr) {
+    // 128 bits of the mask from bit `rel` on, ones for the context before it
+    const int lo = rel >> 6, sh = rel & 63;
+    uint64_t w[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      w[i] = lo + i < 0                ? ~uint64_t{0}
+             : lo + i < a.mask_words ? static_cast<uint64_t>(mask[lo + i])
+                                     : 0;
+    }
+    bits[0] = sh == 0 ? w[0] : (w[0] >> sh) | (w[1] << (64 - sh));
+    bits[1] = sh == 0 ? w[1] : (w[1] >> sh) | (w[2] << (64 - sh));
   }
-  const int left = limit - rel;  // rows from j on before the end
-  return left >= 32 ? bits : left <= 0 ? 0u : bits & ((1u << left) - 1);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int left = limit - rel - 64 * i;  // rows before the end
+    if (left < 64) bits[i] = left <= 0 ? 0 : bits[i] & ((uint64_t{1} << left) - 1);
+  }
 }
 
 // Softmax and epilogue of accumulator w; this thread owns row `row` of the tile.
 template <int D>
-__device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w, Place at, const Place end) {
+__device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w) {
   using S = Shape<D>;
   const int quarter = (threadIdx.x / kWarpSize) % 4;
   const int row = quarter * kWarpSize + threadIdx.x % kWarpSize;
@@ -578,16 +725,18 @@ __device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w, 
   const float kInf = __builtin_huge_valf();
   uint32_t scores_phase = 0, output_phase = 0;
   Segment g;
-  for (int index = 0; next_segment(a, at, end, g); ++index) {
+#pragma unroll 1
+  for (int index = 0; next_segment(a, sy, index, g); ++index) {
     if (threadIdx.x % (4 * kWarpSize) == 0) sy.odd_values[w][(index + 2) & 3] = 0;
     if (w >= g.active) continue;
     const bool any = quarter * kWarpSize < g.rows[w];  // the warp holds rows of the request
     const int at_row = g.row0[w] + (row < g.rows[w] ? row : 0);
-    const int node = at_row / a.group;
-    const int64_t token = g.r.start + node;
+    const int node = a.by_group.divide(at_row);
+    const int64_t token = g.start + node;
     const int64_t* mask =
         a.tree_mask == nullptr ? nullptr : a.tree_mask + token * a.mask_words;
     float ref = -kInf, sum = 0.0f;
+#pragma unroll 1
     for (int step = g.step0; step < g.step1; ++step) {
       // the warp leaves together: the TMEM loads below are collective
       if (!__all_sync(0xffffffffu, wait_phase(&sy.bar[kScoresDone + w], scores_phase, &sy.abort,
@@ -597,15 +746,17 @@ __device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w, 
       scores_phase ^= 1;
       tc_fence_after();
       if (any) {
-        const bool masked = (step + 1) * kTile > g.r.context;
+        const bool masked = (step + 1) * kTile > g.context;
         uint32_t x[4][32];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_load32(scores + 32 * c, x[c]);
         tmem_wait_load();
         if (masked) {
+          uint64_t bits[2];
+          visible(a, g, mask, node, step * kTile, bits);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            const uint32_t see = visible32(a, g.r, mask, node, step * kTile + 32 * c);
+            const auto see = static_cast<uint32_t>(bits[c / 2] >> (32 * (c % 2)));
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               if (!((see >> i) & 1)) x[c][i] = __float_as_uint(-kInf);
@@ -684,7 +835,7 @@ __device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w, 
     if (cut && threadIdx.x % (4 * kWarpSize) == 0 && w == 0) {
       Cut& c = a.cuts[blockIdx.x * 2 + slot];
       c.flags = kCut | (g.front ? kCutFront : 0) | (g.back ? kCutBack : 0);
-      c.token0 = g.r.start;
+      c.token0 = g.start;
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         c.kv_head[x] = g.kv_head[x];
@@ -697,7 +848,7 @@ __device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w, 
       const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
       __nv_bfloat16* out =
           static_cast<__nv_bfloat16*>(a.out) +
-          ((token * a.num_kv_heads + g.kv_head[w]) * a.group + at_row % a.group) * D;
+          ((token * a.num_kv_heads + g.kv_head[w] - node) * a.group + at_row) * D;
 #pragma unroll 1
       for (int c = 0; c < D; c += 16) {
         uint32_t x[16];
@@ -707,12 +858,13 @@ __device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w, 
         for (int i = 0; i < 16; ++i) o[i] = __uint_as_float(x[i]);
         if (odd && row < g.rows[w]) {
           // V values that are not finite, of the rows this node sees: the weights are positive
-          const int first = max(g.step0, g.r.context / kTile) * kTile;
-          const int last = min(g.step1 * kTile, g.r.length);
+          const int first = max(g.step0, g.context / kTile) * kTile;
+          const int last = min(g.step1 * kTile, g.length);
+#pragma unroll 1
           for (int j = first; j < last; ++j) {
-            if (!(visible32(a, g.r, mask, node, j) & 1)) continue;
+            if (!sees(g, mask, node, j)) continue;
             const int page = a.page.divide(j);
-            int64_t block = a.block_tables[g.s * a.max_blocks + page];
+            int64_t block = a.block_tables[static_cast<int64_t>(g.s) * a.max_blocks + page];
             if (block < 0 || block >= a.num_blocks) block = 0;
             const auto* v = static_cast<const uint16_t*>(a.v_cache) +
                             ((block * a.block_size + (j - page * a.block_size)) *
@@ -749,6 +901,27 @@ __device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w, 
   }
 }
 
+// Rows that no item covers are zero: those of requests that were not served, and what lies behind
+// the last. One warp per CTA, every gridDim-th request or row.
+__device__ __forceinline__ void fill_rest(const TreeAttnArgs& a, int64_t row_vecs, int lane) {
+  uint4* out = static_cast<uint4*>(a.out);
+  for (int s = blockIdx.x; s < a.num_seqs; s += gridDim.x) {
+    const Request r = load_request(a, s);
+    if (r.bad && lane == 0) raise_error(a.err, kErrBadIndex);
+    if (r.steps > 0) continue;
+    for (int64_t i = lane; i < static_cast<int64_t>(r.nodes) * row_vecs; i += kWarpSize) {
+      st_global_v4(out + r.start * row_vecs + i, make_uint4(0, 0, 0, 0));
+    }
+  }
+  int64_t tail = a.query_start_loc[a.num_seqs];
+  if (tail < 0) tail = 0;
+  for (int64_t t = tail + blockIdx.x; t < a.num_tokens; t += gridDim.x) {
+    for (int64_t i = lane; i < row_vecs; i += kWarpSize) {
+      st_global_v4(out + t * row_vecs + i, make_uint4(0, 0, 0, 0));
+    }
+  }
+}
+
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
     tree_attention_kernel(const __grid_constant__ CUtensorMap map_k,
@@ -758,112 +931,51 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   __shared__ Sync sy;
   uint8_t* q_tiles = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
-  uint8_t* ring_k = q_tiles + 2 * S::kTileBytes;
-  uint8_t* ring_v = ring_k + S::kStagesK * S::kTileBytes;
+  uint8_t* ring = q_tiles + 2 * S::kTileBytes;
   const int tid = threadIdx.x;
   const int warp = tid / kWarpSize, lane = tid % kWarpSize;
 
-  if (tid == 0) {
-    for (int i = 0; i < kBarriers; ++i) {
-      const bool helpers = i >= kFullQ && i < kLandedV;
-      const bool weights = i == kWeightsDone || i == kWeightsDone + 1;
-      mbar_init(&sy.bar[i], helpers || weights ? 4 * kWarpSize : 1);
-    }
+  if (tid < kBarriers) {
+    mbar_init(&sy.bar[tid], arrivals(tid));
     fence_mbar_init();
+  }
+  if (tid == 0) {
     sy.abort = 0;
     for (int i = 0; i < 8; ++i) sy.odd_values[i / 4][i % 4] = 0;
-    sy.place[0] = sy.place[1] = Place{a.num_seqs, 0, 0};
     a.cuts[blockIdx.x * 2].flags = 0;
     a.cuts[blockIdx.x * 2 + 1].flags = 0;
   }
   if (warp == kMmaWarp) tmem_alloc(&sy.tmem_base, kTmemColumns);
 
-  // this CTA's share of the line: its length, then the requests that hold the share's two ends
-  Request r{};
-  if (tid < a.num_seqs) r = load_request(a, tid);
-  int64_t cost = request_cost(a, r);
-  for (int64_t s = tid + kThreads; s < a.num_seqs; s += kThreads) {
+  // the line's length: every warp adds up a share of the requests
+  const int chunk = (a.num_seqs + kWarps - 1) / kWarps;
+  int64_t cost = 0;
+#pragma unroll 1
+  for (int s = warp * chunk + lane; s < min(a.num_seqs, (warp + 1) * chunk); s += kWarpSize) {
     cost += request_cost(a, load_request(a, s));
   }
 #pragma unroll
   for (int off = 16; off > 0; off /= 2) cost += __shfl_xor_sync(0xffffffffu, cost, off);
-  if (lane == 0) sy.sums[warp] = cost;
+  if (lane == 0) sy.costs[warp] = cost;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  int64_t total = 0;
-#pragma unroll
-  for (int i = 0; i < kThreads / kWarpSize; ++i) total += sy.sums[i];
-  // at least two steps each: a shorter share costs more in the join than it saves
-  int64_t share = (total + gridDim.x - 1) / gridDim.x;
-  if (share < 2) share = 2;
-  const int64_t ends[2] = {blockIdx.x * share, (blockIdx.x + 1) * share};
-  int64_t before = 0;
-  for (int64_t base = 0; base < a.num_seqs; base += kThreads) {
-    if (base > 0) {
-      r = Request{};
-      if (base + tid < a.num_seqs) r = load_request(a, base + tid);
-    }
-    const int64_t own = request_cost(a, r);
-    int64_t upto = own;
-#pragma unroll
-    for (int off = 1; off < kWarpSize; off *= 2) {
-      const int64_t up = __shfl_up_sync(0xffffffffu, upto, off);
-      if (lane >= off) upto += up;
-    }
-    __syncthreads();  // sy.sums has been read
-    if (lane == kWarpSize - 1) sy.sums[warp] = upto;
-    __syncthreads();
-    int64_t chunk = 0;
-#pragma unroll
-    for (int i = 0; i < kThreads / kWarpSize; ++i) {
-      if (i < warp) upto += sy.sums[i];
-      chunk += sy.sums[i];
-    }
-    upto += before;
-    before += chunk;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      if (ends[e] >= upto - own && ends[e] < upto) {
-        sy.place[e] = locate(a, base + tid, r, ends[e] - (upto - own));
-      }
-    }
-  }
-  __syncthreads();
-  const Place at = sy.place[0], end = sy.place[1];
 
   if (warp < kSoftmaxWarps) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
-    softmax<D>(a, sy, warp / 4, at, end);
+    softmax<D>(a, sy, warp / 4);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
-    if (warp < kMmaWarp) {
-      help<D>(a, sy, q_tiles, ring_v, warp - kSoftmaxWarps, lane, at, end);
-    } else if (warp == kLoadWarp || warp == kLoadWarp + 1) {
-      const bool values = warp > kLoadWarp;
-      Loader<D> l{a, sy, values ? &map_v : &map_k, values ? ring_v : ring_k, values, lane};
-      l.run(at, end);
+    if (warp < kLoadWarp) {
+      help<D>(a, sy, q_tiles, ring, warp - kSoftmaxWarps, lane);
+    } else if (warp < kMmaWarp) {
+      Loader<D> l{a, sy, map_k, map_v, ring, warp - kLoadWarp, lane};
+      l.run();
     } else if (warp == kMmaWarp) {
-      issue_products<D>(a, sy, q_tiles, ring_k, ring_v, at, end);
-    }
-  }
-
-  // rows that no item covers are zero: requests that were not served, and what lies behind the last
-  const int64_t row_vecs = static_cast<int64_t>(a.num_kv_heads) * a.group * D / 8;
-  uint4* out = static_cast<uint4*>(a.out);
-  for (int64_t s = blockIdx.x; s < a.num_seqs; s += gridDim.x) {
-    const Request r = load_request(a, s);
-    if (r.bad && tid == 0) raise_error(a.err, kErrBadIndex);
-    if (r.steps > 0) continue;
-    for (int64_t i = tid; i < r.nodes * row_vecs; i += kThreads) {
-      st_global_v4(out + r.start * row_vecs + i, make_uint4(0, 0, 0, 0));
-    }
-  }
-  int64_t tail = a.query_start_loc[a.num_seqs];
-  if (tail < 0) tail = 0;
-  for (int64_t t = tail + blockIdx.x; t < a.num_tokens; t += gridDim.x) {
-    for (int64_t i = tid; i < row_vecs; i += kThreads) {
-      st_global_v4(out + t * row_vecs + i, make_uint4(0, 0, 0, 0));
+      issue_products<D>(a, sy, q_tiles, ring);
+    } else {
+      plan(a, sy, chunk, lane);
+      fill_rest(a, static_cast<int64_t>(a.num_kv_heads) * a.group * D / 8, lane);
     }
   }
 
@@ -893,7 +1005,7 @@ __device__ __forceinline__ float4 ld_global_f32x4(const float* p) {
 // and l the maxima and sums of the segments, M the largest m:
 //   o = sum 2^(m - M) O / sum 2^(m - M) l.
 template <int D>
-__global__ void __launch_bounds__(kJoinRows * D / 4) tree_attention_join_kernel(
+__global__ void __launch_bounds__(kJoinRows * D / 4, 1280 / (kJoinRows * D / 4)) tree_attention_join_kernel(
     const TreeAttnArgs a, int ctas) {
   grid_dependency_sync();
   using S = Shape<D>;
@@ -956,10 +1068,14 @@ __global__ void __launch_bounds__(kJoinRows * D / 4) tree_attention_join_kernel(
       float4 x[kJoinBatch];
 #pragma unroll
       for (int e = 0; e < kJoinBatch; ++e) {
-        const float* p = part(min(i0 + e, n - 1));
-        m[e] = ld_global_f32(p + D * kTile + row);
-        l[e] = ld_global_f32(p + (D + 1) * kTile + row);
-        x[e] = ld_global_f32x4(p + (piece * kTile + row) * 4);
+        m[e] = -kInf;
+        l[e] = 0.0f;
+        if (i0 + e < n) {
+          const float* p = part(i0 + e);
+          m[e] = ld_global_f32(p + D * kTile + row);
+          l[e] = ld_global_f32(p + (D + 1) * kTile + row);
+          x[e] = ld_global_f32x4(p + (piece * kTile + row) * 4);
+        }
       }
       float up = top;
 #pragma unroll
@@ -971,7 +1087,7 @@ __global__ void __launch_bounds__(kJoinRows * D / 4) tree_attention_join_kernel(
 #pragma unroll
       for (int e = 0; e < kJoinBatch; ++e) {
         // a segment of which the node sees nothing has no part
-        if (i0 + e < n && l[e] != 0.0f) {
+        if (l[e] != 0.0f) {
           const float f = exp2_approx(m[e] - base);
           sum = fmaf(f, l[e], sum);
           o.x = fmaf(f, x[e].x, o.x);
@@ -984,9 +1100,10 @@ __global__ void __launch_bounds__(kJoinRows * D / 4) tree_attention_join_kernel(
     }
     if (row >= c.rows[w]) continue;
     const int at_row = c.row0[w] + row;
-    const int64_t token = c.token0 + at_row / a.group;
+    const int node = a.by_group.divide(at_row);
     auto* out = static_cast<__nv_bfloat16*>(a.out) +
-                ((token * a.num_kv_heads + c.kv_head[w]) * a.group + at_row % a.group) * D +
+                ((static_cast<int64_t>(c.token0 + node) * a.num_kv_heads + c.kv_head[w] - node) *
+                     a.group + at_row) * D +
                 piece * 4;
     const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
     if (sum == 0.0f) o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -1028,7 +1145,7 @@ int launch_tree_attention(TreeAttnArgs& a, void* workspace, int device, cudaStre
   const int status = launch_serialized(tree_attention_kernel<D>, dim3(ctas), dim3(kThreads),
                                        Shape<D>::kSmem, stream, 1u, map_k, map_v, a);
   if (status != SVLLM_OK || ctas < 2) return status;
-  return launch(tree_attention_join_kernel<D>, dim3(4 * ctas), dim3(kJoinRows * D / 4), 0, stream,
+  return launch(tree_attention_join_kernel<D>, dim3(5 * ctas), dim3(kJoinRows * D / 4), 0, stream,
                 1u, a, ctas);
 }
 
@@ -1099,12 +1216,15 @@ extern "C" int svllm_tree_attention_bf16(
   a.tree_mask = tree_mask;
   a.q_stride = q_token_stride;
   a.num_blocks = num_blocks;
-  a.num_tokens = num_tokens;
-  a.num_seqs = num_seqs;
+  a.num_tokens = static_cast<int>(num_tokens);
+  a.num_seqs = static_cast<int>(num_seqs);
   a.max_blocks = static_cast<int>(max_blocks);
   a.block_size = static_cast<int>(block_size);
   a.page = make_divider(block_size);
   a.group = static_cast<int>(num_heads / num_kv_heads);
+  a.max_length = static_cast<int>(max_blocks * block_size);
+  a.max_nodes = tree_mask != nullptr ? static_cast<int>(64 * mask_words) : INT32_MAX;
+  a.by_group = make_divider(a.group);
   a.num_kv_heads = static_cast<int>(num_kv_heads);
   a.cache_slots = static_cast<int>(num_blocks * block_size);
   a.box_rows = 128;
