@@ -42,8 +42,8 @@ namespace {
 
 constexpr int kTile = 128;            // query rows per M tile, cached rows per key tile
 constexpr int kSoftmaxWarps = 8;      // two groups of 4: accumulators 0 and 1
-constexpr int kHelperWarps = 2;       // query rows and the check of V
-constexpr int kLoaderWarps = 4;       // K and V
+constexpr int kHelperWarps = 4;       // query rows and the check of V
+constexpr int kLoaderWarps = 2;       // K and V
 constexpr int kLoadWarp = kSoftmaxWarps + kHelperWarps;
 constexpr int kMmaWarp = kLoadWarp + kLoaderWarps;
 constexpr int kPlanWarp = kMmaWarp + 1;  // lists the CTA's segments, zeroes rows without an item
@@ -58,7 +58,6 @@ constexpr uint32_t kScores = 0;       // TMEM columns: S (and P) of accumulator 
 constexpr uint32_t kOutput = 256;     // O at 256 + 128 w
 constexpr float kRescaleAbove = 8.0f;  // in powers of two
 constexpr int kJoinRows = 8;
-constexpr int kJoinBatch = 4;         // segments whose loads are in flight together
 constexpr int kMaxCtas = 256;         // one per SM; the join lists their borders
 
 template <int D>
@@ -71,13 +70,17 @@ struct Shape {
   static constexpr int kPartFloats = (D + 2) * kTile;
 };
 
-// A segment whose item is cut: what the join needs to know of it.
+// A segment whose item is cut, for the join: what one word says of it (0: nothing to join; else
+// kCut, the ends that are cut, and the rows of each accumulator), and where its rows go.
 struct Cut {
-  int flags;                       // 0: none, else kCut and the ends that are cut
   int token0;                      // the request's first token
-  int kv_head[2], row0[2], rows[2];  // per accumulator; rows 0: unused
+  int kv_head[2], row0[2];         // per accumulator
 };
-constexpr int kCut = 1, kCutFront = 2, kCutBack = 4;
+constexpr int kCut = 1, kCutFront = 2, kCutBack = 4, kCutRows = 3, kCutRowBits = 8;
+
+__device__ __forceinline__ int cut_rows(int mark, int w) {
+  return (mark >> (kCutRows + kCutRowBits * w)) & ((1 << kCutRowBits) - 1);
+}
 
 struct TreeAttnArgs {
   void* out;                       // [num_tokens, num_heads, head_dim] bf16, contiguous
@@ -89,6 +92,7 @@ struct TreeAttnArgs {
   const int32_t* query_start_loc;  // [num_seqs + 1]
   const int64_t* tree_mask;        // [num_tokens, mask_words] or null: causal
   float* parts;                    // [CTAs][2][2] partial sums
+  int* marks;                      // [CTAs][2]: a CTA's first and last segment
   Cut* cuts;                       // [CTAs][2]
   int64_t q_stride;
   int64_t num_blocks;
@@ -145,8 +149,8 @@ __device__ __forceinline__ Request load_request(const TreeAttnArgs& a, int s) {
 }
 
 // Steps of the line, weighted: a step over two KV heads loads twice what the others load.
-__device__ __forceinline__ int64_t request_cost(const TreeAttnArgs& a, const Request& r) {
-  return static_cast<int64_t>(a.num_kv_heads) * r.steps * (r.pairs + r.odd);
+__device__ __forceinline__ int request_cost(const TreeAttnArgs& a, const Request& r) {
+  return a.num_kv_heads * r.steps * (r.pairs + r.odd);
 }
 
 // A place on the line: request, item of the request, step of the item.
@@ -154,29 +158,24 @@ struct Place {
   int s, item, step;
 };
 
-__device__ __forceinline__ int64_t quotient(int64_t n, int d) {
-  return n >> 31 == 0 ? static_cast<uint32_t>(n) / static_cast<uint32_t>(d) : n / d;
-}
-
-
-__device__ __forceinline__ Place locate(const TreeAttnArgs& a, int s, const Request& r,
-                                        int64_t at) {
-  const int64_t shared = static_cast<int64_t>(a.num_kv_heads) * r.pairs * r.steps;
-  Place p{s, 0, 0};
-  if (at < shared) {
-    p.item = static_cast<int>(quotient(at, r.steps));
-    p.step = static_cast<int>(at - static_cast<int64_t>(p.item) * r.steps);
-    return p;
-  }
-  at -= shared;
-  const int pair = static_cast<int>(quotient(at, 2 * r.steps));
-  const int64_t rest = at - static_cast<int64_t>(pair) * 2 * r.steps;
-  const bool two = 2 * pair + 1 < a.num_kv_heads;
-  p.item = a.num_kv_heads * r.pairs + pair;
-  p.step = static_cast<int>(two ? (rest + 1) / 2 : rest);
-  if (p.step == r.steps) {  // rounded up to the item's end
-    ++p.item;
-    p.step = 0;
+__device__ __forceinline__ Place locate(const TreeAttnArgs& a, int s, const Request& r, int at) {
+  // items of two M tiles first, of steps that weigh 1; then two KV heads' last tiles, steps of 2
+  const int shared = a.num_kv_heads * r.pairs * r.steps;
+  const int weight = at < shared ? 1 : 2;
+  if (weight == 2) at -= shared;
+  const unsigned length = weight * r.steps;
+  Place p{s, static_cast<int>(at / length), 0};
+  const int rest = at - p.item * static_cast<int>(length);
+  if (weight == 2) {
+    // a last odd KV head is alone in its item, whose steps weigh 1
+    p.step = 2 * p.item + 1 < a.num_kv_heads ? (rest + 1) / 2 : rest;
+    p.item += a.num_kv_heads * r.pairs;
+    if (p.step == r.steps) {  // rounded up to the item's end
+      ++p.item;
+      p.step = 0;
+    }
+  } else {
+    p.step = rest;
   }
   return p;
 }
@@ -216,47 +215,46 @@ struct Sync {
   uint32_t tmem_base;
   int abort;
   int odd_values[2][4];  // per accumulator and segment modulo 4: V held something not finite
-  int64_t costs[kWarps];  // of the warps' shares of the requests
+  int costs[kWarps];     // of the warps' shares of the requests
   Segment list[kSegments];
 };
 
 // The plan warp: this CTA's share of the line, as segments. `chunk` requests make a warp's share
 // of the costs.
 __device__ __forceinline__ void plan(const TreeAttnArgs& a, Sync& sy, int chunk, int lane) {
-  int64_t upto = lane < kWarps ? sy.costs[lane] : 0;
+  int upto = lane < kWarps ? sy.costs[lane] : 0;
 #pragma unroll
   for (int off = 1; off < kWarpSize; off *= 2) {
-    const int64_t up = __shfl_up_sync(0xffffffffu, upto, off);
+    const int up = __shfl_up_sync(0xffffffffu, upto, off);
     if (lane >= off) upto += up;
   }
-  const int64_t total = __shfl_sync(0xffffffffu, upto, kWarpSize - 1);
+  const int total = __shfl_sync(0xffffffffu, upto, kWarpSize - 1);
   // at least two steps each: a shorter share costs more in the join than it saves
-  int64_t share = quotient(total + gridDim.x - 1, gridDim.x);
-  if (share < 2) share = 2;
+  const int share = max(2, static_cast<int>((total + gridDim.x - 1u) / gridDim.x));
   Place places[2];
 #pragma unroll 1
   for (int e = 0; e < 2; ++e) {
-    const int64_t border = (blockIdx.x + e) * share;
+    const int64_t border = static_cast<int64_t>(blockIdx.x + e) * share;
     Place p{a.num_seqs, 0, 0};
     if (border < total) {
       // the warp's share of the requests that holds it, then the request
       const int c = __ffs(static_cast<int>(__ballot_sync(0xffffffffu, border < upto))) - 1;
-      int64_t before = c > 0 ? __shfl_sync(0xffffffffu, upto, c - 1) : 0;
+      int before = c > 0 ? __shfl_sync(0xffffffffu, upto, c - 1) : 0;
 #pragma unroll 1
       for (int s0 = c * chunk;; s0 += kWarpSize) {
         Request r{};
         if (s0 + lane < min(a.num_seqs, (c + 1) * chunk)) r = load_request(a, s0 + lane);
-        const int64_t own = request_cost(a, r);
-        int64_t sum = own;
+        const int own = request_cost(a, r);
+        int sum = own;
 #pragma unroll
         for (int off = 1; off < kWarpSize; off *= 2) {
-          const int64_t up = __shfl_up_sync(0xffffffffu, sum, off);
+          const int up = __shfl_up_sync(0xffffffffu, sum, off);
           if (lane >= off) sum += up;
         }
         const unsigned past = __ballot_sync(0xffffffffu, border < before + sum);
         if (past != 0) {
           const int owner = __ffs(static_cast<int>(past)) - 1;
-          if (lane == owner) p = locate(a, s0 + lane, r, border - (before + sum - own));
+          if (lane == owner) p = locate(a, s0 + lane, r, static_cast<int>(border) - (before + sum - own));
           p.s = __shfl_sync(0xffffffffu, p.s, owner);
           p.item = __shfl_sync(0xffffffffu, p.item, owner);
           p.step = __shfl_sync(0xffffffffu, p.step, owner);
@@ -569,17 +567,23 @@ __device__ __forceinline__ void help(const TreeAttnArgs& a, Sync& sy, uint8_t* q
             if (!ok) break;
             landed ^= 1u << ring_at.slot;
             auto* tile = reinterpret_cast<uint4*>(ring + ring_at.slot * S::kTileBytes);
+            // rows of the tile that are nodes, and behind them whatever the pages hold
+            const int first_row = max(0, g.context - (step - 1) * kTile);
             const int end_row = g.length - (step - 1) * kTile;
             bool odd = false;
+#pragma unroll 1
+            for (int h = 0; h < S::kHalves; ++h) {
 #pragma unroll 4
-            for (int i = warp * kWarpSize + lane; i < S::kTileBytes / 16;
-                 i += kHelperWarps * kWarpSize) {
-              uint4 x = tile[i];
-              if (i * 16 % kHalfBytes / 128 >= end_row) {
-                tile[i] = make_uint4(0, 0, 0, 0);  // behind the request's end, whatever it holds
-              } else if (drop_odd(x.x) | drop_odd(x.y) | drop_odd(x.z) | drop_odd(x.w)) {
-                tile[i] = x;
-                odd = true;
+              for (int i = first_row * 8 + warp * kWarpSize + lane; i < kHalfBytes / 16;
+                   i += kHelperWarps * kWarpSize) {
+                uint4& at = tile[h * (kHalfBytes / 16) + i];
+                uint4 x = at;
+                if (i / 8 >= end_row) {
+                  at = make_uint4(0, 0, 0, 0);
+                } else if (drop_odd(x.x) | drop_odd(x.y) | drop_odd(x.z) | drop_odd(x.w)) {
+                  at = x;
+                  odd = true;
+                }
               }
             }
             if (odd) {
@@ -833,14 +837,15 @@ __device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w) 
     float* part = a.parts + ((static_cast<int64_t>(blockIdx.x) * 2 + slot) * 2 + w) *
                                 S::kPartFloats;
     if (cut && threadIdx.x % (4 * kWarpSize) == 0 && w == 0) {
+      a.marks[blockIdx.x * 2 + slot] = kCut | (g.front ? kCutFront : 0) |
+                                       (g.back ? kCutBack : 0) | g.rows[0] << kCutRows |
+                                       g.rows[1] << (kCutRows + kCutRowBits);
       Cut& c = a.cuts[blockIdx.x * 2 + slot];
-      c.flags = kCut | (g.front ? kCutFront : 0) | (g.back ? kCutBack : 0);
       c.token0 = g.start;
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         c.kv_head[x] = g.kv_head[x];
         c.row0[x] = g.row0[x];
-        c.rows[x] = g.rows[x];
       }
     }
     if (any) {
@@ -858,7 +863,7 @@ __device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w) 
         for (int i = 0; i < 16; ++i) o[i] = __uint_as_float(x[i]);
         if (odd && row < g.rows[w]) {
           // V values that are not finite, of the rows this node sees: the weights are positive
-          const int first = max(g.step0, g.context / kTile) * kTile;
+          const int first = max(g.step0 * kTile, g.context);
           const int last = min(g.step1 * kTile, g.length);
 #pragma unroll 1
           for (int j = first; j < last; ++j) {
@@ -927,7 +932,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     tree_attention_kernel(const __grid_constant__ CUtensorMap map_k,
                           const __grid_constant__ CUtensorMap map_v, const TreeAttnArgs a) {
   using S = Shape<D>;
-  grid_dependency_sync();
   extern __shared__ uint8_t smem_raw[];
   __shared__ Sync sy;
   uint8_t* q_tiles = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
@@ -942,14 +946,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tid == 0) {
     sy.abort = 0;
     for (int i = 0; i < 8; ++i) sy.odd_values[i / 4][i % 4] = 0;
-    a.cuts[blockIdx.x * 2].flags = 0;
-    a.cuts[blockIdx.x * 2 + 1].flags = 0;
   }
   if (warp == kMmaWarp) tmem_alloc(&sy.tmem_base, kTmemColumns);
 
+  grid_dependency_sync();
+  if (tid == 0) {
+    a.marks[blockIdx.x * 2] = 0;
+    a.marks[blockIdx.x * 2 + 1] = 0;
+  }
   // the line's length: every warp adds up a share of the requests
   const int chunk = (a.num_seqs + kWarps - 1) / kWarps;
-  int64_t cost = 0;
+  int cost = 0;
 #pragma unroll 1
   for (int s = warp * chunk + lane; s < min(a.num_seqs, (warp + 1) * chunk); s += kWarpSize) {
     cost += request_cost(a, load_request(a, s));
@@ -999,116 +1006,164 @@ __device__ __forceinline__ float4 ld_global_f32x4(const float* p) {
   return v;
 }
 
-// Joins the segments of each cut item. A border between two CTAs' shares that lies inside an item
-// is the item's if it is the first of those; each block lists these borders (one thread per border)
-// and takes every gridDim-th unit of 8 rows of one accumulator, a thread 16 bytes of a row. With m
-// and l the maxima and sums of the segments, M the largest m:
+// A cut item, as the join's blocks list them.
+struct JoinItem {
+  int first, border, segments;   // cut `first`, then the first cuts of the CTAs from `border` on
+  int mark;                      // of the first cut
+};
+
+constexpr int kJoinUnits = 2 * kTile / kJoinRows;  // per item: 8 rows of one accumulator each
+
+// kUnits units at once, kBatch segments of each at a time, all their loads before any use; a thread
+// does 16 bytes of a row. With m and l the maxima and sums of the segments, M the largest m:
 //   o = sum 2^(m - M) O / sum 2^(m - M) l.
+template <int D, int kUnits, int kBatch>
+__device__ __forceinline__ void join_units(const TreeAttnArgs& a, const JoinItem* items, int unit,
+                                           int stride) {
+  using S = Shape<D>;
+  const float kInf = __builtin_huge_valf();
+  const int piece = threadIdx.x / kJoinRows;
+  int most = 0;
+  float top[kUnits], sum[kUnits];
+  float4 o[kUnits];
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    most = max(most, items[(unit + u * stride) / kJoinUnits].segments);
+    top[u] = -kInf;
+    sum[u] = 0.0f;
+    o[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
+#pragma unroll 1
+  for (int i0 = 0; i0 < most; i0 += kBatch) {
+    float m[kUnits][kBatch], l[kUnits][kBatch];
+    float4 x[kUnits][kBatch];
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const JoinItem& it = items[(unit + u * stride) / kJoinUnits];
+      const int w = (unit + u * stride) % kJoinUnits / (kJoinUnits / 2);
+      const int row = (unit + u * stride) % (kJoinUnits / 2) * kJoinRows +
+                      threadIdx.x % kJoinRows;
+#pragma unroll
+      for (int e = 0; e < kBatch; ++e) {
+        m[u][e] = -kInf;
+        l[u][e] = 0.0f;
+        if (i0 + e < it.segments) {
+          const int64_t slot = i0 + e == 0 ? it.first : (it.border - 1 + i0 + e) * 2;
+          const float* p = a.parts + (slot * 2 + w) * S::kPartFloats + row;
+          m[u][e] = ld_global_f32(p + D * kTile);
+          l[u][e] = ld_global_f32(p + (D + 1) * kTile);
+          x[u][e] = ld_global_f32x4(p + piece * kTile * 4 + row * 3);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      float up = top[u];
+#pragma unroll
+      for (int e = 0; e < kBatch; ++e) up = fmaxf(up, m[u][e]);
+      const float base = up == -kInf ? 0.0f : up;
+      const float f0 = exp2_approx(top[u] - base);
+      sum[u] *= f0;
+      o[u] = make_float4(o[u].x * f0, o[u].y * f0, o[u].z * f0, o[u].w * f0);
+#pragma unroll
+      for (int e = 0; e < kBatch; ++e) {
+        if (l[u][e] != 0.0f) {  // a segment of which the node sees nothing has no part
+          const float f = exp2_approx(m[u][e] - base);
+          sum[u] = fmaf(f, l[u][e], sum[u]);
+          o[u].x = fmaf(f, x[u][e].x, o[u].x);
+          o[u].y = fmaf(f, x[u][e].y, o[u].y);
+          o[u].z = fmaf(f, x[u][e].z, o[u].z);
+          o[u].w = fmaf(f, x[u][e].w, o[u].w);
+        }
+      }
+      top[u] = up;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    const JoinItem& it = items[(unit + u * stride) / kJoinUnits];
+    const int w = (unit + u * stride) % kJoinUnits / (kJoinUnits / 2);
+    const int row =
+        (unit + u * stride) % (kJoinUnits / 2) * kJoinRows + threadIdx.x % kJoinRows;
+    if (row >= cut_rows(it.mark, w)) continue;
+    const Cut& c = a.cuts[it.first];
+    const int at_row = c.row0[w] + row;
+    const int node = a.by_group.divide(at_row);
+    auto* out = static_cast<__nv_bfloat16*>(a.out) +
+                ((static_cast<int64_t>(c.token0 + node) * a.num_kv_heads + c.kv_head[w] - node) *
+                     a.group + at_row) * D + piece * 4;
+    const float inverse = sum[u] == 0.0f ? 0.0f : 1.0f / sum[u];
+    if (sum[u] == 0.0f) o[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    *reinterpret_cast<uint2*>(out) =
+        make_uint2(pack_bf16x2(o[u].x * inverse, o[u].y * inverse),
+                   pack_bf16x2(o[u].z * inverse, o[u].w * inverse));
+  }
+}
+
+// Joins the segments of each cut item. A border between two CTAs' shares that lies inside an item
+// is the item's if it is the first of those; each block lists these items (one thread per border)
+// and takes every gridDim-th unit of them.
 template <int D>
-__global__ void __launch_bounds__(kJoinRows * D / 4, 1280 / (kJoinRows * D / 4)) tree_attention_join_kernel(
+__global__ void __launch_bounds__(kJoinRows * D / 4) tree_attention_join_kernel(
     const TreeAttnArgs a, int ctas) {
   grid_dependency_sync();
-  using S = Shape<D>;
   constexpr int kBlock = kJoinRows * D / 4;
-  constexpr int kUnits = 2 * kTile / kJoinRows;  // per item
-  __shared__ int borders[kMaxCtas], lasts[kMaxCtas];
-  __shared__ uint8_t inside[kMaxCtas + 1];  // the border lies inside an item; 2: as its first
+  __shared__ JoinItem items[kMaxCtas];
+  __shared__ int marks[2 * kMaxCtas];
   __shared__ int warp_counts[kBlock / kWarpSize];
+  __shared__ uint8_t inside[kMaxCtas + 1];  // the border lies inside an item; 2: as its first
   const int tid = threadIdx.x, lane = tid % kWarpSize;
+  for (int i = tid; i < 2 * ctas; i += kBlock) marks[i] = a.marks[i];
+  __syncthreads();
   for (int b = tid; b <= ctas; b += kBlock) {
     uint8_t kind = 0;
-    if (b > 0 && b < ctas && (a.cuts[b * 2].flags & kCutFront)) {
-      // the segment before the border: the previous CTA's second cut one, else its first
-      kind = a.cuts[b * 2 - 1].flags != 0 || !(a.cuts[b * 2 - 2].flags & kCutFront) ? 2 : 1;
+    // the segment before the border: the previous CTA's second cut one, else its first
+    if (b > 0 && b < ctas && (marks[b * 2] & kCutFront)) {
+      kind = marks[b * 2 - 1] != 0 || !(marks[b * 2 - 2] & kCutFront) ? 2 : 1;
     }
     inside[b] = kind;
   }
   __syncthreads();
-  int items = 0;
+  int count = 0;
   for (int b0 = 0; b0 < ctas; b0 += kBlock) {
     const int b = b0 + tid;
     const bool own = b < ctas && inside[b] == 2;
     const unsigned owners = __ballot_sync(0xffffffffu, own);
     if (lane == 0) warp_counts[tid / kWarpSize] = __popc(owners);
     __syncthreads();
-    int at = items + __popc(owners & ((1u << lane) - 1));
+    int at = count + __popc(owners & ((1u << lane) - 1));
     for (int i = 0; i < kBlock / kWarpSize; ++i) {
       if (i < tid / kWarpSize) at += warp_counts[i];
-      items += warp_counts[i];
+      count += warp_counts[i];
     }
     if (own) {
-      int last = b;
-      while (inside[last + 1] == 1) ++last;
-      borders[at] = b;
-      lasts[at] = last;
+      JoinItem it;
+      it.border = b;
+      it.first = b * 2 - (marks[b * 2 - 1] != 0 ? 1 : 2);
+      it.segments = 2;
+      while (inside[b + it.segments - 1] == 1) ++it.segments;
+      it.mark = marks[it.first];
+      items[at] = it;
     }
     __syncthreads();
   }
 
-  const float kInf = __builtin_huge_valf();
-  for (int unit = blockIdx.x; unit < items * kUnits; unit += gridDim.x) {
-    const int border = borders[unit / kUnits];
-    const int first = border * 2 - (a.cuts[border * 2 - 1].flags != 0 ? 1 : 2);
-    const int w = unit % kUnits / (kUnits / 2);
-    const int row = unit % (kUnits / 2) * kJoinRows + tid % kJoinRows;
-    const Cut& c = a.cuts[first];
-    if (unit % (kUnits / 2) * kJoinRows >= c.rows[w]) continue;
-    const int last = lasts[unit / kUnits];
-    const int piece = tid / kJoinRows;
-    const auto part = [&](int i) {  // segment i of the item
-      const int64_t slot = i == 0 ? first : (border - 1 + i) * 2;
-      return a.parts + (slot * 2 + w) * S::kPartFloats;
-    };
-    const int n = last - border + 2;
-    // four segments at a time, all their loads before any use
-    float top = -kInf, sum = 0.0f;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int i0 = 0; i0 < n; i0 += kJoinBatch) {
-      float m[kJoinBatch], l[kJoinBatch];
-      float4 x[kJoinBatch];
-#pragma unroll
-      for (int e = 0; e < kJoinBatch; ++e) {
-        m[e] = -kInf;
-        l[e] = 0.0f;
-        if (i0 + e < n) {
-          const float* p = part(i0 + e);
-          m[e] = ld_global_f32(p + D * kTile + row);
-          l[e] = ld_global_f32(p + (D + 1) * kTile + row);
-          x[e] = ld_global_f32x4(p + (piece * kTile + row) * 4);
-        }
-      }
-      float up = top;
-#pragma unroll
-      for (int e = 0; e < kJoinBatch; ++e) up = fmaxf(up, m[e]);
-      const float base = up == -kInf ? 0.0f : up;
-      const float f0 = exp2_approx(top - base);
-      sum *= f0;
-      o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
-#pragma unroll
-      for (int e = 0; e < kJoinBatch; ++e) {
-        // a segment of which the node sees nothing has no part
-        if (l[e] != 0.0f) {
-          const float f = exp2_approx(m[e] - base);
-          sum = fmaf(f, l[e], sum);
-          o.x = fmaf(f, x[e].x, o.x);
-          o.y = fmaf(f, x[e].y, o.y);
-          o.z = fmaf(f, x[e].z, o.z);
-          o.w = fmaf(f, x[e].w, o.w);
-        }
-      }
-      top = up;
+  // units without a row are passed over
+  const auto empty = [&](int unit) {
+    return unit % (kJoinUnits / 2) * kJoinRows >=
+           cut_rows(items[unit / kJoinUnits].mark, unit % kJoinUnits / (kJoinUnits / 2));
+  };
+  const int total = count * kJoinUnits, stride = gridDim.x;
+  for (int unit = blockIdx.x; unit < total; unit += stride) {
+    if (empty(unit)) continue;
+    const int next = unit + stride;
+    if (next < total && !empty(next) && items[unit / kJoinUnits].segments <= 4 &&
+        items[next / kJoinUnits].segments <= 4) {
+      join_units<D, 2, 4>(a, items, unit, stride);
+      unit = next;
+    } else {
+      join_units<D, 1, 8>(a, items, unit, stride);
     }
-    if (row >= c.rows[w]) continue;
-    const int at_row = c.row0[w] + row;
-    const int node = a.by_group.divide(at_row);
-    auto* out = static_cast<__nv_bfloat16*>(a.out) +
-                ((static_cast<int64_t>(c.token0 + node) * a.num_kv_heads + c.kv_head[w] - node) *
-                     a.group + at_row) * D +
-                piece * 4;
-    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-    if (sum == 0.0f) o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(o.x * inverse, o.y * inverse),
-                                                pack_bf16x2(o.z * inverse, o.w * inverse));
   }
 }
 
@@ -1121,15 +1176,16 @@ inline int attention_ctas(int device) {
 template <int D>
 int64_t workspace_bytes(int ctas) {
   return static_cast<int64_t>(ctas) *
-         (4 * Shape<D>::kPartFloats * 4 + 2 * static_cast<int64_t>(sizeof(Cut)));
+         (4 * Shape<D>::kPartFloats * 4 + 2 * static_cast<int64_t>(sizeof(Cut) + sizeof(int)));
 }
 
 template <int D>
 int launch_tree_attention(TreeAttnArgs& a, void* workspace, int device, cudaStream_t stream) {
   const int ctas = attention_ctas(device);
   a.parts = static_cast<float*>(workspace);
-  a.cuts = reinterpret_cast<Cut*>(a.parts + static_cast<int64_t>(ctas) * 4 *
-                                                Shape<D>::kPartFloats);
+  a.marks = reinterpret_cast<int*>(a.parts + static_cast<int64_t>(ctas) * 4 *
+                                                 Shape<D>::kPartFloats);
+  a.cuts = reinterpret_cast<Cut*>(a.marks + 2 * ctas);
   CUtensorMap map_k, map_v;
   const int64_t cols = static_cast<int64_t>(a.num_kv_heads) * D;
   if (!make_map(&map_k, a.k_cache, a.cache_slots, cols, cols, a.box_rows) ||
@@ -1141,11 +1197,10 @@ int launch_tree_attention(TreeAttnArgs& a, void* workspace, int device, cudaStre
                     Shape<D>::kSmem, device) < 1) {
     return SVLLM_ERR_CUDA;
   }
-  // not scheduled early behind the previous kernel: a CTA takes nearly all of an SM
-  const int status = launch_serialized(tree_attention_kernel<D>, dim3(ctas), dim3(kThreads),
+  const int status = launch(tree_attention_kernel<D>, dim3(ctas), dim3(kThreads),
                                        Shape<D>::kSmem, stream, 1u, map_k, map_v, a);
   if (status != SVLLM_OK || ctas < 2) return status;
-  return launch(tree_attention_join_kernel<D>, dim3(5 * ctas), dim3(kJoinRows * D / 4), 0, stream,
+  return launch(tree_attention_join_kernel<D>, dim3(4 * ctas), dim3(kJoinRows * D / 4), 0, stream,
                 1u, a, ctas);
 }
 
@@ -1201,6 +1256,10 @@ extern "C" int svllm_tree_attention_bf16(
   if (workspace == nullptr || workspace_size < needed || !aligned16(workspace)) {
     return SVLLM_ERR_INVALID_ARGUMENT;
   }
+  // the line of steps is counted in 32 bits: its length is at most this
+  const int64_t most = (max_blocks * block_size / 128 + 1) * num_kv_heads;
+  const int64_t tiles = num_tokens * (num_heads / num_kv_heads) / 128 + num_seqs;
+  if (most >= kMax || tiles >= kMax / most) return SVLLM_ERR_TOO_LARGE;
   int device;
   if (current_device(&device) != SVLLM_OK) return SVLLM_ERR_CUDA;
   int* err = library_error_word(device);
