@@ -32,6 +32,7 @@
 
 #include <cmath>
 #include <cstdint>
+#include <cstring>
 
 #include "common.cuh"
 #include "host_common.h"
@@ -187,6 +188,7 @@ struct Segment {
   int shared;                    // both accumulators take the same K and V
   int active;                    // accumulators in use, 1 or 2; 0: the end of the list
   int kv_head[2], row0[2], rows[2];
+  int lane0;                     // where accumulator 1's rows begin in its tile
   int step0, step1;
   int front, back;               // cut there
 };
@@ -218,6 +220,39 @@ struct Sync {
   int costs[kWarps];     // of the warps' shares of the requests
   Segment list[kSegments];
 };
+
+// The warp waits for a phase together: true for all lanes, or false for all once the pipeline is
+// aborting. The roles' loops are long straight code, bound by instruction fetch, so the common case
+// is a few instructions: a short loop of bounded tries; only then the abort flag and the clock.
+__device__ __forceinline__ bool warp_wait(Sync& sy, int bar, uint32_t parity, int* err) {
+  const uint32_t at = smem_addr(&sy.bar[0]) + bar * 8;
+  uint64_t start = 0;
+  while (true) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\t"
+        "mov.u32 n, 64;\n\t"
+        "TRY:\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "@p bra DONE;\n\t"
+        "sub.u32 n, n, 1;\n\t"
+        "setp.ne.u32 q, n, 0;\n\t"
+        "@q bra TRY;\n\t"
+        "DONE:\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(at), "r"(parity)
+        : "memory");
+    if (__all_sync(0xffffffffu, done != 0)) return true;
+    const uint64_t now = global_timer_ns();
+    if (start == 0) start = now;
+    if (now - start > kWaitLimitNs) {
+      sy.abort = 1;
+      raise_error(err, kErrWaitTimeout);
+    }
+    if (__any_sync(0xffffffffu, *static_cast<volatile int*>(&sy.abort) != 0)) return false;
+  }
+}
 
 // The plan warp: this CTA's share of the line, as segments. `chunk` requests make a warp's share
 // of the costs.
@@ -271,10 +306,7 @@ __device__ __forceinline__ void plan(const TreeAttnArgs& a, Sync& sy, int chunk,
   int loaded = -1;
   const auto list = [&](int index, const Segment& g) {
     const int slot = index % kSegments;
-    if (!__all_sync(0xffffffffu, wait_phase(&sy.bar[kRead + slot], (index / kSegments & 1) ^ 1,
-                                            &sy.abort, a.err))) {
-      return false;
-    }
+    if (!warp_wait(sy, kRead + slot, (index / kSegments & 1) ^ 1, a.err)) return false;
     if (lane == 0) {
       sy.list[slot] = g;
       mbar_arrive(&sy.bar[kListed + slot]);
@@ -319,6 +351,8 @@ __device__ __forceinline__ void plan(const TreeAttnArgs& a, Sync& sy, int chunk,
       g.rows[0] = all_rows - g.row0[0];
       g.rows[1] = g.active == 2 ? g.rows[0] : 0;
     }
+    // one warp of each group works on up to 32 rows: not two that share a scheduler
+    g.lane0 = g.rows[1] <= kTile / 2 ? kTile / 2 : 0;
     g.step0 = at.step;
     g.step1 = at.s == end.s && at.item == end.item ? end.step : r.steps;
     g.front = g.step0 > 0;
@@ -331,16 +365,23 @@ __device__ __forceinline__ void plan(const TreeAttnArgs& a, Sync& sy, int chunk,
   list(index, none);
 }
 
+// One of a pair, without an address: the array stays in registers.
+__device__ __forceinline__ int pick(const int (&pair)[2], int w) {
+  return w == 0 ? pair[0] : pair[1];
+}
+
 // The list's segment `index`, for a warp that reads them all in order; false at its end.
 __device__ __forceinline__ bool next_segment(const TreeAttnArgs& a, Sync& sy, int index,
                                              Segment& g) {
   const int slot = index % kSegments;
-  if (!__all_sync(0xffffffffu, wait_phase(&sy.bar[kListed + slot], index / kSegments & 1,
-                                          &sy.abort, a.err))) {
-    return false;
-  }
-  g = sy.list[slot];
-  __syncwarp();
+  if (!warp_wait(sy, kListed + slot, index / kSegments & 1, a.err)) return false;
+  // broadcast from one lane, so that the compiler knows the warp agrees on them
+  constexpr int kWords = sizeof(Segment) / sizeof(int);
+  const int* from = reinterpret_cast<const int*>(&sy.list[slot]);
+  int words[kWords];
+#pragma unroll
+  for (int i = 0; i < kWords; ++i) words[i] = __shfl_sync(0xffffffffu, from[i], 0);
+  memcpy(&g, words, sizeof(Segment));
   if (threadIdx.x % kWarpSize == 0) mbar_arrive(&sy.bar[kRead + slot]);
   return g.active > 0;
 }
@@ -430,10 +471,7 @@ struct Loader {
   // This warp's part of one tile into the ring's next slot.
   __device__ __forceinline__ bool load(const CUtensorMap* map, int full, const int (&rows)[4],
                                        int kv_head) {
-    if (!__all_sync(0xffffffffu, wait_phase(&sy.bar[kEmpty + at.slot], at.phase ^ 1, &sy.abort,
-                                            a.err))) {
-      return false;
-    }
+    if (!warp_wait(sy, kEmpty + at.slot, at.phase ^ 1, a.err)) return false;
     // boxes (or groups of 4 rows) part, part + kLoaderWarps, ..., both halves of a row together
     const int rows_each = a.box_rows > 1 ? a.box_rows : 4;
     const int count = kTile / rows_each;
@@ -522,7 +560,7 @@ __device__ __forceinline__ void help(const TreeAttnArgs& a, Sync& sy, uint8_t* q
   constexpr int kLanes = D / 8;  // lanes per query row: 16 bytes each
   constexpr int kRowsAtOnce = kWarpSize / kLanes;
   const auto wait = [&](int bar, uint32_t parity) {
-    return __all_sync(0xffffffffu, wait_phase(&sy.bar[bar], parity, &sy.abort, a.err));
+    return warp_wait(sy, bar, parity, a.err);
   };
   Ring ring_at;
   uint32_t landed = 0;  // parity of the next use of each slot's barrier
@@ -537,12 +575,13 @@ __device__ __forceinline__ void help(const TreeAttnArgs& a, Sync& sy, uint8_t* q
 #pragma unroll 1
       for (int r0 = warp * kWarpSize; r0 < kTile; r0 += kHelperWarps * kWarpSize) {
         // row = node * group + head of the KV head
-        const int row = g.row0[w] + r0 + lane;
+        const int r = r0 + lane - (w == 0 ? 0 : g.lane0);
+        const int row = pick(g.row0, w) + max(r, 0);
         const int node = a.by_group.divide(row);
         const int64_t offset =
-            r0 + lane < g.rows[w]
+            r >= 0 && r < pick(g.rows, w)
                 ? (g.start + node) * a.q_stride +
-                      (static_cast<int64_t>(g.kv_head[w] - node) * a.group + row) * D
+                      (static_cast<int64_t>(pick(g.kv_head, w) - node) * a.group + row) * D
                 : -1;
         const int c = lane % kLanes;
         const uint32_t base = smem_addr(q_tiles + w * S::kTileBytes) + (c / 8) * kHalfBytes;
@@ -613,25 +652,25 @@ __device__ __forceinline__ void issue_products(const TreeAttnArgs& a, Sync& sy,
   constexpr uint64_t kTileStep = S::kTileBytes >> 4;
   const uint64_t q_desc = smem_desc_k_sw128(q_tiles), k_desc = smem_desc_k_sw128(ring);
   const uint64_t v_desc = smem_desc_mn_sw128(ring, kHalfBytes);
-  const uint32_t tmem = sy.tmem_base;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, sy.tmem_base, 0);
   Ring ring_at;
   int k_slot = 0, v_slot = 0;           // the tiles in use
   uint32_t full = 0, checked = 0;       // parity of the next use of each slot's barriers
   uint32_t weights_phase = 0;           // one bit per accumulator
   bool ok = true;
   const auto wait = [&](int bar, uint32_t parity) {
-    ok = __all_sync(0xffffffffu, wait_phase(&sy.bar[bar], parity, &sy.abort, a.err));
-    tc_fence_after();
+    ok = warp_wait(sy, bar, parity, a.err);
     return ok;
   };
-  // the ring's next tile
-  const auto take = [&](bool nodes, int& slot) {
-    slot = ring_at.slot;
-    uint32_t& parity = nodes ? checked : full;
-    if (!wait((nodes ? kChecked : kFull) + slot, (parity >> slot) & 1)) return false;
-    parity ^= 1u << slot;
+  // the ring's next tile, and its slot
+  const auto take = [&](bool nodes) {
+    const int slot = ring_at.slot;
+    const uint32_t bit = 1u << slot;
+    wait((nodes ? kChecked : kFull) + slot, ((nodes ? checked : full) & bit) != 0);
+    checked ^= nodes ? bit : 0;
+    full ^= nodes ? 0 : bit;
     ring_at.advance(S::kStages);
-    return true;
+    return slot;
   };
   Segment g;
 #pragma unroll 1
@@ -644,9 +683,10 @@ __device__ __forceinline__ void issue_products(const TreeAttnArgs& a, Sync& sy,
       for (int w = 0; ok && w < g.active; ++w) {
         const bool first_use = !g.shared || w == 0, last_use = !g.shared || w == 1;
         if (step >= g.step0) {
-          if (!wait(kWeightsDone + w, (weights_phase >> w) & 1)) break;
+          if (first_use) v_slot = take(has_nodes(g, step));
+          if (!ok || !wait(kWeightsDone + w, (weights_phase >> w) & 1)) break;
           weights_phase ^= 1u << w;
-          if (first_use && !take(has_nodes(g, step), v_slot)) break;
+          tc_fence_after();  // the weights are in TMEM; the tiles need no such fence
           if (elect_one()) {
             const uint64_t vd = v_desc + v_slot * kTileStep;
             const uint32_t first = step > g.step0;
@@ -661,7 +701,8 @@ __device__ __forceinline__ void issue_products(const TreeAttnArgs& a, Sync& sy,
         }
         if (step + 1 < g.step1) {
           // the next step's scores; they may overwrite these weights: products complete in order
-          if (first_use && !take(false, k_slot)) break;
+          if (first_use) k_slot = take(false);
+          if (!ok) break;
           if (elect_one()) {
             const uint64_t qd = q_desc + w * kTileStep;
             const uint64_t kd = k_desc + k_slot * kTileStep;
@@ -722,7 +763,6 @@ template <int D>
 __device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w) {
   using S = Shape<D>;
   const int quarter = (threadIdx.x / kWarpSize) % 4;
-  const int row = quarter * kWarpSize + threadIdx.x % kWarpSize;
   const uint32_t lanes = static_cast<uint32_t>(quarter * kWarpSize) << 16;
   const uint32_t scores = sy.tmem_base + kScores + w * kTile + lanes;
   const uint32_t output = sy.tmem_base + kOutput + w * kTile + lanes;
@@ -733,8 +773,11 @@ __device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w) 
   for (int index = 0; next_segment(a, sy, index, g); ++index) {
     if (threadIdx.x % (4 * kWarpSize) == 0) sy.odd_values[w][(index + 2) & 3] = 0;
     if (w >= g.active) continue;
-    const bool any = quarter * kWarpSize < g.rows[w];  // the warp holds rows of the request
-    const int at_row = g.row0[w] + (row < g.rows[w] ? row : 0);
+    const int lane0 = w == 0 ? 0 : g.lane0;
+    const int row = quarter * kWarpSize + threadIdx.x % kWarpSize - lane0;
+    const bool valid = row >= 0 && row < pick(g.rows, w);
+    const bool any = __any_sync(0xffffffffu, valid);  // the warp holds rows of the request
+    const int at_row = pick(g.row0, w) + (valid ? row : 0);
     const int node = a.by_group.divide(at_row);
     const int64_t token = g.start + node;
     const int64_t* mask =
@@ -743,10 +786,7 @@ __device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w) 
 #pragma unroll 1
     for (int step = g.step0; step < g.step1; ++step) {
       // the warp leaves together: the TMEM loads below are collective
-      if (!__all_sync(0xffffffffu, wait_phase(&sy.bar[kScoresDone + w], scores_phase, &sy.abort,
-                                              a.err))) {
-        return;
-      }
+      if (!warp_wait(sy, kScoresDone + w, scores_phase, a.err)) return;
       scores_phase ^= 1;
       tc_fence_after();
       if (any) {
@@ -825,10 +865,7 @@ __device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w) 
       mbar_arrive(&sy.bar[kWeightsDone + w]);
     }
 
-    if (!__all_sync(0xffffffffu, wait_phase(&sy.bar[kOutputDone + w], output_phase, &sy.abort,
-                                            a.err))) {
-      return;
-    }
+    if (!warp_wait(sy, kOutputDone + w, output_phase, a.err)) return;
     output_phase ^= 1;
     tc_fence_after();
     const bool cut = g.front || g.back;
@@ -853,7 +890,7 @@ __device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w) 
       const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
       __nv_bfloat16* out =
           static_cast<__nv_bfloat16*>(a.out) +
-          ((token * a.num_kv_heads + g.kv_head[w] - node) * a.group + at_row) * D;
+          ((token * a.num_kv_heads + pick(g.kv_head, w) - node) * a.group + at_row) * D;
 #pragma unroll 1
       for (int c = 0; c < D; c += 16) {
         uint32_t x[16];
@@ -861,7 +898,7 @@ __device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w) 
         float o[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[i] = __uint_as_float(x[i]);
-        if (odd && row < g.rows[w]) {
+        if (odd && valid) {
           // V values that are not finite, of the rows this node sees: the weights are positive
           const int first = max(g.step0 * kTile, g.context);
           const int last = min(g.step1 * kTile, g.length);
@@ -873,7 +910,7 @@ __device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w) 
             if (block < 0 || block >= a.num_blocks) block = 0;
             const auto* v = static_cast<const uint16_t*>(a.v_cache) +
                             ((block * a.block_size + (j - page * a.block_size)) *
-                                 a.num_kv_heads + g.kv_head[w]) * D + c;
+                                 a.num_kv_heads + pick(g.kv_head, w)) * D + c;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               const uint32_t bits = static_cast<uint32_t>(v[i]) << 16;
@@ -881,13 +918,13 @@ __device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w) 
             }
           }
         }
-        if (cut) {
+        if (cut && valid) {
 #pragma unroll
           for (int i = 0; i < 16; i += 4) {
             *reinterpret_cast<float4*>(part + (((c + i) / 4) * kTile + row) * 4) =
                 make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
           }
-        } else if (row < g.rows[w]) {
+        } else if (valid) {
           // a sum of zero: the node saw no row
           float f[8];
 #pragma unroll
@@ -898,7 +935,7 @@ __device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w) 
           }
         }
       }
-      if (cut) {
+      if (cut && valid) {
         part[D * kTile + row] = ref;
         part[(D + 1) * kTile + row] = sum;
       }
@@ -937,7 +974,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* q_tiles = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
   uint8_t* ring = q_tiles + 2 * S::kTileBytes;
   const int tid = threadIdx.x;
-  const int warp = tid / kWarpSize, lane = tid % kWarpSize;
+  const int warp = __shfl_sync(0xffffffffu, tid / kWarpSize, 0), lane = tid % kWarpSize;
 
   if (tid < kBarriers) {
     mbar_init(&sy.bar[tid], arrivals(tid));
