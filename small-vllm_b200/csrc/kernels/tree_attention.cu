@@ -254,10 +254,11 @@ __device__ __forceinline__ bool warp_wait(Sync& sy, int bar, uint32_t parity, in
   }
 }
 
-// The plan warp: this CTA's share of the line, as segments. `chunk` requests make a warp's share
-// of the costs.
-__device__ __forceinline__ void plan(const TreeAttnArgs& a, Sync& sy, int chunk, int lane) {
-  int upto = lane < kWarps ? sy.costs[lane] : 0;
+// The borders of this CTA's share of the line. `cost`: lane i holds the cost of the i-th `chunk` of
+// requests.
+__device__ __forceinline__ void find_share(const TreeAttnArgs& a, int cost, int chunk, int lane,
+                                           Place (&places)[2]) {
+  int upto = cost;
 #pragma unroll
   for (int off = 1; off < kWarpSize; off *= 2) {
     const int up = __shfl_up_sync(0xffffffffu, upto, off);
@@ -266,7 +267,6 @@ __device__ __forceinline__ void plan(const TreeAttnArgs& a, Sync& sy, int chunk,
   const int total = __shfl_sync(0xffffffffu, upto, kWarpSize - 1);
   // at least two steps each: a shorter share costs more in the join than it saves
   const int share = max(2, static_cast<int>((total + gridDim.x - 1u) / gridDim.x));
-  Place places[2];
 #pragma unroll 1
   for (int e = 0; e < 2; ++e) {
     const int64_t border = static_cast<int64_t>(blockIdx.x + e) * share;
@@ -298,10 +298,14 @@ __device__ __forceinline__ void plan(const TreeAttnArgs& a, Sync& sy, int chunk,
         before += __shfl_sync(0xffffffffu, sum, kWarpSize - 1);
       }
     }
-    places[e] = p;
+    if (e == 0) places[0] = p;
+    places[1] = p;
   }
-  Place at = places[0];
-  const Place end = places[1];
+}
+
+// The plan warp: lists the segments of [at, end).
+__device__ __forceinline__ void plan(const TreeAttnArgs& a, Sync& sy, Place at, const Place end,
+                                     int lane) {
   Request r{};
   int loaded = -1;
   const auto list = [&](int index, const Segment& g) {
@@ -991,16 +995,31 @@ __global__ void __launch_bounds__(kThreads, 1)
     a.marks[blockIdx.x * 2] = 0;
     a.marks[blockIdx.x * 2 + 1] = 0;
   }
-  // the line's length: every warp adds up a share of the requests
-  const int chunk = (a.num_seqs + kWarps - 1) / kWarps;
-  int cost = 0;
+  // this CTA's share of the line: a batch of up to 32 requests is planned by one warp while the
+  // others set up; of a larger one every warp adds up a part first
+  const bool few = a.num_seqs <= kWarpSize;
+  const int chunk = few ? 1 : (a.num_seqs + kWarps - 1) / kWarps;
+  if (!few) {
+    int cost = 0;
 #pragma unroll 1
-  for (int s = warp * chunk + lane; s < min(a.num_seqs, (warp + 1) * chunk); s += kWarpSize) {
-    cost += request_cost(a, load_request(a, s));
-  }
+    for (int s = warp * chunk + lane; s < min(a.num_seqs, (warp + 1) * chunk); s += kWarpSize) {
+      cost += request_cost(a, load_request(a, s));
+    }
 #pragma unroll
-  for (int off = 16; off > 0; off /= 2) cost += __shfl_xor_sync(0xffffffffu, cost, off);
-  if (lane == 0) sy.costs[warp] = cost;
+    for (int off = 16; off > 0; off /= 2) cost += __shfl_xor_sync(0xffffffffu, cost, off);
+    if (lane == 0) sy.costs[warp] = cost;
+    __syncthreads();
+  }
+  Place places[2]{};
+  if (warp == kPlanWarp) {
+    int cost = 0;
+    if (!few) {
+      if (lane < kWarps) cost = sy.costs[lane];
+    } else if (lane < a.num_seqs) {
+      cost = request_cost(a, load_request(a, lane));
+    }
+    find_share(a, cost, chunk, lane, places);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -1018,7 +1037,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == kMmaWarp) {
       issue_products<D>(a, sy, q_tiles, ring);
     } else {
-      plan(a, sy, chunk, lane);
+      plan(a, sy, places[0], places[1], lane);
       fill_rest(a, static_cast<int64_t>(a.num_kv_heads) * a.group * D / 8, lane);
     }
   }
