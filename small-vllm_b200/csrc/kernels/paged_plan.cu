@@ -7,11 +7,12 @@
 // sum of the needs, s is served when P_s is at most the list's length (or its need is 0). Block
 // k of the step, counted over all requests, is free_blocks[count - 1 - k].
 //
-// One CTA does the requests: its scans are a few shuffles for 1024 requests, and no grid-wide
-// meeting is needed between giving blocks back and taking them. What bounds it is the chain of
-// dependent loads, not bytes. Tokens are independent of one another (a binary search over the
-// starts, one table entry, a walk up the parents); few of them follow in the same CTA, many get
-// a second kernel over the whole GPU (kFusedTokens).
+// One CTA does the requests, as many threads as there are requests up to 1024: a scan of (tokens,
+// blocks) is a few shuffles, and no grid-wide meeting is needed between giving blocks back and taking
+// them. What bounds it is the chain of dependent loads and barriers, not bytes. Tokens are
+// independent of one another (a binary search over the starts, one table entry, a walk up the
+// parents); few of them follow in the same CTA, the starts and the parents staged in shared memory;
+// many get a second kernel over the whole GPU (kFusedTokens).
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -22,9 +23,10 @@
 namespace svllm::k {
 namespace {
 
-constexpr int kPlanThreads = 1024;
-constexpr int kPlanWarps = kPlanThreads / kWarpSize;
+constexpr int kPlanThreads = 1024;  // at most; as many as there are requests, in whole warps
 constexpr int kTokenThreads = 256;
+constexpr int kStagedStarts = 4096;  // of requests, staged by the tokens' kernel
+constexpr int kOwnBlocks = 8;        // new blocks up to which a request's own lane fetches them
 
 // Up to this many tokens are done by the CTA that did the requests; more get a grid of their own.
 constexpr int64_t kFusedTokens = 4096;
@@ -47,6 +49,7 @@ struct PlanArgs {
   int64_t num_seqs;
   int64_t num_tokens;
   int64_t free_capacity;
+  int64_t max_rows;              // max_blocks * block_size
   int32_t max_blocks;
   int32_t block_size;
   int32_t max_query_len;         // checked where parents are given: the mask's width
@@ -55,37 +58,56 @@ struct PlanArgs {
   int* err;
 };
 
-// Inclusive sum over the CTA's threads; `total` receives the CTA's sum. 64 bits: lengths come
-// from the caller unchecked, and their sum must not wrap.
-__device__ int64_t block_scan(int64_t v, int64_t* warp_sums, int64_t& total) {
+// Lengths come from the caller unchecked: sums stop at the largest int (which no valid one reaches)
+// instead of wrapping.
+__device__ __forceinline__ uint32_t add_up(uint32_t a, uint32_t b) {
+  return min(a + b, static_cast<uint32_t>(INT32_MAX));
+}
+
+// Inclusive sums over the CTA's threads of a pair; `total` receives the CTA's.
+__device__ uint2 block_scan(uint2 v, uint2* warp_sums, uint2& total) {
   const int lane = threadIdx.x % kWarpSize, warp = threadIdx.x / kWarpSize;
+  const int warps = blockDim.x / kWarpSize;
 #pragma unroll
   for (int off = 1; off < kWarpSize; off *= 2) {
-    const int64_t up = __shfl_up_sync(0xffffffffu, v, off);
-    if (lane >= off) v += up;
+    const uint32_t x = __shfl_up_sync(0xffffffffu, v.x, off);
+    const uint32_t y = __shfl_up_sync(0xffffffffu, v.y, off);
+    if (lane >= off) v = make_uint2(add_up(v.x, x), add_up(v.y, y));
+  }
+  if (warps == 1) {
+    total = make_uint2(__shfl_sync(0xffffffffu, v.x, kWarpSize - 1),
+                       __shfl_sync(0xffffffffu, v.y, kWarpSize - 1));
+    return v;
   }
   __syncthreads();  // the previous scan's readers are done
   if (lane == kWarpSize - 1) warp_sums[warp] = v;
   __syncthreads();
-  int64_t s = warp_sums[lane];  // kPlanWarps == kWarpSize: every warp sums the sums itself
+  uint2 s = lane < warps ? warp_sums[lane] : make_uint2(0, 0);  // every warp sums the sums itself
 #pragma unroll
   for (int off = 1; off < kWarpSize; off *= 2) {
-    const int64_t up = __shfl_up_sync(0xffffffffu, s, off);
-    if (lane >= off) s += up;
+    const uint32_t x = __shfl_up_sync(0xffffffffu, s.x, off);
+    const uint32_t y = __shfl_up_sync(0xffffffffu, s.y, off);
+    if (lane >= off) s = make_uint2(add_up(s.x, x), add_up(s.y, y));
   }
-  total = __shfl_sync(0xffffffffu, s, kWarpSize - 1);
-  const int64_t before = __shfl_sync(0xffffffffu, s, warp > 0 ? warp - 1 : 0);
-  return v + (warp > 0 ? before : 0);
+  total = make_uint2(__shfl_sync(0xffffffffu, s.x, kWarpSize - 1),
+                     __shfl_sync(0xffffffffu, s.y, kWarpSize - 1));
+  if (warp > 0) {
+    v.x = add_up(v.x, __shfl_sync(0xffffffffu, s.x, warp - 1));
+    v.y = add_up(v.y, __shfl_sync(0xffffffffu, s.y, warp - 1));
+  }
+  return v;
 }
-static_assert(kPlanWarps == kWarpSize, "block_scan sums one value per warp in one warp");
+static_assert(kPlanThreads <= kWarpSize * kWarpSize, "one value per warp in one warp");
 
-// One token: its request by binary search over the starts, then slot, position and mask. Reads
-// what the requests' part wrote, so plain loads (not the read-only path).
-__device__ void plan_token(const PlanArgs& a, int64_t t) {
-  int64_t lo = 0, hi = a.num_seqs;  // the first request whose end lies beyond t
+// One token: its request by binary search over the starts, then slot, position and mask. `starts`
+// and `parents` may be staged copies. Reads what the requests' part wrote, so plain loads (not the
+// read-only path).
+__device__ void plan_token(const PlanArgs& a, int t, const int32_t* starts,
+                           const int32_t* parents) {
+  int lo = 0, hi = static_cast<int>(a.num_seqs);  // the first request whose end lies beyond t
   while (lo < hi) {
-    const int64_t mid = (lo + hi) / 2;
-    if (a.query_start_loc[mid + 1] > t) {
+    const int mid = (lo + hi) / 2;
+    if (starts[mid + 1] > t) {
       hi = mid;
     } else {
       lo = mid + 1;
@@ -93,15 +115,17 @@ __device__ void plan_token(const PlanArgs& a, int64_t t) {
   }
   const bool live = lo < a.num_seqs && a.seq_lens[lo] > 0;
   int64_t slot = -1, position = 0;
-  int64_t* mask = a.tree_mask == nullptr ? nullptr : a.tree_mask + t * a.mask_words;
+  int64_t* mask =
+      a.tree_mask == nullptr ? nullptr : a.tree_mask + static_cast<int64_t>(t) * a.mask_words;
   int word = a.mask_words;  // mask words from here on are written
   if (live) {
-    const int32_t start = a.query_start_loc[lo];
-    const int i = static_cast<int>(t - start);
-    const int64_t row = static_cast<int64_t>(a.context_lens[lo]) + i;
-    const int64_t page = row / a.block_size;
-    slot = static_cast<int64_t>(a.block_tables[lo * a.max_blocks + page]) * a.block_size +
-           (row - page * a.block_size);
+    const int32_t start = starts[lo];
+    const int i = t - start;
+    const int context = a.context_lens[lo];
+    const int row = context + i;  // at most max_blocks * block_size, which fits
+    const int page = row / a.block_size;
+    slot = static_cast<int64_t>(a.block_tables[static_cast<int64_t>(lo) * a.max_blocks + page]) *
+               a.block_size + (row - page * a.block_size);
     int depth = i;
     if (mask != nullptr) {
       // up the tree: parents come before their children, so the words are met in falling order
@@ -115,7 +139,7 @@ __device__ void plan_token(const PlanArgs& a, int64_t t) {
         }
         bits |= uint64_t{1} << (p % 64);
         ++depth;
-        int up = a.parents[start + p];
+        int up = parents[start + p];
         if (up >= p || up < -1) {  // not a tree: the node counts as a root
           raise_error(a.err, kErrBadIndex);
           up = -1;
@@ -124,7 +148,7 @@ __device__ void plan_token(const PlanArgs& a, int64_t t) {
       }
       mask[--word] = static_cast<int64_t>(bits);
     }
-    position = static_cast<int64_t>(a.context_lens[lo]) + depth;
+    position = static_cast<int64_t>(context) + depth;
   }
   if (mask != nullptr) {
     while (word > 0) mask[--word] = 0;
@@ -133,13 +157,46 @@ __device__ void plan_token(const PlanArgs& a, int64_t t) {
   a.positions[t] = position;
 }
 
+// Copies `count` block ids per lane, src[step * k] -> dst[k]: a lane's own when there are few, else
+// the warp together, lane by lane.
+__device__ __forceinline__ void copy_blocks(int count, const int32_t* src, int step,
+                                            int32_t* dst) {
+  const int most = __reduce_max_sync(0xffffffffu, count);
+  if (most <= kOwnBlocks) {
+    int32_t held[kOwnBlocks];
+#pragma unroll
+    for (int k = 0; k < kOwnBlocks; ++k) {
+      if (k < count) held[k] = src[step * k];
+    }
+#pragma unroll
+    for (int k = 0; k < kOwnBlocks; ++k) {
+      if (k < count) dst[k] = held[k];
+    }
+    return;
+  }
+  for (int l = 0; l < kWarpSize; ++l) {
+    const int n = __shfl_sync(0xffffffffu, count, l);
+    const auto from = reinterpret_cast<const int32_t*>(
+        __shfl_sync(0xffffffffu, reinterpret_cast<int64_t>(src), l));
+    const auto to =
+        reinterpret_cast<int32_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<int64_t>(dst), l));
+    for (int k = threadIdx.x % kWarpSize; k < n; k += kWarpSize) {
+      to[k] = from[static_cast<int64_t>(step) * k];
+    }
+  }
+}
+
 __global__ void __launch_bounds__(kPlanThreads) plan_requests_kernel(const PlanArgs a) {
   grid_dependency_sync();
-  __shared__ int64_t warp_sums[kPlanWarps];
-  __shared__ int64_t sh_off[kPlanThreads];  // blocks given back or taken before this request
-  __shared__ int32_t sh_count[kPlanThreads];
-  __shared__ int32_t sh_owned[kPlanThreads];
-  const int tid = threadIdx.x, lane = tid % kWarpSize, warp = tid / kWarpSize;
+  extern __shared__ int32_t staged[];  // starts, then parents, for the tokens (fused)
+  __shared__ uint2 warp_sums[kPlanThreads / kWarpSize];
+  __shared__ int used;
+  const int tid = threadIdx.x;
+  const int threads = blockDim.x, n_seqs = static_cast<int>(a.num_seqs);
+  if (tid == 0) used = 0;
+  if (a.fused && a.tree_mask != nullptr) {
+    for (int t = tid; t < a.num_tokens; t += threads) staged[n_seqs + 1 + t] = a.parents[t];
+  }
 
   int64_t have = a.free_count[0];
   if (have < 0 || have > a.free_capacity) {
@@ -149,104 +206,109 @@ __global__ void __launch_bounds__(kPlanThreads) plan_requests_kernel(const PlanA
 
   // finished requests: their blocks go on the free list, behind what is there
   int64_t back = 0;
-  for (int64_t base = 0; base < a.num_seqs; base += kPlanThreads) {
-    const int64_t s = base + tid;
-    int64_t give = 0;
-    if (s < a.num_seqs && a.query_lens[s] < 0) {
-      const int32_t owned = a.blocks_owned[s];
+  int query = 0, context = 0, owned = 0;  // of the last chunk read
+  for (int base = 0; base < n_seqs; base += threads) {
+    const int s = base + tid;
+    query = s < n_seqs ? a.query_lens[s] : 0;
+    context = s < n_seqs ? a.context_lens[s] : 0;
+    owned = s < n_seqs ? a.blocks_owned[s] : 0;
+    if (!__syncthreads_or(query < 0)) continue;
+    uint32_t give = 0;
+    if (query < 0) {
       if (owned < 0 || owned > a.max_blocks) {
         raise_error(a.err, kErrBadIndex);
       } else {
         give = owned;
       }
     }
-    int64_t total;
-    const int64_t end = block_scan(give, warp_sums, total);
-    if (total > 0) {  // the same for every thread
-      sh_off[tid] = have + back + end - give;
-      sh_count[tid] = static_cast<int32_t>(give);
-      __syncthreads();
-      for (int k = warp; k < kPlanThreads; k += kPlanWarps) {
-        for (int i = lane; i < sh_count[k]; i += kWarpSize) {
-          const int64_t to = sh_off[k] + i;
-          if (to < a.free_capacity) {
-            a.free_blocks[to] = a.block_tables[(base + k) * a.max_blocks + i];
-          } else {
-            raise_error(a.err, kErrBadIndex);  // no room: the block is dropped
-          }
-        }
-      }
-      __syncthreads();  // the next chunk's counts may be written
-    }
-    back += total;
+    uint2 total;
+    const uint2 end = block_scan(make_uint2(give, 0), warp_sums, total);
+    const int64_t at = have + back + end.x - give;
+    // what finds no room is dropped
+    const int64_t room = a.free_capacity - at;
+    const int fits = room <= 0 ? 0 : room < give ? static_cast<int>(room) : static_cast<int>(give);
+    if (fits < static_cast<int>(give)) raise_error(a.err, kErrBadIndex);
+    const int32_t* row = a.block_tables + static_cast<int64_t>(s) * a.max_blocks;
+    copy_blocks(fits, row, 1, a.free_blocks + at);
+    back += total.x;
   }
   have = have + back < a.free_capacity ? have + back : a.free_capacity;
   __syncthreads();  // blocks given back above may be taken below
 
-  int64_t tokens = 0, needed = 0, used = 0;
-  for (int64_t base = 0; base < a.num_seqs; base += kPlanThreads) {
-    const int64_t s = base + tid;
-    const bool is = s < a.num_seqs;
-    const int64_t query = is ? a.query_lens[s] : 0;
-    const int64_t context = is ? a.context_lens[s] : 0;
-    const int64_t owned = is ? a.blocks_owned[s] : 0;
-    const int64_t n = query > 0 ? query : 0;
-    int64_t total;
-    const int64_t tokens_end = tokens + block_scan(n, warp_sums, total);
-    tokens += total;
+  uint32_t tokens = 0, needed = 0;  // of the chunks before
+  for (int base = 0; base < n_seqs; base += threads) {
+    const int s = base + tid;
+    const bool is = s < n_seqs;
+    if (n_seqs > threads) {  // else they are in registers
+      query = is ? a.query_lens[s] : 0;
+      context = is ? a.context_lens[s] : 0;
+      owned = is ? a.blocks_owned[s] : 0;
+    }
+    const int n = query > 0 ? query : 0;
+    const int64_t rows = static_cast<int64_t>(context) + n;
     bool ok = is && query >= 0;
-    if (ok && (context < 0 || owned < 0 || owned > a.max_blocks || tokens_end > a.num_tokens ||
-               context + n > static_cast<int64_t>(a.max_blocks) * a.block_size ||
-               (a.parents != nullptr && n > a.max_query_len))) {
+    if (ok && (context < 0 || owned < 0 || owned > a.max_blocks || rows > a.max_rows ||
+               (a.tree_mask != nullptr && n > a.max_query_len))) {
       raise_error(a.err, kErrBadIndex);
       ok = false;
     }
-    int64_t need = 0;
+    int need = 0;
     if (ok && n > 0) {
-      need = (context + n + a.block_size - 1) / a.block_size - owned;
+      need = static_cast<int>((static_cast<uint32_t>(rows) + a.block_size - 1) /
+                              static_cast<uint32_t>(a.block_size)) - owned;
       if (need < 0) need = 0;
     }
-    const int64_t need_end = needed + block_scan(need, warp_sums, total);
-    needed += total;
-    const bool served = ok && (need == 0 || need_end <= have);
+    uint2 total;
+    uint2 end = block_scan(make_uint2(n, need), warp_sums, total);
+    end = make_uint2(add_up(end.x, tokens), add_up(end.y, needed));
+    if (ok && n > 0 && end.x > a.num_tokens) {
+      // past the tokens' room; so is every later request with a token, and their needs, counted
+      // in the sums above, come after those of all that are served
+      raise_error(a.err, kErrBadIndex);
+      ok = false;
+    }
+    const bool served = ok && (need == 0 || end.y <= have);
+    const int32_t start = static_cast<int32_t>(
+        end.x < a.num_tokens ? end.x : static_cast<uint32_t>(a.num_tokens));
     if (is) {
-      a.query_start_loc[s + 1] =
-          static_cast<int32_t>(tokens_end < a.num_tokens ? tokens_end : a.num_tokens);
-      a.seq_lens[s] = served ? static_cast<int32_t>(context + n) : 0;
-      a.blocks_owned_out[s] = query < 0 ? 0 : static_cast<int32_t>(served ? owned + need : owned);
+      a.query_start_loc[s + 1] = start;
+      if (a.fused) staged[s + 1] = start;
+      a.seq_lens[s] = served ? static_cast<int32_t>(rows) : 0;
+      a.blocks_owned_out[s] = query < 0 ? 0 : served ? owned + need : owned;
     }
-    if (total > 0) {
-      // needs are not negative, so the served ones among those with a need come first
-      sh_off[tid] = need_end - need;
-      sh_count[tid] = served ? static_cast<int32_t>(need) : 0;
-      sh_owned[tid] = static_cast<int32_t>(owned);
-      __syncthreads();
-      for (int k = warp; k < kPlanThreads; k += kPlanWarps) {
-        for (int i = lane; i < sh_count[k]; i += kWarpSize) {
-          a.block_tables[(base + k) * a.max_blocks + sh_owned[k] + i] =
-              a.free_blocks[have - 1 - sh_off[k] - i];
-        }
-      }
-      __syncthreads();
-    }
-    int64_t took;
-    block_scan(served ? need : 0, warp_sums, took);
-    used += took;
+    const int take = served ? need : 0;
+    if (take > 0) atomicMax(&used, static_cast<int>(end.y));  // the served needs come first
+    const int64_t top = have - 1 - (static_cast<int64_t>(end.y) - need);
+    int32_t* row = a.block_tables + static_cast<int64_t>(s) * a.max_blocks + owned;
+    copy_blocks(take, a.free_blocks + top, -1, row);
+    tokens = add_up(tokens, total.x);
+    needed = add_up(needed, total.y);
   }
   if (tid == 0) {
     a.query_start_loc[0] = 0;
-    a.free_count_out[0] = static_cast<int32_t>(have - used);
+    if (a.fused) staged[0] = 0;
   }
+  __syncthreads();
+  if (tid == 0) a.free_count_out[0] = static_cast<int32_t>(have - used);
   if (a.fused) {
-    __syncthreads();
-    for (int64_t t = tid; t < a.num_tokens; t += kPlanThreads) plan_token(a, t);
+    for (int t = tid; t < a.num_tokens; t += threads) {
+      plan_token(a, t, staged, staged + n_seqs + 1);
+    }
   }
 }
 
 __global__ void __launch_bounds__(kTokenThreads) plan_tokens_kernel(const PlanArgs a) {
   grid_dependency_sync();
+  __shared__ int32_t staged[kStagedStarts + 1];
+  const int n_seqs = static_cast<int>(a.num_seqs);
+  const int32_t* starts = a.query_start_loc;
+  if (n_seqs <= kStagedStarts) {
+    for (int s = threadIdx.x; s <= n_seqs; s += kTokenThreads) staged[s] = starts[s];
+    __syncthreads();
+    starts = staged;
+  }
   const int64_t t = static_cast<int64_t>(blockIdx.x) * kTokenThreads + threadIdx.x;
-  if (t < a.num_tokens) plan_token(a, t);
+  if (t < a.num_tokens) plan_token(a, static_cast<int>(t), starts, a.parents);
 }
 
 }  // namespace
@@ -274,8 +336,8 @@ extern "C" int svllm_paged_plan(
     return SVLLM_ERR_INVALID_ARGUMENT;
   }
   constexpr int64_t kMax = int64_t{1} << 31;
-  if (num_seqs >= kMax / kTokenThreads || num_tokens >= kMax || max_blocks >= kMax ||
-      block_size >= kMax || free_capacity >= kMax ||
+  if (num_seqs >= kMax / kTokenThreads || num_tokens >= kMax - 1 || max_blocks >= kMax ||
+      block_size >= kMax || max_blocks * block_size >= kMax || free_capacity >= kMax ||
       (parents != nullptr && max_query_len > SVLLM_MAX_TREE_NODES)) {
     return SVLLM_ERR_TOO_LARGE;
   }
@@ -302,15 +364,23 @@ extern "C" int svllm_paged_plan(
   a.num_seqs = num_seqs;
   a.num_tokens = num_tokens;
   a.free_capacity = free_capacity;
+  a.max_rows = max_blocks * block_size;
   a.max_blocks = static_cast<int32_t>(max_blocks);
   a.block_size = static_cast<int32_t>(block_size);
   a.max_query_len = static_cast<int32_t>(max_query_len);
   a.mask_words = parents != nullptr ? static_cast<int32_t>((max_query_len + 63) / 64) : 0;
-  a.fused = num_tokens <= kFusedTokens;
+  a.fused = num_tokens <= kFusedTokens && num_seqs <= kPlanThreads;
   a.err = err;
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const int status =
-      launch(plan_requests_kernel, dim3(1), dim3(kPlanThreads), 0, st, 1u, a);
+  // a thread per request, and where the tokens are done here too up to 256 for them
+  int64_t threads = a.fused ? (num_tokens < 256 ? num_tokens : 256) : 1;
+  if (threads < num_seqs) threads = num_seqs;
+  if (threads < 1) threads = 1;
+  threads = threads > kPlanThreads ? kPlanThreads : round_up(threads, kWarpSize);
+  const size_t staged =
+      a.fused ? 4 * static_cast<size_t>(num_seqs + 1 + (parents != nullptr ? num_tokens : 0)) : 0;
+  const int status = launch(plan_requests_kernel, dim3(1), dim3(static_cast<unsigned>(threads)),
+                            staged, st, 1u, a);
   if (status != SVLLM_OK || a.fused) return status;
   return launch(plan_tokens_kernel,
                 dim3(static_cast<unsigned>((num_tokens + kTokenThreads - 1) / kTokenThreads)),

@@ -18,16 +18,17 @@
 // lengths. An item cut by a share's border leaves unnormalised partial sums in the workspace, which
 // a second small kernel joins.
 //
-// In a CTA: four warps bring K and V rows through the block table with TMA into 128-byte-swizzled
-// tiles (any block size: a page may end anywhere in a tile); one thread issues tcgen05.mma: S = Q K^T into TMEM, then O += P V with P read from TMEM and V as
-// the N-major operand, alternating between two accumulators so that the tensor pipe works on one M
-// tile while the other's softmax runs; two groups of 4 warps do the softmax, one thread per row,
-// and write P (bf16, as the second product takes it) over S. The running maximum is a reference
-// that moves only when a row exceeds it by 2^8, so O in TMEM is seldom rescaled; the sums are fp32
-// and the result does not depend on the reference. Masked scores are replaced after the product.
-// Two helper warps bring the query rows and, since 0 * NaN would reach rows that do not see it,
-// zero the values of V that are not finite in the tiles that hold tree nodes; they are added
-// again, for the rows that see them, at the end.
+// In a CTA: two warps bring K and V rows through the block table with TMA into 128-byte-swizzled
+// tiles (any block size: a page may end anywhere in a tile); one thread issues tcgen05.mma: S = Q
+// K^T into TMEM, then O += P V with P read from TMEM and V as the N-major operand, alternating
+// between two accumulators so that the tensor pipe works on one M tile while the other's softmax
+// runs; two groups of 4 warps do the softmax, one thread per row, and write P (bf16, as the second
+// product takes it) over S. The running maximum is a reference that moves only when a row exceeds
+// it by 2^8, so O in TMEM is seldom rescaled; the sums are fp32 and the result does not depend on
+// the reference. Masked scores are replaced after the product. Four helper warps bring the query
+// rows and, since 0 * NaN would reach rows that do not see it, zero the values of V that are not
+// finite in the tiles that hold tree nodes; they are added again, for the rows that see them, at
+// the end. One warp lists the CTA's segments for all others.
 #include <cuda_runtime.h>
 
 #include <cmath>

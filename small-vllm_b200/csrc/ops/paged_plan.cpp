@@ -3,6 +3,7 @@
 #include <ATen/ATen.h>
 #include <c10/util/Exception.h>
 
+#include "ops/common.h"
 #include "ops/paged_plan_kernels.h"
 #include "svllm_kernels.h"
 
@@ -53,15 +54,19 @@ PagedPlan paged_plan(const at::Tensor& context_lens, const at::Tensor& query_len
   p.num_tokens = num_tokens;
   p.block_size = block_size;
   p.max_query_len = max_query_len;
-  p.query_start_loc = at::empty({requests + 1}, i32);
-  p.seq_lens = at::empty({requests}, i32);
-  p.slot_mapping = at::empty({num_tokens}, i64);
-  p.positions = at::empty({num_tokens}, i64);
-  p.blocks_owned_out = at::empty({requests}, i32);
-  p.free_count_out = at::empty({1}, i32);
+  // one allocation for each index type
+  const at::Tensor ints = at::empty({3 * requests + 2}, i32);
+  p.query_start_loc = detail::carve(ints, 0, {requests + 1});
+  p.seq_lens = detail::carve(ints, requests + 1, {requests});
+  p.blocks_owned_out = detail::carve(ints, 2 * requests + 1, {requests});
+  p.free_count_out = detail::carve(ints, 3 * requests + 1, {1});
+  const int64_t words = tree ? (max_query_len + 63) / 64 : 0;
+  const at::Tensor longs = at::empty({(2 + words) * num_tokens}, i64);
+  p.slot_mapping = detail::carve(longs, 0, {num_tokens});
+  p.positions = detail::carve(longs, num_tokens, {num_tokens});
   if (tree) {
     p.parents = *parents;
-    p.tree_mask = at::empty({num_tokens, (max_query_len + 63) / 64}, i64);
+    p.tree_mask = detail::carve(longs, 2 * num_tokens, {num_tokens, words});
   }
   switch (context_lens.device().type()) {
     case c10::DeviceType::CPU:

@@ -3,6 +3,7 @@
 #include <ATen/ATen.h>
 #include <c10/util/Exception.h>
 
+#include "ops/common.h"
 #include "ops/tree_accept_kernels.h"
 #include "svllm_kernels.h"
 
@@ -47,10 +48,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> tree_accept(
   a.seq_lens = seq_lens;
   a.context_lens = context_lens;
   a.max_query_len = max_query_len;
-  a.path = at::empty({requests, max_query_len}, seq_lens.options());
+  // one allocation for each type of output
+  const at::Tensor ints = at::empty({requests * (max_query_len + 2)}, seq_lens.options());
+  a.path = detail::carve(ints, 0, {requests, max_query_len});
+  a.num_accepted = detail::carve(ints, requests * max_query_len, {requests});
+  a.context_lens_out = detail::carve(ints, requests * (max_query_len + 1), {requests});
   a.tokens = at::empty({requests, max_query_len}, targets.options());
-  a.num_accepted = at::empty({requests}, seq_lens.options());
-  a.context_lens_out = at::empty({requests}, seq_lens.options());
   switch (device.type()) {
     case c10::DeviceType::CPU:
       cpu_impl::tree_accept(a);
