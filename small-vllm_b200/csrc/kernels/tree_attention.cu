@@ -217,7 +217,10 @@ struct Sync {
   uint64_t bar[kBarriers];
   uint32_t tmem_base;
   int abort;
-  int odd_values[2][4];  // per accumulator and segment modulo 4: V held something not finite
+  // per helper warp, accumulator and segment modulo 8: V held something not finite. A warp clears its
+  // own word when it begins a segment; no warp is more than kSegments behind another then, so nobody
+  // still reads the one that the segment 8 before left there.
+  int odd_values[kHelperWarps][2][2 * kSegments];
   int costs[kWarps];     // of the warps' shares of the requests
   Segment list[kSegments];
 };
@@ -575,6 +578,8 @@ __device__ __forceinline__ void help(const TreeAttnArgs& a, Sync& sy, uint8_t* q
   for (int index = 0; ok && next_segment(a, sy, index, g); ++index) {
     ok = wait(kEmptyQ, (index & 1) ^ 1);
     if (!ok) break;
+    if (lane < 2) sy.odd_values[warp][lane][index % (2 * kSegments)] = 0;
+    __syncwarp();
 #pragma unroll 1
     for (int w = 0; w < g.active; ++w) {
 #pragma unroll 1
@@ -631,8 +636,8 @@ __device__ __forceinline__ void help(const TreeAttnArgs& a, Sync& sy, uint8_t* q
               }
             }
             if (odd) {
-              sy.odd_values[w][index & 3] = 1;
-              if (g.shared) sy.odd_values[1][index & 3] = 1;
+              sy.odd_values[warp][w][index % (2 * kSegments)] = 1;
+              if (g.shared) sy.odd_values[warp][1][index % (2 * kSegments)] = 1;
             }
             fence_proxy_async_smem();
             mbar_arrive(&sy.bar[kChecked + ring_at.slot]);
@@ -776,7 +781,6 @@ __device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w) 
   Segment g;
 #pragma unroll 1
   for (int index = 0; next_segment(a, sy, index, g); ++index) {
-    if (threadIdx.x % (4 * kWarpSize) == 0) sy.odd_values[w][(index + 2) & 3] = 0;
     if (w >= g.active) continue;
     const int lane0 = w == 0 ? 0 : g.lane0;
     const int row = quarter * kWarpSize + threadIdx.x % kWarpSize - lane0;
@@ -891,7 +895,11 @@ __device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w) 
       }
     }
     if (any) {
-      const bool odd = static_cast<volatile int*>(sy.odd_values[w])[index & 3] != 0;
+      int odd = 0;
+#pragma unroll
+      for (int h = 0; h < kHelperWarps; ++h) {
+        odd |= *static_cast<volatile int*>(&sy.odd_values[h][w][index % (2 * kSegments)]);
+      }
       const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
       __nv_bfloat16* out =
           static_cast<__nv_bfloat16*>(a.out) +
@@ -985,10 +993,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&sy.bar[tid], arrivals(tid));
     fence_mbar_init();
   }
-  if (tid == 0) {
-    sy.abort = 0;
-    for (int i = 0; i < 8; ++i) sy.odd_values[i / 4][i % 4] = 0;
-  }
+  if (tid == 0) sy.abort = 0;
   if (warp == kMmaWarp) tmem_alloc(&sy.tmem_base, kTmemColumns);
 
   grid_dependency_sync();
@@ -1285,38 +1290,40 @@ extern "C" int svllm_tree_attention_bf16(
   using namespace svllm::k;
   if (num_seqs < 0 || num_tokens < 0 || num_heads <= 0 || num_kv_heads <= 0 ||
       num_heads % num_kv_heads != 0 || head_dim <= 0 || block_size <= 0 || max_blocks <= 0 ||
-      num_blocks <= 0 || q_token_stride < num_heads * head_dim || !(scale > 0.0f) ||
-      !std::isfinite(scale) || (tree_mask != nullptr && mask_words <= 0)) {
+      num_blocks <= 0 || !(scale > 0.0f) || !std::isfinite(scale * 2.0f) ||
+      (tree_mask != nullptr && mask_words <= 0)) {
     return SVLLM_ERR_INVALID_ARGUMENT;
   }
+  if (head_dim != 64 && head_dim != 128) return SVLLM_ERR_UNSUPPORTED;
+  constexpr int64_t kMax = int64_t{1} << 31;
+  if (num_seqs >= kMax || num_tokens >= kMax || num_heads >= (int64_t{1} << 20) ||
+      num_tokens * num_heads >= kMax || max_blocks >= kMax || num_blocks >= kMax ||
+      block_size >= (int64_t{1} << 20) || max_blocks * block_size >= kMax ||
+      num_blocks * block_size >= kMax ||
+      (tree_mask != nullptr && mask_words > SVLLM_MAX_TREE_NODES / 64)) {
+    return SVLLM_ERR_TOO_LARGE;
+  }
+  if (q_token_stride < num_heads * head_dim) return SVLLM_ERR_INVALID_ARGUMENT;
   if (num_tokens == 0) return SVLLM_OK;
   if (out == nullptr || q == nullptr || k_cache == nullptr || v_cache == nullptr ||
       query_start_loc == nullptr ||
       (num_seqs > 0 && (block_tables == nullptr || seq_lens == nullptr))) {
     return SVLLM_ERR_INVALID_ARGUMENT;
   }
-  if ((head_dim != 64 && head_dim != 128) || !aligned16(out) || !aligned16(q) ||
-      !aligned16(k_cache) || !aligned16(v_cache) || (q_token_stride * 2) % 16 != 0) {
+  if (!aligned16(out) || !aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) ||
+      (q_token_stride * 2) % 16 != 0) {
     return SVLLM_ERR_UNSUPPORTED;
   }
-  constexpr int64_t kMax = int64_t{1} << 31;
-  if (num_seqs >= kMax || num_tokens * num_heads >= kMax || max_blocks >= kMax ||
-      block_size >= (int64_t{1} << 20) || max_blocks * block_size >= kMax ||
-      num_blocks >= kMax || num_kv_heads >= (int64_t{1} << 20) ||
-      num_blocks * block_size >= kMax ||
-      (tree_mask != nullptr && mask_words > SVLLM_MAX_TREE_NODES / 64)) {
-    return SVLLM_ERR_TOO_LARGE;
-  }
+  // the line of steps is counted in 32 bits: its length is at most this
+  const int64_t most = (max_blocks * block_size / 128 + 1) * num_kv_heads;
+  const int64_t tiles = num_tokens * (num_heads / num_kv_heads) / 128 + num_seqs;
+  if (most >= kMax || tiles >= kMax / most) return SVLLM_ERR_TOO_LARGE;
   int64_t needed = 0;
   const int sized = svllm_tree_attention_workspace_bytes(head_dim, &needed);
   if (sized != SVLLM_OK) return sized;
   if (workspace == nullptr || workspace_size < needed || !aligned16(workspace)) {
     return SVLLM_ERR_INVALID_ARGUMENT;
   }
-  // the line of steps is counted in 32 bits: its length is at most this
-  const int64_t most = (max_blocks * block_size / 128 + 1) * num_kv_heads;
-  const int64_t tiles = num_tokens * (num_heads / num_kv_heads) / 128 + num_seqs;
-  if (most >= kMax || tiles >= kMax / most) return SVLLM_ERR_TOO_LARGE;
   int device;
   if (current_device(&device) != SVLLM_OK) return SVLLM_ERR_CUDA;
   int* err = library_error_word(device);
