@@ -258,49 +258,57 @@ __device__ __forceinline__ bool warp_wait(Sync& sy, int bar, uint32_t parity, in
   }
 }
 
-// The borders of this CTA's share of the line. `cost`: lane i holds the cost of the i-th `chunk` of
-// requests.
-__device__ __forceinline__ void find_share(const TreeAttnArgs& a, int cost, int chunk, int lane,
-                                           Place (&places)[2]) {
-  int upto = cost;
+// Inclusive sum over the warp's lanes.
+__device__ __forceinline__ int sum_up_to_lane(int v, int lane) {
 #pragma unroll
   for (int off = 1; off < kWarpSize; off *= 2) {
-    const int up = __shfl_up_sync(0xffffffffu, upto, off);
-    if (lane >= off) upto += up;
+    const int up = __shfl_up_sync(0xffffffffu, v, off);
+    if (lane >= off) v += up;
   }
+  return v;
+}
+
+// The borders of this CTA's share of the line. `own`: lane i holds the cost of the i-th `chunk` of
+// requests; with a chunk of 1, `r` is the lane's request.
+__device__ __forceinline__ void find_share(const TreeAttnArgs& a, Request r, int own, int chunk,
+                                           int lane, Place (&places)[2]) {
+  const int upto = sum_up_to_lane(own, lane);
   const int total = __shfl_sync(0xffffffffu, upto, kWarpSize - 1);
-  // at least two steps each: a shorter share costs more in the join than it saves
+  // at least two steps each: a shorter share costs more in the join than it saves (1 request of 8
+  // nodes over 128 rows: 12.7 us with 2, 16.4 with 4; 13 requests of up to 37 nodes 27 and 38)
   const int share = max(2, static_cast<int>((total + gridDim.x - 1u) / gridDim.x));
 #pragma unroll 1
   for (int e = 0; e < 2; ++e) {
     const int64_t border = static_cast<int64_t>(blockIdx.x + e) * share;
     Place p{a.num_seqs, 0, 0};
     if (border < total) {
-      // the warp's share of the requests that holds it, then the request
-      const int c = __ffs(static_cast<int>(__ballot_sync(0xffffffffu, border < upto))) - 1;
-      int before = c > 0 ? __shfl_sync(0xffffffffu, upto, c - 1) : 0;
+      // the lane whose chunk of requests holds it, then the request
+      int owner = __ffs(static_cast<int>(__ballot_sync(0xffffffffu, border < upto))) - 1;
+      int before = __shfl_sync(0xffffffffu, upto - own, owner);
+      int s = owner, cost = own;
+      if (chunk > 1) {
+        const int end = min(a.num_seqs, (owner + 1) * chunk);
 #pragma unroll 1
-      for (int s0 = c * chunk;; s0 += kWarpSize) {
-        Request r{};
-        if (s0 + lane < min(a.num_seqs, (c + 1) * chunk)) r = load_request(a, s0 + lane);
-        const int own = request_cost(a, r);
-        int sum = own;
-#pragma unroll
-        for (int off = 1; off < kWarpSize; off *= 2) {
-          const int up = __shfl_up_sync(0xffffffffu, sum, off);
-          if (lane >= off) sum += up;
+        for (int s0 = owner * chunk;; s0 += kWarpSize) {
+          s = s0 + lane;
+          r = Request{};
+          if (s < end) r = load_request(a, s);
+          cost = request_cost(a, r);
+          const int sum = before + sum_up_to_lane(cost, lane);
+          const unsigned past = __ballot_sync(0xffffffffu, border < sum);
+          if (past != 0) {
+            owner = __ffs(static_cast<int>(past)) - 1;
+            s = s0 + owner;
+            before = __shfl_sync(0xffffffffu, sum - cost, owner);
+            break;
+          }
+          before = __shfl_sync(0xffffffffu, sum, kWarpSize - 1);
         }
-        const unsigned past = __ballot_sync(0xffffffffu, border < before + sum);
-        if (past != 0) {
-          const int owner = __ffs(static_cast<int>(past)) - 1;
-          if (lane == owner) p = locate(a, s0 + lane, r, static_cast<int>(border) - (before + sum - own));
-          p.s = __shfl_sync(0xffffffffu, p.s, owner);
-          p.item = __shfl_sync(0xffffffffu, p.item, owner);
-          p.step = __shfl_sync(0xffffffffu, p.step, owner);
-          break;
-        }
-        before += __shfl_sync(0xffffffffu, sum, kWarpSize - 1);
       }
+      if (lane == owner) p = locate(a, s, r, static_cast<int>(border) - before);
+      p.s = __shfl_sync(0xffffffffu, p.s, owner);
+      p.item = __shfl_sync(0xffffffffu, p.item, owner);
+      p.step = __shfl_sync(0xffffffffu, p.step, owner);
     }
     if (e == 0) places[0] = p;
     places[1] = p;
@@ -905,12 +913,13 @@ __device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w) 
           static_cast<__nv_bfloat16*>(a.out) +
           ((token * a.num_kv_heads + pick(g.kv_head, w) - node) * a.group + at_row) * D;
 #pragma unroll 1
-      for (int c = 0; c < D; c += 16) {
-        uint32_t x[16];
-        tmem_load16(output + c, x);
-        float o[16];
+      for (int c = 0; c < D; c += 32) {
+        uint32_t x[32];
+        tmem_load32(output + c, x);
+        tmem_wait_load();
+        float o[32];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[i] = __uint_as_float(x[i]);
+        for (int i = 0; i < 32; ++i) o[i] = __uint_as_float(x[i]);
         if (odd && valid) {
           // V values that are not finite, of the rows this node sees: the weights are positive
           const int first = max(g.step0 * kTile, g.context);
@@ -925,7 +934,7 @@ __device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w) 
                             ((block * a.block_size + (j - page * a.block_size)) *
                                  a.num_kv_heads + pick(g.kv_head, w)) * D + c;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
+            for (int i = 0; i < 32; ++i) {
               const uint32_t bits = static_cast<uint32_t>(v[i]) << 16;
               if ((bits & 0x7f800000u) == 0x7f800000u) o[i] += __uint_as_float(bits);
             }
@@ -933,7 +942,7 @@ __device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w) 
         }
         if (cut && valid) {
 #pragma unroll
-          for (int i = 0; i < 16; i += 4) {
+          for (int i = 0; i < 32; i += 4) {
             *reinterpret_cast<float4*>(part + (((c + i) / 4) * kTile + row) * 4) =
                 make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
           }
@@ -941,7 +950,7 @@ __device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w) 
           // a sum of zero: the node saw no row
           float f[8];
 #pragma unroll
-          for (int i = 0; i < 16; i += 8) {
+          for (int i = 0; i < 32; i += 8) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e] = sum == 0.0f ? 0.0f : o[i + e] * inverse;
             st_global_v4(out + c + i, pack<Bf16>(f));
@@ -1018,13 +1027,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   Place places[2]{};
   if (warp == kPlanWarp) {
+    Request r{};
     int cost = 0;
     if (!few) {
       if (lane < kWarps) cost = sy.costs[lane];
     } else if (lane < a.num_seqs) {
-      cost = request_cost(a, load_request(a, lane));
+      r = load_request(a, lane);
+      cost = request_cost(a, r);
     }
-    find_share(a, cost, chunk, lane, places);
+    find_share(a, r, cost, chunk, lane, places);
   }
   tc_fence_before();
   __syncthreads();
@@ -1261,7 +1272,8 @@ int launch_tree_attention(TreeAttnArgs& a, void* workspace, int device, cudaStre
   }
   const int status = launch(tree_attention_kernel<D>, dim3(ctas), dim3(kThreads),
                                        Shape<D>::kSmem, stream, 1u, map_k, map_v, a);
-  if (status != SVLLM_OK || ctas < 2) return status;
+  // where no table holds more than a tile of rows, items have one step and no border cuts one
+  if (status != SVLLM_OK || ctas < 2 || a.max_length <= kTile) return status;
   return launch(tree_attention_join_kernel<D>, dim3(4 * ctas), dim3(kJoinRows * D / 4), 0, stream,
                 1u, a, ctas);
 }
