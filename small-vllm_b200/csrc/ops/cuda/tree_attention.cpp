@@ -1,5 +1,6 @@
 // CUDA side of ops::tree_attention: a thin LibTorch -> C ABI shim.
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -19,7 +20,7 @@ void tree_attention(const at::Tensor& out, const at::Tensor& q, const at::Tensor
   int64_t bytes = 0;
   detail::check_status("tree_attention", svllm_tree_attention_workspace_bytes(dim, &bytes));
   // from the caching allocator per call: calls on other streams, and captured graphs, get their own
-  const at::Tensor workspace = at::empty({bytes}, q.options().dtype(at::kByte));
+  const c10::DataPtr workspace = c10::cuda::CUDACachingAllocator::get()->allocate(bytes);
   detail::check_status(
       "tree_attention",
       svllm_tree_attention_bf16(
@@ -30,7 +31,7 @@ void tree_attention(const at::Tensor& out, const at::Tensor& q, const at::Tensor
           seq_lens.numel(), tokens, heads, k_cache.size(2), dim,
           tree_mask.defined() ? tree_mask.const_data_ptr<int64_t>() : nullptr,
           tree_mask.defined() ? tree_mask.size(1) : 0, static_cast<float>(scale),
-          workspace.mutable_data_ptr(), bytes, stream));
+          workspace.get(), bytes, stream));
 }
 
 }  // namespace svllm::ops::cuda_impl

@@ -42,8 +42,6 @@ PagedPlan paged_plan(const at::Tensor& context_lens, const at::Tensor& query_len
                 SVLLM_MAX_TREE_NODES, "] where parents are given");
   }
 
-  const auto i32 = context_lens.options();
-  const auto i64 = i32.dtype(at::kLong);
   PagedPlanTensors p;
   p.context_lens = context_lens;
   p.query_lens = query_lens;
@@ -54,20 +52,23 @@ PagedPlan paged_plan(const at::Tensor& context_lens, const at::Tensor& query_len
   p.num_tokens = num_tokens;
   p.block_size = block_size;
   p.max_query_len = max_query_len;
-  // one allocation for each index type
-  const at::Tensor ints = at::empty({3 * requests + 2}, i32);
-  p.query_start_loc = detail::carve(ints, 0, {requests + 1});
-  p.seq_lens = detail::carve(ints, requests + 1, {requests});
-  p.blocks_owned_out = detail::carve(ints, 2 * requests + 1, {requests});
-  p.free_count_out = detail::carve(ints, 3 * requests + 1, {1});
   const int64_t words = tree ? (max_query_len + 63) / 64 : 0;
-  const at::Tensor longs = at::empty({(2 + words) * num_tokens}, i64);
-  p.slot_mapping = detail::carve(longs, 0, {num_tokens});
-  p.positions = detail::carve(longs, num_tokens, {num_tokens});
+  using detail::Outputs;
+  Outputs out(Outputs::size(at::kLong, num_tokens) * 2 +
+                  Outputs::size(at::kLong, num_tokens * words) +
+                  Outputs::size(at::kInt, requests + 1) + Outputs::size(at::kInt, requests) * 2 +
+                  Outputs::size(at::kInt, 1),
+              context_lens.options());
+  p.slot_mapping = out.take(at::kLong, {num_tokens});
+  p.positions = out.take(at::kLong, {num_tokens});
   if (tree) {
     p.parents = *parents;
-    p.tree_mask = detail::carve(longs, 2 * num_tokens, {num_tokens, words});
+    p.tree_mask = out.take(at::kLong, {num_tokens, words});
   }
+  p.query_start_loc = out.take(at::kInt, {requests + 1});
+  p.seq_lens = out.take(at::kInt, {requests});
+  p.blocks_owned_out = out.take(at::kInt, {requests});
+  p.free_count_out = out.take(at::kInt, {1});
   switch (context_lens.device().type()) {
     case c10::DeviceType::CPU:
       cpu_impl::paged_plan(p);

@@ -48,12 +48,15 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> tree_accept(
   a.seq_lens = seq_lens;
   a.context_lens = context_lens;
   a.max_query_len = max_query_len;
-  // one allocation for each type of output
-  const at::Tensor ints = at::empty({requests * (max_query_len + 2)}, seq_lens.options());
-  a.path = detail::carve(ints, 0, {requests, max_query_len});
-  a.num_accepted = detail::carve(ints, requests * max_query_len, {requests});
-  a.context_lens_out = detail::carve(ints, requests * (max_query_len + 1), {requests});
-  a.tokens = at::empty({requests, max_query_len}, targets.options());
+  using detail::Outputs;
+  Outputs out(Outputs::size(at::kLong, requests * max_query_len) +
+                  Outputs::size(at::kInt, requests * max_query_len) +
+                  Outputs::size(at::kInt, requests) * 2,
+              targets.options());
+  a.tokens = out.take(at::kLong, {requests, max_query_len});
+  a.path = out.take(at::kInt, {requests, max_query_len});
+  a.num_accepted = out.take(at::kInt, {requests});
+  a.context_lens_out = out.take(at::kInt, {requests});
   switch (device.type()) {
     case c10::DeviceType::CPU:
       cpu_impl::tree_accept(a);
