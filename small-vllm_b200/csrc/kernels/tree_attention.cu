@@ -1085,23 +1085,37 @@ struct JoinItem {
   int mark;                      // of the first cut
 };
 
-constexpr int kJoinUnits = 2 * kTile / kJoinRows;  // per item: 8 rows of one accumulator each
+// 8 rows of one accumulator of an item. Units are counted row group by row group over all items, so
+// that those with rows lie together and spread over the blocks.
+struct JoinUnit {
+  int item, w, row0;
+};
+
+__device__ __forceinline__ JoinUnit join_unit(int unit, int items) {
+  const int group = unit / (2 * items), rest = unit - group * 2 * items;
+  return JoinUnit{rest >> 1, rest & 1, group * kJoinRows};
+}
 
 // kUnits units at once, kBatch segments of each at a time, all their loads before any use; a thread
 // does 16 bytes of a row. With m and l the maxima and sums of the segments, M the largest m:
 //   o = sum 2^(m - M) O / sum 2^(m - M) l.
 template <int D, int kUnits, int kBatch>
-__device__ __forceinline__ void join_units(const TreeAttnArgs& a, const JoinItem* items, int unit,
-                                           int stride) {
+__device__ __forceinline__ void join_units(const TreeAttnArgs& a, const JoinItem* items,
+                                           const JoinUnit (&units)[kUnits]) {
   using S = Shape<D>;
   const float kInf = __builtin_huge_valf();
   const int piece = threadIdx.x / kJoinRows;
-  int most = 0;
+  int most = 0, token0[kUnits], kv_head[kUnits], row0[kUnits];
   float top[kUnits], sum[kUnits];
   float4 o[kUnits];
 #pragma unroll
   for (int u = 0; u < kUnits; ++u) {
-    most = max(most, items[(unit + u * stride) / kJoinUnits].segments);
+    const JoinItem& it = items[units[u].item];
+    const Cut& c = a.cuts[it.first];
+    token0[u] = c.token0;
+    kv_head[u] = c.kv_head[units[u].w];
+    row0[u] = c.row0[units[u].w];
+    most = max(most, it.segments);
     top[u] = -kInf;
     sum[u] = 0.0f;
     o[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -1112,17 +1126,15 @@ __device__ __forceinline__ void join_units(const TreeAttnArgs& a, const JoinItem
     float4 x[kUnits][kBatch];
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
-      const JoinItem& it = items[(unit + u * stride) / kJoinUnits];
-      const int w = (unit + u * stride) % kJoinUnits / (kJoinUnits / 2);
-      const int row = (unit + u * stride) % (kJoinUnits / 2) * kJoinRows +
-                      threadIdx.x % kJoinRows;
+      const JoinItem& it = items[units[u].item];
+      const int row = units[u].row0 + threadIdx.x % kJoinRows;
 #pragma unroll
       for (int e = 0; e < kBatch; ++e) {
         m[u][e] = -kInf;
         l[u][e] = 0.0f;
         if (i0 + e < it.segments) {
           const int64_t slot = i0 + e == 0 ? it.first : (it.border - 1 + i0 + e) * 2;
-          const float* p = a.parts + (slot * 2 + w) * S::kPartFloats + row;
+          const float* p = a.parts + (slot * 2 + units[u].w) * S::kPartFloats + row;
           m[u][e] = ld_global_f32(p + D * kTile);
           l[u][e] = ld_global_f32(p + (D + 1) * kTile);
           x[u][e] = ld_global_f32x4(p + piece * kTile * 4 + row * 3);
@@ -1154,16 +1166,12 @@ __device__ __forceinline__ void join_units(const TreeAttnArgs& a, const JoinItem
   }
 #pragma unroll
   for (int u = 0; u < kUnits; ++u) {
-    const JoinItem& it = items[(unit + u * stride) / kJoinUnits];
-    const int w = (unit + u * stride) % kJoinUnits / (kJoinUnits / 2);
-    const int row =
-        (unit + u * stride) % (kJoinUnits / 2) * kJoinRows + threadIdx.x % kJoinRows;
-    if (row >= cut_rows(it.mark, w)) continue;
-    const Cut& c = a.cuts[it.first];
-    const int at_row = c.row0[w] + row;
+    const int row = units[u].row0 + threadIdx.x % kJoinRows;
+    if (row >= cut_rows(items[units[u].item].mark, units[u].w)) continue;
+    const int at_row = row0[u] + row;
     const int node = a.by_group.divide(at_row);
     auto* out = static_cast<__nv_bfloat16*>(a.out) +
-                ((static_cast<int64_t>(c.token0 + node) * a.num_kv_heads + c.kv_head[w] - node) *
+                ((static_cast<int64_t>(token0[u] + node) * a.num_kv_heads + kv_head[u] - node) *
                      a.group + at_row) * D + piece * 4;
     const float inverse = sum[u] == 0.0f ? 0.0f : 1.0f / sum[u];
     if (sum[u] == 0.0f) o[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -1221,22 +1229,22 @@ __global__ void __launch_bounds__(kJoinRows * D / 4) tree_attention_join_kernel(
     __syncthreads();
   }
 
-  // units without a row are passed over
-  const auto empty = [&](int unit) {
-    return unit % (kJoinUnits / 2) * kJoinRows >=
-           cut_rows(items[unit / kJoinUnits].mark, unit % kJoinUnits / (kJoinUnits / 2));
+  const int total = count * 2 * (kTile / kJoinRows), stride = gridDim.x;
+  const auto has_rows = [&](const JoinUnit& u) {
+    return u.row0 < cut_rows(items[u.item].mark, u.w);
   };
-  const int total = count * kJoinUnits, stride = gridDim.x;
   for (int unit = blockIdx.x; unit < total; unit += stride) {
-    if (empty(unit)) continue;
-    const int next = unit + stride;
-    if (next < total && !empty(next) && items[unit / kJoinUnits].segments <= 4 &&
-        items[next / kJoinUnits].segments <= 4) {
-      join_units<D, 2, 4>(a, items, unit, stride);
-      unit = next;
-    } else {
-      join_units<D, 1, 8>(a, items, unit, stride);
+    const JoinUnit first = join_unit(unit, count);
+    if (!has_rows(first)) continue;
+    if (unit + stride < total) {
+      const JoinUnit next = join_unit(unit + stride, count);
+      if (has_rows(next) && items[first.item].segments <= 4 && items[next.item].segments <= 4) {
+        join_units<D, 2, 4>(a, items, {first, next});
+        unit += stride;
+        continue;
+      }
     }
+    join_units<D, 1, 8>(a, items, {first});
   }
 }
 
