@@ -374,15 +374,17 @@ int svllm_paged_plan(const int32_t* context_lens, const int32_t* query_lens, int
  * over the rows j < context and those of the nodes j - context whose bit tree_mask[t] has; with
  * tree_mask == NULL the nodes up to i (causal). Rows j as in svllm_paged_decode_attention_bf16,
  * likewise the cache, q (q_token_stride) and the block tables. out: [num_tokens, num_heads,
- * head_dim] contiguous. tree_mask: [num_tokens, mask_words] int64. A token that sees no row, every
- * token of a request with seq_lens 0, and every row of out behind the last request is zero. A value
- * that a token does not see never reaches its output, NaN and infinities included. bf16, fp32
+ * head_dim] contiguous, not overlapping q. tree_mask: [num_tokens, mask_words] int64. A token that
+ * sees no row, or no score above -infinity, every token of a request with seq_lens 0, and every row
+ * of out behind the last request is zero. A value that a token does not see never reaches its
+ * output, NaN and infinities included. bf16, fp32
  * softmax and accumulation, the softmax numerators rounded to bf16 for the second product.
  * head_dim 64 or 128, any number of query heads per KV head, 16-byte aligned out, q and caches, a
  * q_token_stride of whole 16 bytes, else SVLLM_ERR_UNSUPPORTED. scale must be positive and finite.
  * Zeros with SVLLM_DEVERR_BAD_INDEX: a request whose seq_lens is below its number of tokens or
  * past its block table, or whose tree is wider than the mask. With the same bit, a request whose
- * query_start_loc falls or ends past num_tokens has no rows (none of out is written for it). A
+ * query_start_loc falls or ends past num_tokens has no rows (none of out is written for it), nor
+ * has any request where those left overlap into more work than num_tokens tokens can be. A
  * table entry outside the cache raises the bit and reads block 0. workspace: at
  * least svllm_tree_attention_workspace_bytes bytes of device memory, 16-byte aligned, any
  * contents; calls that overlap on the GPU must not share it.
@@ -426,7 +428,8 @@ int svllm_tree_accept(const void* ids, int id_type, const int64_t* targets,
  * value, so the arrays may be freed when the call returns. path: [num_seqs, max_query_len]. A row
  * with a negative slot does not move. SVLLM_DEVERR_BAD_INDEX: a slot past num_slots (the row does
  * not move), a path that does not rise or leaves the request (no row from there on moves), a count
- * past the request's tokens (nothing of it moves). No two tokens of the step may share a slot.
+ * past the request's tokens (nothing of it moves). No two tokens of the step may share a slot, and no
+ * two caches memory: the same pointer twice is SVLLM_ERR_INVALID_ARGUMENT.
  */
 int svllm_tree_commit(void* const* k_caches, void* const* v_caches, int64_t num_layers,
                       int64_t num_slots, int64_t row_bytes, const int32_t* path,

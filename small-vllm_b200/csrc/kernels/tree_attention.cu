@@ -103,6 +103,7 @@ struct TreeAttnArgs {
   int max_blocks;
   int max_length;                  // rows that a block table holds
   int max_nodes;                   // nodes that the mask's words hold
+  int most_steps;                  // the longest line that requests without overlap make
   int block_size;
   Divider page;                    // by the block size
   int group;                       // query heads per KV head
@@ -153,6 +154,12 @@ __device__ __forceinline__ Request load_request(const TreeAttnArgs& a, int s) {
 // Steps of the line, weighted: a step over two KV heads loads twice what the others load.
 __device__ __forceinline__ int request_cost(const TreeAttnArgs& a, const Request& r) {
   return a.num_kv_heads * r.steps * (r.pairs + r.odd);
+}
+
+// Lengths come from the device unchecked: sums of costs stop at the largest int instead of wrapping.
+__device__ __forceinline__ int add_costs(int a, int b) {
+  return static_cast<int>(min(static_cast<unsigned>(a) + static_cast<unsigned>(b),
+                              static_cast<unsigned>(INT32_MAX)));
 }
 
 // A place on the line: request, item of the request, step of the item.
@@ -258,12 +265,12 @@ __device__ __forceinline__ bool warp_wait(Sync& sy, int bar, uint32_t parity, in
   }
 }
 
-// Inclusive sum over the warp's lanes.
+// Inclusive sum of costs over the warp's lanes.
 __device__ __forceinline__ int sum_up_to_lane(int v, int lane) {
 #pragma unroll
   for (int off = 1; off < kWarpSize; off *= 2) {
     const int up = __shfl_up_sync(0xffffffffu, v, off);
-    if (lane >= off) v += up;
+    if (lane >= off) v = add_costs(v, up);
   }
   return v;
 }
@@ -273,7 +280,11 @@ __device__ __forceinline__ int sum_up_to_lane(int v, int lane) {
 __device__ __forceinline__ void find_share(const TreeAttnArgs& a, Request r, int own, int chunk,
                                            int lane, Place (&places)[2]) {
   const int upto = sum_up_to_lane(own, lane);
-  const int total = __shfl_sync(0xffffffffu, upto, kWarpSize - 1);
+  int total = __shfl_sync(0xffffffffu, upto, kWarpSize - 1);
+  if (total > a.most_steps) {  // requests overlap: the starts fall somewhere. Nothing is done
+    if (lane == 0) raise_error(a.err, kErrBadIndex);
+    total = 0;
+  }
   // at least two steps each: a shorter share costs more in the join than it saves (1 request of 8
   // nodes over 128 rows: 12.7 us with 2, 16.4 with 4; 13 requests of up to 37 nodes 27 and 38)
   const int share = max(2, static_cast<int>((total + gridDim.x - 1u) / gridDim.x));
@@ -294,7 +305,7 @@ __device__ __forceinline__ void find_share(const TreeAttnArgs& a, Request r, int
           r = Request{};
           if (s < end) r = load_request(a, s);
           cost = request_cost(a, r);
-          const int sum = before + sum_up_to_lane(cost, lane);
+          const int sum = add_costs(before, sum_up_to_lane(cost, lane));
           const unsigned past = __ballot_sync(0xffffffffu, border < sum);
           if (past != 0) {
             owner = __ffs(static_cast<int>(past)) - 1;
@@ -1018,10 +1029,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     int cost = 0;
 #pragma unroll 1
     for (int s = warp * chunk + lane; s < min(a.num_seqs, (warp + 1) * chunk); s += kWarpSize) {
-      cost += request_cost(a, load_request(a, s));
+      cost = add_costs(cost, request_cost(a, load_request(a, s)));
     }
 #pragma unroll
-    for (int off = 16; off > 0; off /= 2) cost += __shfl_xor_sync(0xffffffffu, cost, off);
+    for (int off = 16; off > 0; off /= 2) {
+      cost = add_costs(cost, __shfl_xor_sync(0xffffffffu, cost, off));
+    }
     if (lane == 0) sy.costs[warp] = cost;
     __syncthreads();
   }
@@ -1366,6 +1379,7 @@ extern "C" int svllm_tree_attention_bf16(
   a.page = make_divider(block_size);
   a.group = static_cast<int>(num_heads / num_kv_heads);
   a.max_length = static_cast<int>(max_blocks * block_size);
+  a.most_steps = static_cast<int>(most * tiles);
   a.max_nodes = tree_mask != nullptr ? static_cast<int>(64 * mask_words) : INT32_MAX;
   a.by_group = make_divider(a.group);
   a.num_kv_heads = static_cast<int>(num_kv_heads);

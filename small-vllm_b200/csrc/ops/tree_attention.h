@@ -13,8 +13,8 @@ namespace svllm::ops {
 //             context and the nodes j - context whose bit tree_mask[t] has; without a mask the nodes
 //             up to t's own (causal). Row j of request b is row block_tables[b][j / block_size] *
 //             block_size + j % block_size of the cache, KV head h / (heads / KV heads); context =
-//             seq_lens[b] - (query_start_loc[b + 1] - query_start_loc[b]). A token that sees no row,
-//             a token of a request with seq_lens 0, and one behind the last request gets zeros.
+//             seq_lens[b] - (query_start_loc[b + 1] - query_start_loc[b]). A token that sees no row, or
+//             no score above -infinity, a token of a request with seq_lens 0, and one behind the last request gets zeros.
 //             What a token does not see never reaches its output, NaN and infinities included.
 // Domain:     q [T, heads, D] with contiguous heads (any token stride: a view of the qkv
 //             projection); k_cache, v_cache [blocks, block_size, KV heads, D] contiguous, heads a

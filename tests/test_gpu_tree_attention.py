@@ -201,6 +201,22 @@ def test_bad_lengths_and_blocks_raise_the_error_word(cuda):
     assert svllm_ops.read_device_error(0, True) == 1
 
 
+def test_requests_that_overlap_do_no_more_than_they_could(cuda):
+    """Starts that rise and fall 10000 times: 10000 requests of the same 4096 tokens over 32768
+    rows, 262144 steps each. Counted in 32 bits their sum would wrap; nothing of them runs."""
+    requests, tokens, bs = 20001, 4096, 32768
+    q = torch.ones(tokens, 64, 64, dtype=torch.bfloat16, device=cuda)
+    cache = torch.ones(1, bs, 8, 64, dtype=torch.bfloat16, device=cuda)
+    starts = torch.zeros(requests + 1, dtype=torch.int32, device=cuda)
+    starts[1::2] = tokens
+    seq = torch.full((requests,), bs, dtype=torch.int32, device=cuda)
+    tables = torch.zeros(requests, 1, dtype=torch.int32, device=cuda)
+    svllm_ops.read_device_error(0, True)
+    svllm_ops.tree_attention(q, cache, cache, tables, seq, starts)
+    torch.cuda.synchronize()
+    assert svllm_ops.read_device_error(0, True) == 1
+
+
 def test_on_another_stream_and_two_at_once(cuda):
     a = build(cuda, [33, 64, 9], [4000, 100, 2500], 16, 8, 128, 16, seed=1)
     b = build(cuda, [64] * 4, [3000] * 4, 16, 8, 128, 16, seed=2)
