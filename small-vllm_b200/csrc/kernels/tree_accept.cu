@@ -186,6 +186,36 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const Commi
   }
 }
 
+// Whether two of the planes K and V are the same: a small hash table of those seen, past its room
+// each against all before it (a model has a few dozen layers; up to 256 take the table).
+bool any_plane_twice(void* const* k, void* const* v, int64_t layers) {
+  constexpr int kSlots = 1024;
+  const auto plane = [&](int64_t i) { return i < layers ? k[i] : v[i - layers]; };
+  const void* seen[kSlots];
+  if (4 * layers > kSlots) {
+    for (int64_t i = 0; i < 2 * layers; ++i) {
+      for (int64_t j = 0; j < i; ++j) {
+        if (plane(i) == plane(j)) return true;
+      }
+    }
+    return false;
+  }
+  int slots = 32;
+  while (slots < 4 * layers) slots *= 2;
+  for (int i = 0; i < slots; ++i) seen[i] = nullptr;
+  for (int64_t i = 0; i < 2 * layers; ++i) {
+    const void* p = plane(i);
+    // the upper half of a product with an odd constant mixes the page bits down
+    int at = static_cast<int>((reinterpret_cast<uint64_t>(p) * 0x9e3779b97f4a7c15u) >> 40) &
+             (slots - 1);
+    for (; seen[at] != nullptr; at = (at + 1) & (slots - 1)) {
+      if (seen[at] == p) return true;
+    }
+    seen[at] = p;
+  }
+  return false;
+}
+
 }  // namespace
 }  // namespace svllm::k
 
@@ -258,6 +288,7 @@ extern "C" int svllm_tree_commit(void* const* k_caches, void* const* v_caches, i
       num_tokens >= (int64_t{1} << 31)) {
     return SVLLM_ERR_TOO_LARGE;
   }
+  if (any_plane_twice(k_caches, v_caches, num_layers)) return SVLLM_ERR_INVALID_ARGUMENT;
   int device;
   if (current_device(&device) != SVLLM_OK) return SVLLM_ERR_CUDA;
   int* err = library_error_word(device);

@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <cstring>
+#include <functional>
 #include <utility>
 #include <vector>
 
@@ -71,6 +72,13 @@ void tree_commit(const std::vector<at::Tensor>& k_caches, const std::vector<at::
   const auto* start = query_start_loc.const_data_ptr<int32_t>();
   const int64_t requests = num_accepted.numel(), width = path.size(1);
   check_starts("tree_commit", start, requests, slot_mapping.numel());
+  std::vector<const void*> planes;
+  for (const auto* caches : {&k_caches, &v_caches}) {
+    for (const at::Tensor& c : *caches) planes.push_back(c.const_data_ptr());
+  }
+  std::sort(planes.begin(), planes.end(), std::less<const void*>());
+  TORCH_CHECK(std::adjacent_find(planes.begin(), planes.end()) == planes.end(),
+              "tree_commit: invalid argument: a cache is given twice");
   std::vector<std::pair<int64_t, int64_t>> moves;  // source and destination, in order
   for (int64_t s = 0; s < requests; ++s) {
     const int64_t n = start[s + 1] - start[s];

@@ -36,7 +36,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> tree_accept(
 // Domain:     k_caches, v_caches: one contiguous [blocks, block_size, KV heads, D] (or [slots, KV
 //             heads, D]) tensor per layer, all of one shape and dtype (on CUDA, rows of whole 16
 //             bytes); path and num_accepted as tree_accept returns them; slot_mapping [T] int64 and
-//             query_start_loc [S + 1] int32 of the step, no slot in it twice.
+//             query_start_loc [S + 1] int32 of the step, no slot in it twice. No two caches share memory;
+//             the same one twice is refused.
 // Throws:     c10::Error on dtype, shape, layout or device mismatches, and on CPU for a path or slot
 //             out of range; on CUDA those raise the device error word and the rows do not move.
 void tree_commit(const std::vector<at::Tensor>& k_caches, const std::vector<at::Tensor>& v_caches,

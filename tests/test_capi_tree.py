@@ -94,6 +94,14 @@ def test_bad_arguments(call, change, status):
     assert call(**change) == status
 
 
+def test_a_cache_given_twice():
+    assert commit() == INVALID  # K and V the same
+    planes = (ctypes.c_void_p * 400)(*(P + 16 * i for i in range(400)))
+    for layers in (2, 200):
+        at = [ctypes.cast(ctypes.byref(planes, 8 * i), ctypes.c_void_p) for i in (0, layers - 1)]
+        assert commit(k_caches=at[0], v_caches=at[1], num_layers=layers) == INVALID
+
+
 def test_nothing_to_do_is_ok():
     assert attention(num_tokens=0) == 0
     assert accept(num_seqs=0) == 0

@@ -307,6 +307,19 @@ def test_tree_commit_rejects_bad_inputs():
             call(**change)
 
 
+def test_tree_commit_refuses_a_cache_given_twice(device):
+    """Its rows would move twice. 1 to 300 layers: a table of the caches seen, then all pairs."""
+    small = [torch.zeros(2, 4, 1, 8, device=device) for _ in range(600)]
+    lists = (i32([[0, 2, -1]], device), i32([2], device),
+             torch.tensor([0, 1, 2], device=device), i32([0, 3], device))
+    for layers in (1, 2, 36, 256, 257, 300):
+        k, v = small[:layers], small[300: 300 + layers]
+        svllm_ops.tree_commit(k, v, *lists)
+        for bad in (v[:-1] + k[:1], v[:-1] + v[:1] if layers > 1 else k):
+            with pytest.raises(RuntimeError, match="invalid argument"):
+                svllm_ops.tree_commit(k, bad, *lists)
+
+
 @pytest.mark.gpu
 def test_tree_commit_bad_paths_on_cuda(cuda):
     """A path that does not rise moves no row from there on, a slot past the cache leaves its
