@@ -59,7 +59,7 @@ constexpr uint32_t kTmemColumns = 512;
 constexpr uint32_t kScores = 0;       // TMEM columns: S (and P) of accumulator w at 128 w,
 constexpr uint32_t kOutput = 256;     // O at 256 + 128 w
 constexpr float kRescaleAbove = 8.0f;  // in powers of two
-constexpr int kJoinRows = 8;
+constexpr int kJoinThreads = 2;       // of a join block, per element of head_dim
 constexpr int kMaxCtas = 256;         // one per SM; the join lists their borders
 
 template <int D>
@@ -1098,116 +1098,117 @@ struct JoinItem {
   int mark;                      // of the first cut
 };
 
-// 8 rows of one accumulator of an item. Units are counted row group by row group over all items, so
-// that those with rows lie together and spread over the blocks.
-struct JoinUnit {
-  int item, w, row0;
-};
-
-__device__ __forceinline__ JoinUnit join_unit(int unit, int items) {
-  const int group = unit / (2 * items), rest = unit - group * 2 * items;
-  return JoinUnit{rest >> 1, rest & 1, group * kJoinRows};
-}
-
-// kUnits units at once, kBatch segments of each at a time, all their loads before any use; a thread
-// does 16 bytes of a row. With m and l the maxima and sums of the segments, M the largest m:
+// Joins units of kRows rows of one accumulator of an item: every gridDim-th of them, counted row
+// group by row group over all items, so that those with rows lie together and spread over the
+// blocks. A thread does kPieces times 16 bytes of a row, kBatch segments at a time, all their loads
+// before any use. With m and l the maxima and sums of the segments, M the largest m:
 //   o = sum 2^(m - M) O / sum 2^(m - M) l.
-template <int D, int kUnits, int kBatch>
+template <int D, int kRows, int kBatch>
 __device__ __forceinline__ void join_units(const TreeAttnArgs& a, const JoinItem* items,
-                                           const JoinUnit (&units)[kUnits]) {
+                                           const Cut* cuts, int count) {
   using S = Shape<D>;
+  constexpr int kApart = kJoinThreads * D / kRows;  // between a thread's pieces
+  constexpr int kPieces = D / 4 / kApart;
   const float kInf = __builtin_huge_valf();
-  const int piece = threadIdx.x / kJoinRows;
-  int most = 0, token0[kUnits], kv_head[kUnits], row0[kUnits];
-  float top[kUnits], sum[kUnits];
-  float4 o[kUnits];
-#pragma unroll
-  for (int u = 0; u < kUnits; ++u) {
-    const JoinItem& it = items[units[u].item];
-    const Cut& c = a.cuts[it.first];
-    token0[u] = c.token0;
-    kv_head[u] = c.kv_head[units[u].w];
-    row0[u] = c.row0[units[u].w];
-    most = max(most, it.segments);
-    top[u] = -kInf;
-    sum[u] = 0.0f;
-    o[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  }
+  const int piece = threadIdx.x / kRows;
+  const int total = count * 2 * (kTile / kRows);
 #pragma unroll 1
-  for (int i0 = 0; i0 < most; i0 += kBatch) {
-    float m[kUnits][kBatch], l[kUnits][kBatch];
-    float4 x[kUnits][kBatch];
+  for (int unit = blockIdx.x; unit < total; unit += gridDim.x) {
+    const int group = unit / (2 * count), rest = unit - group * 2 * count, w = rest & 1;
+    const JoinItem& it = items[rest >> 1];
+    const int row = group * kRows + threadIdx.x % kRows, rows = cut_rows(it.mark, w);
+    if (group * kRows >= rows) continue;
+    float top = -kInf, sum = 0.0f;
+    float4 o[kPieces];
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-      const JoinItem& it = items[units[u].item];
-      const int row = units[u].row0 + threadIdx.x % kJoinRows;
+    for (int i = 0; i < kPieces; ++i) o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const float* const parts =
+        a.parts + w * S::kPartFloats + (piece * kTile + row) * 4;
+    const int to_stats = D * kTile - piece * kTile * 4 - row * 3;
+    constexpr int64_t kSlotFloats = 2 * S::kPartFloats;
+#pragma unroll 1
+    for (int e0 = 0; e0 < it.segments; e0 += kBatch) {
+      float m[kBatch], l[kBatch];
+      float4 x[kBatch][kPieces];
 #pragma unroll
       for (int e = 0; e < kBatch; ++e) {
-        m[u][e] = -kInf;
-        l[u][e] = 0.0f;
-        if (i0 + e < it.segments) {
-          const int64_t slot = i0 + e == 0 ? it.first : (it.border - 1 + i0 + e) * 2;
-          const float* p = a.parts + (slot * 2 + units[u].w) * S::kPartFloats + row;
-          m[u][e] = ld_global_f32(p + D * kTile);
-          l[u][e] = ld_global_f32(p + (D + 1) * kTile);
-          x[u][e] = ld_global_f32x4(p + piece * kTile * 4 + row * 3);
+        m[e] = -kInf;
+        l[e] = 0.0f;
+        if (e0 + e < it.segments) {
+          const int slot = e0 + e == 0 ? it.first : (it.border - 1 + e0 + e) * 2;
+          const float* p = parts + slot * kSlotFloats;
+          m[e] = ld_global_f32(p + to_stats);
+          l[e] = ld_global_f32(p + to_stats + kTile);
+#pragma unroll
+          for (int i = 0; i < kPieces; ++i) {
+            x[e][i] = ld_global_f32x4(p + i * kApart * kTile * 4);
+          }
         }
       }
-    }
+      float up = top;
 #pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-      float up = top[u];
-#pragma unroll
-      for (int e = 0; e < kBatch; ++e) up = fmaxf(up, m[u][e]);
+      for (int e = 0; e < kBatch; ++e) up = fmaxf(up, m[e]);
       const float base = up == -kInf ? 0.0f : up;
-      const float f0 = exp2_approx(top[u] - base);
-      sum[u] *= f0;
-      o[u] = make_float4(o[u].x * f0, o[u].y * f0, o[u].z * f0, o[u].w * f0);
+      const float f0 = exp2_approx(top - base);
+      top = up;
+      sum *= f0;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) {
+        o[i] = make_float4(o[i].x * f0, o[i].y * f0, o[i].z * f0, o[i].w * f0);
+      }
 #pragma unroll
       for (int e = 0; e < kBatch; ++e) {
-        if (l[u][e] != 0.0f) {  // a segment of which the node sees nothing has no part
-          const float f = exp2_approx(m[u][e] - base);
-          sum[u] = fmaf(f, l[u][e], sum[u]);
-          o[u].x = fmaf(f, x[u][e].x, o[u].x);
-          o[u].y = fmaf(f, x[u][e].y, o[u].y);
-          o[u].z = fmaf(f, x[u][e].z, o[u].z);
-          o[u].w = fmaf(f, x[u][e].w, o[u].w);
+        if (l[e] != 0.0f) {  // a segment of which the node sees nothing has no part
+          const float f = exp2_approx(m[e] - base);
+          sum = fmaf(f, l[e], sum);
+#pragma unroll
+          for (int i = 0; i < kPieces; ++i) {
+            o[i].x = fmaf(f, x[e][i].x, o[i].x);
+            o[i].y = fmaf(f, x[e][i].y, o[i].y);
+            o[i].z = fmaf(f, x[e][i].z, o[i].z);
+            o[i].w = fmaf(f, x[e][i].w, o[i].w);
+          }
         }
       }
-      top[u] = up;
     }
-  }
-#pragma unroll
-  for (int u = 0; u < kUnits; ++u) {
-    const int row = units[u].row0 + threadIdx.x % kJoinRows;
-    if (row >= cut_rows(items[units[u].item].mark, units[u].w)) continue;
-    const int at_row = row0[u] + row;
+    if (row >= rows) continue;
+    const Cut& c = cuts[it.first];
+    const int at_row = pick(c.row0, w) + row;
     const int node = a.by_group.divide(at_row);
     auto* out = static_cast<__nv_bfloat16*>(a.out) +
-                ((static_cast<int64_t>(token0[u] + node) * a.num_kv_heads + kv_head[u] - node) *
-                     a.group + at_row) * D + piece * 4;
-    const float inverse = sum[u] == 0.0f ? 0.0f : 1.0f / sum[u];
-    if (sum[u] == 0.0f) o[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    *reinterpret_cast<uint2*>(out) =
-        make_uint2(pack_bf16x2(o[u].x * inverse, o[u].y * inverse),
-                   pack_bf16x2(o[u].z * inverse, o[u].w * inverse));
+                ((static_cast<int64_t>(c.token0 + node) * a.num_kv_heads + pick(c.kv_head, w) -
+                  node) * a.group + at_row) * D + piece * 4;
+    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;  // zero: the node saw no row
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      if (sum == 0.0f) o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      *reinterpret_cast<uint2*>(out + i * kApart * 4) =
+          make_uint2(pack_bf16x2(o[i].x * inverse, o[i].y * inverse),
+                     pack_bf16x2(o[i].z * inverse, o[i].w * inverse));
+    }
   }
 }
 
 // Joins the segments of each cut item. A border between two CTAs' shares that lies inside an item
 // is the item's if it is the first of those; each block lists these items (one thread per border)
-// and takes every gridDim-th unit of them.
+// and takes every gridDim-th unit of them: of 16 rows, whose segments are mostly two or three (each
+// row's factors are then worked out by half as many threads), or where that leaves blocks without
+// work, with long items of many segments, of 8.
 template <int D>
-__global__ void __launch_bounds__(kJoinRows * D / 4) tree_attention_join_kernel(
+__global__ void __launch_bounds__(kJoinThreads * D, 256 / D) tree_attention_join_kernel(
     const TreeAttnArgs a, int ctas) {
   grid_dependency_sync();
-  constexpr int kBlock = kJoinRows * D / 4;
+  constexpr int kBlock = kJoinThreads * D;
   __shared__ JoinItem items[kMaxCtas];
   __shared__ int marks[2 * kMaxCtas];
+  __shared__ Cut cuts[2 * kMaxCtas];
   __shared__ int warp_counts[kBlock / kWarpSize];
   __shared__ uint8_t inside[kMaxCtas + 1];  // the border lies inside an item; 2: as its first
   const int tid = threadIdx.x, lane = tid % kWarpSize;
-  for (int i = tid; i < 2 * ctas; i += kBlock) marks[i] = a.marks[i];
+  for (int i = tid; i < 2 * ctas; i += kBlock) {
+    marks[i] = a.marks[i];
+    cuts[i] = a.cuts[i];  // anything where the mark is 0
+  }
   __syncthreads();
   for (int b = tid; b <= ctas; b += kBlock) {
     uint8_t kind = 0;
@@ -1242,22 +1243,10 @@ __global__ void __launch_bounds__(kJoinRows * D / 4) tree_attention_join_kernel(
     __syncthreads();
   }
 
-  const int total = count * 2 * (kTile / kJoinRows), stride = gridDim.x;
-  const auto has_rows = [&](const JoinUnit& u) {
-    return u.row0 < cut_rows(items[u.item].mark, u.w);
-  };
-  for (int unit = blockIdx.x; unit < total; unit += stride) {
-    const JoinUnit first = join_unit(unit, count);
-    if (!has_rows(first)) continue;
-    if (unit + stride < total) {
-      const JoinUnit next = join_unit(unit + stride, count);
-      if (has_rows(next) && items[first.item].segments <= 4 && items[next.item].segments <= 4) {
-        join_units<D, 2, 4>(a, items, {first, next});
-        unit += stride;
-        continue;
-      }
-    }
-    join_units<D, 1, 8>(a, items, {first});
+  if (count * 2 * (kTile / 16) >= static_cast<int>(gridDim.x)) {
+    join_units<D, 16, 3>(a, items, cuts, count);
+  } else {
+    join_units<D, 8, 8>(a, items, cuts, count);
   }
 }
 
@@ -1295,8 +1284,9 @@ int launch_tree_attention(TreeAttnArgs& a, void* workspace, int device, cudaStre
                                        Shape<D>::kSmem, stream, 1u, map_k, map_v, a);
   // where no table holds more than a tile of rows, items have one step and no border cuts one
   if (status != SVLLM_OK || ctas < 2 || a.max_length <= kTile) return status;
-  return launch(tree_attention_join_kernel<D>, dim3(4 * ctas), dim3(kJoinRows * D / 4), 0, stream,
-                1u, a, ctas);
+  // as many blocks as are resident at once
+  return launch(tree_attention_join_kernel<D>, dim3(256 / D * ctas), dim3(kJoinThreads * D), 0,
+                stream, 1u, a, ctas);
 }
 
 }  // namespace
