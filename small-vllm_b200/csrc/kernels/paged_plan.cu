@@ -12,7 +12,9 @@
 // them. What bounds it is the chain of dependent loads and barriers, not bytes. Tokens are
 // independent of one another (a binary search over the starts, one table entry, a walk up the
 // parents); few of them follow in the same CTA, the starts and the parents staged in shared memory;
-// many get a second kernel over the whole GPU (kFusedTokens).
+// many get a second kernel over the whole GPU (kFusedTokens). Measured in a graph: 4 requests of 8
+// nodes 2.9 us, 64 of 16 5.1, 1024 of 64 9.1 (2.1 MB read and written, 0.3 us of HBM time: latency
+// is all there is); a call from the host costs it some 6.5 us.
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -28,8 +30,11 @@ constexpr int kTokenThreads = 256;
 constexpr int kStagedStarts = 4096;  // of requests, staged by the tokens' kernel
 constexpr int kOwnBlocks = 8;        // new blocks up to which a request's own lane fetches them
 
-// Up to this many tokens are done by the CTA that did the requests; more get a grid of their own.
-constexpr int64_t kFusedTokens = 4096;
+// Up to this many tokens, times the words of a mask, are done by the CTA that did the requests; more
+// get a grid of their own. us in a graph, one kernel against two: 32 tokens 2.9 and 4.1, 256 3.5 and
+// 4.5, 1024 5.1 and 4.7 (a second launch costs the host some 2 us), 2048 7.1 and 4.7, 4096 10.7 and
+// 5.4; one tree of 1024 nodes, 16 words each, 14.3 and 8.7.
+constexpr int64_t kFusedTokens = 1024;
 
 struct PlanArgs {
   const int32_t* context_lens;   // [num_seqs]
@@ -157,8 +162,9 @@ __device__ void plan_token(const PlanArgs& a, int t, const int32_t* starts,
   a.positions[t] = position;
 }
 
-// Copies `count` block ids per lane, src[step * k] -> dst[k]: a lane's own when there are few, else
-// the warp together, lane by lane.
+// Copies `count` block ids per lane, src[step * k] -> dst[k]: a lane's own when there are up to
+// kOwnBlocks, else the warp together, four lanes' at a time. us in a graph, a lane's own against
+// together: 64 requests of 1 block 5.3 and 6.8, 1024 of 4 9.1 and 11.7, 1024 of 16 19.7 and 11.8.
 __device__ __forceinline__ void copy_blocks(int count, const int32_t* src, int step,
                                             int32_t* dst) {
   const int most = __reduce_max_sync(0xffffffffu, count);
@@ -174,14 +180,32 @@ __device__ __forceinline__ void copy_blocks(int count, const int32_t* src, int s
     }
     return;
   }
-  for (int l = 0; l < kWarpSize; ++l) {
-    const int n = __shfl_sync(0xffffffffu, count, l);
-    const auto from = reinterpret_cast<const int32_t*>(
-        __shfl_sync(0xffffffffu, reinterpret_cast<int64_t>(src), l));
-    const auto to =
-        reinterpret_cast<int32_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<int64_t>(dst), l));
-    for (int k = threadIdx.x % kWarpSize; k < n; k += kWarpSize) {
-      to[k] = from[static_cast<int64_t>(step) * k];
+  constexpr int kLanes = 4;
+#pragma unroll 1
+  for (int l = 0; l < kWarpSize; l += kLanes) {
+    int n[kLanes], longest = 0;
+    const int32_t* from[kLanes];
+    int32_t* to[kLanes];
+#pragma unroll
+    for (int e = 0; e < kLanes; ++e) {
+      n[e] = __shfl_sync(0xffffffffu, count, l + e);
+      from[e] = reinterpret_cast<const int32_t*>(
+          __shfl_sync(0xffffffffu, reinterpret_cast<int64_t>(src), l + e));
+      to[e] = reinterpret_cast<int32_t*>(
+          __shfl_sync(0xffffffffu, reinterpret_cast<int64_t>(dst), l + e));
+      longest = max(longest, n[e]);
+    }
+#pragma unroll 1
+    for (int k = threadIdx.x % kWarpSize; k < longest; k += kWarpSize) {
+      int32_t held[kLanes];
+#pragma unroll
+      for (int e = 0; e < kLanes; ++e) {
+        if (k < n[e]) held[e] = from[e][static_cast<int64_t>(step) * k];
+      }
+#pragma unroll
+      for (int e = 0; e < kLanes; ++e) {
+        if (k < n[e]) to[e][k] = held[e];
+      }
     }
   }
 }
@@ -369,12 +393,13 @@ extern "C" int svllm_paged_plan(
   a.block_size = static_cast<int32_t>(block_size);
   a.max_query_len = static_cast<int32_t>(max_query_len);
   a.mask_words = parents != nullptr ? static_cast<int32_t>((max_query_len + 63) / 64) : 0;
-  a.fused = num_tokens <= kFusedTokens && num_seqs <= kPlanThreads;
+  a.fused = num_tokens * (a.mask_words > 1 ? a.mask_words : 1) <= kFusedTokens &&
+            num_seqs <= kPlanThreads;
   a.err = err;
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  // a thread per request, and where the tokens are done here too up to 256 for them
-  int64_t threads = a.fused ? (num_tokens < 256 ? num_tokens : 256) : 1;
-  if (threads < num_seqs) threads = num_seqs;
+  // a thread per request, and per token where those are done here too (1024 tokens by 256 threads
+  // took 6.6 us)
+  int64_t threads = a.fused && num_tokens > num_seqs ? num_tokens : num_seqs;
   if (threads < 1) threads = 1;
   threads = threads > kPlanThreads ? kPlanThreads : round_up(threads, kWarpSize);
   const size_t staged =

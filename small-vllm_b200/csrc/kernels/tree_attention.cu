@@ -1025,6 +1025,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // others set up; of a larger one every warp adds up a part first
   const bool few = a.num_seqs <= kWarpSize;
   const int chunk = few ? 1 : (a.num_seqs + kWarps - 1) / kWarps;
+  static_assert(kWarpSize > kWarps, "a chunk of 1 request is one that its lane has loaded");
   if (!few) {
     int cost = 0;
 #pragma unroll 1
