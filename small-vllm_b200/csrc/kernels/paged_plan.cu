@@ -8,8 +8,8 @@
 // k of the step, counted over all requests, is free_blocks[count - 1 - k].
 //
 // One CTA does the requests, as many threads as there are requests up to 1024: a scan of (tokens,
-// blocks) is a few shuffles, and no grid-wide meeting is needed between giving blocks back and taking
-// them. What bounds it is the chain of dependent loads and barriers, not bytes. Tokens are
+// blocks) is a few shuffles, and no grid-wide meeting is needed between giving blocks back and
+// taking them. What bounds it is the chain of dependent loads and barriers, not bytes. Tokens are
 // independent of one another (a binary search over the starts, one table entry, a walk up the
 // parents); few of them follow in the same CTA, the starts and the parents staged in shared memory;
 // many get a second kernel over the whole GPU (kFusedTokens). Measured in a graph: 4 requests of 8
@@ -30,10 +30,10 @@ constexpr int kTokenThreads = 256;
 constexpr int kStagedStarts = 4096;  // of requests, staged by the tokens' kernel
 constexpr int kOwnBlocks = 8;        // new blocks up to which a request's own lane fetches them
 
-// Up to this many tokens, times the words of a mask, are done by the CTA that did the requests; more
-// get a grid of their own. us in a graph, one kernel against two: 32 tokens 2.9 and 4.1, 256 3.5 and
-// 4.5, 1024 5.1 and 4.7 (a second launch costs the host some 2 us), 2048 7.1 and 4.7, 4096 10.7 and
-// 5.4; one tree of 1024 nodes, 16 words each, 14.3 and 8.7.
+// Up to this many tokens, times the words of a mask, are done by the CTA that did the requests;
+// more get a grid of their own. us in a graph, one kernel against two: 32 tokens 2.9 and 4.1, 256
+// 3.5 and 4.5, 1024 5.1 and 4.7 (a second launch costs the host some 2 us), 2048 7.1 and 4.7, 4096
+// 10.7 and 5.4; one tree of 1024 nodes, 16 words each, 14.3 and 8.7.
 constexpr int64_t kFusedTokens = 1024;
 
 struct PlanArgs {

@@ -3,11 +3,14 @@
 // tree_accept: node 0 of a request is its last accepted token, whose successors were drafted.
 // From cur = 0: the model's token after cur is targets[cur]; the walk goes on at the first child
 // of cur that holds it, and ends where no child does. The tokens emitted are targets along the
-// path, so every request with a node emits at least one.
+// path, so every request with a node emits at least one. What bounds it is the chain of steps down
+// the tree. Measured in a graph: 4 requests of 8 nodes 3.3 us, 1024 of 32 to 64 4.8 (1.8 MB, 0.3 us
+// of HBM time); a call costs its host some 6 us.
 //
 // tree_commit: the step wrote node i of a request to the slot of row context + i; row context +
 // j of the sequence, j < accepted, must be node path[j]. Paths rise (a parent comes before its
-// child), so path[j] >= j.
+// child), so path[j] >= j. A copy: 128 requests of 12 to 24 nodes in 28 layers, 143 MB, 20.7 us in
+// a graph (6.9 TB/s, part of it from L2); one request of 16 nodes 3.8 us.
 #include <cuda_runtime.h>
 
 #include <cstdint>

@@ -29,6 +29,17 @@
 // rows and, since 0 * NaN would reach rows that do not see it, zero the values of V that are not
 // finite in the tiles that hold tree nodes; they are added again, for the rows that see them, at
 // the end. One warp lists the CTA's segments for all others.
+//
+// Measured in a graph, inputs past L2, head_dim 128 where not said: 64 requests of 48 to
+// 64 nodes over 2048 to 4096 rows, 16 heads on 8 KV heads, 203 us (1.08 GB, 5.3 TB/s: 0.82 of the
+// copy rate; 219 us under a load that runs into the power limit), the main kernel 185 and the join
+// the rest: the stream over K and V, which the chain of products and softmax keeps from being quite
+// full. 8 requests of 100 to 128 nodes over 1024 to 4096, 32 heads on 4 KV heads, 86 us (0.75
+// PFLOP/s), main kernel 73: per key tile and
+// accumulator the softmax takes some 1250 cycles, its exponentials first, the two products 512 and
+// 512, and those of one accumulator wait for each other. 32 nodes over 32768 rows 41 us, 20 of them
+// the stream, 10 the join of some 37 segments per item. 8 nodes over 128 rows 8.7 us: one tile's
+// chain of dependent steps, most of it the first fetch of the roles' code.
 #include <cuda_runtime.h>
 
 #include <cmath>
@@ -156,7 +167,8 @@ __device__ __forceinline__ int request_cost(const TreeAttnArgs& a, const Request
   return a.num_kv_heads * r.steps * (r.pairs + r.odd);
 }
 
-// Lengths come from the device unchecked: sums of costs stop at the largest int instead of wrapping.
+// Lengths come from the device unchecked: sums of costs stop at the largest int instead of
+// wrapping.
 __device__ __forceinline__ int add_costs(int a, int b) {
   return static_cast<int>(min(static_cast<unsigned>(a) + static_cast<unsigned>(b),
                               static_cast<unsigned>(INT32_MAX)));
@@ -201,9 +213,9 @@ struct Segment {
   int front, back;               // cut there
 };
 
-// Barriers and flags of one CTA. A V tile with tree nodes lands on its own barrier, for the helpers,
-// which signal when it is checked; kFull stands for all other tiles. (A slot's parity counts the
-// uses of one barrier, so every waiter of a barrier has to see all of them.)
+// Barriers and flags of one CTA. A V tile with tree nodes lands on its own barrier, for the
+// helpers, which signal when it is checked; kFull stands for all other tiles. (A slot's parity
+// counts the uses of one barrier, so every waiter of a barrier has to see all of them.)
 constexpr int kMaxStages = 10;
 constexpr int kSegments = 4;    // of the list's ring
 constexpr int kFull = 0, kLanded = kFull + kMaxStages;
@@ -224,9 +236,9 @@ struct Sync {
   uint64_t bar[kBarriers];
   uint32_t tmem_base;
   int abort;
-  // per helper warp, accumulator and segment modulo 8: V held something not finite. A warp clears its
-  // own word when it begins a segment; no warp is more than kSegments behind another then, so nobody
-  // still reads the one that the segment 8 before left there.
+  // per helper warp, accumulator and segment modulo 8: V held something not finite. A warp clears
+  // its own word when it begins a segment; no warp is more than kSegments behind another then, so
+  // nobody still reads the one that the segment 8 before left there.
   int odd_values[kHelperWarps][2][2 * kSegments];
   int costs[kWarps];     // of the warps' shares of the requests
   Segment list[kSegments];
@@ -455,9 +467,13 @@ __device__ __forceinline__ bool has_nodes(const Segment& g, int step) {
 }
 
 // One of the warps that bring K and V, tile after tile in the order in which the tensor cores take
-// them: every kLoaderWarps-th TMA instruction of each tile (one costs its issuer some 100 cycles, a
-// tile of 16-row pages has 16). Where the block size allows, a TMA box is a run of 8 to 128 rows
-// that no page border can fall into, gcd(block_size, 128); otherwise an instruction gathers 4 rows.
+// them: every kLoaderWarps-th TMA instruction of each tile (one costs its issuer some 60 cycles, a
+// tile of 16-row pages has 16; four loaders, two of them from the helpers, were no faster). Where
+// the block size allows, a TMA box is a run of 8 to 128 rows that no page border can fall into,
+// gcd(block_size, 128); otherwise an instruction gathers 4 rows, some 45 cycles each. With pages of
+// one row that costs 345 us where the 64 requests above take 203; copies of 16 bytes per thread
+// (cp.async) took 290 there and more than the gather in every smaller case. Issued by all lanes
+// at once, each its own rows, the gather took 603.
 template <int D>
 struct Loader {
   using S = Shape<D>;
@@ -1014,15 +1030,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_mbar_init();
   }
   if (tid == 0) sy.abort = 0;
-  if (warp == kMmaWarp) tmem_alloc(&sy.tmem_base, kTmemColumns);
 
   grid_dependency_sync();
+  // not before: no CTA holds TMEM while it waits for another grid
+  if (warp == kMmaWarp) tmem_alloc(&sy.tmem_base, kTmemColumns);
   if (tid == 0) {
     a.marks[blockIdx.x * 2] = 0;
     a.marks[blockIdx.x * 2 + 1] = 0;
   }
   // this CTA's share of the line: a batch of up to 32 requests is planned by one warp while the
-  // others set up; of a larger one every warp adds up a part first
+  // others set up; of a larger one every warp adds up a part first, which for small batches too
+  // took 12.7 us instead of 12.2 (1 request), 27.8 instead of 24.9 (13), 93.7 instead of 90.5 (8)
   const bool few = a.num_seqs <= kWarpSize;
   const int chunk = few ? 1 : (a.num_seqs + kWarps - 1) / kWarps;
   static_assert(kWarpSize > kWarps, "a chunk of 1 request is one that its lane has loaded");
@@ -1194,7 +1212,10 @@ __device__ __forceinline__ void join_units(const TreeAttnArgs& a, const JoinItem
 // is the item's if it is the first of those; each block lists these items (one thread per border)
 // and takes every gridDim-th unit of them: of 16 rows, whose segments are mostly two or three (each
 // row's factors are then worked out by half as many threads), or where that leaves blocks without
-// work, with long items of many segments, of 8.
+// work, with long items of many segments, of 8. With 8 rows everywhere 8 requests of up to 128
+// nodes took 93 us instead of 86, with 16 everywhere one of 32 nodes over 32768 51 instead of 41.
+// The join moves up to 39 MB through L2 once more: 6 us for small batches, 13 to 15 for the
+// largest.
 template <int D>
 __global__ void __launch_bounds__(kJoinThreads * D, 256 / D) tree_attention_join_kernel(
     const TreeAttnArgs a, int ctas) {
