@@ -30,14 +30,15 @@
 // finite in the tiles that hold tree nodes; they are added again, for the rows that see them, at
 // the end. One warp lists the CTA's segments for all others.
 //
-// Measured in a graph, inputs past L2, head_dim 128 where not said: 64 requests of 48 to
-// 64 nodes over 2048 to 4096 rows, 16 heads on 8 KV heads, 203 us (1.08 GB, 5.3 TB/s: 0.82 of the
-// copy rate; 219 us under a load that runs into the power limit), the main kernel 185 and the join
-// the rest: the stream over K and V, which the chain of products and softmax keeps from being quite
-// full. 8 requests of 100 to 128 nodes over 1024 to 4096, 32 heads on 4 KV heads, 86 us (0.75
-// PFLOP/s), main kernel 73: per key tile and
-// accumulator the softmax takes some 1250 cycles, its exponentials first, the two products 512 and
-// 512, and those of one accumulator wait for each other. 32 nodes over 32768 rows 41 us, 20 of them
+// Measured in a graph, inputs past L2, head_dim 128: 64 requests of 48 to 64 nodes over 2048 to
+// 4096 rows, 16 heads on 8 KV heads, 203 us (1.08 GB, 5.3 TB/s: 0.82 of the copy rate; 219 us under
+// a load that runs into the power limit). The main kernel takes 185 of them, in steady state at the
+// copy rate, a tenth of it start and ends of segments; the join takes the rest. 8 requests of 100
+// to 128 nodes over 1024 to 4096, 32 heads on 4 KV heads, 86 us (0.75 PFLOP/s), main kernel 73: a
+// KV head's rows go to four items, 5.6 TB/s through L2, and a step takes 3500 cycles where its
+// products take 2048: per accumulator those and the softmax (1580 cycles, 1260 of them the
+// exponentials) wait for each other. Parts of 64 cached rows with their scores a part ahead took
+// 119: products of N = 64 take as long as those of 128. 32 nodes over 32768 rows 41 us, 20 of them
 // the stream, 10 the join of some 37 segments per item. 8 nodes over 128 rows 8.7 us: one tile's
 // chain of dependent steps, most of it the first fetch of the roles' code.
 #include <cuda_runtime.h>
