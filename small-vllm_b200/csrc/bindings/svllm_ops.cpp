@@ -22,6 +22,29 @@
 
 namespace py = pybind11;
 
+namespace {
+
+// The tensors of a list or tuple. A model's caches are dozens of tensors a call, for which pybind's
+// own conversion takes 3 us, this one a fifth.
+std::vector<at::Tensor> tensor_list(const py::object& list, const char* name) {
+  if (!PyList_Check(list.ptr()) && !PyTuple_Check(list.ptr())) {
+    throw py::type_error(std::string(name) + ": expected a list of tensors");
+  }
+  const Py_ssize_t size = PySequence_Fast_GET_SIZE(list.ptr());
+  PyObject** items = PySequence_Fast_ITEMS(list.ptr());
+  std::vector<at::Tensor> tensors;
+  tensors.reserve(size);
+  for (Py_ssize_t i = 0; i < size; ++i) {
+    if (!THPVariable_Check(items[i])) {
+      throw py::type_error(std::string(name) + ": expected a list of tensors");
+    }
+    tensors.push_back(THPVariable_Unpack(items[i]));
+  }
+  return tensors;
+}
+
+}  // namespace
+
 PYBIND11_MODULE(svllm_ops, m) {
   m.attr("__version__") = SVLLM_VERSION;
 #ifdef SVLLM_CUDA
@@ -81,9 +104,17 @@ PYBIND11_MODULE(svllm_ops, m) {
   m.def("tree_accept", &svllm::ops::tree_accept, py::arg("ids"), py::arg("targets"),
         py::arg("parents"), py::arg("query_start_loc"), py::arg("seq_lens"),
         py::arg("context_lens"), py::arg("max_query_len"));
-  m.def("tree_commit", &svllm::ops::tree_commit, py::arg("k_caches"), py::arg("v_caches"),
-        py::arg("path"), py::arg("num_accepted"), py::arg("slot_mapping"),
-        py::arg("query_start_loc"));
+  m.def(
+      "tree_commit",
+      [](const py::object& k_caches, const py::object& v_caches, const at::Tensor& path,
+         const at::Tensor& num_accepted, const at::Tensor& slot_mapping,
+         const at::Tensor& query_start_loc) {
+        svllm::ops::tree_commit(tensor_list(k_caches, "k_caches"),
+                                tensor_list(v_caches, "v_caches"), path, num_accepted,
+                                slot_mapping, query_start_loc);
+      },
+      py::arg("k_caches"), py::arg("v_caches"), py::arg("path"), py::arg("num_accepted"),
+      py::arg("slot_mapping"), py::arg("query_start_loc"));
   m.def("read_device_error", &svllm::ops::read_device_error, py::arg("device_index"),
         py::arg("reset") = true);
 

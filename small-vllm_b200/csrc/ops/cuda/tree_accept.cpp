@@ -31,6 +31,8 @@ void tree_commit(const std::vector<at::Tensor>& k_caches, const std::vector<at::
   const c10::cuda::CUDAGuard device_guard(first.device());
   const auto stream = reinterpret_cast<svllm_stream>(c10::cuda::getCurrentCUDAStream().stream());
   std::vector<void*> k, v;
+  k.reserve(k_caches.size());
+  v.reserve(v_caches.size());
   for (const at::Tensor& c : k_caches) k.push_back(c.mutable_data_ptr());
   for (const at::Tensor& c : v_caches) v.push_back(c.mutable_data_ptr());
   detail::check_status(

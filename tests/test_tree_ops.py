@@ -307,6 +307,17 @@ def test_tree_commit_rejects_bad_inputs():
             call(**change)
 
 
+def test_tree_commit_takes_lists_and_tuples_of_tensors():
+    lists = (i32([[0, 2, -1]], "cpu"), i32([2], "cpu"), torch.tensor([0, 1, 2]), i32([0, 3], "cpu"))
+    k = torch.arange(64, dtype=torch.float32).view(2, 4, 1, 8)
+    v = torch.nn.Parameter(-k, requires_grad=False)
+    svllm_ops.tree_commit((k,), [v], *lists)
+    assert torch.equal(k[0, 1], k[0, 2]) and torch.equal(v[0, 1], v[0, 2])
+    for bad in (k, None, [None], [[k]], (k, 1)):
+        with pytest.raises(TypeError, match="k_caches"):
+            svllm_ops.tree_commit(bad, [v], *lists)
+
+
 def test_tree_commit_refuses_a_cache_given_twice(device):
     """Its rows would move twice. 1 to 300 layers: a table of the caches seen, then all pairs."""
     small = [torch.zeros(2, 4, 1, 8, device=device) for _ in range(600)]
