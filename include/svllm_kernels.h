@@ -357,7 +357,8 @@ int svllm_lm_head_argmax_static_bf16(const void* hidden, int64_t num_rows, int64
  * max_blocks], more rows than the table holds, tokens past num_tokens, more nodes than
  * max_query_len (which only counts with parents; at most SVLLM_MAX_TREE_NODES). The same bit tells
  * of a parent that does not come before its child (the node counts as a root), a free_count
- * outside [0, free_capacity] (clamped), and blocks given back past free_capacity (dropped).
+ * outside [0, free_capacity] (clamped), and blocks given back past free_capacity (dropped). No
+ * array that is written overlaps another one.
  */
 int svllm_paged_plan(const int32_t* context_lens, const int32_t* query_lens, int64_t num_seqs,
                      int32_t* block_tables, int64_t max_blocks, const int32_t* blocks_owned,

@@ -12,9 +12,10 @@
 // taking them. What bounds it is the chain of dependent loads and barriers, not bytes. Tokens are
 // independent of one another (a binary search over the starts, one table entry, a walk up the
 // parents); few of them follow in the same CTA, the starts and the parents staged in shared memory;
-// many get a second kernel over the whole GPU (kFusedTokens). Measured in a graph: 4 requests of 8
-// nodes 2.9 us, 64 of 16 5.1, 1024 of 64 9.1 (2.1 MB read and written, 0.3 us of HBM time: latency
-// is all there is); a call from the host costs it some 6.5 us.
+// many get a second kernel over the whole GPU (kFusedTokens), which works out the starts and walks
+// up the trees while the first runs (1024 requests of 64 nodes: 10.9 us before, 6.9 with). Measured
+// in a graph: 4 requests of 8 nodes 3.2 us, 64 of 16 4.0, 1024 of 64 6.9 (2.1 MB read and written,
+// 0.3 us of HBM time: latency is all there is); a call from the host costs it some 6.5 us.
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -31,10 +32,10 @@ constexpr int kStagedStarts = 4096;  // of requests, staged by the tokens' kerne
 constexpr int kOwnBlocks = 8;        // new blocks up to which a request's own lane fetches them
 
 // Up to this many tokens, times the words of a mask, are done by the CTA that did the requests;
-// more get a grid of their own. us in a graph, one kernel against two: 32 tokens 2.9 and 4.1, 256
-// 3.5 and 4.5, 1024 5.1 and 4.7 (a second launch costs the host some 2 us), 2048 7.1 and 4.7, 4096
-// 10.7 and 5.4; one tree of 1024 nodes, 16 words each, 14.3 and 8.7.
-constexpr int64_t kFusedTokens = 1024;
+// more get a grid of their own. us in a graph, one kernel against two: 32 tokens 3.2 and 3.6, 256
+// 3.8 and 3.7, 512 4.2 and 3.9 (a second launch costs the host some 2 us), 1024 5.4 and 4.0, 4096
+// 10.7 and 4.7.
+constexpr int64_t kFusedTokens = 512;
 
 struct PlanArgs {
   const int32_t* context_lens;   // [num_seqs]
@@ -104,12 +105,9 @@ __device__ uint2 block_scan(uint2 v, uint2* warp_sums, uint2& total) {
 }
 static_assert(kPlanThreads <= kWarpSize * kWarpSize, "one value per warp in one warp");
 
-// One token: its request by binary search over the starts, then slot, position and mask. `starts`
-// and `parents` may be staged copies. Reads what the requests' part wrote, so plain loads (not the
-// read-only path).
-__device__ void plan_token(const PlanArgs& a, int t, const int32_t* starts,
-                           const int32_t* parents) {
-  int lo = 0, hi = static_cast<int>(a.num_seqs);  // the first request whose end lies beyond t
+// A token's request: the first whose end lies beyond it, by binary search over the starts.
+__device__ int request_of(const PlanArgs& a, int t, const int32_t* starts) {
+  int lo = 0, hi = static_cast<int>(a.num_seqs);
   while (lo < hi) {
     const int mid = (lo + hi) / 2;
     if (starts[mid + 1] > t) {
@@ -118,21 +116,54 @@ __device__ void plan_token(const PlanArgs& a, int t, const int32_t* starts,
       lo = mid + 1;
     }
   }
-  const bool live = lo < a.num_seqs && a.seq_lens[lo] > 0;
+  return lo;
+}
+
+// The way from a node up its tree, for masks of one word.
+struct Walk {
+  uint64_t bits = 0;
+  int depth = -1;
+  bool bad = false;  // not a tree: the node that hangs on a later one counts as a root
+};
+
+__device__ Walk walk_up(const int32_t* parents, int node) {
+  Walk w;
+  for (int p = node; p >= 0;) {
+    w.bits |= uint64_t{1} << p;
+    ++w.depth;
+    int up = parents[p];
+    if (up >= p || up < -1) {
+      w.bad = true;
+      up = -1;
+    }
+    p = up;
+  }
+  return w;
+}
+
+// A token of request `s`, which starts at token `start`: slot, position and mask. `parents` (of
+// the request's first node) may be a staged copy; `w` counts for masks of one word. Reads what the
+// requests' part wrote, so plain loads (not the read-only path).
+__device__ void plan_token(const PlanArgs& a, int t, int s, int start, const int32_t* parents,
+                           const Walk& w) {
+  const bool live = s < a.num_seqs && a.seq_lens[s] > 0;
   int64_t slot = -1, position = 0;
   int64_t* mask =
       a.tree_mask == nullptr ? nullptr : a.tree_mask + static_cast<int64_t>(t) * a.mask_words;
   int word = a.mask_words;  // mask words from here on are written
   if (live) {
-    const int32_t start = starts[lo];
     const int i = t - start;
-    const int context = a.context_lens[lo];
+    const int context = a.context_lens[s];
     const int row = context + i;  // at most max_blocks * block_size, which fits
     const int page = row / a.block_size;
-    slot = static_cast<int64_t>(a.block_tables[static_cast<int64_t>(lo) * a.max_blocks + page]) *
+    slot = static_cast<int64_t>(a.block_tables[static_cast<int64_t>(s) * a.max_blocks + page]) *
                a.block_size + (row - page * a.block_size);
     int depth = i;
-    if (mask != nullptr) {
+    if (a.mask_words == 1) {
+      mask[--word] = static_cast<int64_t>(w.bits);
+      depth = w.depth;
+      if (w.bad) raise_error(a.err, kErrBadIndex);
+    } else if (mask != nullptr) {
       // up the tree: parents come before their children, so the words are met in falling order
       depth = -1;
       uint64_t bits = 0;
@@ -144,7 +175,7 @@ __device__ void plan_token(const PlanArgs& a, int t, const int32_t* starts,
         }
         bits |= uint64_t{1} << (p % 64);
         ++depth;
-        int up = parents[start + p];
+        int up = parents[p];
         if (up >= p || up < -1) {  // not a tree: the node counts as a root
           raise_error(a.err, kErrBadIndex);
           up = -1;
@@ -160,6 +191,11 @@ __device__ void plan_token(const PlanArgs& a, int t, const int32_t* starts,
   }
   a.slot_mapping[t] = slot;
   a.positions[t] = position;
+}
+
+// The walk of a token whose request may not be served yet: a node past the mask has none.
+__device__ Walk walk_of(const PlanArgs& a, int node, const int32_t* parents) {
+  return a.mask_words == 1 && node < 64 ? walk_up(parents, node) : Walk{};
 }
 
 // Copies `count` block ids per lane, src[step * k] -> dst[k]: a lane's own when there are up to
@@ -316,23 +352,63 @@ __global__ void __launch_bounds__(kPlanThreads) plan_requests_kernel(const PlanA
   if (tid == 0) a.free_count_out[0] = static_cast<int32_t>(have - used);
   if (a.fused) {
     for (int t = tid; t < a.num_tokens; t += threads) {
-      plan_token(a, t, staged, staged + n_seqs + 1);
+      const int s = request_of(a, t, staged), start = staged[s];
+      const int32_t* parents = staged + n_seqs + 1 + start;
+      const bool in = s < n_seqs;
+      plan_token(a, t, s, start, parents, in ? walk_of(a, t - start, parents) : Walk{});
     }
   }
 }
 
+// The tokens, after plan_requests_kernel, which lets this kernel start as soon as what came before
+// it has completed: the starts (worked out once more from the query lengths) and the walks need
+// nothing that it writes, so they are done while it runs.
 __global__ void __launch_bounds__(kTokenThreads) plan_tokens_kernel(const PlanArgs a) {
-  grid_dependency_sync();
   __shared__ int32_t staged[kStagedStarts + 1];
-  const int n_seqs = static_cast<int>(a.num_seqs);
+  __shared__ uint2 warp_sums[kTokenThreads / kWarpSize];
+  __shared__ uint32_t ends[kTokenThreads];
+  const int n_seqs = static_cast<int>(a.num_seqs), tid = threadIdx.x;
   const int32_t* starts = a.query_start_loc;
-  if (n_seqs <= kStagedStarts) {
-    for (int s = threadIdx.x; s <= n_seqs; s += kTokenThreads) staged[s] = starts[s];
+  const bool early = n_seqs <= kStagedStarts;
+  if (early) {
+    const int each = (n_seqs + kTokenThreads - 1) / kTokenThreads;
+    const int first = min(n_seqs, tid * each), last = min(n_seqs, first + each);
+    uint32_t sum = 0;
+    for (int s = first; s < last; ++s) {
+      sum = add_up(sum, static_cast<uint32_t>(max(__ldcg(a.query_lens + s), 0)));
+      staged[s + 1] = static_cast<int32_t>(sum);
+    }
+    uint2 total;
+    ends[tid] = block_scan(make_uint2(sum, 0), warp_sums, total).x;
+    __syncthreads();
+    const uint32_t limit = static_cast<uint32_t>(a.num_tokens);
+    const uint32_t before = tid == 0 ? 0 : ends[tid - 1];
+    for (int s = first; s < last; ++s) {
+      staged[s + 1] = static_cast<int32_t>(
+          min(add_up(before, static_cast<uint32_t>(staged[s + 1])), limit));
+    }
+    if (tid == 0) staged[0] = 0;
     __syncthreads();
     starts = staged;
+  } else {
+    grid_dependency_sync();
   }
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * kTokenThreads + threadIdx.x;
-  if (t < a.num_tokens) plan_token(a, static_cast<int>(t), starts, a.parents);
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * kTokenThreads + tid;
+  const bool in_range = t < a.num_tokens;
+  int s = n_seqs, start = 0;
+  Walk w;
+  if (in_range) {
+    s = request_of(a, static_cast<int>(t), starts);
+    if (s < n_seqs) {
+      start = starts[s];
+      if (a.mask_words == 1) w = walk_of(a, static_cast<int>(t) - start, a.parents + start);
+    }
+  }
+  if (early) grid_dependency_sync();
+  if (in_range) {
+    plan_token(a, static_cast<int>(t), s, start,
+               a.parents == nullptr ? nullptr : a.parents + start, w);
+  }
 }
 
 }  // namespace
@@ -397,8 +473,8 @@ extern "C" int svllm_paged_plan(
             num_seqs <= kPlanThreads;
   a.err = err;
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  // a thread per request, and per token where those are done here too (1024 tokens by 256 threads
-  // took 6.6 us)
+  // a thread per request, and per token where those are done here too (512 tokens by 256 threads
+  // took 4.7 us instead of 3.9)
   int64_t threads = a.fused && num_tokens > num_seqs ? num_tokens : num_seqs;
   if (threads < 1) threads = 1;
   threads = threads > kPlanThreads ? kPlanThreads : round_up(threads, kWarpSize);

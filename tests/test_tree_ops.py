@@ -56,7 +56,7 @@ def make_plan_case(seed, requests, nodes, context, bs, *, tree, short, finish, p
     return {"context_lens": ctx, "query_lens": query, "block_tables": tables,
             "blocks_owned": owned, "free_blocks": ids[at:] + [0] * sum(owned),
             "free_count": count, "num_tokens": sum(q0) + pad, "block_size": bs,
-            "parents": random_parents(seed, q0) if tree else None,
+            "parents": random_parents(seed, q0) + [-1] * pad if tree else None,
             "max_query_len": max(1, nodes)}
 
 
@@ -71,6 +71,9 @@ def make_plan_case(seed, requests, nodes, context, bs, *, tree, short, finish, p
     (1030, 3, 40, 16, True, True, 7, 0),      # more requests than one pass of a CTA takes
     (1500, 7, 64, 8, True, False, 5, 0),      # many tokens: the second kernel
     (2100, 4, 64, 8, False, True, 0, 9),
+    (300, 64, 100, 16, True, True, 5, 7),     # full mask words, the second kernel
+    (4200, 2, 20, 16, True, False, 0, 3),     # more starts than that one keeps
+    (64, 40, 30, 1, True, False, 0, 0),       # long runs of blocks
 ], ids=str)
 def test_paged_plan(device, requests, nodes, context, bs, tree, short, finish, pad):
     case = make_plan_case(requests * 31 + nodes, requests, nodes, context, bs, tree=tree,
@@ -152,6 +155,36 @@ def test_paged_plan_bad_lengths_on_cuda(cuda):
     out, _, _ = run_plan(cuda, case)
     assert svllm_ops.read_device_error(0, True) == 1
     assert out[1].tolist() == [6, 0, 0, 0, 0, 0] and out[0].tolist()[-1] == 12
+
+
+@pytest.mark.gpu
+def test_paged_plan_bad_lengths_of_many_tokens_on_cuda(cuda):
+    """The same where the tokens have a kernel of their own: a length of 2^31 - 1 in the middle,
+    with which sums of lengths stop short of wrapping."""
+    requests, at = 600, 400
+    query = [3] * requests
+    query[7], query[at] = 9, 2 ** 31 - 1   # wider than the mask; past every token
+    case = {"context_lens": [4] * requests, "query_lens": query,
+            "block_tables": [[0, 0, 0, 0]] * requests, "blocks_owned": [4] * requests,
+            "free_blocks": [0], "free_count": 0, "num_tokens": 3 * requests + 6, "block_size": 4,
+            "parents": ([-1, 0, 0] * 7 + [-1] * 9 + [-1, 0, 5] + [-1, 0, 1] * requests)[
+                : 3 * requests + 6], "max_query_len": 8}
+    svllm_ops.read_device_error(0, True)
+    out, _, _ = run_plan(cuda, case)
+    assert svllm_ops.read_device_error(0, True) == 1
+    start = [0]
+    for q in query:
+        start.append(min(start[-1] + q, case["num_tokens"]))
+    assert out[0].tolist() == start
+    served = [7 if s != 7 and s < at else 0 for s in range(requests)]
+    assert out[1].tolist() == served
+    live = torch.tensor([s != 7 for s, q in enumerate(query[:at]) for _ in range(q)] +
+                        [False] * (case["num_tokens"] - start[at]))
+    masks, positions = out[4].flatten().cpu(), out[3].cpu()
+    assert ((masks != 0) == live).all() and ((out[2].cpu() >= 0) == live).all()
+    assert masks[:6].tolist() == [1, 3, 5, 1, 3, 5]
+    assert masks[30:36].tolist() == [1, 3, 4, 1, 3, 7]  # a parent that comes later: a root
+    assert positions[30:36].tolist() == [4, 5, 4, 4, 5, 6]
 
 
 # ------------------------------------------------------------------------------ tree_accept
