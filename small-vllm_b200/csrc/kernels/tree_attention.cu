@@ -115,6 +115,7 @@ struct TreeAttnArgs {
   int max_blocks;
   int max_length;                  // rows that a block table holds
   int max_nodes;                   // nodes that the mask's words hold
+  int whole;                       // 1: items are not cut
   int most_steps;                  // the longest line that requests without overlap make
   int block_size;
   Divider page;                    // by the block size
@@ -330,6 +331,10 @@ __device__ __forceinline__ void find_share(const TreeAttnArgs& a, Request r, int
         }
       }
       if (lane == owner) p = locate(a, s, r, static_cast<int>(border) - before);
+      if (a.whole && p.step > 0) {  // on to the next item
+        ++p.item;
+        p.step = 0;
+      }
       p.s = __shfl_sync(0xffffffffu, p.s, owner);
       p.item = __shfl_sync(0xffffffffu, p.item, owner);
       p.step = __shfl_sync(0xffffffffu, p.step, owner);
@@ -1285,6 +1290,21 @@ int64_t workspace_bytes(int ctas) {
          (4 * Shape<D>::kPartFloats * 4 + 2 * static_cast<int64_t>(sizeof(Cut) + sizeof(int)));
 }
 
+// Whether items stay whole, so that there is nothing to join. A join costs 4 us and more with the
+// rows, a longer share of one item some 1.3 us a tile: whole items where no table holds more than
+// two tiles, and up to four where there is work for every CTA all the same. us cut and whole, 16
+// heads on 8 KV heads of 128, rows of a table: 208, 1 request of 8 nodes 12.0 and 10.9; 240, 64 of
+// 40 34.4 and 24.8; 416, 1 of 8 12.3 and 15.4, 4 of 8 13.4 and 15.5, 16 of 8 19.1 and 16.2; 448, 64
+// of 40 42.6 and 36.1; 912, 64 of 8 45.3 and 53.2.
+inline bool whole_items(const TreeAttnArgs& a, int ctas) {
+  const int64_t steps = (a.max_length + kTile - 1) / kTile;
+  if (steps <= 2) return true;
+  if (steps > 4 || a.num_seqs == 0) return false;
+  const int64_t nodes = (a.num_tokens + a.num_seqs - 1) / a.num_seqs;  // of a request, on average
+  const int64_t tiles = (nodes * a.group + kTile - 1) / kTile;
+  return a.num_seqs * a.num_kv_heads * steps * ((tiles + 1) / 2) >= 2 * ctas;
+}
+
 template <int D>
 int launch_tree_attention(TreeAttnArgs& a, void* workspace, int device, cudaStream_t stream) {
   const int ctas = attention_ctas(device);
@@ -1292,6 +1312,7 @@ int launch_tree_attention(TreeAttnArgs& a, void* workspace, int device, cudaStre
   a.marks = reinterpret_cast<int*>(a.parts + static_cast<int64_t>(ctas) * 4 *
                                                  Shape<D>::kPartFloats);
   a.cuts = reinterpret_cast<Cut*>(a.marks + 2 * ctas);
+  a.whole = whole_items(a, ctas);
   CUtensorMap map_k, map_v;
   const int64_t cols = static_cast<int64_t>(a.num_kv_heads) * D;
   if (!make_map(&map_k, a.k_cache, a.cache_slots, cols, cols, a.box_rows) ||
@@ -1305,8 +1326,7 @@ int launch_tree_attention(TreeAttnArgs& a, void* workspace, int device, cudaStre
   }
   const int status = launch(tree_attention_kernel<D>, dim3(ctas), dim3(kThreads),
                                        Shape<D>::kSmem, stream, 1u, map_k, map_v, a);
-  // where no table holds more than a tile of rows, items have one step and no border cuts one
-  if (status != SVLLM_OK || ctas < 2 || a.max_length <= kTile) return status;
+  if (status != SVLLM_OK || ctas < 2 || a.whole) return status;
   // as many blocks as are resident at once
   return launch(tree_attention_join_kernel<D>, dim3(256 / D * ctas), dim3(kJoinThreads * D), 0,
                 stream, 1u, a, ctas);

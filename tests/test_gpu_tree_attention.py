@@ -77,6 +77,11 @@ def check(s, out=None):
     ([5] * 32, [64 * s for s in range(32)], 32, 8, 64, 16, "chain"),
     ([300, 1, 90], [1000, 250, 0], 4, 2, 128, 16, "chain"),
     ([2000], [0], 2, 1, 64, 16, "chain"),           # a causal prompt
+    ([9], [200], 16, 8, 128, 16, "tree"),           # tables of two tiles: items stay whole
+    ([130, 2, 0, 33], [110, 0, 7, 215], 6, 3, 64, 16, "tree"),
+    ([8] * 40, [11 * s for s in range(40)], 16, 8, 128, 16, "tree"),  # of four, enough for all
+    ([40, 7, 99] * 11, [400, 0, 313] * 11, 21, 3, 128, 12, "tree"),
+    ([6] * 60, [7 * s for s in range(60)], 9, 9, 64, 32, "chain"),
 ], ids=str)
 def test_matches_the_definition(cuda, counts, context, heads, kv_heads, dim, bs, shape):
     check(build(cuda, counts, context, heads, kv_heads, dim, bs, shape=shape,
