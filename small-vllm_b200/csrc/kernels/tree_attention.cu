@@ -475,11 +475,11 @@ __device__ __forceinline__ bool has_nodes(const Segment& g, int step) {
 // One of the warps that bring K and V, tile after tile in the order in which the tensor cores take
 // them: every kLoaderWarps-th TMA instruction of each tile (one costs its issuer some 60 cycles, a
 // tile of 16-row pages has 16; four loaders, two of them from the helpers, were no faster). Where
-// the block size allows, a TMA box is a run of 8 to 128 rows that no page border can fall into,
-// gcd(block_size, 128); otherwise an instruction gathers 4 rows, some 45 cycles each. With pages of
-// one row that costs 345 us where the 64 requests above take 203; copies of 16 bytes per thread
-// (cp.async) took 290 there and more than the gather in every smaller case. Issued by all lanes
-// at once, each its own rows, the gather took 603.
+// the block size allows, a TMA box is a run of 4 to 128 rows that no page border can fall into,
+// gcd(block_size, 128); otherwise an instruction gathers 4 rows. With 12-row pages the 64 requests
+// above take 268 us in boxes of 4 rows and 329 gathered; with pages of one row 345, where copies
+// of 16 bytes per thread (cp.async) took 290 and more than the gather in every smaller case. Issued
+// by all lanes at once, each its own rows, the gather took 603.
 template <int D>
 struct Loader {
   using S = Shape<D>;
@@ -835,19 +835,20 @@ __device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w) 
     float ref = -kInf, sum = 0.0f;
 #pragma unroll 1
     for (int step = g.step0; step < g.step1; ++step) {
+      // the mask's words are fetched while the scores are on their way
+      const bool masked = any && (step + 1) * kTile > g.context;
+      uint64_t bits[2] = {};
+      if (masked) visible(a, g, mask, node, step * kTile, bits);
       // the warp leaves together: the TMEM loads below are collective
       if (!warp_wait(sy, kScoresDone + w, scores_phase, a.err)) return;
       scores_phase ^= 1;
       tc_fence_after();
       if (any) {
-        const bool masked = (step + 1) * kTile > g.context;
         uint32_t x[4][32];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_load32(scores + 32 * c, x[c]);
         tmem_wait_load();
         if (masked) {
-          uint64_t bits[2];
-          visible(a, g, mask, node, step * kTile, bits);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const auto see = static_cast<uint32_t>(bits[c / 2] >> (32 * (c % 2)));
@@ -1419,7 +1420,7 @@ extern "C" int svllm_tree_attention_bf16(
   a.cache_slots = static_cast<int>(num_blocks * block_size);
   a.box_rows = 128;
   while (block_size % a.box_rows != 0) a.box_rows /= 2;
-  if (a.box_rows < 8) a.box_rows = 1;
+  if (a.box_rows < 4) a.box_rows = 1;
   a.mask_words = static_cast<int>(mask_words);
   a.scale_log2 = static_cast<float>(static_cast<double>(scale) / std::log(2.0));
   a.err = err;
