@@ -18,17 +18,17 @@
 // lengths. An item cut by a share's border leaves unnormalised partial sums in the workspace, which
 // a second small kernel joins.
 //
-// In a CTA: two warps bring K and V rows through the block table with TMA into 128-byte-swizzled
-// tiles (any block size: a page may end anywhere in a tile); one thread issues tcgen05.mma: S = Q
-// K^T into TMEM, then O += P V with P read from TMEM and V as the N-major operand, alternating
-// between two accumulators so that the tensor pipe works on one M tile while the other's softmax
-// runs; two groups of 4 warps do the softmax, one thread per row, and write P (bf16, as the second
-// product takes it) over S. The running maximum is a reference that moves only when a row exceeds
-// it by 2^8, so O in TMEM is seldom rescaled; the sums are fp32 and the result does not depend on
-// the reference. Masked scores are replaced after the product. Four helper warps bring the query
-// rows and, since 0 * NaN would reach rows that do not see it, zero the values of V that are not
-// finite in the tiles that hold tree nodes; they are added again, for the rows that see them, at
-// the end. One warp lists the CTA's segments for all others.
+// In a CTA: two or four warps bring K and V rows through the block table with TMA into
+// 128-byte-swizzled tiles (any block size: a page may end anywhere in a tile); one thread issues
+// tcgen05.mma: S = Q K^T into TMEM, then O += P V with P read from TMEM and V as the N-major
+// operand, alternating between two accumulators so that the tensor pipe works on one M tile while
+// the other's softmax runs; two groups of 4 warps do the softmax, one thread per row, and write P
+// (bf16, as the second product takes it) over S. The running maximum is a reference that moves only
+// when a row exceeds it by 2^8, so O in TMEM is seldom rescaled; the sums are fp32 and the result
+// does not depend on the reference. Masked scores are replaced after the product. Four or two
+// helper warps bring the query rows and, since 0 * NaN would reach rows that do not see it, zero
+// the values of V that are not finite in the tiles that hold tree nodes; they are added again, for
+// the rows that see them, at the end. One warp lists the CTA's segments for all others.
 //
 // Measured in a graph, inputs past L2, head_dim 128: 64 requests of 48 to 64 nodes over 2048 to
 // 4096 rows, 16 heads on 8 KV heads, 203 us (1.08 GB, 5.3 TB/s: 0.82 of the copy rate; 219 us under
@@ -39,7 +39,7 @@
 // products take 2048: per accumulator those and the softmax (1580 cycles, 1260 of them the
 // exponentials) wait for each other. Parts of 64 cached rows with their scores a part ahead took
 // 119: products of N = 64 take as long as those of 128. 32 nodes over 32768 rows 41 us, 20 of them
-// the stream, 10 the join of some 37 segments per item. 8 nodes over 128 rows 8.7 us: one tile's
+// the stream, 10 the join of some 37 segments per item. 8 nodes over 128 rows 8.2 us: one tile's
 // chain of dependent steps, most of it the first fetch of the roles' code.
 #include <cuda_runtime.h>
 
@@ -56,10 +56,8 @@ namespace {
 
 constexpr int kTile = 128;            // query rows per M tile, cached rows per key tile
 constexpr int kSoftmaxWarps = 8;      // two groups of 4: accumulators 0 and 1
-constexpr int kHelperWarps = 4;       // query rows and the check of V
-constexpr int kLoaderWarps = 2;       // K and V
-constexpr int kLoadWarp = kSoftmaxWarps + kHelperWarps;
-constexpr int kMmaWarp = kLoadWarp + kLoaderWarps;
+constexpr int kSideWarps = 6;         // helpers (query rows, check of V), then loaders (K, V)
+constexpr int kMmaWarp = kSoftmaxWarps + kSideWarps;
 constexpr int kPlanWarp = kMmaWarp + 1;  // lists the CTA's segments, zeroes rows without an item
 constexpr int kThreads = (kPlanWarp + 1) * kWarpSize;
 constexpr int kWarps = kThreads / kWarpSize;
@@ -72,6 +70,11 @@ constexpr uint32_t kScores = 0;       // TMEM columns: S (and P) of accumulator 
 constexpr uint32_t kOutput = 256;     // O at 256 + 128 w
 constexpr float kRescaleAbove = 8.0f;  // in powers of two
 constexpr int kJoinThreads = 2;       // of a join block, per element of head_dim
+// Boxes of fewer rows than this take four loaders and two helpers, others two and four. us with two
+// and four loaders: 12-row pages (boxes of 4), the 64 requests above 268 and 213, 32 chains of 5
+// nodes 65 and 50, 13 short requests 22.7 and 23.4; 8-row pages 214 and 207, 50 and 44, but 1
+// request of 8 nodes 8.7 and 9.3, 8 of up to 128 86 and 90; 16-row pages no gain.
+constexpr int kSmallBox = 8;
 constexpr int kMaxCtas = 256;         // one per SM; the join lists their borders
 
 template <int D>
@@ -227,9 +230,9 @@ constexpr int kScoresDone = kEmptyQ + 1, kWeightsDone = kScoresDone + 2;
 constexpr int kOutputDone = kWeightsDone + 2, kDrain = kOutputDone + 2;
 constexpr int kListed = kDrain + 1, kRead = kListed + kSegments, kBarriers = kRead + kSegments;
 
-__device__ __forceinline__ int arrivals(int bar) {
-  if (bar < kChecked) return kLoaderWarps;
-  if (bar < kEmpty) return kHelperWarps * kWarpSize;
+__device__ __forceinline__ int arrivals(int bar, int helpers) {
+  if (bar < kChecked) return kSideWarps - helpers;
+  if (bar < kEmpty) return helpers * kWarpSize;
   if (bar >= kRead) return kPlanWarp;  // every other warp
   return bar == kWeightsDone || bar == kWeightsDone + 1 ? 4 * kWarpSize : 1;
 }
@@ -241,7 +244,7 @@ struct Sync {
   // per helper warp, accumulator and segment modulo 8: V held something not finite. A warp clears
   // its own word when it begins a segment; no warp is more than kSegments behind another then, so
   // nobody still reads the one that the segment 8 before left there.
-  int odd_values[kHelperWarps][2][2 * kSegments];
+  int odd_values[kSideWarps][2][2 * kSegments];
   int costs[kWarps];     // of the warps' shares of the requests
   Segment list[kSegments];
 };
@@ -443,9 +446,8 @@ struct Ring {
   }
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
-               "r"(take ? 16 : 0)
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src)
                : "memory");
 }
 
@@ -474,13 +476,13 @@ __device__ __forceinline__ bool has_nodes(const Segment& g, int step) {
 
 // One of the warps that bring K and V, tile after tile in the order in which the tensor cores take
 // them: every kLoaderWarps-th TMA instruction of each tile (one costs its issuer some 60 cycles, a
-// tile of 16-row pages has 16; four loaders, two of them from the helpers, were no faster). Where
-// the block size allows, a TMA box is a run of 4 to 128 rows that no page border can fall into,
-// gcd(block_size, 128); otherwise an instruction gathers 4 rows. With 12-row pages the 64 requests
-// above take 268 us in boxes of 4 rows and 329 gathered; with pages of one row 345, where copies
-// of 16 bytes per thread (cp.async) took 290 and more than the gather in every smaller case. Issued
-// by all lanes at once, each its own rows, the gather took 603.
-template <int D>
+// tile of 16-row pages has 16). Where the block size allows, a TMA box is a run of 4 to 128 rows
+// that no page border can fall into, gcd(block_size, 128); otherwise an instruction gathers 4 rows.
+// With 12-row pages and two loaders the 64 requests above took 268 us in boxes of 4 rows and 329
+// gathered; with pages of one row the gather takes 254 with four loaders. Copies of 16 bytes per
+// thread (cp.async) took 290 there and more than the gather in every smaller case. Issued by all
+// lanes at once, each its own rows, the gather took 603.
+template <int D, int kLoaderWarps>
 struct Loader {
   using S = Shape<D>;
   const TreeAttnArgs& a;
@@ -602,7 +604,7 @@ static_assert(kChecked <= 64, "one bit per barrier that a copy may signal");
 
 // The helper warps: the query rows of each segment, and the V tiles that hold tree nodes,
 // whose values that are not finite are zeroed before the tensor cores see them.
-template <int D>
+template <int D, int kHelperWarps>
 __device__ __forceinline__ void help(const TreeAttnArgs& a, Sync& sy, uint8_t* q_tiles,
                                      uint8_t* ring, int warp, int lane) {
   using S = Shape<D>;
@@ -623,26 +625,28 @@ __device__ __forceinline__ void help(const TreeAttnArgs& a, Sync& sy, uint8_t* q
     __syncwarp();
 #pragma unroll 1
     for (int w = 0; w < g.active; ++w) {
+      // row = node * group + head of the KV head; what lies outside the request's rows of the tile
+      // stays as it was: nothing reads the products of those
+      const int rows = pick(g.rows, w), lane0 = w == 0 ? 0 : g.lane0, c = lane % kLanes;
+      const uint32_t base = smem_addr(q_tiles + w * S::kTileBytes) + (c / 8) * kHalfBytes;
+      const auto* src = static_cast<const __nv_bfloat16*>(a.q) + c * 8;
+      // the warps share the rows, up to 32 at a time, whose places a lane each works out
+      const int share = (rows + kHelperWarps - 1) / kHelperWarps;
+      const int block =
+          min(kWarpSize, (share + kRowsAtOnce - 1) / kRowsAtOnce * kRowsAtOnce);
 #pragma unroll 1
-      for (int r0 = warp * kWarpSize; r0 < kTile; r0 += kHelperWarps * kWarpSize) {
-        // row = node * group + head of the KV head
-        const int r = r0 + lane - (w == 0 ? 0 : g.lane0);
-        const int row = pick(g.row0, w) + max(r, 0);
+      for (int r0 = warp * block; r0 < rows; r0 += kHelperWarps * block) {
+        const int row = pick(g.row0, w) + min(r0 + lane, rows - 1);
         const int node = a.by_group.divide(row);
         const int64_t offset =
-            r >= 0 && r < pick(g.rows, w)
-                ? (g.start + node) * a.q_stride +
-                      (static_cast<int64_t>(pick(g.kv_head, w) - node) * a.group + row) * D
-                : -1;
-        const int c = lane % kLanes;
-        const uint32_t base = smem_addr(q_tiles + w * S::kTileBytes) + (c / 8) * kHalfBytes;
-        const auto* src = static_cast<const __nv_bfloat16*>(a.q) + c * 8;
+            (g.start + node) * a.q_stride +
+            (static_cast<int64_t>(pick(g.kv_head, w) - node) * a.group + row) * D;
+        const int count = min(block, rows - r0);
 #pragma unroll 4
-        for (int i = 0; i < kWarpSize / kRowsAtOnce; ++i) {
-          const int x = i * kRowsAtOnce + lane / kLanes;
-          const int64_t from = __shfl_sync(0xffffffffu, offset, x);
-          cp_async16(base + (r0 + x) * 128 + (((c % 8) ^ (x & 7)) << 4),
-                     src + (from < 0 ? 0 : from), from >= 0);
+        for (int i = 0; i < count; i += kRowsAtOnce) {
+          const int r = i + lane / kLanes, x = lane0 + r0 + r;
+          const int64_t from = __shfl_sync(0xffffffffu, offset, r);
+          if (r < count) cp_async16(base + x * 128 + (((c % 8) ^ (x & 7)) << 4), src + from);
         }
       }
     }
@@ -810,7 +814,7 @@ __device__ __forceinline__ void visible(const TreeAttnArgs& a, const Segment& g,
 }
 
 // Softmax and epilogue of accumulator w; this thread owns row `row` of the tile.
-template <int D>
+template <int D, int kHelperWarps>
 __device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w) {
   using S = Shape<D>;
   const int quarter = (threadIdx.x / kWarpSize) % 4;
@@ -872,7 +876,7 @@ __device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w) 
         // the reference moves when it is the first or is exceeded by 2^8
         float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * a.scale_log2;
         if (ref != -kInf && !(top > ref + kRescaleAbove)) top = ref;
-        const bool moved = top != ref;
+        const bool moved = valid && top != ref;
         if (step > g.step0 && __any_sync(0xffffffffu, moved)) {
           const float f = moved ? exp2_approx(ref - top) : 1.0f;
           sum *= f;
@@ -1020,11 +1024,12 @@ __device__ __forceinline__ void fill_rest(const TreeAttnArgs& a, int64_t row_vec
   }
 }
 
-template <int D>
+template <int D, int kHelperWarps>
 __global__ void __launch_bounds__(kThreads, 1)
     tree_attention_kernel(const __grid_constant__ CUtensorMap map_k,
                           const __grid_constant__ CUtensorMap map_v, const TreeAttnArgs a) {
   using S = Shape<D>;
+  constexpr int kLoadWarp = kSoftmaxWarps + kHelperWarps;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Sync sy;
   uint8_t* q_tiles = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
@@ -1033,7 +1038,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = __shfl_sync(0xffffffffu, tid / kWarpSize, 0), lane = tid % kWarpSize;
 
   if (tid < kBarriers) {
-    mbar_init(&sy.bar[tid], arrivals(tid));
+    mbar_init(&sy.bar[tid], arrivals(tid, kHelperWarps));
     fence_mbar_init();
   }
   if (tid == 0) sy.abort = 0;
@@ -1082,13 +1087,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp < kSoftmaxWarps) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
-    softmax<D>(a, sy, warp / 4);
+    softmax<D, kHelperWarps>(a, sy, warp / 4);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters));
     if (warp < kLoadWarp) {
-      help<D>(a, sy, q_tiles, ring, warp - kSoftmaxWarps, lane);
+      help<D, kHelperWarps>(a, sy, q_tiles, ring, warp - kSoftmaxWarps, lane);
     } else if (warp < kMmaWarp) {
-      Loader<D> l{a, sy, map_k, map_v, ring, warp - kLoadWarp, lane};
+      Loader<D, kSideWarps - kHelperWarps> l{a, sy, map_k, map_v, ring, warp - kLoadWarp, lane};
       l.run();
     } else if (warp == kMmaWarp) {
       issue_products<D>(a, sy, q_tiles, ring);
@@ -1321,12 +1326,14 @@ int launch_tree_attention(TreeAttnArgs& a, void* workspace, int device, cudaStre
     return SVLLM_ERR_CUDA;
   }
   // raises the kernel's shared-memory limit on its first use
-  if (blocks_per_sm(reinterpret_cast<const void*>(tree_attention_kernel<D>), kThreads,
-                    Shape<D>::kSmem, device) < 1) {
+  const auto kernel =
+      a.box_rows < kSmallBox ? tree_attention_kernel<D, 2> : tree_attention_kernel<D, 4>;
+  if (blocks_per_sm(reinterpret_cast<const void*>(kernel), kThreads, Shape<D>::kSmem, device) <
+      1) {
     return SVLLM_ERR_CUDA;
   }
-  const int status = launch(tree_attention_kernel<D>, dim3(ctas), dim3(kThreads),
-                                       Shape<D>::kSmem, stream, 1u, map_k, map_v, a);
+  const int status = launch(kernel, dim3(ctas), dim3(kThreads), Shape<D>::kSmem, stream, 1u,
+                            map_k, map_v, a);
   if (status != SVLLM_OK || ctas < 2 || a.whole) return status;
   // as many blocks as are resident at once
   return launch(tree_attention_join_kernel<D>, dim3(256 / D * ctas), dim3(kJoinThreads * D), 0,
