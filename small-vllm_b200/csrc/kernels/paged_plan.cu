@@ -482,7 +482,7 @@ extern "C" int svllm_paged_plan(
       a.fused ? 4 * static_cast<size_t>(num_seqs + 1 + (parents != nullptr ? num_tokens : 0)) : 0;
   const int status = launch(plan_requests_kernel, dim3(1), dim3(static_cast<unsigned>(threads)),
                             staged, st, 1u, a);
-  if (status != SVLLM_OK || a.fused) return status;
+  if (status != SVLLM_OK || a.fused || num_tokens == 0) return status;
   return launch(plan_tokens_kernel,
                 dim3(static_cast<unsigned>((num_tokens + kTokenThreads - 1) / kTokenThreads)),
                 dim3(kTokenThreads), 0, st, 1u, a);

@@ -74,6 +74,7 @@ def make_plan_case(seed, requests, nodes, context, bs, *, tree, short, finish, p
     (300, 64, 100, 16, True, True, 5, 7),     # full mask words, the second kernel
     (4200, 2, 20, 16, True, False, 0, 3),     # more starts than that one keeps
     (64, 40, 30, 1, True, False, 0, 0),       # long runs of blocks
+    (1100, 0, 64, 16, False, False, 2, 0),    # nobody has a token, nor is there any
 ], ids=str)
 def test_paged_plan(device, requests, nodes, context, bs, tree, short, finish, pad):
     case = make_plan_case(requests * 31 + nodes, requests, nodes, context, bs, tree=tree,
