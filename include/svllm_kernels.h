@@ -383,9 +383,8 @@ int svllm_paged_plan(const int32_t* context_lens, const int32_t* query_lens, int
  * head_dim 64 or 128, any number of query heads per KV head, 16-byte aligned out, q and caches, a
  * q_token_stride of whole 16 bytes, else SVLLM_ERR_UNSUPPORTED. scale must be positive and finite.
  * Zeros with SVLLM_DEVERR_BAD_INDEX: a request whose seq_lens is below its number of tokens or
- * past its block table, or whose tree is wider than the mask. With the same bit, a request whose
- * query_start_loc falls or ends past num_tokens has no rows (none of out is written for it), nor
- * has any request where those left overlap into more work than num_tokens tokens can be. A
+ * past its block table, or whose tree is wider than the mask; all of out where query_start_loc does
+ * not rise from 0 to at most num_tokens, since nothing then says whose its rows are. A
  * table entry outside the cache raises the bit and reads block 0. workspace: at
  * least svllm_tree_attention_workspace_bytes bytes of device memory, 16-byte aligned, any
  * contents; calls that overlap on the GPU must not share it.

@@ -119,7 +119,6 @@ struct TreeAttnArgs {
   int max_length;                  // rows that a block table holds
   int max_nodes;                   // nodes that the mask's words hold
   int whole;                       // 1: items are not cut
-  int most_steps;                  // the longest line that requests without overlap make
   int block_size;
   Divider page;                    // by the block size
   int group;                       // query heads per KV head
@@ -138,7 +137,8 @@ struct Request {
   int steps;                          // key tiles
   int pairs;                          // items of two M tiles per KV head
   int odd;                            // 1: a last single M tile, in items of two KV heads
-  bool bad;                           // lengths out of range
+  bool bad;                           // starts or lengths out of range
+  bool astray;                        // starts that fall or lie outside the tokens
 };
 
 __device__ __forceinline__ Request load_request(const TreeAttnArgs& a, int s) {
@@ -146,7 +146,7 @@ __device__ __forceinline__ Request load_request(const TreeAttnArgs& a, int s) {
   const int begin = a.query_start_loc[s], end = a.query_start_loc[s + 1];
   const int length = a.seq_lens[s];
   if (begin < 0 || end < begin || end > a.num_tokens) {
-    r.bad = true;
+    r.bad = r.astray = true;
     return r;
   }
   r.start = begin;
@@ -172,8 +172,8 @@ __device__ __forceinline__ int request_cost(const TreeAttnArgs& a, const Request
   return a.num_kv_heads * r.steps * (r.pairs + r.odd);
 }
 
-// Lengths come from the device unchecked: sums of costs stop at the largest int instead of
-// wrapping.
+// Costs of requests whose starts rise from 0 add up to an int (checked on the host from the sizes).
+// Of others, of which nothing is done, the sum stops at the largest int instead of wrapping.
 __device__ __forceinline__ int add_costs(int a, int b) {
   return static_cast<int>(min(static_cast<unsigned>(a) + static_cast<unsigned>(b),
                               static_cast<unsigned>(INT32_MAX)));
@@ -293,15 +293,12 @@ __device__ __forceinline__ int sum_up_to_lane(int v, int lane) {
 }
 
 // The borders of this CTA's share of the line. `own`: lane i holds the cost of the i-th `chunk` of
-// requests; with a chunk of 1, `r` is the lane's request.
+// requests; with a chunk of 1, `r` is the lane's request. `astray`: the starts do not rise from 0
+// to at most the number of tokens, so no request has items.
 __device__ __forceinline__ void find_share(const TreeAttnArgs& a, Request r, int own, int chunk,
-                                           int lane, Place (&places)[2]) {
+                                           bool astray, int lane, Place (&places)[2]) {
   const int upto = sum_up_to_lane(own, lane);
-  int total = __shfl_sync(0xffffffffu, upto, kWarpSize - 1);
-  if (total > a.most_steps) {  // requests overlap: the starts fall somewhere. Nothing is done
-    if (lane == 0) raise_error(a.err, kErrBadIndex);
-    total = 0;
-  }
+  const int total = astray ? 0 : __shfl_sync(0xffffffffu, upto, kWarpSize - 1);
   // at least two steps each: a shorter share costs more in the join than it saves (1 request of 8
   // nodes over 128 rows: 12.7 us with 2, 16.4 with 4; 13 requests of up to 37 nodes 27 and 38)
   const int share = max(2, static_cast<int>((total + gridDim.x - 1u) / gridDim.x));
@@ -1004,10 +1001,13 @@ __device__ __forceinline__ void softmax(const TreeAttnArgs& a, Sync& sy, int w) 
 }
 
 // Rows that no item covers are zero: those of requests that were not served, and what lies behind
-// the last. One warp per CTA, every gridDim-th request or row.
-__device__ __forceinline__ void fill_rest(const TreeAttnArgs& a, int64_t row_vecs, int lane) {
+// the last; all of them where the starts lead astray. One warp per CTA, every gridDim-th request or
+// row.
+__device__ __forceinline__ void fill_rest(const TreeAttnArgs& a, bool astray, int64_t row_vecs,
+                                          int lane) {
   uint4* out = static_cast<uint4*>(a.out);
-  for (int s = blockIdx.x; s < a.num_seqs; s += gridDim.x) {
+  if (astray && lane == 0) raise_error(a.err, kErrBadIndex);
+  for (int s = blockIdx.x; !astray && s < a.num_seqs; s += gridDim.x) {
     const Request r = load_request(a, s);
     if (r.bad && lane == 0) raise_error(a.err, kErrBadIndex);
     if (r.steps > 0) continue;
@@ -1015,8 +1015,7 @@ __device__ __forceinline__ void fill_rest(const TreeAttnArgs& a, int64_t row_vec
       st_global_v4(out + r.start * row_vecs + i, make_uint4(0, 0, 0, 0));
     }
   }
-  int64_t tail = a.query_start_loc[a.num_seqs];
-  if (tail < 0) tail = 0;
+  const int64_t tail = astray ? 0 : a.query_start_loc[a.num_seqs];
   for (int64_t t = tail + blockIdx.x; t < a.num_tokens; t += gridDim.x) {
     for (int64_t i = lane; i < row_vecs; i += kWarpSize) {
       st_global_v4(out + t * row_vecs + i, make_uint4(0, 0, 0, 0));
@@ -1056,18 +1055,21 @@ __global__ void __launch_bounds__(kThreads, 1)
   const bool few = a.num_seqs <= kWarpSize;
   const int chunk = few ? 1 : (a.num_seqs + kWarps - 1) / kWarps;
   static_assert(kWarpSize > kWarps, "a chunk of 1 request is one that its lane has loaded");
+  bool astray = false;
   if (!few) {
     int cost = 0;
 #pragma unroll 1
     for (int s = warp * chunk + lane; s < min(a.num_seqs, (warp + 1) * chunk); s += kWarpSize) {
-      cost = add_costs(cost, request_cost(a, load_request(a, s)));
+      const Request r = load_request(a, s);
+      cost = add_costs(cost, request_cost(a, r));
+      astray |= r.astray;
     }
 #pragma unroll
     for (int off = 16; off > 0; off /= 2) {
       cost = add_costs(cost, __shfl_xor_sync(0xffffffffu, cost, off));
     }
     if (lane == 0) sy.costs[warp] = cost;
-    __syncthreads();
+    astray = __syncthreads_or(astray);
   }
   Place places[2]{};
   if (warp == kPlanWarp) {
@@ -1079,7 +1081,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       r = load_request(a, lane);
       cost = request_cost(a, r);
     }
-    find_share(a, r, cost, chunk, lane, places);
+    astray = __any_sync(0xffffffffu, astray | r.astray | (a.query_start_loc[0] != 0));
+    find_share(a, r, cost, chunk, astray, lane, places);
   }
   tc_fence_before();
   __syncthreads();
@@ -1099,7 +1102,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       issue_products<D>(a, sy, q_tiles, ring);
     } else {
       plan(a, sy, places[0], places[1], lane);
-      fill_rest(a, static_cast<int64_t>(a.num_kv_heads) * a.group * D / 8, lane);
+      fill_rest(a, astray, static_cast<int64_t>(a.num_kv_heads) * a.group * D / 8, lane);
     }
   }
 
@@ -1388,7 +1391,7 @@ extern "C" int svllm_tree_attention_bf16(
       (q_token_stride * 2) % 16 != 0) {
     return SVLLM_ERR_UNSUPPORTED;
   }
-  // the line of steps is counted in 32 bits: its length is at most this
+  // the line of steps is counted in 32 bits: its length is at most most * tiles
   const int64_t most = (max_blocks * block_size / 128 + 1) * num_kv_heads;
   const int64_t tiles = num_tokens * (num_heads / num_kv_heads) / 128 + num_seqs;
   if (most >= kMax || tiles >= kMax / most) return SVLLM_ERR_TOO_LARGE;
@@ -1420,7 +1423,6 @@ extern "C" int svllm_tree_attention_bf16(
   a.page = make_divider(block_size);
   a.group = static_cast<int>(num_heads / num_kv_heads);
   a.max_length = static_cast<int>(max_blocks * block_size);
-  a.most_steps = static_cast<int>(most * tiles);
   a.max_nodes = tree_mask != nullptr ? static_cast<int>(64 * mask_words) : INT32_MAX;
   a.by_group = make_divider(a.group);
   a.num_kv_heads = static_cast<int>(num_kv_heads);

@@ -25,7 +25,8 @@ namespace svllm::ops {
 // Returns:    A new [T, heads, D] tensor.
 // Throws:     c10::Error on dtype, shape, layout or device mismatches, and on CPU for lengths or
 //             blocks out of range; on CUDA those raise the device error word (the request's rows
-//             are zero, a block outside the cache reads block 0).
+//             are zero, all rows where query_start_loc does not rise from 0 to at most T; a block
+//             outside the cache reads block 0).
 at::Tensor tree_attention(const at::Tensor& q, const at::Tensor& k_cache,
                           const at::Tensor& v_cache, const at::Tensor& block_tables,
                           const at::Tensor& seq_lens, const at::Tensor& query_start_loc,

@@ -7,6 +7,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+import svllm_capi
 import svllm_ops
 from tree_reference import (attention_bound, attention_reference, make_pages, masks_of, pack_lists,
                             random_parents)
@@ -280,3 +281,35 @@ def test_refusals(cuda):
     with pytest.raises(RuntimeError, match="elsewhere"):
         svllm_ops.tree_attention(s["q"], s["k"], s["v"], s["tables"].cpu(), s["seq"], s["starts"],
                                  s["mask"])
+
+
+@pytest.mark.parametrize("starts", [
+    [2, 4, 8, 12],    # rises, but not from 0
+    [0, 4, 3, 12],    # falls
+    [0, 12, 4, 12],   # falls, and the requests left overlap
+    [0, 4, 8, 40],    # ends past the tokens
+    [-1, 4, 8, 12],
+    [3],              # no request, and yet a first token
+], ids=str)
+@pytest.mark.parametrize("repeat", [1, 17], ids=["few", "many"])  # 3 or 51 requests
+def test_starts_that_contradict_themselves_leave_nothing_unwritten(cuda, starts, repeat):
+    """query_start_loc has to rise from 0 to at most the number of tokens. Where it does not the
+    error word says so, and all of the output is zero: nothing of what its memory held before, and
+    no row that depends on which of two requests wrote it last."""
+    s = build(cuda, [4, 4, 4] * repeat, [30, 200, 30] * repeat, 16, 8, 128, 16)
+    if len(starts) > 1:
+        good = s["starts"].tolist()
+        starts = starts[:-1] + good[3:-1] + [starts[-1] + 12 * (repeat - 1)]
+    else:
+        s["tables"], s["seq"] = s["tables"][:0], s["seq"][:0]
+    s["starts"] = torch.tensor(starts, dtype=torch.int32, device=cuda)
+    workspace = torch.empty(svllm_capi.tree_attention_workspace_bytes(128), dtype=torch.uint8,
+                            device=cuda)
+    for mask in (s["mask"], None):
+        svllm_ops.read_device_error(0, True)
+        out = torch.full(s["q"].shape, 7.0, dtype=torch.bfloat16, device=cuda)
+        svllm_capi.tree_attention(out, s["q"], s["k"], s["v"], s["tables"], s["seq"], s["starts"],
+                                  mask, s["scale"], workspace)
+        torch.cuda.synchronize()
+        assert svllm_ops.read_device_error(0, True) == 1
+        assert (out == 0).all()
