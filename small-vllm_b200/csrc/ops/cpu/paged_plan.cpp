@@ -46,6 +46,13 @@ void paged_plan(const PagedPlanTensors& p) {
               p.num_tokens);
   TORCH_CHECK(have + back <= capacity, "paged_plan: ", back, " blocks come back to ", have,
               " free ones, free_blocks holds ", capacity);
+  const auto* parents = tree ? p.parents.const_data_ptr<int32_t>() : nullptr;
+  for (int64_t s = 0, t = 0; tree && s < requests; ++s) {
+    for (int32_t i = 0; i < query[s]; ++i, ++t) {
+      TORCH_CHECK(parents[t] >= -1 && parents[t] < i, "paged_plan: parent ", parents[t],
+                  " of node ", i, " of request ", s, " does not come before it");
+    }
+  }
 
   for (int64_t s = 0; s < requests; ++s) {
     for (int32_t i = 0; query[s] < 0 && i < owned[s]; ++i) stack[have++] = tables[s * width + i];
@@ -80,7 +87,6 @@ void paged_plan(const PagedPlanTensors& p) {
   auto* positions = p.positions.mutable_data_ptr<int64_t>();
   auto* mask = tree ? p.tree_mask.mutable_data_ptr<int64_t>() : nullptr;
   const int64_t words = tree ? p.tree_mask.size(1) : 0;
-  const auto* parents = tree ? p.parents.const_data_ptr<int32_t>() : nullptr;
   std::fill(slots, slots + p.num_tokens, -1);
   std::fill(positions, positions + p.num_tokens, 0);
   std::fill(mask, mask + p.num_tokens * words, 0);
@@ -93,8 +99,6 @@ void paged_plan(const PagedPlanTensors& p) {
       depth[i] = i;
       if (tree) {
         const int64_t up = parents[t];
-        TORCH_CHECK(up >= -1 && up < i, "paged_plan: parent ", up, " of node ", i, " of request ",
-                    s, " does not come before it");
         depth[i] = up < 0 ? 0 : depth[up] + 1;
         if (up >= 0) {
           std::copy(mask + (start[s] + up) * words, mask + (start[s] + up + 1) * words,

@@ -134,6 +134,36 @@ def test_paged_plan_rejects_bad_inputs():
             call(**change)
 
 
+def test_paged_plan_refusals_write_nothing():
+    """What a refused call was given is as it was: the tables and the free list, to which a finished
+    request's blocks would have come back and from which two more would have been taken."""
+    def lists():
+        return dict(context_lens=i32([4, 8, 4, 4], "cpu"), query_lens=i32([2, -1, 3, 4], "cpu"),
+                    block_tables=i32([[1, 0, 0, 0], [2, 3, 0, 0], [4, 0, 0, 0], [5, 0, 0, 0]],
+                                     "cpu"),
+                    blocks_owned=i32([1, 2, 1, 1], "cpu"),
+                    free_blocks=i32([6, 0, 0, 0], "cpu"), free_count=i32([0], "cpu"),
+                    num_tokens=9, block_size=4, parents=i32([-1, 0, -1, 0, 1, -1, 0, 1, 2], "cpu"),
+                    max_query_len=4)
+
+    served = lists()
+    assert svllm_ops.paged_plan(**served)[1].tolist() == [6, 0, 7, 0]
+    assert served["block_tables"][0, 1] == 3 and served["free_blocks"].tolist() == [2, 3, 0, 0]
+    for change in [
+        {"parents": i32([-1, 1, -1, 0, 1, -1, 0, 1, 2], "cpu")},   # of the first request
+        {"parents": i32([-1, 0, -1, 0, -2, -1, 0, 1, 2], "cpu")},  # of the last that is served
+        {"parents": i32([-1, 0, -1, 0, 1, -1, 0, 1, 7], "cpu")},   # of one that is not
+        {"max_query_len": 3}, {"context_lens": i32([4, 8, 14, 4], "cpu")},
+        {"blocks_owned": i32([1, 2, 1, 5], "cpu")}, {"free_count": i32([3], "cpu")},
+        {"num_tokens": 8, "parents": i32([-1, 0, -1, 0, 1, -1, 0, 1], "cpu")},
+    ]:
+        a = {**lists(), **change}
+        with pytest.raises(RuntimeError, match="paged_plan"):
+            svllm_ops.paged_plan(**a)
+        assert torch.equal(a["block_tables"], lists()["block_tables"]), change
+        assert torch.equal(a["free_blocks"], lists()["free_blocks"]), change
+
+
 @pytest.mark.gpu
 def test_paged_plan_bad_lengths_on_cuda(cuda):
     """What the CPU refuses raises the bad-index bit, and only the request it concerns goes
