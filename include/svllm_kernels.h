@@ -356,7 +356,8 @@ int svllm_lm_head_argmax_static_bf16(const void* hidden, int64_t num_rows, int64
  * Not served, with SVLLM_DEVERR_BAD_INDEX: a negative context, blocks_owned outside [0,
  * max_blocks], more rows than the table holds, tokens past num_tokens, more nodes than
  * max_query_len (which only counts with parents; at most SVLLM_MAX_TREE_NODES). The same bit tells
- * of a parent that does not come before its child (the node counts as a root), a free_count
+ * of a parent that does not come before its child (the node counts as a root; of requests that are
+ * not served too, up to the mask's width), a free_count
  * outside [0, free_capacity] (clamped), and blocks given back past free_capacity (dropped). No
  * array that is written overlaps another one.
  */

@@ -12,10 +12,13 @@
 // taking them. What bounds it is the chain of dependent loads and barriers, not bytes. Tokens are
 // independent of one another (a binary search over the starts, one table entry, a walk up the
 // parents); few of them follow in the same CTA, the starts and the parents staged in shared memory;
-// many get a second kernel over the whole GPU (kFusedTokens), which works out the starts and walks
-// up the trees while the first runs (1024 requests of 64 nodes: 10.9 us before, 6.9 with). Measured
-// in a graph: 4 requests of 8 nodes 3.2 us, 64 of 16 4.0, 1024 of 64 6.9 (2.1 MB read and written,
-// 0.3 us of HBM time: latency is all there is); a call from the host costs it some 6.5 us.
+// of many (kFusedTokens) the part that depends on the inputs alone, the walks with the masks and
+// positions, is done by more CTAs of the same launch, and a second kernel adds the slots. (It reads
+// only what the first wrote: inputs that it read itself before its dependency wait would come from
+// kernels of which nothing promises that their writes are visible to it.) Measured in a graph: 4
+// requests of 8 nodes 3.2 us, 64 of 16 3.9, 1024 of 64 that take 4 blocks each 7.1 (2.1 MB read and
+// written, 0.3 us of HBM time: latency is all there is); a call from the host costs it some 7.5 us,
+// 10 with two launches.
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -28,13 +31,13 @@ namespace {
 
 constexpr int kPlanThreads = 1024;  // at most; as many as there are requests, in whole warps
 constexpr int kTokenThreads = 256;
-constexpr int kStagedStarts = 4096;  // of requests, staged by the tokens' kernel
+constexpr int kStagedStarts = 4096;  // of requests, staged by the CTAs of the walks
 constexpr int kOwnBlocks = 8;        // new blocks up to which a request's own lane fetches them
 
 // Up to this many tokens, times the words of a mask, are done by the CTA that did the requests;
-// more get a grid of their own. us in a graph, one kernel against two: 32 tokens 3.2 and 3.6, 256
-// 3.8 and 3.7, 512 4.2 and 3.9 (a second launch costs the host some 2 us), 1024 5.4 and 4.0, 4096
-// 10.7 and 4.7.
+// more get CTAs and a second kernel. us in a graph, one kernel against two: 32 tokens 3.2 and 3.5,
+// 256 4.0 and 3.8, 512 4.2 and 3.8 (a second launch costs the host some 2 us), 1024 5.3 and 3.8,
+// 4096 10.2 and 4.3.
 constexpr int64_t kFusedTokens = 512;
 
 struct PlanArgs {
@@ -60,7 +63,8 @@ struct PlanArgs {
   int32_t block_size;
   int32_t max_query_len;         // checked where parents are given: the mask's width
   int32_t mask_words;
-  int fused;                     // this CTA does the tokens too
+  int fused;                     // CTA 0 does the tokens too
+  int walks;                     // the CTAs from 1 on do the tokens' walks
   int* err;
 };
 
@@ -119,88 +123,93 @@ __device__ int request_of(const PlanArgs& a, int t, const int32_t* starts) {
   return lo;
 }
 
-// The way from a node up its tree, for masks of one word.
-struct Walk {
-  uint64_t bits = 0;
-  int depth = -1;
-  bool bad = false;  // not a tree: the node that hangs on a later one counts as a root
+// A token's request and its row there; s < 0: none, or none that its table has room for.
+struct TokenRow {
+  int s = -1, row = 0;
 };
 
-__device__ Walk walk_up(const int32_t* parents, int node) {
-  Walk w;
-  for (int p = node; p >= 0;) {
-    w.bits |= uint64_t{1} << p;
-    ++w.depth;
-    int up = parents[p];
-    if (up >= p || up < -1) {
-      w.bad = true;
-      up = -1;
+__device__ TokenRow row_of(const PlanArgs& a, int t, int s, int start) {
+  TokenRow r;
+  if (s < a.num_seqs) {
+    const int64_t row = static_cast<int64_t>(a.context_lens[s]) + (t - start);
+    if (row >= 0 && row < a.max_rows) {
+      r.s = s;
+      r.row = static_cast<int>(row);
     }
-    p = up;
   }
-  return w;
+  return r;
 }
 
-// A token of request `s`, which starts at token `start`: slot, position and mask. `parents` (of
-// the request's first node) may be a staged copy; `w` counts for masks of one word. Reads what the
-// requests' part wrote, so plain loads (not the read-only path).
-__device__ void plan_token(const PlanArgs& a, int t, int s, int start, const int32_t* parents,
-                           const Walk& w) {
-  const bool live = s < a.num_seqs && a.seq_lens[s] > 0;
-  int64_t slot = -1, position = 0;
-  int64_t* mask =
-      a.tree_mask == nullptr ? nullptr : a.tree_mask + static_cast<int64_t>(t) * a.mask_words;
-  int word = a.mask_words;  // mask words from here on are written
-  if (live) {
-    const int i = t - start;
-    const int context = a.context_lens[s];
-    const int row = context + i;  // at most max_blocks * block_size, which fits
-    const int page = row / a.block_size;
-    slot = static_cast<int64_t>(a.block_tables[static_cast<int64_t>(s) * a.max_blocks + page]) *
-               a.block_size + (row - page * a.block_size);
-    int depth = i;
-    if (a.mask_words == 1) {
-      mask[--word] = static_cast<int64_t>(w.bits);
-      depth = w.depth;
-      if (w.bad) raise_error(a.err, kErrBadIndex);
-    } else if (mask != nullptr) {
-      // up the tree: parents come before their children, so the words are met in falling order
-      depth = -1;
-      uint64_t bits = 0;
-      int p = i;
-      while (p >= 0) {
-        for (; word - 1 > p / 64; --word) {
-          mask[word - 1] = static_cast<int64_t>(bits);
+// Position and mask of token `t`, node `i` of a request, as if the request were served. `parents`
+// (of its first node; null: a chain) may be a staged copy.
+__device__ void write_tree(const PlanArgs& a, int t, int i, int row, const int32_t* parents) {
+  int depth = i;
+  if (parents != nullptr) {
+    if (i >= 64 * a.mask_words) return;  // a request wider than the mask: not served
+    const int own = parents[i];
+    int64_t* mask = a.tree_mask + static_cast<int64_t>(t) * a.mask_words;
+    uint64_t bits = 0;
+    depth = -1;
+    if (a.mask_words == 1) {  // 1024 requests of 64 nodes: 7.1 us, 7.6 by the loop below
+      for (int p = i; p >= 0;) {
+        bits |= uint64_t{1} << p;
+        ++depth;
+        const int up = parents[p];
+        p = up >= p ? -1 : up;  // not a tree: the node counts as a root
+      }
+      *mask = static_cast<int64_t>(bits);
+    } else {
+      // parents come before their children, so the words are met in falling order
+      int word = a.mask_words - 1;
+      for (int p = i; p >= 0;) {
+        for (; word > p >> 6; --word) {
+          mask[word] = static_cast<int64_t>(bits);
           bits = 0;
         }
-        bits |= uint64_t{1} << (p % 64);
+        bits |= uint64_t{1} << (p & 63);
         ++depth;
-        int up = parents[p];
-        if (up >= p || up < -1) {  // not a tree: the node counts as a root
-          raise_error(a.err, kErrBadIndex);
-          up = -1;
-        }
-        p = up;
+        const int up = parents[p];
+        p = up >= p ? -1 : up;
       }
-      mask[--word] = static_cast<int64_t>(bits);
+      for (; word >= 0; --word) {
+        mask[word] = static_cast<int64_t>(bits);
+        bits = 0;
+      }
     }
-    position = static_cast<int64_t>(context) + depth;
+    if (own >= i || own < -1) raise_error(a.err, kErrBadIndex);
   }
-  if (mask != nullptr) {
-    while (word > 0) mask[--word] = 0;
-  }
-  a.slot_mapping[t] = slot;
-  a.positions[t] = position;
+  a.positions[t] = static_cast<int64_t>(row) - i + depth;
 }
 
-// The walk of a token whose request may not be served yet: a node past the mask has none.
-__device__ Walk walk_of(const PlanArgs& a, int node, const int32_t* parents) {
-  return a.mask_words == 1 && node < 64 ? walk_up(parents, node) : Walk{};
+// A token's slot: what the requests' part wrote, read with plain loads.
+struct TokenSlot {
+  int64_t slot = 0;
+  bool live = false;  // its request is served
+};
+
+__device__ TokenSlot find_slot(const PlanArgs& a, const TokenRow& r) {
+  TokenSlot x;
+  if (r.s >= 0) {
+    const int page = r.row / a.block_size;
+    const int block = a.block_tables[static_cast<int64_t>(r.s) * a.max_blocks + page];
+    x.live = a.seq_lens[r.s] > 0;
+    x.slot = static_cast<int64_t>(block) * a.block_size + (r.row - page * a.block_size);
+  }
+  return x;
+}
+
+__device__ void write_slot(const PlanArgs& a, int t, const TokenSlot& x) {
+  a.slot_mapping[t] = x.live ? x.slot : -1;
+  if (x.live) return;
+  a.positions[t] = 0;
+  for (int w = 0; w < a.mask_words; ++w) {
+    a.tree_mask[static_cast<int64_t>(t) * a.mask_words + w] = 0;
+  }
 }
 
 // Copies `count` block ids per lane, src[step * k] -> dst[k]: a lane's own when there are up to
 // kOwnBlocks, else the warp together, four lanes' at a time. us in a graph, a lane's own against
-// together: 64 requests of 1 block 5.3 and 6.8, 1024 of 4 9.1 and 11.7, 1024 of 16 19.7 and 11.8.
+// together: 64 requests of 1 block 3.4 and 4.8, 1024 of 4 5.8 and 9.3, 1024 of 16 16.4 and 9.5.
 __device__ __forceinline__ void copy_blocks(int count, const int32_t* src, int step,
                                             int32_t* dst) {
   const int most = __reduce_max_sync(0xffffffffu, count);
@@ -246,13 +255,53 @@ __device__ __forceinline__ void copy_blocks(int count, const int32_t* src, int s
   }
 }
 
+// The walks of blockDim tokens, by one of the CTAs beside the requests': position and mask, and in
+// slot_mapping, for the kernel that follows, the token's request and row. The starts it needs are
+// summed up once more.
+__device__ void walk_tokens(const PlanArgs& a, int32_t* starts, uint2* warp_sums) {
+  const int n_seqs = static_cast<int>(a.num_seqs), tid = threadIdx.x, threads = blockDim.x;
+  uint32_t* ends = reinterpret_cast<uint32_t*>(starts + n_seqs + 1);  // of the threads' requests
+  const int each = (n_seqs + threads - 1) / threads;
+  const int first = min(n_seqs, tid * each), last = min(n_seqs, first + each);
+  uint32_t sum = 0;
+  for (int s = first; s < last; ++s) {
+    sum = add_up(sum, static_cast<uint32_t>(max(a.query_lens[s], 0)));
+    starts[s + 1] = static_cast<int32_t>(sum);
+  }
+  uint2 total;
+  ends[tid] = block_scan(make_uint2(sum, 0), warp_sums, total).x;
+  __syncthreads();
+  const uint32_t limit = static_cast<uint32_t>(a.num_tokens);
+  const uint32_t before = tid == 0 ? 0 : ends[tid - 1];
+  for (int s = first; s < last; ++s) {
+    starts[s + 1] = static_cast<int32_t>(
+        min(add_up(before, static_cast<uint32_t>(starts[s + 1])), limit));
+  }
+  if (tid == 0) starts[0] = 0;
+  __syncthreads();
+  const int64_t at = static_cast<int64_t>(blockIdx.x - 1) * threads + tid;
+  if (at >= a.num_tokens) return;
+  const int t = static_cast<int>(at);
+  const int s = request_of(a, t, starts), start = s < n_seqs ? starts[s] : 0;
+  const TokenRow r = row_of(a, t, s, start);
+  a.slot_mapping[t] = static_cast<int64_t>(r.s) * (int64_t{1} << 32) + r.row;
+  if (s < n_seqs) {
+    write_tree(a, t, t - start, r.row, a.parents == nullptr ? nullptr : a.parents + start);
+  }
+}
+
 __global__ void __launch_bounds__(kPlanThreads) plan_requests_kernel(const PlanArgs a) {
   grid_dependency_sync();
-  extern __shared__ int32_t staged[];  // starts, then parents, for the tokens (fused)
+  // starts; then parents, for the tokens (fused), or the threads' sums (the CTAs of the walks)
+  extern __shared__ int32_t staged[];
   __shared__ uint2 warp_sums[kPlanThreads / kWarpSize];
   __shared__ int used;
   const int tid = threadIdx.x;
   const int threads = blockDim.x, n_seqs = static_cast<int>(a.num_seqs);
+  if (blockIdx.x > 0) {
+    walk_tokens(a, staged, warp_sums);
+    return;
+  }
   if (tid == 0) used = 0;
   if (a.fused && a.tree_mask != nullptr) {
     for (int t = tid; t < a.num_tokens; t += threads) staged[n_seqs + 1 + t] = a.parents[t];
@@ -352,63 +401,39 @@ __global__ void __launch_bounds__(kPlanThreads) plan_requests_kernel(const PlanA
   if (tid == 0) a.free_count_out[0] = static_cast<int32_t>(have - used);
   if (a.fused) {
     for (int t = tid; t < a.num_tokens; t += threads) {
-      const int s = request_of(a, t, staged), start = staged[s];
-      const int32_t* parents = staged + n_seqs + 1 + start;
-      const bool in = s < n_seqs;
-      plan_token(a, t, s, start, parents, in ? walk_of(a, t - start, parents) : Walk{});
+      const int s = request_of(a, t, staged), start = s < n_seqs ? staged[s] : 0;
+      const TokenRow r = row_of(a, t, s, start);
+      const TokenSlot x = find_slot(a, r);
+      if (s < n_seqs) {
+        write_tree(a, t, t - start, r.row,
+                   a.parents == nullptr ? nullptr : staged + n_seqs + 1 + start);
+      }
+      write_slot(a, t, x);
     }
   }
 }
 
-// The tokens, after plan_requests_kernel, which lets this kernel start as soon as what came before
-// it has completed: the starts (worked out once more from the query lengths) and the walks need
-// nothing that it writes, so they are done while it runs.
+// The tokens' slots, after plan_requests_kernel; the walks too where that had too many starts to
+// stage.
 __global__ void __launch_bounds__(kTokenThreads) plan_tokens_kernel(const PlanArgs a) {
-  __shared__ int32_t staged[kStagedStarts + 1];
-  __shared__ uint2 warp_sums[kTokenThreads / kWarpSize];
-  __shared__ uint32_t ends[kTokenThreads];
-  const int n_seqs = static_cast<int>(a.num_seqs), tid = threadIdx.x;
-  const int32_t* starts = a.query_start_loc;
-  const bool early = n_seqs <= kStagedStarts;
-  if (early) {
-    const int each = (n_seqs + kTokenThreads - 1) / kTokenThreads;
-    const int first = min(n_seqs, tid * each), last = min(n_seqs, first + each);
-    uint32_t sum = 0;
-    for (int s = first; s < last; ++s) {
-      sum = add_up(sum, static_cast<uint32_t>(max(__ldcg(a.query_lens + s), 0)));
-      staged[s + 1] = static_cast<int32_t>(sum);
-    }
-    uint2 total;
-    ends[tid] = block_scan(make_uint2(sum, 0), warp_sums, total).x;
-    __syncthreads();
-    const uint32_t limit = static_cast<uint32_t>(a.num_tokens);
-    const uint32_t before = tid == 0 ? 0 : ends[tid - 1];
-    for (int s = first; s < last; ++s) {
-      staged[s + 1] = static_cast<int32_t>(
-          min(add_up(before, static_cast<uint32_t>(staged[s + 1])), limit));
-    }
-    if (tid == 0) staged[0] = 0;
-    __syncthreads();
-    starts = staged;
+  grid_dependency_sync();
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * kTokenThreads + threadIdx.x;
+  if (at >= a.num_tokens) return;
+  const int t = static_cast<int>(at);
+  TokenRow r;
+  if (a.walks) {
+    const int64_t left = a.slot_mapping[t];
+    r.s = static_cast<int>(left >> 32);
+    r.row = static_cast<int>(left & 0xffffffff);
   } else {
-    grid_dependency_sync();
-  }
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * kTokenThreads + tid;
-  const bool in_range = t < a.num_tokens;
-  int s = n_seqs, start = 0;
-  Walk w;
-  if (in_range) {
-    s = request_of(a, static_cast<int>(t), starts);
-    if (s < n_seqs) {
-      start = starts[s];
-      if (a.mask_words == 1) w = walk_of(a, static_cast<int>(t) - start, a.parents + start);
+    const int s = request_of(a, t, a.query_start_loc);
+    if (s < a.num_seqs) {
+      const int start = a.query_start_loc[s];
+      r = row_of(a, t, s, start);
+      write_tree(a, t, t - start, r.row, a.parents == nullptr ? nullptr : a.parents + start);
     }
   }
-  if (early) grid_dependency_sync();
-  if (in_range) {
-    plan_token(a, static_cast<int>(t), s, start,
-               a.parents == nullptr ? nullptr : a.parents + start, w);
-  }
+  write_slot(a, t, find_slot(a, r));
 }
 
 }  // namespace
@@ -471,17 +496,21 @@ extern "C" int svllm_paged_plan(
   a.mask_words = parents != nullptr ? static_cast<int32_t>((max_query_len + 63) / 64) : 0;
   a.fused = num_tokens * (a.mask_words > 1 ? a.mask_words : 1) <= kFusedTokens &&
             num_seqs <= kPlanThreads;
+  a.walks = !a.fused && num_seqs <= kStagedStarts;
   a.err = err;
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   // a thread per request, and per token where those are done here too (512 tokens by 256 threads
   // took 4.7 us instead of 3.9)
   int64_t threads = a.fused && num_tokens > num_seqs ? num_tokens : num_seqs;
-  if (threads < 1) threads = 1;
+  if (threads < (a.walks ? kTokenThreads : 1)) threads = a.walks ? kTokenThreads : 1;
   threads = threads > kPlanThreads ? kPlanThreads : round_up(threads, kWarpSize);
-  const size_t staged =
-      a.fused ? 4 * static_cast<size_t>(num_seqs + 1 + (parents != nullptr ? num_tokens : 0)) : 0;
-  const int status = launch(plan_requests_kernel, dim3(1), dim3(static_cast<unsigned>(threads)),
-                            staged, st, 1u, a);
+  const int64_t beside = a.walks ? (num_tokens + threads - 1) / threads : 0;
+  int64_t staged = 0;  // ints
+  if (a.fused) staged = num_seqs + 1 + (parents != nullptr ? num_tokens : 0);
+  if (a.walks) staged = num_seqs + 1 + threads;
+  const int status = launch(plan_requests_kernel, dim3(static_cast<unsigned>(1 + beside)),
+                            dim3(static_cast<unsigned>(threads)), static_cast<size_t>(staged) * 4,
+                            st, 1u, a);
   if (status != SVLLM_OK || a.fused || num_tokens == 0) return status;
   return launch(plan_tokens_kernel,
                 dim3(static_cast<unsigned>((num_tokens + kTokenThreads - 1) / kTokenThreads)),

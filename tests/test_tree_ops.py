@@ -218,6 +218,63 @@ def test_paged_plan_bad_lengths_of_many_tokens_on_cuda(cuda):
     assert positions[30:36].tolist() == [4, 5, 4, 4, 5, 6]
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("requests", [40, 300, 4200])
+def test_paged_plan_behind_the_kernel_that_makes_its_lengths(cuda, requests):
+    """The lists of a plan come from the kernels right before it, and the tables it fills lie in one
+    buffer with the parents it reads, in the same 32 bytes where they meet: captured, and replayed
+    with other lists."""
+    nodes, bs = 40, 4
+    width = (64 + nodes) // bs + 1
+    g = torch.Generator().manual_seed(requests)
+    starts = i32([nodes * s for s in range(requests + 1)], cuda)
+    ones = i32([1] * requests, cuda)
+    targets = torch.ones(requests * nodes, dtype=torch.int64, device=cuda)
+    tokens = requests * nodes
+    buffer = torch.zeros(requests * width + tokens, dtype=torch.int32, device=cuda)
+    tables = buffer[: requests * width].view(requests, width)
+    parents = buffer[requests * width:]
+    new_parents = torch.zeros_like(parents)
+    ids, context = torch.zeros_like(targets), i32([0] * requests, cuda)
+    owned = i32([0] * requests, cuda)
+    stack = torch.arange(requests * width, dtype=torch.int32, device=cuda)
+    count = i32([requests * width], cuda)
+
+    def step():
+        tables.zero_()
+        parents.copy_(new_parents)
+        # chains of which every request accepts as many as its ids say
+        _, _, query, after = svllm_ops.tree_accept(ids, targets, None, starts, ones, context,
+                                                   nodes)
+        return (query, after) + svllm_ops.paged_plan(after, query, tables, owned, stack, count,
+                                                     tokens, bs, parents, nodes)
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(4):
+        length = torch.randint(1, nodes + 1, (requests,), generator=g)
+        before = torch.randint(0, 24, (requests,), generator=g)
+        packed = random_parents(requests, length.tolist())
+        ids.copy_((torch.arange(nodes) < length[:, None]).long().flatten())
+        context.copy_(before)
+        new_parents.copy_(i32(packed + [-1] * (tokens - len(packed)), "cpu"))
+        graph.replay()
+        case = {"context_lens": (before + length).tolist(), "query_lens": length.tolist(),
+                "block_tables": [[0] * width] * requests, "blocks_owned": [0] * requests,
+                "free_blocks": list(range(requests * width)), "free_count": requests * width,
+                "num_tokens": tokens, "block_size": bs,
+                "parents": packed + [-1] * (tokens - len(packed)), "max_query_len": nodes}
+        want, want_tables, _ = plan_reference(case)
+        assert out[0].tolist() == case["query_lens"] and out[1].tolist() == case["context_lens"]
+        for name, got in zip(("query_start_loc", "seq_lens", "slot_mapping", "positions",
+                              "tree_mask", "blocks_owned", "free_count"), out[2:]):
+            assert torch.equal(got.cpu(), want[name]), name
+        assert torch.equal(tables.cpu(), want_tables)
+        assert parents.tolist() == case["parents"]
+
+
 # ------------------------------------------------------------------------------ tree_accept
 
 @pytest.mark.parametrize("counts", [[1], [8], [0, 3, 0, 17], [64, 65, 33, 1], [200, 31, 0, 128],
