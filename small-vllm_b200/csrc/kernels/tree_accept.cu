@@ -115,12 +115,10 @@ struct CommitArgs {
   int64_t num_tokens;
   int64_t row_vecs;                // 16-byte vectors per row
   int max_query_len;
-  int planes;
-  int planes_per_cta;
   int* err;
 };
 
-// One CTA: one request, some planes (K or V of a layer). A thread moves the same 16-byte column
+// One CTA: one request, one plane (K or V of a layer). A thread moves the same 16-byte column
 // of every row in order, eight rows loaded before they are stored. That order is enough: row i
 // is written after every source path[j], j <= i, has been read, and no later source is row i,
 // since path[j] >= j > i.
@@ -165,24 +163,20 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const Commi
   }
   __syncthreads();
   count = sh_limit;
-  const int first = blockIdx.y * a.planes_per_cta;
-  const int last = min(a.planes, first + a.planes_per_cta);
-  for (int p = first; p < last; ++p) {
-    uint4* rows = static_cast<uint4*>(a.plane[p]);
-    for (int64_t v = tid; v < a.row_vecs; v += kCommitThreads) {
-      for (int base = 1; base < count; base += kCommitBatch) {
-        uint4 held[kCommitBatch];
+  uint4* rows = static_cast<uint4*>(a.plane[blockIdx.y]);
+  for (int64_t v = tid; v < a.row_vecs; v += kCommitThreads) {
+    for (int base = 1; base < count; base += kCommitBatch) {
+      uint4 held[kCommitBatch];
 #pragma unroll
-        for (int e = 0; e < kCommitBatch; ++e) {
-          if (base + e < count && sh_src[base + e] >= 0) {
-            held[e] = rows[sh_src[base + e] * a.row_vecs + v];
-          }
+      for (int e = 0; e < kCommitBatch; ++e) {
+        if (base + e < count && sh_src[base + e] >= 0) {
+          held[e] = rows[sh_src[base + e] * a.row_vecs + v];
         }
+      }
 #pragma unroll
-        for (int e = 0; e < kCommitBatch; ++e) {
-          if (base + e < count && sh_src[base + e] >= 0) {
-            rows[sh_dst[base + e] * a.row_vecs + v] = held[e];
-          }
+      for (int e = 0; e < kCommitBatch; ++e) {
+        if (base + e < count && sh_src[base + e] >= 0) {
+          rows[sh_dst[base + e] * a.row_vecs + v] = held[e];
         }
       }
     }
@@ -305,16 +299,14 @@ extern "C" int svllm_tree_commit(void* const* k_caches, void* const* v_caches, i
   a.num_tokens = num_tokens;
   a.row_vecs = row_bytes / 16;
   a.max_query_len = static_cast<int>(max_query_len);
-  a.planes_per_cta = 1;
   a.err = err;
   for (int64_t l = 0; l < num_layers; l += kCommitPlanes / 2) {
-    a.planes = 0;
+    unsigned planes = 0;
     for (int64_t m = l; m < num_layers && m < l + kCommitPlanes / 2; ++m) {
-      a.plane[a.planes++] = k_caches[m];
-      a.plane[a.planes++] = v_caches[m];
+      a.plane[planes++] = k_caches[m];
+      a.plane[planes++] = v_caches[m];
     }
-    const dim3 grid(static_cast<unsigned>(num_seqs),
-                    static_cast<unsigned>((a.planes + a.planes_per_cta - 1) / a.planes_per_cta));
+    const dim3 grid(static_cast<unsigned>(num_seqs), planes);
     const int status = launch(tree_commit_kernel, grid, dim3(kCommitThreads),
                               static_cast<size_t>(max_query_len) * 16,
                               reinterpret_cast<cudaStream_t>(stream), 1u, a);
