@@ -313,3 +313,61 @@ def test_starts_that_contradict_themselves_leave_nothing_unwritten(cuda, starts,
         torch.cuda.synchronize()
         assert svllm_ops.read_device_error(0, True) == 1
         assert (out == 0).all()
+
+
+@pytest.mark.parametrize("counts, context, heads, kv_heads, dim, bs, shape", [
+    ([8, 60], [120, 500], 16, 8, 128, 8, "tree"),      # boxes of 8 rows: two loaders
+    ([37, 9, 1], [777, 130, 2], 20, 4, 128, 24, "tree"),
+    ([130, 6], [300, 900], 4, 2, 64, 40, "tree"),
+    ([8, 60], [120, 500], 16, 8, 128, 4, "tree"),      # of 4: four
+    ([5] * 9, [100 * s for s in range(9)], 32, 8, 64, 20, "chain"),
+    ([37, 9, 1], [777, 130, 2], 20, 4, 128, 1, "tree"),  # gathered rows, over several tiles
+    ([130, 6], [300, 900], 8, 1, 128, 3, "tree"),
+    ([200], [0], 4, 2, 128, 6, "chain"),
+], ids=str)
+def test_page_sizes_on_both_sides_of_each_way_to_load(cuda, counts, context, heads, kv_heads, dim,
+                                                      bs, shape):
+    check(build(cuda, counts, context, heads, kv_heads, dim, bs, shape=shape, seed=bs))
+
+
+@pytest.mark.parametrize("bs", [1, 3, 4, 8, 12, 16])
+@pytest.mark.parametrize("node", [0, 3, 30, 69, 101])  # rows that different helper warps check
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")], ids=str)
+def test_masked_values_do_not_leak_from_pages_of_any_size(cuda, bs, node, bad):
+    """As above, for each way to load pages and both numbers of helper warps: a V that is not
+    finite in one column reaches that column of the nodes that see it and nothing else."""
+    s = build(cuda, [7, 110], [20, 300], 16, 8, 128, bs, seed=node)
+    clean = run(s)
+    row, table = 300 + node, s["tables"][1].tolist()
+    sees = ((s["mask"][7:, node // 64] >> (node % 64)) & 1).bool()
+    assert sees.any() and (node == 0 or not sees.all())
+    s["v"] = s["v"].clone()
+    s["v"][table[row // bs], row % bs, :, 70] = bad
+    if 410 % bs:  # the rest of the last page
+        s["v"][table[410 // bs], 410 % bs:] = bad
+    out = run(s)
+    seeing = torch.zeros(117, dtype=torch.bool, device=cuda)
+    seeing[7:] = sees
+    assert torch.equal(out[~seeing], clean[~seeing])
+    other = [d for d in range(128) if d != 70]
+    assert torch.equal(out[seeing][..., other], clean[seeing][..., other])
+    got = out[seeing][..., 70]
+    assert (got.isnan() if bad != bad else got == bad).all()
+
+
+@pytest.mark.parametrize("counts, context, heads, kv_heads, dim, bs", [
+    ([8], [120], 16, 8, 128, 16),
+    ([40] * 64, [200] * 64, 16, 8, 128, 16),
+    ([31, 1, 0, 64, 17], [500, 3, 70, 0, 102], 28, 4, 128, 12),
+    ([200, 7], [90, 300], 5, 1, 64, 1),
+], ids=str)
+def test_tables_wider_than_any_request(cuda, counts, context, heads, kv_heads, dim, bs):
+    """A table of a fixed width, as a captured step has: what stands behind a request's pages is not
+    read, and the items of short requests may be cut, which those over a fitted table are not."""
+    s = build(cuda, counts, context, heads, kv_heads, dim, bs, seed=7)
+    wide = torch.full((len(counts), 4096 // bs), 2 ** 31 - 1, dtype=torch.int32, device=cuda)
+    for i, (n, c) in enumerate(zip(counts, context)):
+        pages = -(-(n + c) // bs)
+        wide[i, :pages] = s["tables"][i, :pages]
+    out = run(dict(s, tables=wide))
+    check(s, out)

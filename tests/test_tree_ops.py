@@ -93,6 +93,33 @@ def test_paged_plan(device, requests, nodes, context, bs, tree, short, finish, p
         assert (want["seq_lens"] == 0).any()  # the case means what it says
 
 
+@pytest.mark.parametrize("requests, nodes, tree, finish", [
+    (7, 130, True, 3), (40, 9, False, 4), (300, 64, True, 5), (1030, 3, True, 7),
+    (4200, 2, True, 2),
+], ids=str)
+def test_paged_plan_again_on_its_own_lists(device, requests, nodes, tree, finish):
+    """A second call with the same lengths and counts, on the tables and the free list that the first
+    has written, gives and writes the same: blocks that came back are where they were put, and those
+    taken are taken again."""
+    case = make_plan_case(requests + nodes, requests, nodes, 60, 8, tree=tree, short=True,
+                          finish=finish, pad=3)
+    want, want_tables, want_stack = plan_reference(case)
+    lists = [i32(case[k], device) for k in ("context_lens", "query_lens", "block_tables",
+                                            "blocks_owned", "free_blocks")]
+    count = i32([case["free_count"]], device)
+    parents = i32(case["parents"], device) if tree else None
+    for _ in range(3):
+        out = svllm_ops.paged_plan(*lists, count, case["num_tokens"], case["block_size"], parents,
+                                   case["max_query_len"])
+        for name, got in zip(("query_start_loc", "seq_lens", "slot_mapping", "positions",
+                              "tree_mask", "blocks_owned", "free_count"), out):
+            assert got is None if name == "tree_mask" and not tree else torch.equal(
+                got.cpu(), want[name]), name
+        assert torch.equal(lists[2].cpu(), want_tables)
+        assert torch.equal(lists[4].cpu(), want_stack)
+    assert (want["seq_lens"] == 0).any() and want_stack.tolist() != case["free_blocks"]
+
+
 def test_paged_plan_without_requests(device):
     e = i32([], device)
     out = svllm_ops.paged_plan(e, e, torch.zeros(0, 3, dtype=torch.int32, device=device), e,
