@@ -9,8 +9,9 @@
 //
 // tree_commit: the step wrote node i of a request to the slot of row context + i; row context +
 // j of the sequence, j < accepted, must be node path[j]. Paths rise (a parent comes before its
-// child), so path[j] >= j. A copy: 128 requests of 12 to 24 nodes in 28 layers, 143 MB, 20.7 us in
-// a graph (6.9 TB/s, part of it from L2); one request of 16 nodes 3.8 us.
+// child), so path[j] >= j. A copy: 128 requests of 12 to 24 nodes in 28 layers, 143 MB, 23.8 us in
+// calls on caches in turn (6.0 TB/s, 0.91 of the copy rate); 20.7 us over and over in a graph, less
+// than HBM would take, part of it from L2; one request of 16 nodes 3.8 us in a graph.
 #include <cuda_runtime.h>
 
 #include <cstdint>
