@@ -32,11 +32,11 @@
 //
 // Measured in a graph, inputs past L2, head_dim 128: 64 requests of 48 to 64 nodes over 2048 to
 // 4096 rows, 16 heads on 8 KV heads, 203 us (1.08 GB, 5.3 TB/s: 0.82 of the copy rate; 219 to 237
-// under a load that runs into the power limit). The main kernel takes 185 of them, in steady state at the
-// copy rate, a tenth of it start and ends of segments; the join takes the rest. 8 requests of 100
-// to 128 nodes over 1024 to 4096, 32 heads on 4 KV heads, 86 us (0.75 PFLOP/s), main kernel 73: a
-// KV head's rows go to four items, 5.6 TB/s through L2, and a step takes 3500 cycles where its
-// products take 2048: per accumulator those and the softmax (1580 cycles, 1260 of them the
+// under a load that runs into the power limit). The main kernel takes 185 of them, in steady state
+// at the copy rate, a tenth of it start and ends of segments; the join takes the rest. 8 requests
+// of 100 to 128 nodes over 1024 to 4096, 32 heads on 4 KV heads, 86 us (0.75 PFLOP/s), main kernel
+// 73: a KV head's rows go to four items, 5.6 TB/s through L2, and a step takes 3500 cycles where
+// its products take 2048: per accumulator those and the softmax (1580 cycles, 1260 of them the
 // exponentials) wait for each other. Parts of 64 cached rows with their scores a part ahead took
 // 119: products of N = 64 take as long as those of 128. 32 nodes over 32768 rows 41 us, 20 of them
 // the stream, 10 the join of some 37 segments per item. 8 nodes over 128 rows 8.2 us: one tile's
@@ -1309,8 +1309,8 @@ int64_t workspace_bytes(int ctas) {
 // 40 34.4 and 24.8; 416, 1 of 8 12.3 and 15.4, 4 of 8 13.4 and 15.5, 16 of 8 19.1 and 16.2; 448, 64
 // of 40 42.6 and 36.1; 912, 64 of 8 45.3 and 53.2. The host knows the tables' width, not the
 // lengths: short requests over wide tables (of a captured step, say) are cut and joined. 1 request
-// of 8 nodes over 128 rows takes 8.2 us with a table of 128 rows and 10.2 with one of 4096, 64 of 40
-// over 240 rows 23.9 and 34.1, 8 of 16 over 416 14.6 with both.
+// of 8 nodes over 128 rows takes 8.2 us with a table of 128 rows and 10.2 with one of 4096, 64 of
+// 40 over 240 rows 23.9 and 34.1, 8 of 16 over 416 14.6 with both.
 inline bool whole_items(const TreeAttnArgs& a, int ctas) {
   const int64_t steps = (a.max_length + kTile - 1) / kTile;
   if (steps <= 2) return true;

@@ -246,6 +246,35 @@ def test_paged_plan_bad_lengths_of_many_tokens_on_cuda(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("more", [0, 300, 5000], ids=["one launch", "two", "two, many starts"])
+@pytest.mark.parametrize("fault", ["parent", "width"])
+def test_paged_plan_requests_that_are_not_served_on_cuda(cuda, more, fault):
+    """A parent of a request that finds no blocks is checked like any other, and one whose tree has
+    more nodes than the words of the mask has none of them written: both go without a slot, a
+    position and a mask, and nobody else does."""
+    nodes = [3, 70 if fault == "width" else 3, 3] + [3] * more
+    case = {"context_lens": [4] * len(nodes), "query_lens": nodes,
+            "block_tables": [[5] + [0] * 19] * len(nodes),
+            "blocks_owned": [2] + [1 if fault == "parent" else 20] + [2] * (1 + more),
+            "free_blocks": [9], "free_count": 0, "num_tokens": sum(nodes), "block_size": 4,
+            "parents": [-1, 0, 1] + ([-1, 2, 0] if fault == "parent" else [-1] + [0] * 69) +
+            [-1, 0, 0] * (1 + more), "max_query_len": 40}
+    svllm_ops.read_device_error(0, True)
+    out, tables, _ = run_plan(cuda, case)
+    assert svllm_ops.read_device_error(0, True) == 1
+    first, end = 3, 3 + nodes[1]
+    assert out[1].tolist() == [7, 0] + [7] * (1 + more)
+    assert out[2][first:end].tolist() == [-1] * nodes[1]
+    assert out[3][first:end].tolist() == [0] * nodes[1]
+    assert out[4][first:end].flatten().tolist() == [0] * nodes[1]
+    assert out[2][:3].tolist() == [0, 1, 2] and out[4][:3].flatten().tolist() == [1, 3, 7]
+    assert out[2][end:].tolist() == [0, 1, 2] * (1 + more)
+    assert out[3][end:].tolist() == [4, 5, 5] * (1 + more)
+    assert out[4][end:].flatten().tolist() == [1, 3, 5] * (1 + more)
+    assert torch.equal(tables.cpu(), torch.tensor(case["block_tables"], dtype=torch.int32))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("requests", [40, 300, 4200])
 def test_paged_plan_behind_the_kernel_that_makes_its_lengths(cuda, requests):
     """The lists of a plan come from the kernels right before it, and the tables it fills lie in one
