@@ -439,6 +439,81 @@ int svllm_tree_commit(void* const* k_caches, void* const* v_caches, int64_t num_
                       int64_t max_query_len, svllm_stream stream);
 
 /*
+ * svllm_tree_commit for the scales of an 8-bit cache (below): k_scales, v_scales HOST arrays of
+ * num_layers device pointers, each [num_slots, num_kv_heads] bytes, at any alignment.
+ */
+int svllm_tree_commit_scales(void* const* k_scales, void* const* v_scales, int64_t num_layers,
+                             int64_t num_slots, int64_t num_kv_heads, const int32_t* path,
+                             const int32_t* num_accepted, const int64_t* slot_mapping,
+                             const int32_t* query_start_loc, int64_t num_seqs, int64_t num_tokens,
+                             int64_t max_query_len, svllm_stream stream);
+
+/*
+ * The 8-bit paged KV cache. A row x of head_dim values (one slot, one KV head; K or V) is held as
+ * e4m3 codes, k_cache / v_cache [num_slots, num_kv_heads, head_dim] bytes, and one power-of-two
+ * scale, k_scale / v_scale [num_slots, num_kv_heads] bytes in e8m0 (e + 127): e is the least
+ * integer with max |x_i| <= 448 * 2^e, clamped to [-60, 60], code i is e4m3(x_i * 2^-e), rounded to
+ * nearest even and saturated. A value that is not finite becomes the NaN code and does not count
+ * for the maximum. A code times its scale is a bf16 value. head_dim 64 or 128 and 16-byte aligned
+ * caches, else SVLLM_ERR_UNSUPPORTED. New ops: the reference's paged cache is planned in the
+ * activations' type (docs/ROADMAP.md:24-25).
+ */
+
+/*
+ * The rotary step (svllm_qk_norm_rope_cache_bf16, svllm_rope_cache_bf16) with the 8-bit cache's
+ * write in the same pass. q is rotated in place, k and v are read only; for a token with slot s >=
+ * 0 its rotated k and its v are quantised into slot s. The norm and the rotation are fp32 and every
+ * result is rounded once, where it is stored; the angle position * inv_freq[i] is not rounded to
+ * fp32 before it is reduced. Negative slots and slots past the cache as in
+ * svllm_qk_norm_rope_cache_bf16. No slot may be given twice.
+ */
+int svllm_qk_norm_rope_cache_fp8_bf16(void* q, const void* k, const void* v, const void* q_weight,
+                                      const void* k_weight, const void* positions, int pos_type,
+                                      const int64_t* slot_mapping, void* k_cache, void* v_cache,
+                                      void* k_scale, void* v_scale, int64_t num_slots,
+                                      int64_t num_tokens, int64_t num_heads, int64_t num_kv_heads,
+                                      int64_t head_dim, int64_t q_row_stride,
+                                      int64_t k_row_stride, int64_t v_row_stride, float eps,
+                                      const float* inv_freq, svllm_stream stream);
+int svllm_rope_cache_fp8_bf16(void* q, const void* k, const void* v, const void* positions,
+                              int pos_type, const int64_t* slot_mapping, void* k_cache,
+                              void* v_cache, void* k_scale, void* v_scale, int64_t num_slots,
+                              int64_t num_tokens, int64_t num_heads, int64_t num_kv_heads,
+                              int64_t head_dim, int64_t q_row_stride, int64_t k_row_stride,
+                              int64_t v_row_stride, const float* inv_freq, svllm_stream stream);
+
+/*
+ * The cached rows of whole requests back in bf16, exactly: k_out, v_out [num_seqs, max_blocks *
+ * block_size, num_kv_heads, head_dim], row j of request s from slot block_tables[s][j / block_size]
+ * * block_size + j % block_size for j < seq_lens[s], zeros behind. Seen as [num_seqs * max_blocks,
+ * block_size, ...] the outputs are a paged bf16 cache in which page p of request s is block s *
+ * max_blocks + p. A length outside [0, max_blocks * block_size] is clamped and a table entry
+ * outside the cache read as block 0, either with SVLLM_DEVERR_BAD_INDEX.
+ */
+int svllm_cache_read_fp8_bf16(void* k_out, void* v_out, const void* k_cache, const void* v_cache,
+                              const void* k_scale, const void* v_scale, int64_t num_blocks,
+                              int64_t block_size, const int32_t* block_tables, int64_t max_blocks,
+                              const int32_t* seq_lens, int64_t num_seqs, int64_t num_kv_heads,
+                              int64_t head_dim, svllm_stream stream);
+
+/*
+ * Decode attention (svllm_paged_decode_attention_bf16) over the 8-bit cache: out[b, h] =
+ * softmax_j(scale * q[b, h] . k_j) v_j over the rows j < seq_lens[b], k_j and v_j codes times
+ * scales. Any number of query heads per KV head; q 16-byte aligned with a q_token_stride of whole
+ * 16 bytes, else SVLLM_ERR_UNSUPPORTED; scale positive and finite. Products in f16 on exact codes,
+ * the softmax numerators rounded to f16 for the second; scores, maxima and sums in fp32. A request
+ * of length 0, and a head with no score above -infinity, gives zeros. Lengths and table entries out
+ * of range as in svllm_cache_read_fp8_bf16.
+ */
+int svllm_decode_attention_fp8_bf16(void* out, const void* q, int64_t q_token_stride,
+                                    const void* k_cache, const void* v_cache, const void* k_scale,
+                                    const void* v_scale, int64_t num_blocks, int64_t block_size,
+                                    const int32_t* block_tables, int64_t max_blocks,
+                                    const int32_t* seq_lens, int64_t num_seqs, int64_t num_heads,
+                                    int64_t num_kv_heads, int64_t head_dim, float scale,
+                                    svllm_stream stream);
+
+/*
  * Reads (and with reset != 0 clears) the library's own error word on `device`. Synchronises
  * that device. For validation, not for the hot path.
  */

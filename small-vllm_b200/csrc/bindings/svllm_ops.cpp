@@ -11,6 +11,8 @@
 #include "model/config.h"
 #include "model/qwen3.h"
 #include "ops/add_rms_norm.h"
+#include "ops/cache_fp8.h"
+#include "ops/decode_attention_fp8.h"
 #include "ops/embedding.h"
 #include "ops/paged_plan.h"
 #include "ops/rms_norm.h"
@@ -82,6 +84,20 @@ PYBIND11_MODULE(svllm_ops, m) {
   m.def("rope_cache", &svllm::ops::rope_cache, py::arg("q"), py::arg("k"), py::arg("v"),
         py::arg("positions"), py::arg("slot_mapping"), py::arg("k_cache"), py::arg("v_cache"),
         py::arg("theta"), py::arg("rope_scaling") = std::nullopt);
+  m.def("qk_norm_rope_cache_fp8", &svllm::ops::qk_norm_rope_cache_fp8, py::arg("q"), py::arg("k"),
+        py::arg("v"), py::arg("q_weight"), py::arg("k_weight"), py::arg("positions"),
+        py::arg("slot_mapping"), py::arg("k_cache"), py::arg("v_cache"), py::arg("k_scale"),
+        py::arg("v_scale"), py::arg("eps"), py::arg("theta"),
+        py::arg("rope_scaling") = std::nullopt);
+  m.def("rope_cache_fp8", &svllm::ops::rope_cache_fp8, py::arg("q"), py::arg("k"), py::arg("v"),
+        py::arg("positions"), py::arg("slot_mapping"), py::arg("k_cache"), py::arg("v_cache"),
+        py::arg("k_scale"), py::arg("v_scale"), py::arg("theta"),
+        py::arg("rope_scaling") = std::nullopt);
+  m.def("cache_read_fp8", &svllm::ops::cache_read_fp8, py::arg("k_cache"), py::arg("v_cache"),
+        py::arg("k_scale"), py::arg("v_scale"), py::arg("block_tables"), py::arg("seq_lens"));
+  m.def("decode_attention_fp8", &svllm::ops::decode_attention_fp8, py::arg("q"),
+        py::arg("k_cache"), py::arg("v_cache"), py::arg("k_scale"), py::arg("v_scale"),
+        py::arg("block_tables"), py::arg("seq_lens"), py::arg("scale") = std::nullopt);
   m.def("rope_inv_freq", &svllm::ops::rope_inv_freq, py::arg("theta"), py::arg("head_dim"),
         py::arg("rope_scaling") = std::nullopt);
   m.def("silu_and_mul",
@@ -108,13 +124,19 @@ PYBIND11_MODULE(svllm_ops, m) {
       "tree_commit",
       [](const py::object& k_caches, const py::object& v_caches, const at::Tensor& path,
          const at::Tensor& num_accepted, const at::Tensor& slot_mapping,
-         const at::Tensor& query_start_loc) {
+         const at::Tensor& query_start_loc, const py::object& k_scales,
+         const py::object& v_scales) {
+        const auto scales = [](const py::object& list, const char* name) {
+          return list.is_none() ? std::vector<at::Tensor>() : tensor_list(list, name);
+        };
         svllm::ops::tree_commit(tensor_list(k_caches, "k_caches"),
                                 tensor_list(v_caches, "v_caches"), path, num_accepted,
-                                slot_mapping, query_start_loc);
+                                slot_mapping, query_start_loc, scales(k_scales, "k_scales"),
+                                scales(v_scales, "v_scales"));
       },
       py::arg("k_caches"), py::arg("v_caches"), py::arg("path"), py::arg("num_accepted"),
-      py::arg("slot_mapping"), py::arg("query_start_loc"));
+      py::arg("slot_mapping"), py::arg("query_start_loc"), py::arg("k_scales") = py::none(),
+      py::arg("v_scales") = py::none());
   m.def("read_device_error", &svllm::ops::read_device_error, py::arg("device_index"),
         py::arg("reset") = true);
 
@@ -152,7 +174,7 @@ PYBIND11_MODULE(svllm_ops, m) {
       .def(py::init<const ModelConfig&, const std::unordered_map<std::string, at::Tensor>&>(),
            py::arg("config"), py::arg("weights"))
       .def("allocate_kv_cache", &Model::allocate_kv_cache, py::arg("num_blocks"),
-           py::arg("block_size"))
+           py::arg("block_size"), py::arg("fp8") = false)
       .def(
           "forward",
           [](Model& self, const at::Tensor& ids, const at::Tensor& positions,
@@ -174,7 +196,9 @@ PYBIND11_MODULE(svllm_ops, m) {
       .def_property_readonly("block_size", &Model::block_size)
       .def_property_readonly("num_blocks", &Model::num_blocks)
       .def_property_readonly("k_cache", &Model::k_cache)
-      .def_property_readonly("v_cache", &Model::v_cache);
+      .def_property_readonly("v_cache", &Model::v_cache)
+      .def_property_readonly("k_scale", &Model::k_scale)
+      .def_property_readonly("v_scale", &Model::v_scale);
 
   using svllm::model::DecodeGraphs;
   py::class_<DecodeGraphs>(m, "DecodeGraphs")

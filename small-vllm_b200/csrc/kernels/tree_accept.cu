@@ -107,14 +107,14 @@ constexpr int kCommitPlanes = 128;  // K and V planes of one launch, their point
 constexpr int kCommitBatch = 8;     // rows a thread holds between its loads and its stores
 
 struct CommitArgs {
-  void* plane[kCommitPlanes];      // [num_slots, row_vecs * 16 bytes] each
+  void* plane[kCommitPlanes];      // [num_slots, row_vecs units] each
   const int32_t* path;             // [num_seqs, max_query_len]
   const int32_t* num_accepted;     // [num_seqs]
   const int64_t* slot_mapping;     // [num_tokens]
   const int32_t* query_start_loc;  // [num_seqs + 1]
   int64_t num_slots;
   int64_t num_tokens;
-  int64_t row_vecs;                // 16-byte vectors per row
+  int64_t row_vecs;                // units per row: 16-byte vectors, or bytes of scales
   int max_query_len;
   int* err;
 };
@@ -122,7 +122,9 @@ struct CommitArgs {
 // One CTA: one request, one plane (K or V of a layer). A thread moves the same 16-byte column
 // of every row in order, eight rows loaded before they are stored. That order is enough: row i
 // is written after every source path[j], j <= i, has been read, and no later source is row i,
-// since path[j] >= j > i.
+// since path[j] >= j > i. Unit: uint4, or uint8_t for the scales of an 8-bit cache, whose rows are
+// a few bytes.
+template <class Unit>
 __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const CommitArgs a) {
   grid_dependency_sync();
   extern __shared__ int64_t sh[];
@@ -164,10 +166,10 @@ __global__ void __launch_bounds__(kCommitThreads) tree_commit_kernel(const Commi
   }
   __syncthreads();
   count = sh_limit;
-  uint4* rows = static_cast<uint4*>(a.plane[blockIdx.y]);
+  Unit* rows = static_cast<Unit*>(a.plane[blockIdx.y]);
   for (int64_t v = tid; v < a.row_vecs; v += kCommitThreads) {
     for (int base = 1; base < count; base += kCommitBatch) {
-      uint4 held[kCommitBatch];
+      Unit held[kCommitBatch];
 #pragma unroll
       for (int e = 0; e < kCommitBatch; ++e) {
         if (base + e < count && sh_src[base + e] >= 0) {
@@ -262,12 +264,15 @@ extern "C" int svllm_tree_accept(const void* ids, int id_type, const int64_t* ta
                 1u, a);
 }
 
-extern "C" int svllm_tree_commit(void* const* k_caches, void* const* v_caches, int64_t num_layers,
-                                 int64_t num_slots, int64_t row_bytes, const int32_t* path,
-                                 const int32_t* num_accepted, const int64_t* slot_mapping,
-                                 const int32_t* query_start_loc, int64_t num_seqs,
-                                 int64_t num_tokens, int64_t max_query_len, svllm_stream stream) {
-  using namespace svllm::k;
+namespace svllm::k {
+namespace {
+
+template <class Unit>
+int launch_commit(void* const* k_caches, void* const* v_caches, int64_t num_layers,
+                  int64_t num_slots, int64_t row_bytes, const int32_t* path,
+                  const int32_t* num_accepted, const int64_t* slot_mapping,
+                  const int32_t* query_start_loc, int64_t num_seqs, int64_t num_tokens,
+                  int64_t max_query_len, svllm_stream stream) {
   if (num_seqs < 0 || num_tokens < 0 || num_layers < 0 || num_slots < 0 || row_bytes <= 0 ||
       max_query_len <= 0) {
     return SVLLM_ERR_INVALID_ARGUMENT;
@@ -279,9 +284,12 @@ extern "C" int svllm_tree_commit(void* const* k_caches, void* const* v_caches, i
   }
   for (int64_t l = 0; l < num_layers; ++l) {
     if (k_caches[l] == nullptr || v_caches[l] == nullptr) return SVLLM_ERR_INVALID_ARGUMENT;
-    if (!aligned16(k_caches[l]) || !aligned16(v_caches[l])) return SVLLM_ERR_UNSUPPORTED;
+    if (reinterpret_cast<uintptr_t>(k_caches[l]) % sizeof(Unit) != 0 ||
+        reinterpret_cast<uintptr_t>(v_caches[l]) % sizeof(Unit) != 0) {
+      return SVLLM_ERR_UNSUPPORTED;
+    }
   }
-  if (row_bytes % 16 != 0) return SVLLM_ERR_UNSUPPORTED;
+  if (row_bytes % static_cast<int64_t>(sizeof(Unit)) != 0) return SVLLM_ERR_UNSUPPORTED;
   if (max_query_len > SVLLM_MAX_TREE_NODES || num_seqs >= (int64_t{1} << 31) ||
       num_tokens >= (int64_t{1} << 31)) {
     return SVLLM_ERR_TOO_LARGE;
@@ -298,7 +306,7 @@ extern "C" int svllm_tree_commit(void* const* k_caches, void* const* v_caches, i
   a.query_start_loc = query_start_loc;
   a.num_slots = num_slots;
   a.num_tokens = num_tokens;
-  a.row_vecs = row_bytes / 16;
+  a.row_vecs = row_bytes / static_cast<int64_t>(sizeof(Unit));
   a.max_query_len = static_cast<int>(max_query_len);
   a.err = err;
   for (int64_t l = 0; l < num_layers; l += kCommitPlanes / 2) {
@@ -308,10 +316,35 @@ extern "C" int svllm_tree_commit(void* const* k_caches, void* const* v_caches, i
       a.plane[planes++] = v_caches[m];
     }
     const dim3 grid(static_cast<unsigned>(num_seqs), planes);
-    const int status = launch(tree_commit_kernel, grid, dim3(kCommitThreads),
+    const int status = launch(tree_commit_kernel<Unit>, grid, dim3(kCommitThreads),
                               static_cast<size_t>(max_query_len) * 16,
                               reinterpret_cast<cudaStream_t>(stream), 1u, a);
     if (status != SVLLM_OK) return status;
   }
   return SVLLM_OK;
+}
+
+}  // namespace
+}  // namespace svllm::k
+
+extern "C" int svllm_tree_commit(void* const* k_caches, void* const* v_caches, int64_t num_layers,
+                                 int64_t num_slots, int64_t row_bytes, const int32_t* path,
+                                 const int32_t* num_accepted, const int64_t* slot_mapping,
+                                 const int32_t* query_start_loc, int64_t num_seqs,
+                                 int64_t num_tokens, int64_t max_query_len, svllm_stream stream) {
+  return svllm::k::launch_commit<uint4>(k_caches, v_caches, num_layers, num_slots, row_bytes, path,
+                                        num_accepted, slot_mapping, query_start_loc, num_seqs,
+                                        num_tokens, max_query_len, stream);
+}
+
+extern "C" int svllm_tree_commit_scales(void* const* k_scales, void* const* v_scales,
+                                        int64_t num_layers, int64_t num_slots,
+                                        int64_t num_kv_heads, const int32_t* path,
+                                        const int32_t* num_accepted, const int64_t* slot_mapping,
+                                        const int32_t* query_start_loc, int64_t num_seqs,
+                                        int64_t num_tokens, int64_t max_query_len,
+                                        svllm_stream stream) {
+  return svllm::k::launch_commit<uint8_t>(k_scales, v_scales, num_layers, num_slots, num_kv_heads,
+                                          path, num_accepted, slot_mapping, query_start_loc,
+                                          num_seqs, num_tokens, max_query_len, stream);
 }

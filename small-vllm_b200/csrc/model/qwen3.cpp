@@ -8,6 +8,8 @@
 #include <utility>
 
 #include "ops/add_rms_norm.h"
+#include "ops/cache_fp8.h"
+#include "ops/decode_attention_fp8.h"
 #include "ops/embedding.h"
 #include "ops/rms_norm.h"
 #include "ops/rope.h"
@@ -97,15 +99,29 @@ Model::Model(const ModelConfig& config,
   }
 }
 
-void Model::allocate_kv_cache(int64_t num_blocks, int64_t block_size) {
+void Model::allocate_kv_cache(int64_t num_blocks, int64_t block_size, bool fp8) {
   TORCH_CHECK(num_blocks > 0 && block_size > 0, "allocate_kv_cache: num_blocks ", num_blocks,
               " and block_size ", block_size, " must be positive");
+  TORCH_CHECK(!fp8 || config_.head_dim == 64 || config_.head_dim == 128,
+              "allocate_kv_cache: the fp8 cache takes head_dim 64 or 128, not ", config_.head_dim);
   k_cache_.clear();
   v_cache_.clear();
+  k_scale_.clear();
+  v_scale_.clear();
+  const int64_t shape[] = {num_blocks, block_size, config_.num_kv_heads, config_.head_dim};
+  const at::IntArrayRef rows(shape, 3);
   for (int64_t l = 0; l < config_.num_layers; ++l) {
-    const auto shape = {num_blocks, block_size, config_.num_kv_heads, config_.head_dim};
-    k_cache_.push_back(at::zeros(shape, embed_.options()));
-    v_cache_.push_back(at::zeros(shape, embed_.options()));
+    if (fp8) {
+      // zero codes under a scale of 1
+      const auto bytes = embed_.options().dtype(at::kByte);
+      k_cache_.push_back(at::zeros(shape, bytes).view(at::kFloat8_e4m3fn));
+      v_cache_.push_back(at::zeros(shape, bytes).view(at::kFloat8_e4m3fn));
+      k_scale_.push_back(at::full(rows, 127, bytes).view(at::kFloat8_e8m0fnu));
+      v_scale_.push_back(at::full(rows, 127, bytes).view(at::kFloat8_e8m0fnu));
+    } else {
+      k_cache_.push_back(at::zeros(shape, embed_.options()));
+      v_cache_.push_back(at::zeros(shape, embed_.options()));
+    }
   }
   num_blocks_ = num_blocks;
   block_size_ = block_size;
@@ -182,6 +198,22 @@ at::Tensor Model::paged_decode_attention(const at::Tensor& q, int64_t layer,
 #endif
 }
 
+at::Tensor Model::fp8_attention(const at::Tensor& q, int64_t layer, const AttentionMetadata& meta,
+                                const at::Tensor& tables, const at::Tensor& lens,
+                                const at::Tensor& starts) const {
+  if (meta.decode) {
+    return ops::decode_attention_fp8(q, k_cache_[layer], v_cache_[layer], k_scale_[layer],
+                                     v_scale_[layer], tables, lens, std::nullopt);
+  }
+  const auto [k, v] = ops::cache_read_fp8(k_cache_[layer], v_cache_[layer], k_scale_[layer],
+                                          v_scale_[layer], tables, lens);
+  const int64_t pages = tables.numel();
+  const auto shape = {pages, block_size_, config_.num_kv_heads, config_.head_dim};
+  const at::Tensor in_order = at::arange(pages, tables.options()).view(tables.sizes());
+  return ops::tree_attention(q, k.view(shape), v.view(shape), in_order, lens, starts,
+                             meta.tree_mask, std::nullopt);
+}
+
 at::Tensor Model::forward(const at::Tensor& ids, const at::Tensor& positions,
                           const AttentionMetadata& meta) {
   TORCH_CHECK(!k_cache_.empty(), "Model::forward: allocate_kv_cache first");
@@ -199,10 +231,12 @@ at::Tensor Model::forward(const at::Tensor& ids, const at::Tensor& positions,
   const int64_t T = ids.size(0);
   const int64_t Hq = config_.num_heads, Hk = config_.num_kv_heads, D = config_.head_dim;
   const double eps = config_.rms_norm_eps;
-  const bool paged = paged_decode_ok(meta);
-  const AttentionPlan plan = paged || meta.tree ? AttentionPlan{} : plan_attention(T, meta);
+  const bool fp8 = !k_scale_.empty();
+  const bool paged = !fp8 && paged_decode_ok(meta);
+  const AttentionPlan plan =
+      paged || meta.tree || fp8 ? AttentionPlan{} : plan_attention(T, meta);
   at::Tensor tables, lens, starts;
-  if (meta.tree) {
+  if (meta.tree || fp8) {
     tables = meta.block_tables.to(at::kInt).contiguous();
     lens = meta.seq_lens.to(at::kInt).contiguous();
     starts = meta.query_start_loc.to(at::kInt).contiguous();
@@ -222,7 +256,14 @@ at::Tensor Model::forward(const at::Tensor& ids, const at::Tensor& positions,
     const at::Tensor q = qkv.narrow(1, 0, Hq * D).view({T, Hq, D});
     const at::Tensor k = qkv.narrow(1, Hq * D, Hk * D).view({T, Hk, D});
     const at::Tensor v = qkv.narrow(1, (Hq + Hk) * D, Hk * D).view({T, Hk, D});
-    if (config_.qk_norm) {
+    if (fp8 && config_.qk_norm) {
+      ops::qk_norm_rope_cache_fp8(q, k, v, layer.q_norm, layer.k_norm, positions,
+                                  meta.slot_mapping, k_cache_[l], v_cache_[l], k_scale_[l],
+                                  v_scale_[l], eps, config_.rope_theta, config_.rope_scaling);
+    } else if (fp8) {
+      ops::rope_cache_fp8(q, k, v, positions, meta.slot_mapping, k_cache_[l], v_cache_[l],
+                          k_scale_[l], v_scale_[l], config_.rope_theta, config_.rope_scaling);
+    } else if (config_.qk_norm) {
       ops::qk_norm_rope_cache(q, k, v, layer.q_norm, layer.k_norm, positions, meta.slot_mapping,
                               k_cache_[l], v_cache_[l], eps, config_.rope_theta,
                               config_.rope_scaling);
@@ -231,9 +272,11 @@ at::Tensor Model::forward(const at::Tensor& ids, const at::Tensor& positions,
                       config_.rope_theta, config_.rope_scaling);
     }
     const at::Tensor attn =
-        meta.tree ? ops::tree_attention(q, k_cache_[l], v_cache_[l], tables, lens, starts,
+        fp8 ? fp8_attention(q, static_cast<int64_t>(l), meta, tables, lens, starts)
+                  .view({T, Hq * D})
+        : meta.tree ? ops::tree_attention(q, k_cache_[l], v_cache_[l], tables, lens, starts,
                                         meta.tree_mask, std::nullopt)
-                        .view({T, Hq * D})
+                          .view({T, Hq * D})
         : paged ? paged_decode_attention(q, static_cast<int64_t>(l), meta)
                 : attention(q, static_cast<int64_t>(l), plan);
     hidden = project(attn, layer.o_proj);

@@ -58,7 +58,9 @@ class Model {
 
   // Allocates a zeroed paged KV cache of num_blocks blocks of block_size tokens per layer,
   // [num_blocks, block_size, num_kv_heads, head_dim] each, on the weights' device.
-  void allocate_kv_cache(int64_t num_blocks, int64_t block_size);
+  // With fp8 the cache is the 8-bit one (ops/rope.h, qk_norm_rope_cache_fp8; head_dim 64 or 128):
+  // half the bytes, for steps whose K and V carry e4m3's four significant bits.
+  void allocate_kv_cache(int64_t num_blocks, int64_t block_size, bool fp8 = false);
 
   // The final-norm hidden states [T, hidden] of the tokens ids [T] at positions [T]; writes
   // every token's k and v into the cache first.
@@ -91,6 +93,9 @@ class Model {
   int64_t num_blocks() const { return num_blocks_; }
   const std::vector<at::Tensor>& k_cache() const { return k_cache_; }
   const std::vector<at::Tensor>& v_cache() const { return v_cache_; }
+  // The scales of an 8-bit cache, [num_blocks, block_size, num_kv_heads] each; empty otherwise.
+  const std::vector<at::Tensor>& k_scale() const { return k_scale_; }
+  const std::vector<at::Tensor>& v_scale() const { return v_scale_; }
 
  private:
   struct Layer {
@@ -115,6 +120,11 @@ class Model {
   bool paged_decode_ok(const AttentionMetadata& meta) const;
   at::Tensor paged_decode_attention(const at::Tensor& q, int64_t layer,
                                     const AttentionMetadata& meta) const;
+  // Steps over the 8-bit cache. Decode: its attention straight from the codes. Others: the requests'
+  // rows read back in bf16, which are a paged cache in order, and attention over that.
+  at::Tensor fp8_attention(const at::Tensor& q, int64_t layer, const AttentionMetadata& meta,
+                           const at::Tensor& tables, const at::Tensor& lens,
+                           const at::Tensor& starts) const;
 
   ModelConfig config_;
   at::Tensor embed_;       // [V, H]
@@ -123,6 +133,8 @@ class Model {
   std::vector<Layer> layers_;
   std::vector<at::Tensor> k_cache_;
   std::vector<at::Tensor> v_cache_;
+  std::vector<at::Tensor> k_scale_;
+  std::vector<at::Tensor> v_scale_;
   int64_t block_size_ = 0;
   int64_t num_blocks_ = 0;
 };

@@ -35,6 +35,18 @@ void tree_commit(const std::vector<at::Tensor>& k_caches, const std::vector<at::
   v.reserve(v_caches.size());
   for (const at::Tensor& c : k_caches) k.push_back(c.mutable_data_ptr());
   for (const at::Tensor& c : v_caches) v.push_back(c.mutable_data_ptr());
+  if (first.scalar_type() == at::kFloat8_e8m0fnu) {  // scales, seen as [..., num_kv_heads, 1]
+    detail::check_status(
+        "tree_commit",
+        svllm_tree_commit_scales(k.data(), v.data(), static_cast<int64_t>(k.size()), num_slots,
+                                 first.size(-1) * first.size(-2),
+                                 path.const_data_ptr<int32_t>(),
+                                 num_accepted.const_data_ptr<int32_t>(),
+                                 slot_mapping.const_data_ptr<int64_t>(),
+                                 query_start_loc.const_data_ptr<int32_t>(), num_accepted.numel(),
+                                 slot_mapping.numel(), path.size(1), stream));
+    return;
+  }
   detail::check_status(
       "tree_commit",
       svllm_tree_commit(k.data(), v.data(), static_cast<int64_t>(k.size()), num_slots,

@@ -9,6 +9,7 @@
 #include <tuple>
 #include <vector>
 
+#include "ops/cache_fp8.h"
 #include "ops/rope_kernels.h"
 
 namespace svllm::ops {
@@ -59,12 +60,15 @@ at::Tensor token_view(const char* op, const char* name, const at::Tensor& t) {
   return t.view({-1, heads, head_dim});
 }
 
-// Cache-write operands of the *_cache ops (all undefined for plain rope / qk_norm_rope).
+// Cache-write operands of the *_cache ops (all undefined for plain rope / qk_norm_rope; the scales
+// undefined unless the cache is the 8-bit one).
 struct KvCacheArgs {
   at::Tensor v;
   at::Tensor slot_mapping;
   at::Tensor k_cache;
   at::Tensor v_cache;
+  at::Tensor k_scale;
+  at::Tensor v_scale;
 };
 
 void check_and_run(const char* op, const at::Tensor& q, const at::Tensor& k,
@@ -106,12 +110,20 @@ void check_and_run(const char* op, const at::Tensor& q, const at::Tensor& k,
               ", positions on ", positions.device(), ")");
 
   const bool with_cache = cache.v.defined();
-  at::Tensor v3, kc, vc;
-  if (with_cache) {
+  const bool fp8 = cache.k_scale.defined();
+  at::Tensor v3, kc, vc, ks, vs;
+  if (fp8) {
+    TORCH_CHECK(cache.v.scalar_type() == q.scalar_type(), op, ": expected bf16 v, got ",
+                cache.v.scalar_type());
+    detail::check_fp8_cache(op, cache.k_cache, cache.v_cache, cache.k_scale, cache.v_scale,
+                            q.device());
+  } else if (with_cache) {
     TORCH_CHECK(cache.v.scalar_type() == q.scalar_type() &&
                     cache.k_cache.scalar_type() == q.scalar_type() &&
                     cache.v_cache.scalar_type() == q.scalar_type(),
                 op, ": expected bf16 v, k_cache and v_cache");
+  }
+  if (with_cache) {
     v3 = token_view(op, "v", cache.v);
     TORCH_CHECK(v3.sizes() == k3.sizes(), op, ": v of shape ", cache.v.sizes(),
                 " does not match k of shape ", k.sizes());
@@ -137,12 +149,23 @@ void check_and_run(const char* op, const at::Tensor& q, const at::Tensor& k,
                 " but v, slot_mapping or a cache is elsewhere");
     kc = cache.k_cache.view({-1, kv_heads, head_dim});
     vc = cache.v_cache.view({-1, kv_heads, head_dim});
+    if (fp8) {
+      ks = cache.k_scale.view({-1, kv_heads});
+      vs = cache.v_scale.view({-1, kv_heads});
+    }
   }
 
   const std::vector<float>& inv_freq = cached_inv_freq(theta, head_dim, rope_scaling);
 
   switch (q.device().type()) {
     case c10::DeviceType::CPU: {
+      if (fp8) {
+        const int64_t bad =
+            cpu_impl::rope_cache_fp8(q3, k3, v3, q_weight, k_weight, positions, cache.slot_mapping,
+                                     kc, vc, ks, vs, eps, inv_freq.data());
+        TORCH_CHECK(bad == 0, op, ": ", bad, " slots past the cache's ", kc.size(0));
+        break;
+      }
       cpu_impl::rope(q3, k3, q_weight, k_weight, positions, eps, inv_freq.data());
       if (with_cache) {
         const int64_t bad = cpu_impl::write_kv_cache(k3, v3, cache.slot_mapping, kc, vc);
@@ -151,7 +174,10 @@ void check_and_run(const char* op, const at::Tensor& q, const at::Tensor& k,
       break;
     }
     case c10::DeviceType::CUDA:
-      if (with_cache) {
+      if (fp8) {
+        cuda_impl::rope_cache_fp8(q3, k3, v3, q_weight, k_weight, positions, cache.slot_mapping,
+                                  kc, vc, ks, vs, eps, inv_freq.data());
+      } else if (with_cache) {
         cuda_impl::rope_cache(q3, k3, v3, q_weight, k_weight, positions, cache.slot_mapping, kc,
                               vc, eps, inv_freq.data());
       } else {
@@ -232,6 +258,27 @@ void rope_cache(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                 const std::optional<Llama3RopeScaling>& rope_scaling) {
   check_and_run("rope_cache", q, k, at::Tensor(), at::Tensor(), positions, 0.0, theta,
                 rope_scaling, {v, slot_mapping, k_cache, v_cache});
+}
+
+void qk_norm_rope_cache_fp8(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                            const at::Tensor& q_weight, const at::Tensor& k_weight,
+                            const at::Tensor& positions, const at::Tensor& slot_mapping,
+                            const at::Tensor& k_cache, const at::Tensor& v_cache,
+                            const at::Tensor& k_scale, const at::Tensor& v_scale, double eps,
+                            double theta, const std::optional<Llama3RopeScaling>& rope_scaling) {
+  TORCH_CHECK(q_weight.defined() && k_weight.defined(),
+              "qk_norm_rope_cache_fp8: q_weight and k_weight are required");
+  check_and_run("qk_norm_rope_cache_fp8", q, k, q_weight, k_weight, positions, eps, theta,
+                rope_scaling, {v, slot_mapping, k_cache, v_cache, k_scale, v_scale});
+}
+
+void rope_cache_fp8(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                    const at::Tensor& positions, const at::Tensor& slot_mapping,
+                    const at::Tensor& k_cache, const at::Tensor& v_cache,
+                    const at::Tensor& k_scale, const at::Tensor& v_scale, double theta,
+                    const std::optional<Llama3RopeScaling>& rope_scaling) {
+  check_and_run("rope_cache_fp8", q, k, at::Tensor(), at::Tensor(), positions, 0.0, theta,
+                rope_scaling, {v, slot_mapping, k_cache, v_cache, k_scale, v_scale});
 }
 
 }  // namespace svllm::ops

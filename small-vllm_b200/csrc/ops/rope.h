@@ -62,6 +62,34 @@ void rope_cache(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                 const at::Tensor& k_cache, const at::Tensor& v_cache, double theta,
                 const std::optional<Llama3RopeScaling>& rope_scaling);
 
+// Definition: The rotary step with the 8-bit cache's write in the same pass: qk_norm_rope_cache /
+//             rope_cache for a cache of e4m3 codes with one power-of-two scale per row.
+// Formula:    y = rotate(norm(x)) per head of q and k as in qk_norm_rope / rope, but in fp32 with
+//             the one rounding at the end, and with the angle position * inv_freq[i] kept exact
+//             where fp32 would round it. q holds bf16(y); k and v stay as they were. For every
+//             token t with s = slot_mapping[t] >= 0 and every KV head, y of k and the v row are
+//             quantised: e the least integer with max |x_i| <= 448 * 2^e, clamped to [-60, 60];
+//             scale 2^e, codes e4m3(x_i * 2^-e), saturating. Values that are not finite become
+//             the NaN code and do not count for the maximum.
+// Domain:     As qk_norm_rope_cache, head_dim 64 or 128; k_cache and v_cache contiguous
+//             float8_e4m3fn [..., num_kv_heads, head_dim]; k_scale and v_scale contiguous
+//             float8_e8m0fnu [..., num_kv_heads]. No slot twice in slot_mapping.
+// Returns:    Nothing; q and the slots' codes and scales hold the results. A negative slot skips
+//             its token's cache write (padding).
+// Throws:     As qk_norm_rope_cache.
+void qk_norm_rope_cache_fp8(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                            const at::Tensor& q_weight, const at::Tensor& k_weight,
+                            const at::Tensor& positions, const at::Tensor& slot_mapping,
+                            const at::Tensor& k_cache, const at::Tensor& v_cache,
+                            const at::Tensor& k_scale, const at::Tensor& v_scale, double eps,
+                            double theta, const std::optional<Llama3RopeScaling>& rope_scaling);
+
+void rope_cache_fp8(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                    const at::Tensor& positions, const at::Tensor& slot_mapping,
+                    const at::Tensor& k_cache, const at::Tensor& v_cache,
+                    const at::Tensor& k_scale, const at::Tensor& v_scale, double theta,
+                    const std::optional<Llama3RopeScaling>& rope_scaling);
+
 // Definition: The inverse-frequency table rope() uses, computed on the CPU with torch's own fp32
 //             ops in Hugging Face's order (_compute_default_rope_parameters, and
 //             _compute_llama3_parameters when rope_scaling is given), so it equals Hugging Face's

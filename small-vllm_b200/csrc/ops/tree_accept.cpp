@@ -72,10 +72,14 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> tree_accept(
 
 void tree_commit(const std::vector<at::Tensor>& k_caches, const std::vector<at::Tensor>& v_caches,
                  const at::Tensor& path, const at::Tensor& num_accepted,
-                 const at::Tensor& slot_mapping, const at::Tensor& query_start_loc) {
+                 const at::Tensor& slot_mapping, const at::Tensor& query_start_loc,
+                 const std::vector<at::Tensor>& k_scales,
+                 const std::vector<at::Tensor>& v_scales) {
   TORCH_CHECK(!k_caches.empty() && k_caches.size() == v_caches.size(), "tree_commit: ",
               k_caches.size(), " K caches and ", v_caches.size(), " V caches");
   const at::Tensor& first = k_caches[0];
+  TORCH_CHECK(first.scalar_type() != at::kFloat8_e8m0fnu,
+              "tree_commit: float8_e8m0fnu caches are scales: pass them as k_scales and v_scales");
   TORCH_CHECK(first.dim() >= 3 && first.numel() > 0,
               "tree_commit: caches must be [..., num_kv_heads, head_dim], got shape ",
               first.sizes());
@@ -87,6 +91,23 @@ void tree_commit(const std::vector<at::Tensor>& k_caches, const std::vector<at::
                   "first K cache is ", first.scalar_type(), " ", first.sizes(), " on ",
                   first.device(), ", another ", c.scalar_type(), " ", c.sizes(), " on ",
                   c.device());
+    }
+  }
+  const bool scaled = !k_scales.empty() || !v_scales.empty();
+  std::vector<at::Tensor> ks, vs;  // as [..., KV heads, 1]
+  if (scaled) {
+    TORCH_CHECK(k_scales.size() == k_caches.size() && v_scales.size() == v_caches.size(),
+                "tree_commit: ", k_scales.size(), " K scales and ", v_scales.size(),
+                " V scales for ", k_caches.size(), " layers");
+    const at::IntArrayRef rows = first.sizes().slice(0, first.dim() - 1);
+    for (const auto* scales : {&k_scales, &v_scales}) {
+      for (const at::Tensor& c : *scales) {
+        TORCH_CHECK(c.sizes() == rows && c.scalar_type() == at::kFloat8_e8m0fnu &&
+                        c.device() == first.device() && c.is_contiguous(),
+                    "tree_commit: scales must be contiguous float8_e8m0fnu ", rows, " on ",
+                    first.device(), ", got ", c.scalar_type(), " ", c.sizes(), " on ", c.device());
+        (scales == &k_scales ? ks : vs).push_back(c.unsqueeze(-1));
+      }
     }
   }
   const at::Device device = first.device();
@@ -103,10 +124,18 @@ void tree_commit(const std::vector<at::Tensor>& k_caches, const std::vector<at::
     case c10::DeviceType::CPU:
       cpu_impl::tree_commit(k_caches, v_caches, num_slots, path, num_accepted, slot_mapping,
                             query_start_loc);
+      if (scaled) {
+        cpu_impl::tree_commit(ks, vs, num_slots, path, num_accepted, slot_mapping,
+                              query_start_loc);
+      }
       break;
     case c10::DeviceType::CUDA:
       cuda_impl::tree_commit(k_caches, v_caches, num_slots, path, num_accepted, slot_mapping,
                              query_start_loc);
+      if (scaled) {
+        cuda_impl::tree_commit(ks, vs, num_slots, path, num_accepted, slot_mapping,
+                               query_start_loc);
+      }
       break;
     default:
       TORCH_CHECK(false, "tree_commit: unsupported device ", device);

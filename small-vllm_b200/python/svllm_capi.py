@@ -77,6 +77,15 @@ SIGNATURES = {
     "svllm_tree_attention_workspace_bytes": [_I64, _P],
     "svllm_tree_accept": [_P, _I, _P, _P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _P, _P, _P],
     "svllm_tree_commit": [_P, _P, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _P],
+    "svllm_tree_commit_scales": [_P, _P, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _P],
+    "svllm_qk_norm_rope_cache_fp8_bf16": [_P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _I64,
+                                          _I64, _I64, _I64, _I64, _I64, _I64, _I64, _F, _P, _P],
+    "svllm_rope_cache_fp8_bf16": [_P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64,
+                                  _I64, _I64, _I64, _I64, _P, _P],
+    "svllm_cache_read_fp8_bf16": [_P, _P, _P, _P, _P, _P, _I64, _I64, _P, _I64, _P, _I64, _I64,
+                                  _I64, _P],
+    "svllm_decode_attention_fp8_bf16": [_P, _P, _I64, _P, _P, _P, _P, _I64, _I64, _P, _I64, _P,
+                                        _I64, _I64, _I64, _I64, _F, _P],
     "svllm_read_device_error": [_I, _I, _P],
 }
 
