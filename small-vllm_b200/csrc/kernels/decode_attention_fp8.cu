@@ -19,15 +19,21 @@
 // f16 (2^-11 of each, an eighth of a bf16 rounding) because the product takes no wider operand.
 //
 // Layout. A warp takes steps of 32 cached rows, lane = 4 g + t:
-//   S^T[16 rows x 8 heads] = K[16 x D] . Q^T[D x 8]: lane loads rows g, g + 8 of K, 16 bytes at
+//   S^T[16 rows x 8 heads] = K[16 x D] . Q^T[D x 8]: lane holds rows g, g + 8 of K, 16 bytes at
 //     64 c + 16 t of piece c; a 4-byte word of it is one k-step (the same permutation of the
 //     head dimension on both sides);
-//   O^T[D x 8] += V^T[D x 16 rows] . P^T[16 x 8]: lane loads rows 2t, 2t + 1, 2t + 8, 2t + 9 of V,
+//   O^T[D x 8] += V^T[D x 16 rows] . P^T[16 x 8]: lane holds rows 2t, 2t + 1, 2t + 8, 2t + 9 of V,
 //     D / 8 bytes at g * D / 8. V's transpose is two byte permutations of a word of two rows, which
 //     pair their codes before the conversion; P^T comes from S^T by movmatrix.
-// A CTA takes one (request, KV head, group of up to eight query heads) and a split of the rows;
-// its warps share the split. The splits of one such item form a thread-block cluster that merges
-// its (max, sum, partial output) through distributed shared memory.
+//
+// Work. An item is one (request, KV head, group of up to eight query heads). Rows travel by cp.async,
+// 16 bytes a lane, into a ring of stages that each warp owns. Two kernels:
+//   * By lines (long tables, or many items): the steps of all items form one line, in that order,
+//     of which each warp takes an equal share, found from the device-side lengths. A warp runs on
+//     from item to item without waiting for another; the parts of items that are cut go to a
+//     workspace, and a third kernel joins them in a fixed order.
+//   * By items (short tables and few items): a CTA takes an item, its warps deal the steps among
+//     them and merge through shared memory. One launch.
 #include <cuda_runtime.h>
 
 #include <cfloat>
@@ -41,10 +47,25 @@
 namespace svllm::k {
 namespace {
 
-constexpr int kMaxSplits = 8;    // the portable cluster size
 constexpr int kStepRows = 32;    // cached rows a warp takes at a time
-constexpr int kGroup = 8;        // query heads of a CTA: the N of the products
-constexpr float kWeightBits = 14.0f;  // weights reach 2^14, so that f16 keeps small ones
+constexpr int kGroup = 8;        // query heads of an item: the N of the products
+constexpr int kStages = 2;       // of a warp's ring
+constexpr int kLineWarps = 8;    // of a CTA by lines, one per SM
+constexpr int kItemWarps = 8;    // of a CTA by items
+constexpr int kMinShare = 2;     // steps of a warp's share at least
+constexpr int64_t kItemRows = 512;  // by items up to this many rows of a table
+constexpr int kJoinThreads = 256;
+constexpr int kJoinBatch = 8;    // parts a thread of the join has in flight
+// The running maximum is moved only when a score passes it by kSlack, so that most steps need one
+// vote instead of a maximum over the warp. Weights reach 2^(kWeightBits + kSlack).
+constexpr float kWeightBits = 6.0f, kSlack = 8.0f;
+
+// Where an item's parts are: the first share that holds one, and how many (1: the item is whole, and
+// its output written).
+struct JoinEntry {
+  int share;
+  int parts;
+};
 
 struct AttnArgs {
   void* out;      // [num_seqs, num_heads, D] bf16, contiguous
@@ -55,8 +76,14 @@ struct AttnArgs {
   const uint8_t* v_scale;
   const int32_t* block_tables;  // [num_seqs, max_blocks]
   const int32_t* seq_lens;      // [num_seqs]
+  // What the warps by lines leave of cut items, for the join: [shares][2][heads of an item], of the
+  // item that a share continues and of one that it begins.
+  JoinEntry* table;  // [items]
+  float2* part_ml;   // maximum and sum
+  float* part_acc;   // [D] each
   int64_t q_stride;
   int64_t num_blocks;
+  int num_seqs;
   int max_blocks;
   int max_rows;  // max_blocks * block_size
   int block_size;
@@ -64,8 +91,8 @@ struct AttnArgs {
   int num_heads;
   int num_kv_heads;
   int group;   // query heads per KV head
-  int groups;  // CTAs they are dealt to
-  int splits;
+  int groups;  // items they are dealt to
+  int shares;  // warps by lines
   float scale_log2;
   int* err;
 };
@@ -76,82 +103,139 @@ __device__ __forceinline__ uint32_t transpose8x8_b16(uint32_t x) {
   return y;
 }
 
-// This lane's bytes of a V row: 16 at D = 128, 8 at D = 64.
+// 16 bytes to shared memory, zeros where !valid.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(valid ? 16 : 0)
+               : "memory");
+}
+
+__device__ __forceinline__ void cp_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "r"(a)
+               : "memory");
+  return r;
+}
+
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 r;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a) : "memory");
+  return r;
+}
+
+// Where 16-byte chunk c of row r lies in a tile of 32 rows: permuted so that both products' reads
+// (a quarter of a warp: two rows times four chunks of K, four even or odd rows times two chunks of
+// V) touch every bank once.
 template <int D>
-struct VPart {
-  uint32_t w[D / 32];
-  __device__ __forceinline__ void load(const uint8_t* p) {
-    if constexpr (D == 128) {
-      const uint4 x = ld_global_nc_v4(p);
-      w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
-    } else {
-      asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];"
-                   : "=r"(w[0]), "=r"(w[1])
-                   : "l"(p));
-    }
+__device__ __forceinline__ uint32_t tile_at(int r, int c) {
+  if constexpr (D == 128) {
+    return static_cast<uint32_t>(r * 128 + ((c ^ (r & 7)) << 4));
+  } else {
+    return static_cast<uint32_t>((r >> 1) * 128 + (((r ^ (r >> 2)) & 1) << 6) +
+                                 ((c ^ (((r >> 1) & 1) << 1)) << 4));
   }
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) w[i] = 0;
+}
+
+// A request's length, and the steps of its items: one at least, so that a request without rows
+// gets its zeros.
+__device__ __forceinline__ int clamp_len(const AttnArgs& a, int n) {
+  return max(0, min(n, a.max_rows));
+}
+
+__device__ __forceinline__ int item_steps(int len) {
+  return max(1, (len + kStepRows - 1) / kStepRows);
+}
+
+// The query heads of an item: the first one's index, and how many.
+struct Heads {
+  int first, count;
+  __device__ __forceinline__ Heads(const AttnArgs& a, int sub) {
+    const int kh = sub / a.groups, hg = sub - kh * a.groups;
+    first = kh * a.group + hg * kGroup;
+    count = min(kGroup, a.group - hg * kGroup);
   }
 };
 
-template <int D, int kWarps>
-__global__ void __launch_bounds__(kWarps * kWarpSize) decode_attention_fp8_kernel(
-    const __grid_constant__ AttnArgs a) {
-  grid_dependency_sync();
-  constexpr int kThreads = kWarps * kWarpSize;
-  constexpr int kPieces = D / 64;  // 16-byte pieces per lane of a K row
-  constexpr int kTiles = D / 16;   // m-tiles of O^T
-  extern __shared__ __align__(16) float shared[];  // warp_acc [kWarps][heads][D], part [heads][D]
-  __shared__ float warp_m[kWarps][kGroup], warp_l[kWarps][kGroup];
-  __shared__ float m_sm[kGroup], l_sm[kGroup];
+// One step's copies: 32 rows of K, then of V.
+template <int D>
+struct Loader {
+  static constexpr int kChunks = D / 16;  // 16-byte chunks of a row
+  static constexpr int kTileBytes = kStepRows * D;
+  static constexpr int kStageBytes = 2 * kTileBytes;
+  static constexpr int kLoads = kStepRows * kChunks / kWarpSize;  // a lane, K and V each
+  static constexpr int kRowsALoad = kWarpSize / kChunks;
 
-  const int split = static_cast<int>(blockIdx.x % a.splits);
-  const int64_t item = blockIdx.x / a.splits;
-  const int hg = static_cast<int>(item % a.groups);
-  const int kh = static_cast<int>(item / a.groups % a.num_kv_heads);
-  const int64_t b = item / a.groups / a.num_kv_heads;
-  const int heads = min(kGroup, a.group - hg * kGroup);  // this CTA's
-  const int head0 = kh * a.group + hg * kGroup;
-  const int warp = threadIdx.x / kWarpSize;
-  const int lane = threadIdx.x % kWarpSize;
-  const int g = lane >> 2;
-  const int t = lane & 3;
-  float* part = shared + kWarps * heads * D;
-
-  int seq_len = a.seq_lens[b];
-  if (seq_len < 0 || seq_len > a.max_rows) {
-    if (threadIdx.x == 0) raise_error(a.err, kErrBadIndex);
-    seq_len = seq_len < 0 ? 0 : a.max_rows;
+  // The table entry of lane r's row of a step; any where the row does not exist.
+  static __device__ __forceinline__ int block_of(const AttnArgs& a, int b, int step, int len) {
+    const int j = step * kStepRows + static_cast<int>(threadIdx.x) % kWarpSize;
+    if (j >= len) return 0;
+    return __ldg(a.block_tables + static_cast<int64_t>(b) * a.max_blocks + a.page.divide(j));
   }
-  // this CTA's split of the rows, then this warp's share of it, both in whole steps
-  const int steps = (seq_len + kStepRows - 1) / kStepRows;
-  const int split_steps = (steps + a.splits - 1) / a.splits;
-  const int warp_steps = (split_steps + kWarps - 1) / kWarps;
-  const int step0 = min(steps, split * split_steps + warp * warp_steps);
-  const int step1 = min(steps, min((split + 1) * split_steps, step0 + warp_steps));
-  const int w_begin = step0 * kStepRows;
-  const int w_end = min(seq_len, step1 * kStepRows);
-  const int32_t* table = a.block_tables + b * a.max_blocks;
 
-  // Q^T's B fragments in f16: head g, this lane's dims. Scaled by a power of two per head.
-  uint32_t qf[kPieces][8];
+  // Copies the step's rows to `dst` and loads lane r's row's scale bytes, which nothing waits for
+  // here.
+  static __device__ __forceinline__ void issue(const AttnArgs& a, uint32_t dst, int block, int kh,
+                                               int step, int len, uint32_t& k_scale,
+                                               uint32_t& v_scale) {
+    const int lane = static_cast<int>(threadIdx.x) % kWarpSize;
+    const int r0 = step * kStepRows, j = r0 + lane;
+    uint32_t slot = 0;
+    k_scale = v_scale = kScaleBias;
+    if (j < len) {
+      if (static_cast<uint64_t>(block) >= static_cast<uint64_t>(a.num_blocks)) {
+        raise_error(a.err, kErrBadIndex);  // an entry outside the cache: read block 0
+        block = 0;
+      }
+      slot = static_cast<uint32_t>(block) * static_cast<uint32_t>(a.block_size) +
+             static_cast<uint32_t>(j - a.page.divide(j) * a.block_size);
+      const int64_t at = static_cast<int64_t>(slot) * a.num_kv_heads + kh;
+      k_scale = __ldg(a.k_scale + at);
+      v_scale = __ldg(a.v_scale + at);
+    }
+    const int c = lane % kChunks;
+    const int64_t row_bytes = static_cast<int64_t>(a.num_kv_heads) * D;
+    const uint8_t* k = a.k_cache + static_cast<int64_t>(kh) * D + c * 16;
+    const int64_t v = a.v_cache - a.k_cache;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int r = i * kRowsALoad + lane / kChunks;
+      const uint8_t* p = k + __shfl_sync(0xffffffffu, slot, r) * row_bytes;
+      const bool valid = r0 + r < len;  // zeros past the end: 0 * w, never NaN
+      cp_async16(dst + tile_at<D>(r, c), p, valid);
+      cp_async16(dst + kTileBytes + tile_at<D>(r, c), p + v, valid);
+    }
+  }
+};
+
+// Q^T's B fragments in f16: head g, this lane's dims, scaled by a power of two per head.
+template <int D>
+struct Queries {
+  static constexpr int kPieces = D / 64;  // 16-byte pieces per lane of a K row
+  uint32_t f[kPieces][8];
   float x_scale[2];  // of the scores of heads 2t and 2t + 1
-  {
+
+  // chunk(i): 16-byte chunk i of query head g; zeros for a head that does not exist.
+  template <class Chunk>
+  __device__ __forceinline__ void set(float scale_log2, const Chunk& chunk) {
+    const int t = static_cast<int>(threadIdx.x) & 3;
     uint32_t raw[kPieces][8];
     uint32_t amax = 0;
 #pragma unroll
     for (int c = 0; c < kPieces; ++c) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) raw[c][i] = 0;
-      if (g < heads) {
-        const uint8_t* qp = static_cast<const uint8_t*>(a.q) +
-                            (b * a.q_stride + static_cast<int64_t>(head0 + g) * D + 64 * c + 16 * t) * 2;
-        const uint4 q0 = ld_global_nc_v4(qp), q1 = ld_global_nc_v4(qp + 16);
-        raw[c][0] = q0.x, raw[c][1] = q0.y, raw[c][2] = q0.z, raw[c][3] = q0.w;
-        raw[c][4] = q1.x, raw[c][5] = q1.y, raw[c][6] = q1.z, raw[c][7] = q1.w;
-      }
+      const uint4 q0 = chunk(8 * c + 2 * t), q1 = chunk(8 * c + 2 * t + 1);
+      raw[c][0] = q0.x, raw[c][1] = q0.y, raw[c][2] = q0.z, raw[c][3] = q0.w;
+      raw[c][4] = q1.x, raw[c][5] = q1.y, raw[c][6] = q1.z, raw[c][7] = q1.w;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         amax = max(amax, max(raw[c][i] & 0x7fffu, (raw[c][i] >> 16) & 0x7fffu));
@@ -159,7 +243,7 @@ __global__ void __launch_bounds__(kWarps * kWarpSize) decode_attention_fp8_kerne
     }
     amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    // the largest magnitude's exponent; the shift to 14 as two factors, either inside fp32
+    // the largest magnitude's exponent to 14, as two factors, either inside fp32
     const int shift = 14 - (static_cast<int>(amax >> 7) - 127);  // [-114, 141]
     const int s0 = shift / 2, s1 = shift - s0;
     const float f0 = exp2_int(s0), f1 = exp2_int(s1);
@@ -167,79 +251,43 @@ __global__ void __launch_bounds__(kWarps * kWarpSize) decode_attention_fp8_kerne
     for (int c = 0; c < kPieces; ++c) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        qf[c][i] = pack_f16x2(__uint_as_float(raw[c][i] << 16) * f0 * f1,
-                              __uint_as_float(raw[c][i] & 0xffff0000u) * f0 * f1);
+        f[c][i] = pack_f16x2(__uint_as_float(raw[c][i] << 16) * f0 * f1,
+                             __uint_as_float(raw[c][i] & 0xffff0000u) * f0 * f1);
       }
     }
-    const float back = a.scale_log2 * exp2_int(-s0) * exp2_int(-s1);
+    const float back = scale_log2 * exp2_int(-s0) * exp2_int(-s1);
     x_scale[0] = __shfl_sync(0xffffffffu, back, 8 * t);      // lane of head 2t
     x_scale[1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);  // of head 2t + 1
   }
+};
 
+// A warp's running sums over an item's rows.
+template <int D>
+struct Sums {
+  static constexpr int kTiles = D / 16;  // m-tiles of O^T
+  // O^T element (dim, head): m-tile i holds dims g * D / 8 + 2 i (elements 0, 1: heads 2t, 2t + 1)
+  // and + 1 (elements 2, 3)
   float acc[kTiles][4];
+  // the running maximum of y of heads 2t, 2t + 1; finite, so that no difference with a score of
+  // -infinity is NaN
+  float m[2];
+  float l[2];  // this lane's rows only, until reduce()
+
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-  for (int i = 0; i < kTiles; ++i) {
+    for (int i = 0; i < kTiles; ++i) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[i][e] = 0.0f;
+      for (int e = 0; e < 4; ++e) acc[i][e] = 0.0f;
+    }
+    m[0] = m[1] = -FLT_MAX;
+    l[0] = l[1] = 0.0f;
   }
-  // the running maximum of y of heads 2t, 2t + 1; finite, so that no difference with a score
-  // of -infinity is NaN
-  float m[2] = {-FLT_MAX, -FLT_MAX};
-  float l[2] = {0.0f, 0.0f};  // this lane's rows only, summed over the warp at the end
 
-  const int64_t row_bytes = static_cast<int64_t>(a.num_kv_heads) * D;
-  const uint8_t* kc = a.k_cache + static_cast<int64_t>(kh) * D + 16 * t;
-  const uint8_t* vc = a.v_cache + static_cast<int64_t>(kh) * D + g * (D / 8);
-
-  // lane r's row of a step: its slot and its two scale bytes (1 past the end, and unused)
-  uint32_t slot = 0, scales = 0;
-  const auto look_up = [&](int r0) {
-    const int j = r0 + lane;
-    slot = 0;
-    scales = (kScaleBias << 8) | kScaleBias;
-    if (j < w_end) {
-      const int page = a.page.divide(j);
-      int blk = __ldg(table + page);
-      if (static_cast<uint64_t>(blk) >= static_cast<uint64_t>(a.num_blocks)) {
-        raise_error(a.err, kErrBadIndex);  // an entry outside the cache: read block 0
-        blk = 0;
-      }
-      slot = static_cast<uint32_t>(blk) * static_cast<uint32_t>(a.block_size) +
-             static_cast<uint32_t>(j - page * a.block_size);
-      const int64_t at = static_cast<int64_t>(slot) * a.num_kv_heads + kh;
-      scales = __ldg(a.k_scale + at) | (static_cast<uint32_t>(__ldg(a.v_scale + at)) << 8);
-    }
-  };
-
-  if (w_begin < w_end) look_up(w_begin);
-  for (int r0 = w_begin; r0 < w_end; r0 += kStepRows) {
-    uint4 k[2][2][kPieces];  // tile, row g or g + 8, piece
-    VPart<D> v[2][4];        // tile, rows 2t, 2t + 1, 2t + 8, 2t + 9
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = 16 * i + 8 * e + g;
-        const uint8_t* p = kc + __shfl_sync(0xffffffffu, slot, r) * row_bytes;
-#pragma unroll
-        for (int c = 0; c < kPieces; ++c) {
-          k[i][e][c] = r0 + r < w_end ? ld_global_nc_v4(p + 64 * c) : make_uint4(0, 0, 0, 0);
-        }
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = 16 * i + 8 * (e >> 1) + 2 * t + (e & 1);
-        const uint8_t* p = vc + __shfl_sync(0xffffffffu, slot, r) * row_bytes;
-        if (r0 + r < w_end) v[i][e].load(p);
-        else v[i][e].clear();  // codes of rows past the end are zeros: 0 * w, never NaN
-      }
-    }
-    const uint32_t step_scales = scales;
-    if (r0 + kStepRows < w_end) look_up(r0 + kStepRows);
-
+  // Adds a step: the tile in shared memory, lane r's row's scale bytes, how many rows exist.
+  __device__ __forceinline__ void step(uint32_t tile, uint32_t scales, int live,
+                                       const Queries<D>& q) {
+    const int lane = static_cast<int>(threadIdx.x) % kWarpSize;
+    const int g = lane >> 2, t = lane & 3;
     // S^T: lane holds rows g, g + 8 of both tiles x heads 2t, 2t + 1
     float y[2][4];
     float unscale[2][2];  // 2^-ev
@@ -248,35 +296,37 @@ __global__ void __launch_bounds__(kWarps * kWarpSize) decode_attention_fp8_kerne
     for (int i = 0; i < 2; ++i) {
       float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int c = 0; c < kPieces; ++c) {
+      for (int c = 0; c < Queries<D>::kPieces; ++c) {
+        const uint4 k0 = lds128(tile + tile_at<D>(16 * i + g, 4 * c + t));
+        const uint4 k1 = lds128(tile + tile_at<D>(16 * i + 8 + g, 4 * c + t));
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const uint32_t w0 = word(k[i][0][c], w), w1 = word(k[i][1][c], w);
+          const uint32_t w0 = word(k0, w), w1 = word(k1, w);
           mma_16816_f16(s, e4m3_to_f16x2_lo(w0), e4m3_to_f16x2_lo(w1), e4m3_to_f16x2_hi(w0),
-                        e4m3_to_f16x2_hi(w1), qf[c][2 * w], qf[c][2 * w + 1]);
+                        e4m3_to_f16x2_hi(w1), q.f[c][2 * w], q.f[c][2 * w + 1]);
         }
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int r = 16 * i + 8 * e + g;
-        const uint32_t sc = __shfl_sync(0xffffffffu, step_scales, r);
+        const uint32_t sc = __shfl_sync(0xffffffffu, scales, r);
         const float ks = scale_value(sc & 0xffu);
         const float ev = static_cast<float>(static_cast<int>(sc >> 8) - kScaleBias);
         unscale[i][e] = scale_value(2 * kScaleBias - (sc >> 8));
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float v = fmaf(s[2 * e + h], x_scale[h] * ks, ev);
-          y[i][2 * e + h] = r0 + r < w_end ? v : -__builtin_huge_valf();
+          const float v = fmaf(s[2 * e + h], q.x_scale[h] * ks, ev);
+          y[i][2 * e + h] = r < live ? v : -__builtin_huge_valf();
           top[h] = fmaxf(top[h], y[i][2 * e + h]);
         }
       }
     }
+    if (__any_sync(0xffffffffu, top[0] > m[0] + kSlack || top[1] > m[1] + kSlack)) {
 #pragma unroll
-    for (int off = 4; off < kWarpSize; off *= 2) {
-      top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], off));
-      top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], off));
-    }
-    if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {  // the maximum moved
+      for (int off = 4; off < kWarpSize; off *= 2) {
+        top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], off));
+        top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], off));
+      }
       const float al[2] = {exp2_approx(m[0] - top[0]), exp2_approx(m[1] - top[1])};
       l[0] *= al[0];
       l[1] *= al[1];
@@ -298,12 +348,25 @@ __global__ void __launch_bounds__(kWarps * kWarpSize) decode_attention_fp8_kerne
       }
       const uint32_t b0 = transpose8x8_b16(pack_f16x2(p[0], p[1]));  // rows 2t, 2t + 1 of head g
       const uint32_t b1 = transpose8x8_b16(pack_f16x2(p[2], p[3]));  // and + 8
+      uint32_t v[4][D / 32];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 16 * i + 8 * (e >> 1) + 2 * t + (e & 1);
+        const uint32_t at = tile + Loader<D>::kTileBytes;
+        if constexpr (D == 128) {
+          const uint4 x = lds128(at + tile_at<D>(r, g));
+          v[e][0] = x.x, v[e][1] = x.y, v[e][2] = x.z, v[e][3] = x.w;
+        } else {
+          const uint2 x = lds64(at + tile_at<D>(r, g >> 1) + 8 * (g & 1));
+          v[e][0] = x.x, v[e][1] = x.y;
+        }
+      }
 #pragma unroll
       for (int w = 0; w < D / 32; ++w) {
-        const uint32_t lo0 = __byte_perm(v[i][0].w[w], v[i][1].w[w], 0x5140);
-        const uint32_t hi0 = __byte_perm(v[i][0].w[w], v[i][1].w[w], 0x7362);
-        const uint32_t lo1 = __byte_perm(v[i][2].w[w], v[i][3].w[w], 0x5140);
-        const uint32_t hi1 = __byte_perm(v[i][2].w[w], v[i][3].w[w], 0x7362);
+        const uint32_t lo0 = __byte_perm(v[0][w], v[1][w], 0x5140);
+        const uint32_t hi0 = __byte_perm(v[0][w], v[1][w], 0x7362);
+        const uint32_t lo1 = __byte_perm(v[2][w], v[3][w], 0x5140);
+        const uint32_t hi1 = __byte_perm(v[2][w], v[3][w], 0x7362);
         mma_16816_f16(acc[2 * w], e4m3_to_f16x2_lo(lo0), e4m3_to_f16x2_hi(lo0),
                       e4m3_to_f16x2_lo(lo1), e4m3_to_f16x2_hi(lo1), b0, b1);
         mma_16816_f16(acc[2 * w + 1], e4m3_to_f16x2_lo(hi0), e4m3_to_f16x2_hi(hi0),
@@ -311,123 +374,514 @@ __global__ void __launch_bounds__(kWarps * kWarpSize) decode_attention_fp8_kerne
       }
     }
   }
-#pragma unroll
-  for (int off = 4; off < kWarpSize; off *= 2) {
-    l[0] += __shfl_xor_sync(0xffffffffu, l[0], off);
-    l[1] += __shfl_xor_sync(0xffffffffu, l[1], off);
-  }
-  // O^T element (dim, head): m-tile i holds dims g * D / 8 + 2 i (elements 0, 1: heads 2t, 2t + 1)
-  // and + 1 (elements 2, 3)
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    if (2 * t + h < heads) {
-      if (g == 0) {
-        warp_m[warp][2 * t + h] = m[h];
-        warp_l[warp][2 * t + h] = l[h];
-      }
-      float* dst = shared + (warp * heads + 2 * t + h) * D + g * (D / 8);
-#pragma unroll
-      for (int i = 0; i < kTiles; ++i) {
-        *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(acc[i][h], acc[i][2 + h]);
-      }
-    }
-  }
-  __syncthreads();
-  // the warps' (max, sum, partial) merged into the CTA's
-  if (threadIdx.x < heads) {
-    const int h = threadIdx.x;
-    float mx = warp_m[0][h];
-#pragma unroll
-    for (int w = 1; w < kWarps; ++w) mx = fmaxf(mx, warp_m[w][h]);
-    float ls = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) ls += warp_l[w][h] * exp2_approx(warp_m[w][h] - mx);
-    m_sm[h] = mx;
-    l_sm[h] = ls;
-  }
-  for (int idx = threadIdx.x; idx < heads * D; idx += kThreads) {
-    const int h = idx / D;
-    float mx = warp_m[0][h];
-#pragma unroll
-    for (int w = 1; w < kWarps; ++w) mx = fmaxf(mx, warp_m[w][h]);
-    float o = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) o += shared[w * heads * D + idx] * exp2_approx(warp_m[w][h] - mx);
-    part[idx] = o;
-  }
-  __syncthreads();
 
-  __nv_bfloat16* out =
-      static_cast<__nv_bfloat16*>(a.out) + (b * a.num_heads + head0) * static_cast<int64_t>(D);
-  if (a.splits == 1) {
-    for (int idx = threadIdx.x; idx < heads * D; idx += kThreads) {
-      const float ls = l_sm[idx / D];
-      out[idx] = __float2bfloat16_rn(ls == 0.0f ? 0.0f : part[idx] / ls);
+  // l of the whole warp.
+  __device__ __forceinline__ void reduce() {
+#pragma unroll
+    for (int off = 4; off < kWarpSize; off *= 2) {
+      l[0] += __shfl_xor_sync(0xffffffffu, l[0], off);
+      l[1] += __shfl_xor_sync(0xffffffffu, l[1], off);
     }
-    return;
   }
-  // CTA r of the cluster combines and writes output elements [r * per, (r + 1) * per)
-  cluster_sync_all();
-  const int per = heads * D / a.splits;
-  const int first = static_cast<int>(cluster_rank()) * per;
-  for (int idx = first + threadIdx.x; idx < first + per; idx += kThreads) {
-    const int h = idx / D;
-    float mr[kMaxSplits], lr[kMaxSplits], pr[kMaxSplits];
-#pragma unroll
-    for (int r = 0; r < kMaxSplits; ++r) {
-      if (r < a.splits) {
-        mr[r] = ld_remote_f32(&m_sm[h], r);
-        lr[r] = ld_remote_f32(&l_sm[h], r);
-        pr[r] = ld_remote_f32(&part[idx], r);
-      }
-    }
-    float mx = mr[0];
-#pragma unroll
-    for (int r = 1; r < kMaxSplits; ++r) {
-      if (r < a.splits) mx = fmaxf(mx, mr[r]);
-    }
-    float o = 0.0f, ls = 0.0f;
-#pragma unroll
-    for (int r = 0; r < kMaxSplits; ++r) {
-      if (r < a.splits) {
-        const float w = exp2_approx(mr[r] - mx);
-        o += w * pr[r];
-        ls += w * lr[r];
-      }
-    }
-    out[idx] = __float2bfloat16_rn(ls == 0.0f ? 0.0f : o / ls);
+};
+
+// ------------------------------------------------------------------------------------- by lines
+
+// A run of steps of one item.
+struct Segment {
+  int b;
+  int sub;    // KV head * groups + group of query heads
+  int first;  // its first step in the item
+  int n;      // its steps
+  int steps;  // the item's
+  int len;
+  int left;   // steps of the share from this segment on
+};
+
+// The line as every warp sees it.
+struct Line {
+  int total;   // steps
+  int shares;  // no more than steps, so that none is empty
+  int base, extra;  // steps of a share, and how many shares have one more
+  int b0;      // the share's first request; lane i holds the length of request b0 + i
+  int len;
+
+  __device__ __forceinline__ int begin(int c) const { return c * base + min(c, extra); }
+  // The first share that begins at step `at` or behind it.
+  __device__ __forceinline__ int first_from(int at) const {
+    const int wide = extra * (base + 1);
+    return at <= wide ? (at + base) / (base + 1) : extra + (at - wide + base - 1) / base;
   }
-  cluster_sync_all();  // every CTA's shared memory stays valid until the others have read it
+};
+
+__device__ __forceinline__ int length_of(const AttnArgs& a, const Line& line, int b) {
+  const int held = __shfl_sync(0xffffffffu, line.len, (b - line.b0) & (kWarpSize - 1));
+  return b - line.b0 < kWarpSize ? held : clamp_len(a, __ldg(a.seq_lens + b));
 }
 
-template <int D, int kWarps>
-int launch_attention(const AttnArgs& a, int64_t blocks, int device, cudaStream_t stream) {
-  const int heads = a.group < kGroup ? a.group : kGroup;
-  const size_t smem = static_cast<size_t>(kWarps + 1) * heads * D * 4;
-  const auto kernel = decode_attention_fp8_kernel<D, kWarps>;
-  if (blocks_per_sm(reinterpret_cast<const void*>(kernel), kWarps * kWarpSize, smem, device) <= 0) {
-    return SVLLM_ERR_CUDA;
+// The segment after s; s.left tells whether there is one. Every lane of a warp.
+__device__ __forceinline__ void next_segment(const AttnArgs& a, const Line& line, Segment& s) {
+  s.left -= s.n;
+  s.first = 0;
+  if (++s.sub == a.num_kv_heads * a.groups) {
+    s.sub = 0;
+    ++s.b;
+    if (s.left > 0) {
+      s.len = length_of(a, line, s.b);
+      s.steps = item_steps(s.len);
+    }
   }
-  return launch_serialized(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kWarps * kWarpSize),
-                           smem, stream, static_cast<unsigned>(a.splits), a);
+  s.n = min(s.steps, s.left);
+}
+
+// Share c of the line: its first segment. A lane takes a run of requests.
+__device__ __forceinline__ Segment first_segment(const AttnArgs& a, int c, Line& line) {
+  const int lane = static_cast<int>(threadIdx.x) % kWarpSize;
+  const int subs = a.num_kv_heads * a.groups;
+  const int per = (a.num_seqs + kWarpSize - 1) / kWarpSize;
+  const int begin = min(a.num_seqs, lane * per), end = min(a.num_seqs, begin + per);
+  int sum = 0, len = 0;
+  bool bad = false;
+#pragma unroll 4
+  for (int b = begin; b < end; ++b) {
+    const int n = __ldg(a.seq_lens + b);
+    bad |= n < 0 || n > a.max_rows;
+    len = clamp_len(a, n);
+    sum += item_steps(len) * subs;
+  }
+  if (bad && c == 0) raise_error(a.err, kErrBadIndex);
+  int scan = sum;
+#pragma unroll
+  for (int off = 1; off < kWarpSize; off *= 2) {
+    const int up = __shfl_up_sync(0xffffffffu, scan, off);
+    if (lane >= off) scan += up;
+  }
+  line.total = __shfl_sync(0xffffffffu, scan, kWarpSize - 1);
+  line.shares = min(a.shares, (line.total + kMinShare - 1) / kMinShare);
+  line.base = line.total / line.shares;
+  line.extra = line.total - line.base * line.shares;
+  Segment s{};
+  if (c >= line.shares) return s;
+  const int lo = line.begin(c);
+  // the lane whose requests hold the share's first step walks them
+  int found = begin, off = lo - (scan - sum);
+  const bool mine = off >= 0 && off < sum;
+  if (mine && per > 1) {
+    for (;; ++found) {
+      const int n = item_steps(clamp_len(a, __ldg(a.seq_lens + found))) * subs;
+      if (off < n) break;
+      off -= n;
+    }
+  }
+  const int owner = __ffs(static_cast<int>(__ballot_sync(0xffffffffu, mine))) - 1;
+  s.b = __shfl_sync(0xffffffffu, found, owner);
+  off = __shfl_sync(0xffffffffu, off, owner);
+  if (per == 1) {  // a lane holds a request's length already
+    line.b0 = 0;
+    line.len = len;
+  } else {
+    line.b0 = s.b;
+    line.len = s.b + lane < a.num_seqs ? clamp_len(a, __ldg(a.seq_lens + s.b + lane)) : 0;
+  }
+  s.len = length_of(a, line, s.b);
+  s.steps = item_steps(s.len);
+  s.sub = off / s.steps;
+  s.first = off - s.sub * s.steps;
+  s.left = line.begin(c + 1) - lo;
+  s.n = min(s.steps - s.first, s.left);
+  return s;
 }
 
 template <int D>
-int dispatch(const AttnArgs& a, int64_t blocks, int64_t split_steps, int device,
-             cudaStream_t stream) {
-  const int64_t sms = sm_count(device);
-  if (blocks <= sms && split_steps >= 8) return launch_attention<D, 8>(a, blocks, device, stream);
-  return launch_attention<D, 4>(a, blocks, device, stream);
+__global__ void __launch_bounds__(kLineWarps * kWarpSize, 1) decode_attention_fp8_lines(
+    const __grid_constant__ AttnArgs a) {
+  grid_dependency_sync();
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x / kWarpSize;
+  const int lane = threadIdx.x % kWarpSize;
+  const int g = lane >> 2;
+  const int t = lane & 3;
+  const int held_heads = min(a.group, kGroup);
+  const uint32_t ring = smem_addr(smem) + warp * kStages * Loader<D>::kStageBytes;
+
+  // neighbouring shares on different SMs, so that few shares find many SMs
+  const int share = warp * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x);
+  Line line;
+  Segment seg = first_segment(a, share, line);
+  if (seg.left <= 0) return;
+
+  // ---- loads: `ahead` walks the share in front of the products
+  Segment ahead = seg;
+  int ahead_step = 0;
+  int block = Loader<D>::block_of(a, ahead.b, ahead.first, ahead.len);
+  uint32_t k_scales[kStages - 1], v_scales[kStages - 1];  // of the stages in flight
+  const auto load = [&](int stage, uint32_t& k_scale, uint32_t& v_scale) {
+    if (ahead.left > 0) {
+      Loader<D>::issue(a, ring + stage * Loader<D>::kStageBytes, block, ahead.sub / a.groups,
+                       ahead.first + ahead_step, ahead.len, k_scale, v_scale);
+      if (++ahead_step == ahead.n) {
+        next_segment(a, line, ahead);
+        ahead_step = 0;
+      }
+      if (ahead.left > 0) {
+        block = Loader<D>::block_of(a, ahead.b, ahead.first + ahead_step, ahead.len);
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) load(i, k_scales[i], v_scales[i]);
+
+  Queries<D> q;
+  Sums<D> sums;
+  int stage = 0, at = 0;  // `at`: the step of the segment
+  while (true) {
+    const Heads heads(a, seg.sub);
+    if (at == 0) {  // rows are on their way meanwhile
+      const uint8_t* src = static_cast<const uint8_t*>(a.q) +
+                           (seg.b * a.q_stride + static_cast<int64_t>(heads.first + g) * D) * 2;
+      q.set(a.scale_log2, [&](int i) {
+        return g < heads.count ? ld_global_nc_v4(src + i * 16) : make_uint4(0, 0, 0, 0);
+      });
+      sums.clear();
+    }
+    cp_async_wait<kStages - 2>();
+    __syncwarp();  // every lane's copies have landed, and every lane is done with the stage before
+    const uint32_t scales = k_scales[0] | (v_scales[0] << 8);
+#pragma unroll
+    for (int i = 0; i + 1 < kStages - 1; ++i) {
+      k_scales[i] = k_scales[i + 1];
+      v_scales[i] = v_scales[i + 1];
+    }
+    load(stage == 0 ? kStages - 1 : stage - 1, k_scales[kStages - 2], v_scales[kStages - 2]);
+    sums.step(ring + stage * Loader<D>::kStageBytes, scales,
+              seg.len - (seg.first + at) * kStepRows, q);
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+    if (++at < seg.n) continue;
+
+    // ---- the segment's end: the item's output, or a part
+    sums.reduce();
+    const bool cut = seg.n < seg.steps;
+    const int64_t out0 = (static_cast<int64_t>(seg.b) * a.num_heads + heads.first) * D;
+    if (seg.first == 0 && lane == 0) {
+      // the item ends behind this share by the steps that it lacks
+      const int end = line.begin(share + 1) + seg.steps - seg.n;
+      a.table[static_cast<int64_t>(seg.b) * a.num_kv_heads * a.groups + seg.sub] = {
+          share, cut ? line.first_from(end) - share : 1};
+    }
+    const int64_t part = (2 * static_cast<int64_t>(share) + (seg.first == 0 ? 1 : 0)) * held_heads;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int head = 2 * t + h;
+      if (head >= heads.count) continue;
+      if (cut) {
+        if (g == 0) a.part_ml[part + head] = make_float2(sums.m[h], sums.l[h]);
+        float4* dst = reinterpret_cast<float4*>(a.part_acc + (part + head) * D + g * (D / 8));
+#pragma unroll
+        for (int i = 0; i < Sums<D>::kTiles; i += 2) {
+          dst[i / 2] = make_float4(sums.acc[i][h], sums.acc[i][2 + h], sums.acc[i + 1][h],
+                                   sums.acc[i + 1][2 + h]);
+        }
+      } else {
+        const float f = sums.l[h] == 0.0f ? 0.0f : 1.0f / sums.l[h];
+        uint32_t w[Sums<D>::kTiles];
+#pragma unroll
+        for (int i = 0; i < Sums<D>::kTiles; ++i) {
+          w[i] = pack_bf16x2(sums.acc[i][h] * f, sums.acc[i][2 + h] * f);
+        }
+        uint8_t* dst = static_cast<uint8_t*>(a.out) + (out0 + head * D + g * (D / 8)) * 2;
+#pragma unroll
+        for (int i = 0; i < Sums<D>::kTiles; i += 4) {
+          st_global_v4(dst + i * 4, make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]));
+        }
+      }
+    }
+    next_segment(a, line, seg);
+    at = 0;
+    if (seg.left <= 0) break;
+  }
+}
+
+// Joins the parts of the items that were cut: blockIdx.x the item, `spread` warps for each 32 of its
+// outputs. A lane takes four dims of every 4 spread-th part, kJoinBatch of them in flight; its
+// fellows' sums come by shuffles, the other warps' through shared memory. The order is fixed by the
+// sizes, so results repeat.
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads) decode_attention_fp8_join(
+    const __grid_constant__ AttnArgs a, int spread) {
+  grid_dependency_sync();
+  constexpr int kWarps = kJoinThreads / kWarpSize;
+  constexpr int kRuns = D / 32;  // of 32 dims in a head
+  __shared__ float4 others[kWarps][8];
+  __shared__ float2 others_ml[kWarps];
+  const JoinEntry entry = a.table[blockIdx.x];
+  if (entry.parts <= 1) return;
+  const int subs = a.num_kv_heads * a.groups;
+  const int b = static_cast<int>(blockIdx.x) / subs;
+  const Heads heads(a, static_cast<int>(blockIdx.x) - b * subs);
+  const int held_heads = min(a.group, kGroup);
+  const int warp = threadIdx.x / kWarpSize, lane = threadIdx.x % kWarpSize;
+  const int mate = warp % spread;  // this warp's place among those of its run
+  const int run = (static_cast<int>(blockIdx.y) * kWarps + warp) / spread;
+  const int head = run / kRuns;
+  const bool real = head < heads.count;
+  const int d = run % kRuns * 32 + lane % 8 * 4;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float m = -FLT_MAX, l = 0.0f;
+  const int step = 4 * spread;
+  for (int p0 = lane / 8 * spread + mate; real && p0 < entry.parts; p0 += step * kJoinBatch) {
+    float2 ml[kJoinBatch];
+    float4 x[kJoinBatch];
+#pragma unroll
+    for (int i = 0; i < kJoinBatch; ++i) {
+      const int p = p0 + i * step;
+      ml[i] = make_float2(-FLT_MAX, 0.0f);
+      x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (p < entry.parts) {
+        // the first part is the one that begins the item; the others continue it
+        const int64_t at =
+            (2 * static_cast<int64_t>(entry.share + p) + (p == 0 ? 1 : 0)) * held_heads + head;
+        ml[i] = a.part_ml[at];
+        x[i] = *reinterpret_cast<const float4*>(a.part_acc + at * D + d);
+      }
+    }
+    float mx = m;
+#pragma unroll
+    for (int i = 0; i < kJoinBatch; ++i) mx = fmaxf(mx, ml[i].x);
+    const float f = exp2_approx(m - mx);
+    l *= f;
+    acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+#pragma unroll
+    for (int i = 0; i < kJoinBatch; ++i) {
+      const float w = exp2_approx(ml[i].x - mx);
+      l = fmaf(ml[i].y, w, l);
+      acc = make_float4(fmaf(x[i].x, w, acc.x), fmaf(x[i].y, w, acc.y), fmaf(x[i].z, w, acc.z),
+                        fmaf(x[i].w, w, acc.w));
+    }
+    m = mx;
+  }
+#pragma unroll
+  for (int off = 8; off < kWarpSize; off *= 2) {
+    const float mx = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+    const float f = exp2_approx(m - mx);
+    m = mx;
+    l *= f;
+    acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+    l += __shfl_xor_sync(0xffffffffu, l, off);
+    acc.x += __shfl_xor_sync(0xffffffffu, acc.x, off);
+    acc.y += __shfl_xor_sync(0xffffffffu, acc.y, off);
+    acc.z += __shfl_xor_sync(0xffffffffu, acc.z, off);
+    acc.w += __shfl_xor_sync(0xffffffffu, acc.w, off);
+  }
+  if (spread > 1) {
+    if (lane < 8) {
+      others[warp][lane] = acc;
+      if (lane == 0) others_ml[warp] = make_float2(m, l);
+    }
+    __syncthreads();
+    if (mate != 0) return;
+    for (int w = warp + 1; w < warp + spread; ++w) {
+      const float2 ml = others_ml[w];
+      const float4 x = others[w][lane % 8];
+      const float mx = fmaxf(m, ml.x);
+      const float f0 = exp2_approx(m - mx), f1 = exp2_approx(ml.x - mx);
+      m = mx;
+      l = l * f0 + ml.y * f1;
+      acc = make_float4(acc.x * f0 + x.x * f1, acc.y * f0 + x.y * f1, acc.z * f0 + x.z * f1,
+                        acc.w * f0 + x.w * f1);
+    }
+  }
+  if (lane < 8 && real) {
+    const float r = l == 0.0f ? 0.0f : 1.0f / l;
+    uint8_t* dst = static_cast<uint8_t*>(a.out) +
+                   ((static_cast<int64_t>(b) * a.num_heads + heads.first + head) * D + d) * 2;
+    *reinterpret_cast<uint2*>(dst) =
+        make_uint2(pack_bf16x2(acc.x * r, acc.y * r), pack_bf16x2(acc.z * r, acc.w * r));
+  }
+}
+
+// ------------------------------------------------------------------------------------- by items
+
+template <int D>
+__global__ void __launch_bounds__(kItemWarps * kWarpSize, 1) decode_attention_fp8_items(
+    const __grid_constant__ AttnArgs a) {
+  grid_dependency_sync();
+  constexpr int kThreads = kItemWarps * kWarpSize;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float warp_m[kItemWarps][kGroup], warp_l[kItemWarps][kGroup];
+  const int warp = threadIdx.x / kWarpSize;
+  const int lane = threadIdx.x % kWarpSize;
+  const int g = lane >> 2;
+  const int t = lane & 3;
+  const int subs = a.num_kv_heads * a.groups;
+  const int b = static_cast<int>(blockIdx.x) / subs, sub = static_cast<int>(blockIdx.x) % subs;
+  const Heads heads(a, sub);
+  const uint32_t ring = smem_addr(smem) + warp * kStages * Loader<D>::kStageBytes;
+
+  const int n = __ldg(a.seq_lens + b);
+  if (threadIdx.x == 0 && (n < 0 || n > a.max_rows)) raise_error(a.err, kErrBadIndex);
+  const int len = clamp_len(a, n), steps = item_steps(len);
+
+  int block = Loader<D>::block_of(a, b, warp, len);
+  uint32_t k_scales[kStages], v_scales[kStages];
+  const auto load = [&](int stage, int step, uint32_t& k_scale, uint32_t& v_scale) {
+    k_scale = v_scale = kScaleBias;
+    if (step < steps) {
+      Loader<D>::issue(a, ring + stage * Loader<D>::kStageBytes, block, sub / a.groups, step, len,
+                       k_scale, v_scale);
+      block = Loader<D>::block_of(a, b, step + kItemWarps, len);
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages; ++i) {
+    load(i, warp + i * kItemWarps, k_scales[i], v_scales[i]);
+  }
+  Queries<D> q;
+  const uint8_t* src = static_cast<const uint8_t*>(a.q) +
+                       (b * a.q_stride + static_cast<int64_t>(heads.first + g) * D) * 2;
+  q.set(a.scale_log2, [&](int i) {
+    return g < heads.count ? ld_global_nc_v4(src + i * 16) : make_uint4(0, 0, 0, 0);
+  });
+  Sums<D> sums;
+  sums.clear();
+  int stage = 0;
+  for (int step = warp; step < steps; step += kItemWarps) {
+    cp_async_wait<kStages - 1>();
+    __syncwarp();
+    sums.step(ring + stage * Loader<D>::kStageBytes, k_scales[0] | (v_scales[0] << 8),
+              len - step * kStepRows, q);
+#pragma unroll
+    for (int i = 0; i + 1 < kStages; ++i) {
+      k_scales[i] = k_scales[i + 1];
+      v_scales[i] = v_scales[i + 1];
+    }
+    __syncwarp();  // every lane is done with the stage
+    load(stage, step + kStages * kItemWarps, k_scales[kStages - 1], v_scales[kStages - 1]);
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+  }
+  sums.reduce();
+  cp_async_wait<0>();
+  __syncthreads();  // the rings are free
+  float* accs = reinterpret_cast<float*>(smem);  // [warps][heads][D]
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int head = 2 * t + h;
+    if (head >= heads.count) continue;
+    if (g == 0) {
+      warp_m[warp][head] = sums.m[h];
+      warp_l[warp][head] = sums.l[h];
+    }
+    float4* dst = reinterpret_cast<float4*>(accs + (warp * heads.count + head) * D + g * (D / 8));
+#pragma unroll
+    for (int i = 0; i < Sums<D>::kTiles; i += 2) {
+      dst[i / 2] = make_float4(sums.acc[i][h], sums.acc[i][2 + h], sums.acc[i + 1][h],
+                               sums.acc[i + 1][2 + h]);
+    }
+  }
+  __syncthreads();
+  const int64_t out0 = (static_cast<int64_t>(b) * a.num_heads + heads.first) * D;
+  for (int idx = threadIdx.x; idx < heads.count * D; idx += kThreads) {
+    const int h = idx / D;
+    float mx = warp_m[0][h];
+#pragma unroll
+    for (int w = 1; w < kItemWarps; ++w) mx = fmaxf(mx, warp_m[w][h]);
+    float o = 0.0f, ls = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kItemWarps; ++w) {
+      const float f = exp2_approx(warp_m[w][h] - mx);
+      o = fmaf(accs[w * heads.count * D + idx], f, o);
+      ls = fmaf(warp_l[w][h], f, ls);
+    }
+    static_cast<__nv_bfloat16*>(a.out)[out0 + idx] =
+        __float2bfloat16_rn(ls == 0.0f ? 0.0f : o / ls);
+  }
+}
+
+int64_t line_shares(int device) { return static_cast<int64_t>(sm_count(device)) * kLineWarps; }
+
+template <int D>
+int launch_items(const AttnArgs& a, int64_t items, int device, cudaStream_t stream) {
+  const size_t smem = static_cast<size_t>(kItemWarps) * kStages * Loader<D>::kStageBytes;
+  static_assert(kStages * Loader<D>::kStageBytes >= kGroup * D * 4, "the merge takes the rings");
+  const auto kernel = decode_attention_fp8_items<D>;
+  if (blocks_per_sm(reinterpret_cast<const void*>(kernel), kItemWarps * kWarpSize, smem, device) <=
+      0) {
+    return SVLLM_ERR_CUDA;
+  }
+  return launch(kernel, dim3(static_cast<unsigned>(items)), dim3(kItemWarps * kWarpSize), smem,
+                stream, 1u, a);
+}
+
+template <int D>
+int launch_lines(const AttnArgs& a, int64_t items, int device, cudaStream_t stream) {
+  const int heads = a.group < kGroup ? a.group : kGroup;
+  const size_t smem = static_cast<size_t>(kLineWarps) * kStages * Loader<D>::kStageBytes;
+  const auto kernel = decode_attention_fp8_lines<D>;
+  if (blocks_per_sm(reinterpret_cast<const void*>(kernel), kLineWarps * kWarpSize, smem, device) <=
+      0) {
+    return SVLLM_ERR_CUDA;
+  }
+  const unsigned sms = static_cast<unsigned>(sm_count(device));
+  const int status =
+      launch(kernel, dim3(sms), dim3(kLineWarps * kWarpSize), smem, stream, 1u, a);
+  if (status != SVLLM_OK) return status;
+  // up to four parts a lane, as far as the warps of a CTA go
+  const int64_t parts = line_shares(device) / items + 2;
+  int spread = 1;
+  while (spread < kJoinThreads / kWarpSize && parts > 16 * spread) spread *= 2;
+  const int runs = heads * (D / 32) * spread;
+  const unsigned slices = static_cast<unsigned>((runs * kWarpSize + kJoinThreads - 1) / kJoinThreads);
+  return launch(decode_attention_fp8_join<D>, dim3(static_cast<unsigned>(items), slices),
+                dim3(kJoinThreads), 0, stream, 1u, a, spread);
+}
+
+constexpr int64_t kMaxSeqs = 1 << 20, kMaxHeads = 1 << 16;
+
+// The parts of the workspace by lines.
+struct Workspace {
+  int64_t items, ml, acc, bytes;
+  Workspace(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+            int device) {
+    const int64_t group = num_heads / num_kv_heads;
+    const int64_t held = group < kGroup ? group : kGroup;
+    items = num_seqs * num_kv_heads * ((group + kGroup - 1) / kGroup);
+    ml = round_up(items * static_cast<int64_t>(sizeof(JoinEntry)), 256);
+    acc = ml + round_up(2 * line_shares(device) * held * static_cast<int64_t>(sizeof(float2)), 256);
+    bytes = acc + 2 * line_shares(device) * held * head_dim * static_cast<int64_t>(sizeof(float));
+  }
+};
+
+bool by_items(int64_t max_rows, int64_t items, int device) {
+  return max_rows <= kItemRows && items <= 2 * sm_count(device);
 }
 
 }  // namespace
 }  // namespace svllm::k
 
+extern "C" int svllm_decode_attention_fp8_workspace_bytes(int64_t num_seqs, int64_t num_heads,
+                                                          int64_t num_kv_heads, int64_t head_dim,
+                                                          int64_t* bytes) {
+  using namespace svllm::k;
+  if (bytes == nullptr || num_seqs < 0 || num_heads <= 0 || num_kv_heads <= 0 ||
+      num_heads % num_kv_heads != 0) {
+    return SVLLM_ERR_INVALID_ARGUMENT;
+  }
+  if (head_dim != 64 && head_dim != 128) return SVLLM_ERR_UNSUPPORTED;
+  if (num_seqs >= kMaxSeqs || num_heads > kMaxHeads) return SVLLM_ERR_TOO_LARGE;
+  int device;
+  if (current_device(&device) != SVLLM_OK) return SVLLM_ERR_CUDA;
+  const Workspace w(num_seqs, num_heads, num_kv_heads, head_dim, device);
+  *bytes = w.bytes;
+  return SVLLM_OK;
+}
+
 extern "C" int svllm_decode_attention_fp8_bf16(
     void* out, const void* q, int64_t q_token_stride, const void* k_cache, const void* v_cache,
     const void* k_scale, const void* v_scale, int64_t num_blocks, int64_t block_size,
     const int32_t* block_tables, int64_t max_blocks, const int32_t* seq_lens, int64_t num_seqs,
-    int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, float scale, svllm_stream stream) {
+    int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, float scale, void* workspace,
+    int64_t workspace_bytes, svllm_stream stream) {
   using namespace svllm::k;
   if (num_seqs < 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 ||
       block_size <= 0 || max_blocks < 0 || num_blocks <= 0 || head_dim <= 0 ||
@@ -443,18 +897,24 @@ extern "C" int svllm_decode_attention_fp8_bf16(
   constexpr int64_t kInt = int64_t{1} << 31;
   const int64_t group = num_heads / num_kv_heads;
   const int64_t groups = (group + kGroup - 1) / kGroup;
-  if (num_heads > (1 << 16) || block_size >= (1 << 20) || max_blocks >= kInt ||
+  if (num_heads > kMaxHeads || block_size >= (1 << 20) || max_blocks >= kInt ||
       max_blocks * block_size >= kInt - kStepRows || num_blocks >= kInt ||
-      num_blocks * block_size >= kInt || num_seqs >= kInt ||
-      num_seqs * num_kv_heads * groups * kMaxSplits >= kInt) {
+      num_blocks * block_size >= kInt || num_seqs >= kMaxSeqs ||
+      // the line's steps, were every request as long as its table
+      num_seqs * num_kv_heads * groups * (max_blocks * block_size / kStepRows + 1) >= kInt) {
     return SVLLM_ERR_TOO_LARGE;
   }
-  if ((head_dim != 64 && head_dim != 128) || !aligned16(q) || !aligned16(k_cache) ||
+  if ((head_dim != 64 && head_dim != 128) || !aligned16(out) || !aligned16(q) || !aligned16(k_cache) ||
       !aligned16(v_cache) || q_token_stride % 8 != 0) {
     return SVLLM_ERR_UNSUPPORTED;
   }
   int device;
   if (current_device(&device) != SVLLM_OK) return SVLLM_ERR_CUDA;
+  const Workspace w(num_seqs, num_heads, num_kv_heads, head_dim, device);
+  const bool direct = by_items(max_blocks * block_size, w.items, device);
+  if (!direct && (workspace == nullptr || workspace_bytes < w.bytes || !aligned16(workspace))) {
+    return SVLLM_ERR_INVALID_ARGUMENT;
+  }
   AttnArgs a{};
   a.err = library_error_word(device);
   if (a.err == nullptr) return SVLLM_ERR_CUDA;
@@ -477,16 +937,17 @@ extern "C" int svllm_decode_attention_fp8_bf16(
   a.group = static_cast<int>(group);
   a.groups = static_cast<int>(groups);
   a.scale_log2 = static_cast<float>(static_cast<double>(scale) / std::log(2.0));
-  // Split the rows until there are about two CTAs per SM, never below 64 rows per split.
-  const int64_t items = num_seqs * num_kv_heads * groups;
-  int64_t splits = (2 * sm_count(device) + items - 1) / items;
-  const int64_t by_length = (a.max_rows + 63) / 64;
-  splits = splits < by_length ? splits : by_length;
-  int pow2 = 1;
-  while (pow2 * 2 <= splits && pow2 * 2 <= kMaxSplits) pow2 *= 2;
-  a.splits = pow2;
-  const int64_t split_steps = ((a.max_rows + kStepRows - 1) / kStepRows + pow2 - 1) / pow2;
+  a.num_seqs = static_cast<int>(num_seqs);
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return head_dim == 128 ? dispatch<128>(a, items * pow2, split_steps, device, s)
-                         : dispatch<64>(a, items * pow2, split_steps, device, s);
+  if (direct) {
+    return head_dim == 128 ? launch_items<128>(a, w.items, device, s)
+                           : launch_items<64>(a, w.items, device, s);
+  }
+  a.shares = static_cast<int>(line_shares(device));
+  uint8_t* base = static_cast<uint8_t*>(workspace);
+  a.table = reinterpret_cast<JoinEntry*>(base);
+  a.part_ml = reinterpret_cast<float2*>(base + w.ml);
+  a.part_acc = reinterpret_cast<float*>(base + w.acc);
+  return head_dim == 128 ? launch_lines<128>(a, w.items, device, s)
+                         : launch_lines<64>(a, w.items, device, s);
 }

@@ -1,4 +1,6 @@
 // CUDA side of ops::cache_read_fp8 and ops::decode_attention_fp8: thin LibTorch -> C ABI shims.
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -32,6 +34,12 @@ void decode_attention_fp8(const at::Tensor& out, const at::Tensor& q, const at::
   if (requests == 0) return;
   const c10::cuda::CUDAGuard device_guard(q.device());
   const auto stream = reinterpret_cast<svllm_stream>(c10::cuda::getCurrentCUDAStream().stream());
+  int64_t bytes = 0;
+  detail::check_status("decode_attention_fp8",
+                       svllm_decode_attention_fp8_workspace_bytes(
+                           requests, heads, k_cache.size(2), dim, &bytes));
+  // from the caching allocator per call: calls on other streams, and captured graphs, get their own
+  const c10::DataPtr workspace = c10::cuda::CUDACachingAllocator::get()->allocate(bytes);
   detail::check_status(
       "decode_attention_fp8",
       svllm_decode_attention_fp8_bf16(
@@ -40,7 +48,7 @@ void decode_attention_fp8(const at::Tensor& out, const at::Tensor& q, const at::
           v_scale.const_data_ptr(), k_cache.size(0), k_cache.size(1),
           block_tables.const_data_ptr<int32_t>(), block_tables.size(1),
           seq_lens.const_data_ptr<int32_t>(), requests, heads, k_cache.size(2), dim,
-          static_cast<float>(scale), stream));
+          static_cast<float>(scale), workspace.get(), bytes, stream));
 }
 
 }  // namespace svllm::ops::cuda_impl

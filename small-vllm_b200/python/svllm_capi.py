@@ -85,7 +85,8 @@ SIGNATURES = {
     "svllm_cache_read_fp8_bf16": [_P, _P, _P, _P, _P, _P, _I64, _I64, _P, _I64, _P, _I64, _I64,
                                   _I64, _P],
     "svllm_decode_attention_fp8_bf16": [_P, _P, _I64, _P, _P, _P, _P, _I64, _I64, _P, _I64, _P,
-                                        _I64, _I64, _I64, _I64, _F, _P],
+                                        _I64, _I64, _I64, _I64, _F, _P, _I64, _P],
+    "svllm_decode_attention_fp8_workspace_bytes": [_I64, _I64, _I64, _I64, _P],
     "svllm_read_device_error": [_I, _I, _P],
 }
 
