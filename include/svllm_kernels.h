@@ -487,7 +487,7 @@ int svllm_rope_cache_fp8_bf16(void* q, const void* k, const void* v, const void*
  * block_size, num_kv_heads, head_dim], row j of request s from slot block_tables[s][j / block_size]
  * * block_size + j % block_size for j < seq_lens[s], zeros behind. Seen as [num_seqs * max_blocks,
  * block_size, ...] the outputs are a paged bf16 cache in which page p of request s is block s *
- * max_blocks + p. A length outside [0, max_blocks * block_size] is clamped and a table entry
+ * max_blocks + p. k_out and v_out 32-byte aligned, else SVLLM_ERR_UNSUPPORTED. A length outside [0, max_blocks * block_size] is clamped and a table entry
  * outside the cache read as block 0, either with SVLLM_DEVERR_BAD_INDEX.
  */
 int svllm_cache_read_fp8_bf16(void* k_out, void* v_out, const void* k_cache, const void* v_cache,

@@ -73,7 +73,8 @@ def commit(pointer=P, **change):
     (read, {"k_out": None}, INVALID),
     (read, {"v_scale": None}, INVALID),
     (read, {"block_tables": None}, INVALID),
-    (read, {"num_seqs": 1 << 20, "max_blocks": 1 << 12}, TOO_LARGE),
+    (read, {"num_seqs": 1 << 24, "max_blocks": 1 << 12}, TOO_LARGE),
+    (read, {"max_blocks": 1 << 28}, TOO_LARGE),
     (read, {"block_size": 1 << 20}, TOO_LARGE),
     (read, {"head_dim": 96}, UNSUPPORTED),
     (read, {"v_out": P + 8}, UNSUPPORTED),
