@@ -53,7 +53,8 @@ constexpr int kStages = 2;       // of a warp's ring
 constexpr int kLineWarps = 8;    // of a CTA by lines, one per SM
 constexpr int kItemWarps = 8;    // of a CTA by items
 constexpr int kMinShare = 2;     // steps of a warp's share at least
-constexpr int64_t kItemRows = 512;  // by items up to this many rows of a table
+constexpr int kMaxSplits = 8;    // CTAs of an item: the portable cluster size
+constexpr int kItemSteps = 4;    // by items up to this many steps of a warp
 constexpr int kJoinThreads = 256;
 constexpr int kJoinBatch = 8;    // parts a thread of the join has in flight
 // The running maximum is moved only when a score passes it by kSlack, so that most steps need one
@@ -93,6 +94,7 @@ struct AttnArgs {
   int group;   // query heads per KV head
   int groups;  // items they are dealt to
   int shares;  // warps by lines
+  int splits;  // CTAs of an item, by items
   float scale_log2;
   int* err;
 };
@@ -709,20 +711,27 @@ __global__ void __launch_bounds__(kItemWarps * kWarpSize, 1) decode_attention_fp
   constexpr int kThreads = kItemWarps * kWarpSize;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float warp_m[kItemWarps][kGroup], warp_l[kItemWarps][kGroup];
+  __shared__ float split_m[kGroup], split_l[kGroup];
   const int warp = threadIdx.x / kWarpSize;
   const int lane = threadIdx.x % kWarpSize;
   const int g = lane >> 2;
   const int t = lane & 3;
   const int subs = a.num_kv_heads * a.groups;
-  const int b = static_cast<int>(blockIdx.x) / subs, sub = static_cast<int>(blockIdx.x) % subs;
+  const int item = static_cast<int>(blockIdx.x) / a.splits;
+  const int split = static_cast<int>(blockIdx.x) - item * a.splits;
+  const int b = item / subs, sub = item - b * subs;
   const Heads heads(a, sub);
   const uint32_t ring = smem_addr(smem) + warp * kStages * Loader<D>::kStageBytes;
 
   const int n = __ldg(a.seq_lens + b);
   if (threadIdx.x == 0 && (n < 0 || n > a.max_rows)) raise_error(a.err, kErrBadIndex);
-  const int len = clamp_len(a, n), steps = item_steps(len);
+  const int len = clamp_len(a, n);
+  // this split's steps, which the warps deal among them
+  const int of_split = (item_steps(len) + a.splits - 1) / a.splits;
+  const int steps = min(item_steps(len), (split + 1) * of_split);
+  const int begin = split * of_split + warp;
 
-  int block = Loader<D>::block_of(a, b, warp, len);
+  int block = Loader<D>::block_of(a, b, begin, len);
   uint32_t k_scales[kStages], v_scales[kStages];
   const auto load = [&](int stage, int step, uint32_t& k_scale, uint32_t& v_scale) {
     k_scale = v_scale = kScaleBias;
@@ -735,7 +744,7 @@ __global__ void __launch_bounds__(kItemWarps * kWarpSize, 1) decode_attention_fp
   };
 #pragma unroll
   for (int i = 0; i < kStages; ++i) {
-    load(i, warp + i * kItemWarps, k_scales[i], v_scales[i]);
+    load(i, begin + i * kItemWarps, k_scales[i], v_scales[i]);
   }
   Queries<D> q;
   const uint8_t* src = static_cast<const uint8_t*>(a.q) +
@@ -746,7 +755,7 @@ __global__ void __launch_bounds__(kItemWarps * kWarpSize, 1) decode_attention_fp
   Sums<D> sums;
   sums.clear();
   int stage = 0;
-  for (int step = warp; step < steps; step += kItemWarps) {
+  for (int step = begin; step < steps; step += kItemWarps) {
     cp_async_wait<kStages - 1>();
     __syncwarp();
     sums.step(ring + stage * Loader<D>::kStageBytes, k_scales[0] | (v_scales[0] << 8),
@@ -780,7 +789,9 @@ __global__ void __launch_bounds__(kItemWarps * kWarpSize, 1) decode_attention_fp
     }
   }
   __syncthreads();
-  const int64_t out0 = (static_cast<int64_t>(b) * a.num_heads + heads.first) * D;
+  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) +
+                       (static_cast<int64_t>(b) * a.num_heads + heads.first) * D;
+  float* part = accs + kItemWarps * heads.count * D;  // [heads][D], of the split
   for (int idx = threadIdx.x; idx < heads.count * D; idx += kThreads) {
     const int h = idx / D;
     float mx = warp_m[0][h];
@@ -793,9 +804,47 @@ __global__ void __launch_bounds__(kItemWarps * kWarpSize, 1) decode_attention_fp
       o = fmaf(accs[w * heads.count * D + idx], f, o);
       ls = fmaf(warp_l[w][h], f, ls);
     }
-    static_cast<__nv_bfloat16*>(a.out)[out0 + idx] =
-        __float2bfloat16_rn(ls == 0.0f ? 0.0f : o / ls);
+    if (a.splits == 1) {
+      out[idx] = __float2bfloat16_rn(ls == 0.0f ? 0.0f : o / ls);
+    } else {
+      part[idx] = o;
+      if (idx % D == 0) {
+        split_m[h] = mx;
+        split_l[h] = ls;
+      }
+    }
   }
+  if (a.splits == 1) return;
+  // The splits of an item are a thread-block cluster: each joins and writes a slice of the outputs
+  // from all of them, through distributed shared memory.
+  cluster_sync_all();
+  const int per = heads.count * D / a.splits;
+  for (int idx = split * per + threadIdx.x; idx < (split + 1) * per; idx += kThreads) {
+    const int h = idx / D;
+    float m[kMaxSplits], l[kMaxSplits], x[kMaxSplits];
+#pragma unroll
+    for (int r = 0; r < kMaxSplits; ++r) {
+      m[r] = -FLT_MAX;
+      l[r] = x[r] = 0.0f;
+      if (r < a.splits) {
+        m[r] = ld_remote_f32(&split_m[h], r);
+        l[r] = ld_remote_f32(&split_l[h], r);
+        x[r] = ld_remote_f32(&part[idx], r);
+      }
+    }
+    float mx = m[0];
+#pragma unroll
+    for (int r = 1; r < kMaxSplits; ++r) mx = fmaxf(mx, m[r]);
+    float o = 0.0f, ls = 0.0f;
+#pragma unroll
+    for (int r = 0; r < kMaxSplits; ++r) {
+      const float f = exp2_approx(m[r] - mx);
+      o = fmaf(x[r], f, o);
+      ls = fmaf(l[r], f, ls);
+    }
+    out[idx] = __float2bfloat16_rn(ls == 0.0f ? 0.0f : o / ls);
+  }
+  cluster_sync_all();  // every CTA's shared memory stays valid until the others have read it
 }
 
 int64_t line_shares(int device) { return static_cast<int64_t>(sm_count(device)) * kLineWarps; }
@@ -803,14 +852,15 @@ int64_t line_shares(int device) { return static_cast<int64_t>(sm_count(device)) 
 template <int D>
 int launch_items(const AttnArgs& a, int64_t items, int device, cudaStream_t stream) {
   const size_t smem = static_cast<size_t>(kItemWarps) * kStages * Loader<D>::kStageBytes;
-  static_assert(kStages * Loader<D>::kStageBytes >= kGroup * D * 4, "the merge takes the rings");
+  static_assert(kItemWarps * kStages * Loader<D>::kStageBytes >= (kItemWarps + 1) * kGroup * D * 4,
+                "the merge takes the rings");
   const auto kernel = decode_attention_fp8_items<D>;
   if (blocks_per_sm(reinterpret_cast<const void*>(kernel), kItemWarps * kWarpSize, smem, device) <=
       0) {
     return SVLLM_ERR_CUDA;
   }
-  return launch(kernel, dim3(static_cast<unsigned>(items)), dim3(kItemWarps * kWarpSize), smem,
-                stream, 1u, a);
+  return launch(kernel, dim3(static_cast<unsigned>(items * a.splits)),
+                dim3(kItemWarps * kWarpSize), smem, stream, static_cast<unsigned>(a.splits), a);
 }
 
 template <int D>
@@ -852,8 +902,18 @@ struct Workspace {
   }
 };
 
-bool by_items(int64_t max_rows, int64_t items, int device) {
-  return max_rows <= kItemRows && items <= 2 * sm_count(device);
+// CTAs of an item, by items; 0: by lines. `wave`: how many such CTAs run at a time.
+int item_splits(int64_t max_rows, int64_t items, int64_t wave) {
+  int splits = 1;
+  while (2 * splits <= kMaxSplits && 2 * splits * items <= wave &&
+         splits * kItemWarps * kStepRows < max_rows) {
+    splits *= 2;
+  }
+  const int64_t steps = (max_rows + splits * kItemWarps * kStepRows - 1) /
+                        (splits * kItemWarps * kStepRows);
+  const int64_t waves = (items * splits + wave - 1) / wave;
+  const bool fits = waves <= 2 && waves * (steps > 0 ? steps : 1) <= kItemSteps;
+  return fits ? splits : 0;
 }
 
 }  // namespace
@@ -911,8 +971,9 @@ extern "C" int svllm_decode_attention_fp8_bf16(
   int device;
   if (current_device(&device) != SVLLM_OK) return SVLLM_ERR_CUDA;
   const Workspace w(num_seqs, num_heads, num_kv_heads, head_dim, device);
-  const bool direct = by_items(max_blocks * block_size, w.items, device);
-  if (!direct && (workspace == nullptr || workspace_bytes < w.bytes || !aligned16(workspace))) {
+  const int splits = item_splits(max_blocks * block_size, w.items,
+                                 sm_count(device) * (head_dim == 128 ? 1 : 2));
+  if (splits == 0 && (workspace == nullptr || workspace_bytes < w.bytes || !aligned16(workspace))) {
     return SVLLM_ERR_INVALID_ARGUMENT;
   }
   AttnArgs a{};
@@ -939,7 +1000,8 @@ extern "C" int svllm_decode_attention_fp8_bf16(
   a.scale_log2 = static_cast<float>(static_cast<double>(scale) / std::log(2.0));
   a.num_seqs = static_cast<int>(num_seqs);
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (direct) {
+  if (splits > 0) {
+    a.splits = splits;
     return head_dim == 128 ? launch_items<128>(a, w.items, device, s)
                            : launch_items<64>(a, w.items, device, s);
   }

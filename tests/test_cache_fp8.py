@@ -279,6 +279,13 @@ def test_attention(device, heads, kv_heads, dim, block):
     ([2500, 1, 0, 777], 24, 8, 64, 12, None),
     (list(range(0, 520, 4)), 2, 2, 64, 16, None),
     ([30000], 2, 1, 128, 64, None),
+    # by items, as clusters of 8, 4 and 2 CTAs, some of which find no rows
+    ([1000], 16, 8, 128, 16, None),
+    ([1, 2000, 0, 33], 3, 1, 128, 16, None),
+    ([900] * 4, 16, 8, 64, 12, None),
+    ([2000, 1500, 3], 27, 3, 64, 16, None),
+    ([700] * 8, 8, 8, 128, 16, None),
+    ([500, 1] * 10, 16, 16, 64, 16, None),
 ])
 def test_attention_long(cuda, lens, heads, kv_heads, dim, block, width):
     check_attention(cuda, lens, heads, kv_heads, dim, block, width=width)
