@@ -500,11 +500,12 @@ int svllm_cache_read_fp8_bf16(void* k_out, void* v_out, const void* k_cache, con
  * Decode attention (svllm_paged_decode_attention_bf16) over the 8-bit cache: out[b, h] =
  * softmax_j(scale * q[b, h] . k_j) v_j over the rows j < seq_lens[b], k_j and v_j codes times
  * scales. Any number of query heads per KV head; q and out 16-byte aligned, a q_token_stride of whole
- * 16 bytes, else SVLLM_ERR_UNSUPPORTED; scale positive and finite. Products in f16 on exact codes,
+ * 16 bytes, else SVLLM_ERR_UNSUPPORTED; scale positive and finite, as is scale / ln 2. Products in f16 on exact codes,
  * the softmax numerators rounded to f16 for the second; scores, maxima and sums in fp32. A request
  * of length 0, and a head with no score above -infinity, gives zeros. Lengths and table entries out
  * of range as in svllm_cache_read_fp8_bf16. workspace: at least
- * svllm_decode_attention_fp8_workspace_bytes bytes of device memory, 16-byte aligned, any contents;
+ * svllm_decode_attention_fp8_workspace_bytes bytes of device memory (NULL where that is 0), 16-byte
+ * aligned, any contents;
  * calls that overlap on the GPU must not share it. Results repeat bit for bit.
  */
 int svllm_decode_attention_fp8_bf16(void* out, const void* q, int64_t q_token_stride,
@@ -516,10 +517,11 @@ int svllm_decode_attention_fp8_bf16(void* out, const void* q, int64_t q_token_st
                                     void* workspace, int64_t workspace_bytes,
                                     svllm_stream stream);
 
-/* The workspace that svllm_decode_attention_fp8_bf16 needs on the current device for these sizes and
- * any tables and lengths. */
+/* The workspace that svllm_decode_attention_fp8_bf16 needs on the current device for these sizes,
+ * whatever the lengths: 0 for short tables and few heads, whose work needs no joining. */
 int svllm_decode_attention_fp8_workspace_bytes(int64_t num_seqs, int64_t num_heads,
                                                int64_t num_kv_heads, int64_t head_dim,
+                                               int64_t max_blocks, int64_t block_size,
                                                int64_t* bytes);
 
 /*

@@ -886,53 +886,65 @@ int launch_lines(const AttnArgs& a, int64_t items, int device, cudaStream_t stre
                 dim3(kJoinThreads), 0, stream, 1u, a, spread);
 }
 
-constexpr int64_t kMaxSeqs = 1 << 20, kMaxHeads = 1 << 16;
-
-// The parts of the workspace by lines.
-struct Workspace {
-  int64_t items, ml, acc, bytes;
-  Workspace(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
-            int device) {
-    const int64_t group = num_heads / num_kv_heads;
-    const int64_t held = group < kGroup ? group : kGroup;
-    items = num_seqs * num_kv_heads * ((group + kGroup - 1) / kGroup);
-    ml = round_up(items * static_cast<int64_t>(sizeof(JoinEntry)), 256);
-    acc = ml + round_up(2 * line_shares(device) * held * static_cast<int64_t>(sizeof(float2)), 256);
-    bytes = acc + 2 * line_shares(device) * held * head_dim * static_cast<int64_t>(sizeof(float));
-  }
-};
-
-// CTAs of an item, by items; 0: by lines. `wave`: how many such CTAs run at a time.
+// CTAs of an item, by items; 0: by lines. `wave`: how many such CTAs run at a time. Measured, by
+// lines and by items (us in a graph, 16/8 heads of 128): 1 request of 100 rows 7.2, 3.6; 1 of 2000
+// 8.7, 5.6; 8 of 2000 11.7, 9.9; 16 of 500 9.5, 6.1; 32 of 500, two waves, 11.5, 10.8; but 32 of 1000,
+// two waves of four steps, 17.6, 19.1, and 64 of 100, four waves, 10.2, 11.8.
 int item_splits(int64_t max_rows, int64_t items, int64_t wave) {
   int splits = 1;
   while (2 * splits <= kMaxSplits && 2 * splits * items <= wave &&
          splits * kItemWarps * kStepRows < max_rows) {
     splits *= 2;
   }
-  const int64_t steps = (max_rows + splits * kItemWarps * kStepRows - 1) /
-                        (splits * kItemWarps * kStepRows);
+  const int64_t rows = int64_t{splits} * kItemWarps * kStepRows;  // of a step of all warps
+  const int64_t steps = max_rows > rows ? (max_rows + rows - 1) / rows : 1;
   const int64_t waves = (items * splits + wave - 1) / wave;
-  const bool fits = waves <= 2 && waves * (steps > 0 ? steps : 1) <= kItemSteps;
-  return fits ? splits : 0;
+  return waves <= 2 && waves * steps <= kItemSteps ? splits : 0;
 }
+
+constexpr int64_t kInt = int64_t{1} << 31;
+constexpr int64_t kMaxSeqs = 1 << 20, kMaxHeads = 1 << 16, kMaxBlockSize = 1 << 20;
+constexpr int64_t kMaxRows = kInt - kStepRows;
+
+// How a call is dealt to CTAs, and its workspace: none by items.
+struct Workspace {
+  int64_t items, splits, ml, acc, bytes;
+  Workspace(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
+            int64_t max_rows, int device) {
+    const int64_t group = num_heads / num_kv_heads;
+    const int64_t held = group < kGroup ? group : kGroup;
+    items = num_seqs * num_kv_heads * ((group + kGroup - 1) / kGroup);
+    // shared memory leaves room for one CTA by items on an SM at head_dim 128, registers for two at 64
+    splits = item_splits(max_rows, items, sm_count(device) * (head_dim == 128 ? 1 : 2));
+    ml = round_up(items * static_cast<int64_t>(sizeof(JoinEntry)), 256);
+    acc = ml + round_up(2 * line_shares(device) * held * static_cast<int64_t>(sizeof(float2)), 256);
+    bytes = splits > 0 ? 0
+                       : acc + 2 * line_shares(device) * held * head_dim *
+                                   static_cast<int64_t>(sizeof(float));
+  }
+};
 
 }  // namespace
 }  // namespace svllm::k
 
 extern "C" int svllm_decode_attention_fp8_workspace_bytes(int64_t num_seqs, int64_t num_heads,
                                                           int64_t num_kv_heads, int64_t head_dim,
+                                                          int64_t max_blocks, int64_t block_size,
                                                           int64_t* bytes) {
   using namespace svllm::k;
   if (bytes == nullptr || num_seqs < 0 || num_heads <= 0 || num_kv_heads <= 0 ||
-      num_heads % num_kv_heads != 0) {
+      num_heads % num_kv_heads != 0 || max_blocks < 0 || block_size <= 0) {
     return SVLLM_ERR_INVALID_ARGUMENT;
   }
   if (head_dim != 64 && head_dim != 128) return SVLLM_ERR_UNSUPPORTED;
-  if (num_seqs >= kMaxSeqs || num_heads > kMaxHeads) return SVLLM_ERR_TOO_LARGE;
+  if (num_seqs >= kMaxSeqs || num_heads > kMaxHeads || max_blocks >= kInt ||
+      block_size >= kMaxBlockSize || max_blocks * block_size >= kMaxRows) {
+    return SVLLM_ERR_TOO_LARGE;
+  }
   int device;
   if (current_device(&device) != SVLLM_OK) return SVLLM_ERR_CUDA;
-  const Workspace w(num_seqs, num_heads, num_kv_heads, head_dim, device);
-  *bytes = w.bytes;
+  *bytes = Workspace(num_seqs, num_heads, num_kv_heads, head_dim, max_blocks * block_size, device)
+               .bytes;
   return SVLLM_OK;
 }
 
@@ -945,7 +957,8 @@ extern "C" int svllm_decode_attention_fp8_bf16(
   using namespace svllm::k;
   if (num_seqs < 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 ||
       block_size <= 0 || max_blocks < 0 || num_blocks <= 0 || head_dim <= 0 ||
-      q_token_stride < num_heads * head_dim || !(scale > 0.0f) || !std::isfinite(scale)) {
+      q_token_stride < num_heads * head_dim || !(scale > 0.0f) ||
+      !std::isfinite(static_cast<float>(static_cast<double>(scale) / std::log(2.0)))) {
     return SVLLM_ERR_INVALID_ARGUMENT;
   }
   if (num_seqs == 0) return SVLLM_OK;
@@ -954,11 +967,10 @@ extern "C" int svllm_decode_attention_fp8_bf16(
       seq_lens == nullptr) {
     return SVLLM_ERR_INVALID_ARGUMENT;
   }
-  constexpr int64_t kInt = int64_t{1} << 31;
   const int64_t group = num_heads / num_kv_heads;
   const int64_t groups = (group + kGroup - 1) / kGroup;
-  if (num_heads > kMaxHeads || block_size >= (1 << 20) || max_blocks >= kInt ||
-      max_blocks * block_size >= kInt - kStepRows || num_blocks >= kInt ||
+  if (num_heads > kMaxHeads || block_size >= kMaxBlockSize || max_blocks >= kInt ||
+      max_blocks * block_size >= kMaxRows || num_blocks >= kInt ||
       num_blocks * block_size >= kInt || num_seqs >= kMaxSeqs ||
       // the line's steps, were every request as long as its table
       num_seqs * num_kv_heads * groups * (max_blocks * block_size / kStepRows + 1) >= kInt) {
@@ -970,10 +982,8 @@ extern "C" int svllm_decode_attention_fp8_bf16(
   }
   int device;
   if (current_device(&device) != SVLLM_OK) return SVLLM_ERR_CUDA;
-  const Workspace w(num_seqs, num_heads, num_kv_heads, head_dim, device);
-  const int splits = item_splits(max_blocks * block_size, w.items,
-                                 sm_count(device) * (head_dim == 128 ? 1 : 2));
-  if (splits == 0 && (workspace == nullptr || workspace_bytes < w.bytes || !aligned16(workspace))) {
+  const Workspace w(num_seqs, num_heads, num_kv_heads, head_dim, max_blocks * block_size, device);
+  if (w.bytes > 0 && (workspace == nullptr || workspace_bytes < w.bytes || !aligned16(workspace))) {
     return SVLLM_ERR_INVALID_ARGUMENT;
   }
   AttnArgs a{};
@@ -1000,8 +1010,8 @@ extern "C" int svllm_decode_attention_fp8_bf16(
   a.scale_log2 = static_cast<float>(static_cast<double>(scale) / std::log(2.0));
   a.num_seqs = static_cast<int>(num_seqs);
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (splits > 0) {
-    a.splits = splits;
+  if (w.splits > 0) {
+    a.splits = static_cast<int>(w.splits);
     return head_dim == 128 ? launch_items<128>(a, w.items, device, s)
                            : launch_items<64>(a, w.items, device, s);
   }

@@ -37,9 +37,11 @@ void decode_attention_fp8(const at::Tensor& out, const at::Tensor& q, const at::
   int64_t bytes = 0;
   detail::check_status("decode_attention_fp8",
                        svllm_decode_attention_fp8_workspace_bytes(
-                           requests, heads, k_cache.size(2), dim, &bytes));
+                           requests, heads, k_cache.size(2), dim, block_tables.size(1),
+                           k_cache.size(1), &bytes));
   // from the caching allocator per call: calls on other streams, and captured graphs, get their own
-  const c10::DataPtr workspace = c10::cuda::CUDACachingAllocator::get()->allocate(bytes);
+  c10::DataPtr workspace;
+  if (bytes > 0) workspace = c10::cuda::CUDACachingAllocator::get()->allocate(bytes);
   detail::check_status(
       "decode_attention_fp8",
       svllm_decode_attention_fp8_bf16(

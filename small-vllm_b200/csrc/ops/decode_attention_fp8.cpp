@@ -28,7 +28,8 @@ at::Tensor decode_attention_fp8(const at::Tensor& q, const at::Tensor& k_cache,
                                 (requests == 1 || q.stride(0) >= heads * dim)),
               kOp, ": q's heads must be contiguous, got strides ", q.strides());
   const double factor = scale.value_or(std::pow(static_cast<double>(dim), -0.5));
-  TORCH_CHECK(factor > 0.0 && std::isfinite(static_cast<float>(factor)) &&
+  // also in base 2, which is what the kernel takes
+  TORCH_CHECK(factor > 0.0 && std::isfinite(static_cast<float>(factor / std::log(2.0))) &&
                   static_cast<float>(factor) > 0.0f,
               kOp, ": scale must be positive and finite, got ", factor);
   at::Tensor out = at::empty({requests, heads, dim}, q.options());

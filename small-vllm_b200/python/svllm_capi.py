@@ -86,7 +86,7 @@ SIGNATURES = {
                                   _I64, _P],
     "svllm_decode_attention_fp8_bf16": [_P, _P, _I64, _P, _P, _P, _P, _I64, _I64, _P, _I64, _P,
                                         _I64, _I64, _I64, _I64, _F, _P, _I64, _P],
-    "svllm_decode_attention_fp8_workspace_bytes": [_I64, _I64, _I64, _I64, _P],
+    "svllm_decode_attention_fp8_workspace_bytes": [_I64] * 6 + [_P],
     "svllm_read_device_error": [_I, _I, _P],
 }
 
@@ -346,6 +346,78 @@ def tree_commit(k_caches, v_caches, path, num_accepted, slot_mapping, query_star
         row * first.element_size(), path.data_ptr(), num_accepted.data_ptr(),
         slot_mapping.data_ptr(), query_start_loc.data_ptr(), num_accepted.numel(),
         slot_mapping.numel(), path.shape[1], _stream(stream)), "tree_commit")
+
+
+def tree_commit_scales(k_scales, v_scales, path, num_accepted, slot_mapping, query_start_loc,
+                       stream=None) -> None:
+    """tree_commit for an 8-bit cache's scales, [..., Hk] each."""
+    first = k_scales[0]
+    k = (_P * len(k_scales))(*[c.data_ptr() for c in k_scales])
+    v = (_P * len(v_scales))(*[c.data_ptr() for c in v_scales])
+    check(lib().svllm_tree_commit_scales(
+        ctypes.cast(k, _P), ctypes.cast(v, _P), len(k_scales), first.numel() // first.shape[-1],
+        first.shape[-1], path.data_ptr(), num_accepted.data_ptr(), slot_mapping.data_ptr(),
+        query_start_loc.data_ptr(), num_accepted.numel(), slot_mapping.numel(), path.shape[1],
+        _stream(stream)), "tree_commit_scales")
+
+
+def qk_norm_rope_cache_fp8(q, k, v, q_weight, k_weight, positions, slot_mapping, k_cache, v_cache,
+                           k_scale, v_scale, eps: float, inv, stream=None) -> None:
+    """q rotated in place; k (rotated) and v quantised into their slots of the 8-bit cache: codes
+    [num_slots, Hk, D] and e8m0 scales [num_slots, Hk], or shapes that flatten to those."""
+    arr = _inv_array(inv)
+    check(lib().svllm_qk_norm_rope_cache_fp8_bf16(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(),
+        positions.data_ptr(), _index_type(positions), slot_mapping.data_ptr(),
+        k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+        k_scale.numel() // k.shape[1], q.shape[0], q.shape[1], k.shape[1], q.shape[2],
+        q.stride(0), k.stride(0), v.stride(0), eps, ctypes.cast(arr, _P), _stream(stream)),
+        "qk_norm_rope_cache_fp8")
+
+
+def rope_cache_fp8(q, k, v, positions, slot_mapping, k_cache, v_cache, k_scale, v_scale, inv,
+                   stream=None) -> None:
+    arr = _inv_array(inv)
+    check(lib().svllm_rope_cache_fp8_bf16(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), positions.data_ptr(), _index_type(positions),
+        slot_mapping.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+        v_scale.data_ptr(), k_scale.numel() // k.shape[1], q.shape[0], q.shape[1], k.shape[1],
+        q.shape[2], q.stride(0), k.stride(0), v.stride(0), ctypes.cast(arr, _P), _stream(stream)),
+        "rope_cache_fp8")
+
+
+def cache_read_fp8(k_out, v_out, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens,
+                   stream=None) -> None:
+    """k_out, v_out [S, max_blocks * block_size, Hk, D] bf16 = the requests' rows, zeros behind."""
+    num_blocks, block_size, num_kv_heads, head_dim = k_cache.shape
+    check(lib().svllm_cache_read_fp8_bf16(
+        k_out.data_ptr(), v_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+        k_scale.data_ptr(), v_scale.data_ptr(), num_blocks, block_size, block_tables.data_ptr(),
+        block_tables.shape[1], seq_lens.data_ptr(), seq_lens.numel(), num_kv_heads, head_dim,
+        _stream(stream)), "cache_read_fp8")
+
+
+def decode_attention_fp8_workspace_bytes(num_seqs: int, num_heads: int, num_kv_heads: int,
+                                         head_dim: int, max_blocks: int, block_size: int) -> int:
+    size = _I64(0)
+    check(lib().svllm_decode_attention_fp8_workspace_bytes(
+        num_seqs, num_heads, num_kv_heads, head_dim, max_blocks, block_size, ctypes.byref(size)),
+        "decode_attention_fp8_workspace_bytes")
+    return size.value
+
+
+def decode_attention_fp8(out, q, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens,
+                         scale: float, workspace, stream=None) -> None:
+    """out [S, Hq, D] = decode attention of q [S, Hq, D] over the 8-bit caches; workspace: uint8
+    tensor of decode_attention_fp8_workspace_bytes(...), or None where that is 0."""
+    num_seqs, num_heads, head_dim = q.shape
+    num_blocks, block_size, num_kv_heads, _ = k_cache.shape
+    check(lib().svllm_decode_attention_fp8_bf16(
+        out.data_ptr(), q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(),
+        k_scale.data_ptr(), v_scale.data_ptr(), num_blocks, block_size, block_tables.data_ptr(),
+        block_tables.shape[1], seq_lens.data_ptr(), num_seqs, num_heads, num_kv_heads, head_dim,
+        scale, _ptr(workspace), workspace.numel() if workspace is not None else 0,
+        _stream(stream)), "decode_attention_fp8")
 
 
 def read_device_error(device: int = 0, reset: bool = True) -> int:

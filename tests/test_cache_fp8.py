@@ -9,6 +9,7 @@ import pytest
 import torch
 
 import fp8_reference as ref
+import svllm_capi as capi
 import svllm_ops
 from fp8_reference import E4M3, E8M0
 
@@ -375,9 +376,11 @@ def test_attention_strides_streams_and_repeats(cuda):
 
 
 @pytest.mark.gpu
-def test_step_captured_and_replayed(cuda):
-    """Write, attention and read-back of one step in a graph; replays follow the data."""
-    heads, kv_heads, dim, block, lens = 8, 4, 128, 16, [300, 17, 64]
+@pytest.mark.parametrize("lens", [[300, 17, 64], [9000, 17, 64]], ids=["by items", "by lines"])
+def test_step_captured_and_replayed(cuda, lens):
+    """Write, attention and read-back of one step in a graph; replays follow the data, the lengths
+    too."""
+    heads, kv_heads, dim, block = 8, 4, 128, 16
     tables, total = ref.make_tables(3, lens, block)
     caches = [t.to(cuda) for t in ref.make_cache(4, total, block, kv_heads, dim)]
     start = [t.clone() for t in caches]
@@ -399,7 +402,9 @@ def test_step_captured_and_replayed(cuda):
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         held = step(qkv)
-    for seed in range(3):
+    for seed in range(4):
+        if seed == 2:  # other lengths in the same tables, one of them none
+            n.copy_(torch.tensor([lens[0] // 2, 0, 50], dtype=torch.int32))
         fresh = torch.randn(qkv.shape, generator=g).bfloat16().to(cuda)
         for c, s in zip(caches, start):
             c.copy_(s)
@@ -410,6 +415,114 @@ def test_step_captured_and_replayed(cuda):
         graph.replay()
         for a, b in zip(held, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_two_graphs_replay_at_once(cuda):
+    """Graphs of the joined form, captured apart, replayed on two streams: each its own workspace."""
+    block, lens = 16, [6000, 9000]
+    tables, total = ref.make_tables(3, lens, block)
+    caches = [t.to(cuda) for t in ref.make_cache(4, total, block, 2, 64)]
+    t, n = tables.to(cuda), torch.tensor(lens, dtype=torch.int32, device=cuda)
+    g = torch.Generator().manual_seed(5)
+    qs = [torch.randn(2, 4, 64, generator=g).bfloat16().to(cuda) for _ in range(2)]
+    want = [svllm_ops.decode_attention_fp8(q, *caches, t, n) for q in qs]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for q in qs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append([svllm_ops.decode_attention_fp8(q, *caches, t, n) for _ in range(20)])
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(5):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for held, w in zip(outs, want):
+        assert all(torch.equal(o, w) for o in held)
+
+
+@pytest.mark.gpu
+def test_slots_past_32_bits(cuda):
+    """Rows behind 4 GB of codes: written, attended to and read back."""
+    kv_heads, dim, block = 1, 128, 16
+    blocks = (1 << 32) // (block * kv_heads * dim) + 64
+    caches = [torch.zeros(blocks, block, kv_heads, dim, dtype=torch.uint8, device=cuda).view(E4M3)
+              for _ in range(2)]
+    caches += [torch.full((blocks, block, kv_heads), 127, dtype=torch.uint8,
+                          device=cuda).view(E8M0) for _ in range(2)]
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(40, 4, dim, generator=g).bfloat16()
+    pages = torch.tensor([blocks - 1, 3, blocks - 7], dtype=torch.int32)
+    j = torch.arange(40)
+    slots = pages.long()[j // block] * block + j % block
+    q, k, v = (t.contiguous().to(cuda) for t in x.split([2, 1, 1], 1))
+    svllm_ops.rope_cache_fp8(q, k, v, torch.zeros(40, dtype=torch.long, device=cuda),
+                             slots.to(cuda), *caches, THETA)
+    codes, scale, _ = ref.quantise(x[:, 2:].double())  # position 0: nothing turns
+    held = ref.values(codes, scale)
+    n = torch.tensor([40], dtype=torch.int32, device=cuda)
+    k_read, v_read = svllm_ops.cache_read_fp8(*caches, pages[None].to(cuda), n)
+    assert torch.equal(k_read[0, :40, 0].cpu().double(), held[:, 0])
+    assert torch.equal(v_read[0, :40, 0].cpu().double(), held[:, 1])
+    for wide in (3, 2000):  # by items, by lines
+        t = torch.zeros(1, wide, dtype=torch.int32)
+        t[0, :3] = pages
+        out = svllm_ops.decode_attention_fp8(q[-1:], *caches, t.to(cuda), n).cpu()
+        small = [c.cpu()[:, None] for c in (codes[:, :1], codes[:, 1:], scale[:, :1], scale[:, 1:])]
+        want, bound = ref.attention(q[-1:].cpu(), *small, torch.arange(40)[None].int(), [40],
+                                    dim ** -0.5)
+        assert ((out.double() - want).abs() <= bound).all()
+    # nothing else was written: the rows beside them, and those 4 GB below
+    for c, fill in zip(caches, (0, 0, 127, 127)):
+        flat = c.view(torch.uint8).flatten(0, 1)
+        near = torch.cat([slots - 16, slots + 32 * block, slots - (1 << 32) // dim])
+        near = near[(near >= 0) & (near < len(flat))]
+        near = near[~torch.isin(near, slots)]
+        assert (flat[near.to(cuda)] == fill).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("width", [None, 700], ids=["by items", "by lines"])
+def test_c_abi_gives_the_same_bits(cuda, width):
+    """The entry points without LibTorch, a workspace that holds anything and serves calls in turn."""
+    lens, block = [5000, 33, 0], 16
+    tables, total = ref.make_tables(3, lens, block, width=width)
+    caches = [t.to(cuda) for t in ref.make_cache(4, total, block, 2, 128)]
+    t, n = tables.to(cuda), torch.tensor(lens, dtype=torch.int32, device=cuda)
+    g = torch.Generator().manual_seed(5)
+    size = capi.decode_attention_fp8_workspace_bytes(3, 6, 2, 128, t.shape[1], block)
+    assert (size > 0) == (width is not None)
+    workspace = torch.full((size,), 255, dtype=torch.uint8, device=cuda) if size else None
+    for _ in range(3):
+        q = torch.randn(3, 6, 128, generator=g).bfloat16().to(cuda)
+        out = torch.empty_like(q)
+        capi.decode_attention_fp8(out, q, *caches, t, n, 128 ** -0.5, workspace)
+        assert torch.equal(out, svllm_ops.decode_attention_fp8(q, *caches, t, n))
+    if size:
+        for few in (workspace[: size - 1], None):
+            with pytest.raises(capi.CapiError):
+                capi.decode_attention_fp8(out, q, *caches, t, n, 128 ** -0.5, few)
+    k, v = (torch.empty(3, t.shape[1] * block, 2, 128, dtype=torch.bfloat16, device=cuda)
+            for _ in range(2))
+    capi.cache_read_fp8(k, v, *caches, t, n)
+    assert all(torch.equal(a, b) for a, b in
+               zip((k, v), svllm_ops.cache_read_fp8(*caches, t, n)))
+    c = write_case(4, 40, 6, 2, 128)
+    inv = svllm_ops.rope_inv_freq(THETA, 128, None).tolist()
+    for norm in (True, False):
+        want = call_write(c, cuda, 6, 2, 128, norm)
+        q, k, v = split(c["qkv"].to(cuda).clone(), 6, 2, 128)
+        own = [x.clone().to(cuda) for x in c["caches"]]
+        w, pos, slots = c["weights"].to(cuda), c["positions"].to(cuda), c["slots"].to(cuda)
+        if norm:
+            capi.qk_norm_rope_cache_fp8(q, k, v, w[0], w[1], pos, slots, *own, EPS, inv)
+        else:
+            capi.rope_cache_fp8(q, k, v, pos, slots, *own, inv)
+        assert torch.equal(q.cpu(), want[0])
+        assert all(torch.equal(bits(a), bits(b)) for a, b in zip(own, want[1]))
 
 
 @pytest.mark.gpu
@@ -527,6 +640,7 @@ def test_read_and_attention_refuse():
     refused("requests", q=q[:1])
     refused("scale", scale=0.0)
     refused("scale", scale=math.inf)
+    refused("scale", scale=3e38)  # past fp32 in base 2
 
 
 def test_empty_batches(device):
