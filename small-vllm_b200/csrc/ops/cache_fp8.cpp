@@ -4,6 +4,7 @@
 #include <c10/util/Exception.h>
 
 #include "ops/cache_fp8_kernels.h"
+#include "ops/common.h"
 
 namespace svllm::ops {
 
@@ -65,8 +66,10 @@ std::tuple<at::Tensor, at::Tensor> cache_read_fp8(const at::Tensor& k_cache,
   TORCH_CHECK(device.is_cpu() || device.is_cuda(), "cache_read_fp8: unsupported device ", device);
   const int64_t shape[] = {seq_lens.size(0), block_tables.size(1) * k_cache.size(1),
                            k_cache.size(2), k_cache.size(3)};
-  const auto options = k_cache.options().dtype(at::kBFloat16);
-  const at::Tensor k = at::empty(shape, options), v = at::empty(shape, options);
+  const int64_t bytes =
+      detail::Outputs::size(at::kBFloat16, shape[0] * shape[1] * shape[2] * shape[3]);
+  detail::Outputs out(2 * bytes, k_cache.options());
+  const at::Tensor k = out.take(at::kBFloat16, shape), v = out.take(at::kBFloat16, shape);
   if (device.is_cuda()) {
     cuda_impl::cache_read_fp8(k, v, k_cache, v_cache, k_scale, v_scale, block_tables, seq_lens);
   } else {

@@ -70,7 +70,7 @@ int64_t rope_cache_fp8(const at::Tensor& q, const at::Tensor& k, const at::Tenso
                        const at::Tensor& k_scale, const at::Tensor& v_scale, double eps,
                        const float* inv_freq) {
   const int64_t tokens = q.size(0), heads = q.size(1), kv_heads = k.size(1), dim = q.size(2);
-  const int64_t half = dim / 2, num_slots = k_cache.size(0);
+  const int64_t half = dim / 2, num_slots = k_scale.numel() / kv_heads;
   auto* qp = q.mutable_data_ptr<at::BFloat16>();
   const auto* kp = k.const_data_ptr<at::BFloat16>();
   const auto* vp = v.const_data_ptr<at::BFloat16>();

@@ -80,6 +80,7 @@ void rope_cache_fp8(const at::Tensor& q, const at::Tensor& k, const at::Tensor& 
   const auto stream = reinterpret_cast<svllm_stream>(c10::cuda::getCurrentCUDAStream().stream());
   const int pos_type = positions.scalar_type() == at::kLong ? SVLLM_INDEX_I64 : SVLLM_INDEX_I32;
   const auto* slots = slot_mapping.const_data_ptr<int64_t>();
+  const int64_t num_slots = k_scale.numel() / k.size(1);
   // the only token's stride is never used, and torch may report any
   const auto stride = [&](const at::Tensor& x) {
     return num_tokens == 1 ? x.size(1) * x.size(2) : x.stride(0);
@@ -91,7 +92,7 @@ void rope_cache_fp8(const at::Tensor& q, const at::Tensor& k, const at::Tensor& 
             q.mutable_data_ptr(), k.const_data_ptr(), v.const_data_ptr(),
             q_weight.const_data_ptr(), k_weight.const_data_ptr(), positions.const_data_ptr(),
             pos_type, slots, k_cache.mutable_data_ptr(), v_cache.mutable_data_ptr(),
-            k_scale.mutable_data_ptr(), v_scale.mutable_data_ptr(), k_cache.size(0), num_tokens,
+            k_scale.mutable_data_ptr(), v_scale.mutable_data_ptr(), num_slots, num_tokens,
             q.size(1), k.size(1), q.size(2), stride(q), stride(k), stride(v),
             static_cast<float>(eps), inv_freq, stream));
   } else {
@@ -101,7 +102,7 @@ void rope_cache_fp8(const at::Tensor& q, const at::Tensor& k, const at::Tensor& 
             q.mutable_data_ptr(), k.const_data_ptr(), v.const_data_ptr(),
             positions.const_data_ptr(), pos_type, slots, k_cache.mutable_data_ptr(),
             v_cache.mutable_data_ptr(), k_scale.mutable_data_ptr(), v_scale.mutable_data_ptr(),
-            k_cache.size(0), num_tokens, q.size(1), k.size(1), q.size(2), stride(q), stride(k),
+            num_slots, num_tokens, q.size(1), k.size(1), q.size(2), stride(q), stride(k),
             stride(v), inv_freq, stream));
   }
 }

@@ -111,7 +111,7 @@ void check_and_run(const char* op, const at::Tensor& q, const at::Tensor& k,
 
   const bool with_cache = cache.v.defined();
   const bool fp8 = cache.k_scale.defined();
-  at::Tensor v3, kc, vc, ks, vs;
+  at::Tensor v3, kc, vc;
   if (fp8) {
     TORCH_CHECK(cache.v.scalar_type() == q.scalar_type(), op, ": expected bf16 v, got ",
                 cache.v.scalar_type());
@@ -147,11 +147,9 @@ void check_and_run(const char* op, const at::Tensor& q, const at::Tensor& k,
                                    cache.v_cache.device() == q.device();
     TORCH_CHECK(cache_same_device, op, ": q is on ", q.device(),
                 " but v, slot_mapping or a cache is elsewhere");
-    kc = cache.k_cache.view({-1, kv_heads, head_dim});
-    vc = cache.v_cache.view({-1, kv_heads, head_dim});
-    if (fp8) {
-      ks = cache.k_scale.view({-1, kv_heads});
-      vs = cache.v_scale.view({-1, kv_heads});
+    if (!fp8) {  // (a view costs its caller near a microsecond: the 8-bit kernels take sizes)
+      kc = cache.k_cache.view({-1, kv_heads, head_dim});
+      vc = cache.v_cache.view({-1, kv_heads, head_dim});
     }
   }
 
@@ -162,8 +160,10 @@ void check_and_run(const char* op, const at::Tensor& q, const at::Tensor& k,
       if (fp8) {
         const int64_t bad =
             cpu_impl::rope_cache_fp8(q3, k3, v3, q_weight, k_weight, positions, cache.slot_mapping,
-                                     kc, vc, ks, vs, eps, inv_freq.data());
-        TORCH_CHECK(bad == 0, op, ": ", bad, " slots past the cache's ", kc.size(0));
+                                     cache.k_cache, cache.v_cache, cache.k_scale, cache.v_scale,
+                                     eps, inv_freq.data());
+        TORCH_CHECK(bad == 0, op, ": ", bad, " slots past the cache's ",
+                    cache.k_scale.numel() / k3.size(1));
         break;
       }
       cpu_impl::rope(q3, k3, q_weight, k_weight, positions, eps, inv_freq.data());
@@ -176,7 +176,8 @@ void check_and_run(const char* op, const at::Tensor& q, const at::Tensor& k,
     case c10::DeviceType::CUDA:
       if (fp8) {
         cuda_impl::rope_cache_fp8(q3, k3, v3, q_weight, k_weight, positions, cache.slot_mapping,
-                                  kc, vc, ks, vs, eps, inv_freq.data());
+                                  cache.k_cache, cache.v_cache, cache.k_scale, cache.v_scale, eps,
+                                  inv_freq.data());
       } else if (with_cache) {
         cuda_impl::rope_cache(q3, k3, v3, q_weight, k_weight, positions, cache.slot_mapping, kc,
                               vc, eps, inv_freq.data());

@@ -19,8 +19,8 @@ void rope(const at::Tensor& q, const at::Tensor& k, const at::Tensor& q_weight,
 // Returns the number of slots past the cache (their tokens write nothing).
 int64_t write_kv_cache(const at::Tensor& k, const at::Tensor& v, const at::Tensor& slot_mapping,
                        const at::Tensor& k_cache, const at::Tensor& v_cache);
-// The 8-bit cache's step, q in place; scales viewed as [num_slots, num_kv_heads]. Returns the
-// number of slots past the cache.
+// The 8-bit cache's step, q in place; caches [..., num_kv_heads, head_dim] and scales [...,
+// num_kv_heads] as they come. Returns the number of slots past the cache.
 int64_t rope_cache_fp8(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                        const at::Tensor& q_weight, const at::Tensor& k_weight,
                        const at::Tensor& positions, const at::Tensor& slot_mapping,
