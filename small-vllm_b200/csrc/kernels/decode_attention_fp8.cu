@@ -53,6 +53,11 @@ constexpr int kStages = 2;       // of a warp's ring
 constexpr int kLineWarps = 8;    // of a CTA by lines, one per SM
 constexpr int kItemWarps = 8;    // of a CTA by items
 constexpr int kMinShare = 2;     // steps of a warp's share at least
+// KV heads of an item by lines at head_dim 64, so that a row fills a 128-byte line, and from how many
+// steps a warp on, were every request as long as its table (us, one and two, 32/8 heads of 64: 64
+// requests of 2048-4096 rows, 110 steps, 61.4, 43.9; 16 of 2048-4096, 14 steps, 19.8, 19.7; 13 of
+// 140-2500, 24/8 heads, 7 steps, 10.0, 11.8).
+constexpr int kPair = 2, kPairSteps = 14;
 constexpr int kMaxSplits = 8;    // CTAs of an item: the portable cluster size
 constexpr int kItemSteps = 4;    // by items up to this many steps of a warp
 constexpr int kJoinThreads = 256;
@@ -93,6 +98,7 @@ struct AttnArgs {
   int num_kv_heads;
   int group;   // query heads per KV head
   int groups;  // items they are dealt to
+  int subs;    // items of a request
   int shares;  // warps by lines
   int splits;  // CTAs of an item, by items
   float scale_log2;
@@ -136,13 +142,13 @@ __device__ __forceinline__ uint2 lds64(uint32_t a) {
   return r;
 }
 
-// Where 16-byte chunk c of row r lies in a tile of 32 rows: permuted so that both products' reads
-// (a quarter of a warp: two rows times four chunks of K, four even or odd rows times two chunks of
-// V) touch every bank once.
-template <int D>
+// Where 16-byte chunk c of row r lies in a tile of 32 rows of `kWidth` bytes: permuted so that both
+// products' reads (a quarter of a warp: two rows times four chunks of K, four even or odd rows times
+// two chunks of V) touch every bank once.
+template <int kWidth>
 __device__ __forceinline__ uint32_t tile_at(int r, int c) {
-  if constexpr (D == 128) {
-    return static_cast<uint32_t>(r * 128 + ((c ^ (r & 7)) << 4));
+  if constexpr (kWidth == 128) {
+    return static_cast<uint32_t>(r * 128 + ((c ^ (r & 6) ^ ((r & 1) << 2)) << 4));
   } else {
     return static_cast<uint32_t>((r >> 1) * 128 + (((r ^ (r >> 2)) & 1) << 6) +
                                  ((c ^ (((r >> 1) & 1) << 1)) << 4));
@@ -159,21 +165,28 @@ __device__ __forceinline__ int item_steps(int len) {
   return max(1, (len + kStepRows - 1) / kStepRows);
 }
 
-// The query heads of an item: the first one's index, and how many.
+// An item's heads: kHeads neighbouring KV heads (the last item of an odd number of them has one
+// less) and, of each, the same up to eight query heads.
+template <int kHeads>
 struct Heads {
-  int first, count;
+  int kv, live;      // the first KV head, and how many there are
+  int first, count;  // of the first KV head: its first query head, and how many
   __device__ __forceinline__ Heads(const AttnArgs& a, int sub) {
-    const int kh = sub / a.groups, hg = sub - kh * a.groups;
-    first = kh * a.group + hg * kGroup;
+    const int run = a.groups == 1 ? sub : sub / a.groups;
+    const int hg = sub - run * a.groups;
+    kv = run * kHeads;
+    live = min(kHeads, a.num_kv_heads - kv);
+    first = kv * a.group + hg * kGroup;
     count = min(kGroup, a.group - hg * kGroup);
   }
 };
 
-// One step's copies: 32 rows of K, then of V.
-template <int D>
+// One step's copies: 32 rows of K, then of V, of kHeads KV heads side by side.
+template <int D, int kHeads>
 struct Loader {
-  static constexpr int kChunks = D / 16;  // 16-byte chunks of a row
-  static constexpr int kTileBytes = kStepRows * D;
+  static constexpr int kWidth = D * kHeads;
+  static constexpr int kChunks = kWidth / 16;  // 16-byte chunks of a row
+  static constexpr int kTileBytes = kStepRows * kWidth;
   static constexpr int kStageBytes = 2 * kTileBytes;
   static constexpr int kLoads = kStepRows * kChunks / kWarpSize;  // a lane, K and V each
   static constexpr int kRowsALoad = kWarpSize / kChunks;
@@ -185,15 +198,17 @@ struct Loader {
     return __ldg(a.block_tables + static_cast<int64_t>(b) * a.max_blocks + a.page.divide(j));
   }
 
-  // Copies the step's rows to `dst` and loads lane r's row's scale bytes, which nothing waits for
-  // here.
-  static __device__ __forceinline__ void issue(const AttnArgs& a, uint32_t dst, int block, int kh,
-                                               int step, int len, uint32_t& k_scale,
-                                               uint32_t& v_scale) {
+  // Copies the step's rows to `dst` and loads lane r's row's scale bytes (the first KV head's lowest),
+  // which nothing waits for here.
+  static __device__ __forceinline__ void issue(const AttnArgs& a, uint32_t dst, int block,
+                                               const Heads<kHeads>& heads, int step, int len,
+                                               uint32_t (&k_scale)[kHeads],
+                                               uint32_t (&v_scale)[kHeads]) {
     const int lane = static_cast<int>(threadIdx.x) % kWarpSize;
     const int r0 = step * kStepRows, j = r0 + lane;
     uint32_t slot = 0;
-    k_scale = v_scale = kScaleBias;
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) k_scale[i] = v_scale[i] = kScaleBias;
     if (j < len) {
       if (static_cast<uint64_t>(block) >= static_cast<uint64_t>(a.num_blocks)) {
         raise_error(a.err, kErrBadIndex);  // an entry outside the cache: read block 0
@@ -201,21 +216,28 @@ struct Loader {
       }
       slot = static_cast<uint32_t>(block) * static_cast<uint32_t>(a.block_size) +
              static_cast<uint32_t>(j - a.page.divide(j) * a.block_size);
-      const int64_t at = static_cast<int64_t>(slot) * a.num_kv_heads + kh;
-      k_scale = __ldg(a.k_scale + at);
-      v_scale = __ldg(a.v_scale + at);
+      const int64_t at = static_cast<int64_t>(slot) * a.num_kv_heads + heads.kv;
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i) {
+        if (i < heads.live) {
+          k_scale[i] = __ldg(a.k_scale + at + i);
+          v_scale[i] = __ldg(a.v_scale + at + i);
+        }
+      }
     }
     const int c = lane % kChunks;
+    const bool live = kHeads == 1 || c * 16 < heads.live * D;
     const int64_t row_bytes = static_cast<int64_t>(a.num_kv_heads) * D;
-    const uint8_t* k = a.k_cache + static_cast<int64_t>(kh) * D + c * 16;
+    // (a chunk of a KV head that does not exist copies nothing; its address is the first head's)
+    const uint8_t* k = a.k_cache + static_cast<int64_t>(heads.kv) * D + (live ? c * 16 : 0);
     const int64_t v = a.v_cache - a.k_cache;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int r = i * kRowsALoad + lane / kChunks;
       const uint8_t* p = k + __shfl_sync(0xffffffffu, slot, r) * row_bytes;
-      const bool valid = r0 + r < len;  // zeros past the end: 0 * w, never NaN
-      cp_async16(dst + tile_at<D>(r, c), p, valid);
-      cp_async16(dst + kTileBytes + tile_at<D>(r, c), p + v, valid);
+      const bool valid = r0 + r < len && live;  // zeros past the end: 0 * w, never NaN
+      cp_async16(dst + tile_at<kWidth>(r, c), p, valid);
+      cp_async16(dst + kTileBytes + tile_at<kWidth>(r, c), p + v, valid);
     }
   }
 };
@@ -263,8 +285,8 @@ struct Queries {
   }
 };
 
-// A warp's running sums over an item's rows.
-template <int D>
+// A warp's running sums over an item's rows, for one of its KV heads. kWidth: of a row of the tiles.
+template <int D, int kWidth>
 struct Sums {
   static constexpr int kTiles = D / 16;  // m-tiles of O^T
   // O^T element (dim, head): m-tile i holds dims g * D / 8 + 2 i (elements 0, 1: heads 2t, 2t + 1)
@@ -285,9 +307,11 @@ struct Sums {
     l[0] = l[1] = 0.0f;
   }
 
-  // Adds a step: the tile in shared memory, lane r's row's scale bytes, how many rows exist.
-  __device__ __forceinline__ void step(uint32_t tile, uint32_t scales, int live,
+  // Adds a step: the tile in shared memory and the KV head's place in its rows, lane r's row's scale
+  // bytes, how many rows exist.
+  __device__ __forceinline__ void step(uint32_t tile, int place, uint32_t scales, int live,
                                        const Queries<D>& q) {
+    const int chunk = place * (D / 16);
     const int lane = static_cast<int>(threadIdx.x) % kWarpSize;
     const int g = lane >> 2, t = lane & 3;
     // S^T: lane holds rows g, g + 8 of both tiles x heads 2t, 2t + 1
@@ -299,8 +323,8 @@ struct Sums {
       float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int c = 0; c < Queries<D>::kPieces; ++c) {
-        const uint4 k0 = lds128(tile + tile_at<D>(16 * i + g, 4 * c + t));
-        const uint4 k1 = lds128(tile + tile_at<D>(16 * i + 8 + g, 4 * c + t));
+        const uint4 k0 = lds128(tile + tile_at<kWidth>(16 * i + g, chunk + 4 * c + t));
+        const uint4 k1 = lds128(tile + tile_at<kWidth>(16 * i + 8 + g, chunk + 4 * c + t));
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const uint32_t w0 = word(k0, w), w1 = word(k1, w);
@@ -354,12 +378,12 @@ struct Sums {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int r = 16 * i + 8 * (e >> 1) + 2 * t + (e & 1);
-        const uint32_t at = tile + Loader<D>::kTileBytes;
+        const uint32_t at = tile + kStepRows * kWidth;
         if constexpr (D == 128) {
-          const uint4 x = lds128(at + tile_at<D>(r, g));
+          const uint4 x = lds128(at + tile_at<kWidth>(r, chunk + g));
           v[e][0] = x.x, v[e][1] = x.y, v[e][2] = x.z, v[e][3] = x.w;
         } else {
-          const uint2 x = lds64(at + tile_at<D>(r, g >> 1) + 8 * (g & 1));
+          const uint2 x = lds64(at + tile_at<kWidth>(r, chunk + (g >> 1)) + 8 * (g & 1));
           v[e][0] = x.x, v[e][1] = x.y;
         }
       }
@@ -392,7 +416,7 @@ struct Sums {
 // A run of steps of one item.
 struct Segment {
   int b;
-  int sub;    // KV head * groups + group of query heads
+  int sub;    // KV head (or pair) * groups + group of query heads
   int first;  // its first step in the item
   int n;      // its steps
   int steps;  // the item's
@@ -425,7 +449,7 @@ __device__ __forceinline__ int length_of(const AttnArgs& a, const Line& line, in
 __device__ __forceinline__ void next_segment(const AttnArgs& a, const Line& line, Segment& s) {
   s.left -= s.n;
   s.first = 0;
-  if (++s.sub == a.num_kv_heads * a.groups) {
+  if (++s.sub == a.subs) {
     s.sub = 0;
     ++s.b;
     if (s.left > 0) {
@@ -439,7 +463,7 @@ __device__ __forceinline__ void next_segment(const AttnArgs& a, const Line& line
 // Share c of the line: its first segment. A lane takes a run of requests.
 __device__ __forceinline__ Segment first_segment(const AttnArgs& a, int c, Line& line) {
   const int lane = static_cast<int>(threadIdx.x) % kWarpSize;
-  const int subs = a.num_kv_heads * a.groups;
+  const int subs = a.subs;
   const int per = (a.num_seqs + kWarpSize - 1) / kWarpSize;
   const int begin = min(a.num_seqs, lane * per), end = min(a.num_seqs, begin + per);
   int sum = 0, len = 0;
@@ -494,17 +518,18 @@ __device__ __forceinline__ Segment first_segment(const AttnArgs& a, int c, Line&
   return s;
 }
 
-template <int D>
+template <int D, int kHeads>
 __global__ void __launch_bounds__(kLineWarps * kWarpSize, 1) decode_attention_fp8_lines(
     const __grid_constant__ AttnArgs a) {
   grid_dependency_sync();
+  using Load = Loader<D, kHeads>;
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x / kWarpSize;
   const int lane = threadIdx.x % kWarpSize;
   const int g = lane >> 2;
   const int t = lane & 3;
   const int held_heads = min(a.group, kGroup);
-  const uint32_t ring = smem_addr(smem) + warp * kStages * Loader<D>::kStageBytes;
+  const uint32_t ring = smem_addr(smem) + warp * kStages * Load::kStageBytes;
 
   // neighbouring shares on different SMs, so that few shares find many SMs
   const int share = warp * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x);
@@ -515,86 +540,102 @@ __global__ void __launch_bounds__(kLineWarps * kWarpSize, 1) decode_attention_fp
   // ---- loads: `ahead` walks the share in front of the products
   Segment ahead = seg;
   int ahead_step = 0;
-  int block = Loader<D>::block_of(a, ahead.b, ahead.first, ahead.len);
-  uint32_t k_scales[kStages - 1], v_scales[kStages - 1];  // of the stages in flight
-  const auto load = [&](int stage, uint32_t& k_scale, uint32_t& v_scale) {
+  int block = Load::block_of(a, ahead.b, ahead.first, ahead.len);
+  uint32_t k_scales[kStages - 1][kHeads], v_scales[kStages - 1][kHeads];  // of the stages in flight
+  const auto load = [&](int stage, uint32_t (&k_scale)[kHeads], uint32_t (&v_scale)[kHeads]) {
     if (ahead.left > 0) {
-      Loader<D>::issue(a, ring + stage * Loader<D>::kStageBytes, block, ahead.sub / a.groups,
-                       ahead.first + ahead_step, ahead.len, k_scale, v_scale);
+      Load::issue(a, ring + stage * Load::kStageBytes, block, Heads<kHeads>(a, ahead.sub),
+                  ahead.first + ahead_step, ahead.len, k_scale, v_scale);
       if (++ahead_step == ahead.n) {
         next_segment(a, line, ahead);
         ahead_step = 0;
       }
-      if (ahead.left > 0) {
-        block = Loader<D>::block_of(a, ahead.b, ahead.first + ahead_step, ahead.len);
-      }
+      if (ahead.left > 0) block = Load::block_of(a, ahead.b, ahead.first + ahead_step, ahead.len);
     }
     cp_async_commit();
   };
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) load(i, k_scales[i], v_scales[i]);
 
-  Queries<D> q;
-  Sums<D> sums;
+  Queries<D> q[kHeads];
+  Sums<D, Load::kWidth> sums[kHeads];
   int stage = 0, at = 0;  // `at`: the step of the segment
   while (true) {
-    const Heads heads(a, seg.sub);
+    const Heads<kHeads> heads(a, seg.sub);
     if (at == 0) {  // rows are on their way meanwhile
-      const uint8_t* src = static_cast<const uint8_t*>(a.q) +
-                           (seg.b * a.q_stride + static_cast<int64_t>(heads.first + g) * D) * 2;
-      q.set(a.scale_log2, [&](int i) {
-        return g < heads.count ? ld_global_nc_v4(src + i * 16) : make_uint4(0, 0, 0, 0);
-      });
-      sums.clear();
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i) {
+        const uint8_t* src =
+            static_cast<const uint8_t*>(a.q) +
+            (seg.b * a.q_stride + static_cast<int64_t>(heads.first + i * a.group + g) * D) * 2;
+        const bool real = i < heads.live && g < heads.count;
+        q[i].set(a.scale_log2, [&](int n) {
+          return real ? ld_global_nc_v4(src + n * 16) : make_uint4(0, 0, 0, 0);
+        });
+        sums[i].clear();
+      }
     }
     cp_async_wait<kStages - 2>();
     __syncwarp();  // every lane's copies have landed, and every lane is done with the stage before
-    const uint32_t scales = k_scales[0] | (v_scales[0] << 8);
+    uint32_t scales[kHeads];
 #pragma unroll
-    for (int i = 0; i + 1 < kStages - 1; ++i) {
-      k_scales[i] = k_scales[i + 1];
-      v_scales[i] = v_scales[i + 1];
+    for (int i = 0; i < kHeads; ++i) {
+      scales[i] = k_scales[0][i] | (v_scales[0][i] << 8);
+#pragma unroll
+      for (int n = 0; n + 1 < kStages - 1; ++n) {
+        k_scales[n][i] = k_scales[n + 1][i];
+        v_scales[n][i] = v_scales[n + 1][i];
+      }
     }
     load(stage == 0 ? kStages - 1 : stage - 1, k_scales[kStages - 2], v_scales[kStages - 2]);
-    sums.step(ring + stage * Loader<D>::kStageBytes, scales,
-              seg.len - (seg.first + at) * kStepRows, q);
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      sums[i].step(ring + stage * Load::kStageBytes, i, scales[i],
+                   seg.len - (seg.first + at) * kStepRows, q[i]);
+    }
     stage = stage + 1 == kStages ? 0 : stage + 1;
     if (++at < seg.n) continue;
 
     // ---- the segment's end: the item's output, or a part
-    sums.reduce();
     const bool cut = seg.n < seg.steps;
-    const int64_t out0 = (static_cast<int64_t>(seg.b) * a.num_heads + heads.first) * D;
     if (seg.first == 0 && lane == 0) {
       // the item ends behind this share by the steps that it lacks
       const int end = line.begin(share + 1) + seg.steps - seg.n;
-      a.table[static_cast<int64_t>(seg.b) * a.num_kv_heads * a.groups + seg.sub] = {
+      a.table[static_cast<int64_t>(seg.b) * a.subs + seg.sub] = {
           share, cut ? line.first_from(end) - share : 1};
     }
-    const int64_t part = (2 * static_cast<int64_t>(share) + (seg.first == 0 ? 1 : 0)) * held_heads;
+    const int64_t part =
+        (2 * static_cast<int64_t>(share) + (seg.first == 0 ? 1 : 0)) * (kHeads * held_heads);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int head = 2 * t + h;
-      if (head >= heads.count) continue;
-      if (cut) {
-        if (g == 0) a.part_ml[part + head] = make_float2(sums.m[h], sums.l[h]);
-        float4* dst = reinterpret_cast<float4*>(a.part_acc + (part + head) * D + g * (D / 8));
+    for (int i = 0; i < kHeads; ++i) {
+      sums[i].reduce();
 #pragma unroll
-        for (int i = 0; i < Sums<D>::kTiles; i += 2) {
-          dst[i / 2] = make_float4(sums.acc[i][h], sums.acc[i][2 + h], sums.acc[i + 1][h],
-                                   sums.acc[i + 1][2 + h]);
-        }
-      } else {
-        const float f = sums.l[h] == 0.0f ? 0.0f : 1.0f / sums.l[h];
-        uint32_t w[Sums<D>::kTiles];
+      for (int h = 0; h < 2; ++h) {
+        const int head = 2 * t + h;
+        if (i >= heads.live || head >= heads.count) continue;
+        if (cut) {
+          const int64_t at_head = part + i * held_heads + head;
+          if (g == 0) a.part_ml[at_head] = make_float2(sums[i].m[h], sums[i].l[h]);
+          float4* dst = reinterpret_cast<float4*>(a.part_acc + at_head * D + g * (D / 8));
 #pragma unroll
-        for (int i = 0; i < Sums<D>::kTiles; ++i) {
-          w[i] = pack_bf16x2(sums.acc[i][h] * f, sums.acc[i][2 + h] * f);
-        }
-        uint8_t* dst = static_cast<uint8_t*>(a.out) + (out0 + head * D + g * (D / 8)) * 2;
+          for (int n = 0; n < D / 16; n += 2) {
+            dst[n / 2] = make_float4(sums[i].acc[n][h], sums[i].acc[n][2 + h],
+                                     sums[i].acc[n + 1][h], sums[i].acc[n + 1][2 + h]);
+          }
+        } else {
+          const float f = sums[i].l[h] == 0.0f ? 0.0f : 1.0f / sums[i].l[h];
+          uint32_t w[D / 16];
 #pragma unroll
-        for (int i = 0; i < Sums<D>::kTiles; i += 4) {
-          st_global_v4(dst + i * 4, make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]));
+          for (int n = 0; n < D / 16; ++n) {
+            w[n] = pack_bf16x2(sums[i].acc[n][h] * f, sums[i].acc[n][2 + h] * f);
+          }
+          const int64_t out =
+              (static_cast<int64_t>(seg.b) * a.num_heads + heads.first + i * a.group + head) * D;
+          uint8_t* dst = static_cast<uint8_t*>(a.out) + (out + g * (D / 8)) * 2;
+#pragma unroll
+          for (int n = 0; n < D / 16; n += 4) {
+            st_global_v4(dst + n * 4, make_uint4(w[n], w[n + 1], w[n + 2], w[n + 3]));
+          }
         }
       }
     }
@@ -608,7 +649,7 @@ __global__ void __launch_bounds__(kLineWarps * kWarpSize, 1) decode_attention_fp
 // outputs. A lane takes four dims of every 4 spread-th part, kJoinBatch of them in flight; its
 // fellows' sums come by shuffles, the other warps' through shared memory. The order is fixed by the
 // sizes, so results repeat.
-template <int D>
+template <int D, int kHeads>
 __global__ void __launch_bounds__(kJoinThreads) decode_attention_fp8_join(
     const __grid_constant__ AttnArgs a, int spread) {
   grid_dependency_sync();
@@ -618,15 +659,15 @@ __global__ void __launch_bounds__(kJoinThreads) decode_attention_fp8_join(
   __shared__ float2 others_ml[kWarps];
   const JoinEntry entry = a.table[blockIdx.x];
   if (entry.parts <= 1) return;
-  const int subs = a.num_kv_heads * a.groups;
-  const int b = static_cast<int>(blockIdx.x) / subs;
-  const Heads heads(a, static_cast<int>(blockIdx.x) - b * subs);
+  const int b = static_cast<int>(blockIdx.x) / a.subs;
+  const Heads<kHeads> heads(a, static_cast<int>(blockIdx.x) - b * a.subs);
   const int held_heads = min(a.group, kGroup);
   const int warp = threadIdx.x / kWarpSize, lane = threadIdx.x % kWarpSize;
   const int mate = warp % spread;  // this warp's place among those of its run
   const int run = (static_cast<int>(blockIdx.y) * kWarps + warp) / spread;
-  const int head = run / kRuns;
-  const bool real = head < heads.count;
+  const int kv = run / (kRuns * heads.count);  // of the item's KV heads
+  const int head = run / kRuns - kv * heads.count;
+  const bool real = kv < heads.live;
   const int d = run % kRuns * 32 + lane % 8 * 4;
   float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float m = -FLT_MAX, l = 0.0f;
@@ -642,7 +683,8 @@ __global__ void __launch_bounds__(kJoinThreads) decode_attention_fp8_join(
       if (p < entry.parts) {
         // the first part is the one that begins the item; the others continue it
         const int64_t at =
-            (2 * static_cast<int64_t>(entry.share + p) + (p == 0 ? 1 : 0)) * held_heads + head;
+            (2 * static_cast<int64_t>(entry.share + p) + (p == 0 ? 1 : 0)) * (kHeads * held_heads) +
+            kv * held_heads + head;
         ml[i] = a.part_ml[at];
         x[i] = *reinterpret_cast<const float4*>(a.part_acc + at * D + d);
       }
@@ -696,7 +738,8 @@ __global__ void __launch_bounds__(kJoinThreads) decode_attention_fp8_join(
   if (lane < 8 && real) {
     const float r = l == 0.0f ? 0.0f : 1.0f / l;
     uint8_t* dst = static_cast<uint8_t*>(a.out) +
-                   ((static_cast<int64_t>(b) * a.num_heads + heads.first + head) * D + d) * 2;
+                   ((static_cast<int64_t>(b) * a.num_heads + heads.first + kv * a.group + head) *
+                        D + d) * 2;
     *reinterpret_cast<uint2*>(dst) =
         make_uint2(pack_bf16x2(acc.x * r, acc.y * r), pack_bf16x2(acc.z * r, acc.w * r));
   }
@@ -705,7 +748,7 @@ __global__ void __launch_bounds__(kJoinThreads) decode_attention_fp8_join(
 // ------------------------------------------------------------------------------------- by items
 
 template <int D>
-__global__ void __launch_bounds__(kItemWarps * kWarpSize, 1) decode_attention_fp8_items(
+__global__ void __launch_bounds__(kItemWarps * kWarpSize, D == 128 ? 1 : 2) decode_attention_fp8_items(
     const __grid_constant__ AttnArgs a) {
   grid_dependency_sync();
   constexpr int kThreads = kItemWarps * kWarpSize;
@@ -716,12 +759,12 @@ __global__ void __launch_bounds__(kItemWarps * kWarpSize, 1) decode_attention_fp
   const int lane = threadIdx.x % kWarpSize;
   const int g = lane >> 2;
   const int t = lane & 3;
-  const int subs = a.num_kv_heads * a.groups;
+  using Load = Loader<D, 1>;
   const int item = static_cast<int>(blockIdx.x) / a.splits;
   const int split = static_cast<int>(blockIdx.x) - item * a.splits;
-  const int b = item / subs, sub = item - b * subs;
-  const Heads heads(a, sub);
-  const uint32_t ring = smem_addr(smem) + warp * kStages * Loader<D>::kStageBytes;
+  const int b = item / a.subs, sub = item - b * a.subs;
+  const Heads<1> heads(a, sub);
+  const uint32_t ring = smem_addr(smem) + warp * kStages * Load::kStageBytes;
 
   const int n = __ldg(a.seq_lens + b);
   if (threadIdx.x == 0 && (n < 0 || n > a.max_rows)) raise_error(a.err, kErrBadIndex);
@@ -731,14 +774,12 @@ __global__ void __launch_bounds__(kItemWarps * kWarpSize, 1) decode_attention_fp
   const int steps = min(item_steps(len), (split + 1) * of_split);
   const int begin = split * of_split + warp;
 
-  int block = Loader<D>::block_of(a, b, begin, len);
-  uint32_t k_scales[kStages], v_scales[kStages];
-  const auto load = [&](int stage, int step, uint32_t& k_scale, uint32_t& v_scale) {
-    k_scale = v_scale = kScaleBias;
+  int block = Load::block_of(a, b, begin, len);
+  uint32_t k_scales[kStages][1], v_scales[kStages][1];
+  const auto load = [&](int stage, int step, uint32_t (&k_scale)[1], uint32_t (&v_scale)[1]) {
     if (step < steps) {
-      Loader<D>::issue(a, ring + stage * Loader<D>::kStageBytes, block, sub / a.groups, step, len,
-                       k_scale, v_scale);
-      block = Loader<D>::block_of(a, b, step + kItemWarps, len);
+      Load::issue(a, ring + stage * Load::kStageBytes, block, heads, step, len, k_scale, v_scale);
+      block = Load::block_of(a, b, step + kItemWarps, len);
     }
     cp_async_commit();
   };
@@ -752,18 +793,18 @@ __global__ void __launch_bounds__(kItemWarps * kWarpSize, 1) decode_attention_fp
   q.set(a.scale_log2, [&](int i) {
     return g < heads.count ? ld_global_nc_v4(src + i * 16) : make_uint4(0, 0, 0, 0);
   });
-  Sums<D> sums;
+  Sums<D, D> sums;
   sums.clear();
   int stage = 0;
   for (int step = begin; step < steps; step += kItemWarps) {
     cp_async_wait<kStages - 1>();
     __syncwarp();
-    sums.step(ring + stage * Loader<D>::kStageBytes, k_scales[0] | (v_scales[0] << 8),
+    sums.step(ring + stage * Load::kStageBytes, 0, k_scales[0][0] | (v_scales[0][0] << 8),
               len - step * kStepRows, q);
 #pragma unroll
     for (int i = 0; i + 1 < kStages; ++i) {
-      k_scales[i] = k_scales[i + 1];
-      v_scales[i] = v_scales[i + 1];
+      k_scales[i][0] = k_scales[i + 1][0];
+      v_scales[i][0] = v_scales[i + 1][0];
     }
     __syncwarp();  // every lane is done with the stage
     load(stage, step + kStages * kItemWarps, k_scales[kStages - 1], v_scales[kStages - 1]);
@@ -783,7 +824,7 @@ __global__ void __launch_bounds__(kItemWarps * kWarpSize, 1) decode_attention_fp
     }
     float4* dst = reinterpret_cast<float4*>(accs + (warp * heads.count + head) * D + g * (D / 8));
 #pragma unroll
-    for (int i = 0; i < Sums<D>::kTiles; i += 2) {
+    for (int i = 0; i < D / 16; i += 2) {
       dst[i / 2] = make_float4(sums.acc[i][h], sums.acc[i][2 + h], sums.acc[i + 1][h],
                                sums.acc[i + 1][2 + h]);
     }
@@ -851,8 +892,8 @@ int64_t line_shares(int device) { return static_cast<int64_t>(sm_count(device)) 
 
 template <int D>
 int launch_items(const AttnArgs& a, int64_t items, int device, cudaStream_t stream) {
-  const size_t smem = static_cast<size_t>(kItemWarps) * kStages * Loader<D>::kStageBytes;
-  static_assert(kItemWarps * kStages * Loader<D>::kStageBytes >= (kItemWarps + 1) * kGroup * D * 4,
+  const size_t smem = static_cast<size_t>(kItemWarps) * kStages * Loader<D, 1>::kStageBytes;
+  static_assert(kItemWarps * kStages * Loader<D, 1>::kStageBytes >= (kItemWarps + 1) * kGroup * D * 4,
                 "the merge takes the rings");
   const auto kernel = decode_attention_fp8_items<D>;
   if (blocks_per_sm(reinterpret_cast<const void*>(kernel), kItemWarps * kWarpSize, smem, device) <=
@@ -863,11 +904,11 @@ int launch_items(const AttnArgs& a, int64_t items, int device, cudaStream_t stre
                 dim3(kItemWarps * kWarpSize), smem, stream, static_cast<unsigned>(a.splits), a);
 }
 
-template <int D>
+template <int D, int kHeads>
 int launch_lines(const AttnArgs& a, int64_t items, int device, cudaStream_t stream) {
   const int heads = a.group < kGroup ? a.group : kGroup;
-  const size_t smem = static_cast<size_t>(kLineWarps) * kStages * Loader<D>::kStageBytes;
-  const auto kernel = decode_attention_fp8_lines<D>;
+  const size_t smem = static_cast<size_t>(kLineWarps) * kStages * Loader<D, kHeads>::kStageBytes;
+  const auto kernel = decode_attention_fp8_lines<D, kHeads>;
   if (blocks_per_sm(reinterpret_cast<const void*>(kernel), kLineWarps * kWarpSize, smem, device) <=
       0) {
     return SVLLM_ERR_CUDA;
@@ -880,9 +921,9 @@ int launch_lines(const AttnArgs& a, int64_t items, int device, cudaStream_t stre
   const int64_t parts = line_shares(device) / items + 2;
   int spread = 1;
   while (spread < kJoinThreads / kWarpSize && parts > 16 * spread) spread *= 2;
-  const int runs = heads * (D / 32) * spread;
+  const int runs = kHeads * heads * (D / 32) * spread;
   const unsigned slices = static_cast<unsigned>((runs * kWarpSize + kJoinThreads - 1) / kJoinThreads);
-  return launch(decode_attention_fp8_join<D>, dim3(static_cast<unsigned>(items), slices),
+  return launch(decode_attention_fp8_join<D, kHeads>, dim3(static_cast<unsigned>(items), slices),
                 dim3(kJoinThreads), 0, stream, 1u, a, spread);
 }
 
@@ -908,19 +949,29 @@ constexpr int64_t kMaxRows = kInt - kStepRows;
 
 // How a call is dealt to CTAs, and its workspace: none by items.
 struct Workspace {
+  int64_t side_by_side;  // KV heads of an item
+  int64_t subs;          // items of a request
   int64_t items, splits, ml, acc, bytes;
   Workspace(int64_t num_seqs, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim,
             int64_t max_rows, int device) {
     const int64_t group = num_heads / num_kv_heads;
+    const int64_t groups = (group + kGroup - 1) / kGroup;
     const int64_t held = group < kGroup ? group : kGroup;
-    items = num_seqs * num_kv_heads * ((group + kGroup - 1) / kGroup);
+    ml = acc = bytes = 0;
+    side_by_side = 1;
     // shared memory leaves room for one CTA by items on an SM at head_dim 128, registers for two at 64
+    subs = num_kv_heads * groups;
+    items = num_seqs * subs;
     splits = item_splits(max_rows, items, sm_count(device) * (head_dim == 128 ? 1 : 2));
+    if (splits > 0) return;
+    const int64_t steps = items * ((max_rows + kStepRows - 1) / kStepRows) / line_shares(device);
+    side_by_side = head_dim == 64 && steps >= kPairSteps ? kPair : 1;
+    subs = (num_kv_heads + side_by_side - 1) / side_by_side * groups;
+    items = num_seqs * subs;
+    const int64_t parts = 2 * line_shares(device) * side_by_side * held;
     ml = round_up(items * static_cast<int64_t>(sizeof(JoinEntry)), 256);
-    acc = ml + round_up(2 * line_shares(device) * held * static_cast<int64_t>(sizeof(float2)), 256);
-    bytes = splits > 0 ? 0
-                       : acc + 2 * line_shares(device) * held * head_dim *
-                                   static_cast<int64_t>(sizeof(float));
+    acc = ml + round_up(parts * static_cast<int64_t>(sizeof(float2)), 256);
+    bytes = acc + parts * head_dim * static_cast<int64_t>(sizeof(float));
   }
 };
 
@@ -1007,6 +1058,7 @@ extern "C" int svllm_decode_attention_fp8_bf16(
   a.num_kv_heads = static_cast<int>(num_kv_heads);
   a.group = static_cast<int>(group);
   a.groups = static_cast<int>(groups);
+  a.subs = static_cast<int>(w.subs);
   a.scale_log2 = static_cast<float>(static_cast<double>(scale) / std::log(2.0));
   a.num_seqs = static_cast<int>(num_seqs);
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
@@ -1020,6 +1072,7 @@ extern "C" int svllm_decode_attention_fp8_bf16(
   a.table = reinterpret_cast<JoinEntry*>(base);
   a.part_ml = reinterpret_cast<float2*>(base + w.ml);
   a.part_acc = reinterpret_cast<float*>(base + w.acc);
-  return head_dim == 128 ? launch_lines<128>(a, w.items, device, s)
-                         : launch_lines<64>(a, w.items, device, s);
+  if (head_dim == 128) return launch_lines<128, 1>(a, w.items, device, s);
+  return w.side_by_side == kPair ? launch_lines<64, kPair>(a, w.items, device, s)
+                                 : launch_lines<64, 1>(a, w.items, device, s);
 }

@@ -287,6 +287,15 @@ def test_attention(device, heads, kv_heads, dim, block):
     ([2000, 1500, 3], 27, 3, 64, 16, None),
     ([700] * 8, 8, 8, 128, 16, None),
     ([500, 1] * 10, 16, 16, 64, 16, None),
+    # by lines, KV heads of 64 in pairs, the last one alone
+    ([9000, 70, 0, 4000], 9, 3, 64, 16, None),
+    ([9000, 33], 27, 3, 64, 12, None),
+    ([600, 1, 77] * 50, 10, 5, 64, 16, None),
+    ([3000, 5, 2000, 100] * 16, 8, 4, 64, 1, None),
+    ([3000, 5, 2000, 100] * 12, 33, 3, 128, 16, None),
+    ([700, 33, 0, 2000] * 4, 27, 3, 64, 16, 2000),
+    ([700, 33, 1, 2000] * 4, 3, 1, 64, 12, 9000),
+    ([90, 4100], 40, 5, 64, 256, 800),
 ])
 def test_attention_long(cuda, lens, heads, kv_heads, dim, block, width):
     check_attention(cuda, lens, heads, kv_heads, dim, block, width=width)
