@@ -27,13 +27,24 @@
 //     pair their codes before the conversion; P^T comes from S^T by movmatrix.
 //
 // Work. An item is one (request, KV head, group of up to eight query heads). Rows travel by cp.async,
-// 16 bytes a lane, into a ring of stages that each warp owns. Two kernels:
+// 16 bytes a lane, into a ring of two stages that each warp owns. Two kernels:
 //   * By lines (long tables, or many items): the steps of all items form one line, in that order,
 //     of which each warp takes an equal share, found from the device-side lengths. A warp runs on
 //     from item to item without waiting for another; the parts of items that are cut go to a
-//     workspace, and a third kernel joins them in a fixed order.
+//     workspace, and a third kernel joins them in a fixed order. Head_dim 64: two KV heads an item,
+//     so that a row's copy fills a 128-byte line (the L2's requests bound the kernel otherwise).
 //   * By items (short tables and few items): a CTA takes an item, its warps deal the steps among
-//     them and merge through shared memory. One launch.
+//     them and merge through shared memory; up to eight CTAs share an item as a thread-block cluster,
+//     which merges through distributed shared memory. One launch.
+//
+// What bounds it, measured on a B200 (16/8 heads of 128, us in a graph): 64 requests of 2064 to 4096
+// rows, 407 MB, 77-79. The warps stream at 6.6 TB/s once they run, 62 us; 2.5 us go by before the
+// first rows are asked for (lengths, then the table, each a trip to memory), 3 between the first and
+// the last warp's end, 4 in the join, 2 between the kernels. One request of 32760 rows: 19.5, of
+// which 10.5 are the stream. Steps of 32 rows take 600 warp instructions, 38 % of the issue slots.
+// Neither more loads in flight (three stages, twelve or fourteen warps, the next load after the
+// products: 79 to 83 us) nor a CTA per share whose warps merge at every item's end (98) did better;
+// registers instead of shared memory for the rows took 168.
 #include <cuda_runtime.h>
 
 #include <cfloat>
@@ -61,7 +72,10 @@ constexpr int kPair = 2, kPairSteps = 14;
 constexpr int kMaxSplits = 8;    // CTAs of an item: the portable cluster size
 constexpr int kItemSteps = 4;    // by items up to this many steps of a warp
 constexpr int kJoinThreads = 256;
-constexpr int kJoinBatch = 8;    // parts a thread of the join has in flight
+// Parts a lane of the join has in flight: few where an item has few parts, which most lanes do not
+// have (us, 1, 2 and 8: 128 requests of 512-1024 rows, 32/8 heads of 64, 3 parts, 29.0, 29.3, 31.0; 24
+// of 2048-4096, 28/4 of 128, 14 parts, 23.3, 23.6, 21.4).
+constexpr int kJoinFew = 2, kJoinMany = 8, kJoinFewParts = 5;
 // The running maximum is moved only when a score passes it by kSlack, so that most steps need one
 // vote instead of a maximum over the warp. Weights reach 2^(kWeightBits + kSlack).
 constexpr float kWeightBits = 6.0f, kSlack = 8.0f;
@@ -646,10 +660,10 @@ __global__ void __launch_bounds__(kLineWarps * kWarpSize, 1) decode_attention_fp
 }
 
 // Joins the parts of the items that were cut: blockIdx.x the item, `spread` warps for each 32 of its
-// outputs. A lane takes four dims of every 4 spread-th part, kJoinBatch of them in flight; its
+// outputs. A lane takes four dims of every 4 spread-th part, kBatch of them in flight; its
 // fellows' sums come by shuffles, the other warps' through shared memory. The order is fixed by the
 // sizes, so results repeat.
-template <int D, int kHeads>
+template <int D, int kHeads, int kBatch>
 __global__ void __launch_bounds__(kJoinThreads) decode_attention_fp8_join(
     const __grid_constant__ AttnArgs a, int spread) {
   grid_dependency_sync();
@@ -672,11 +686,11 @@ __global__ void __launch_bounds__(kJoinThreads) decode_attention_fp8_join(
   float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float m = -FLT_MAX, l = 0.0f;
   const int step = 4 * spread;
-  for (int p0 = lane / 8 * spread + mate; real && p0 < entry.parts; p0 += step * kJoinBatch) {
-    float2 ml[kJoinBatch];
-    float4 x[kJoinBatch];
+  for (int p0 = lane / 8 * spread + mate; real && p0 < entry.parts; p0 += step * kBatch) {
+    float2 ml[kBatch];
+    float4 x[kBatch];
 #pragma unroll
-    for (int i = 0; i < kJoinBatch; ++i) {
+    for (int i = 0; i < kBatch; ++i) {
       const int p = p0 + i * step;
       ml[i] = make_float2(-FLT_MAX, 0.0f);
       x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -691,12 +705,12 @@ __global__ void __launch_bounds__(kJoinThreads) decode_attention_fp8_join(
     }
     float mx = m;
 #pragma unroll
-    for (int i = 0; i < kJoinBatch; ++i) mx = fmaxf(mx, ml[i].x);
+    for (int i = 0; i < kBatch; ++i) mx = fmaxf(mx, ml[i].x);
     const float f = exp2_approx(m - mx);
     l *= f;
     acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
 #pragma unroll
-    for (int i = 0; i < kJoinBatch; ++i) {
+    for (int i = 0; i < kBatch; ++i) {
       const float w = exp2_approx(ml[i].x - mx);
       l = fmaf(ml[i].y, w, l);
       acc = make_float4(fmaf(x[i].x, w, acc.x), fmaf(x[i].y, w, acc.y), fmaf(x[i].z, w, acc.z),
@@ -923,7 +937,9 @@ int launch_lines(const AttnArgs& a, int64_t items, int device, cudaStream_t stre
   while (spread < kJoinThreads / kWarpSize && parts > 16 * spread) spread *= 2;
   const int runs = kHeads * heads * (D / 32) * spread;
   const unsigned slices = static_cast<unsigned>((runs * kWarpSize + kJoinThreads - 1) / kJoinThreads);
-  return launch(decode_attention_fp8_join<D, kHeads>, dim3(static_cast<unsigned>(items), slices),
+  const auto join = parts <= kJoinFewParts ? decode_attention_fp8_join<D, kHeads, kJoinFew>
+                                           : decode_attention_fp8_join<D, kHeads, kJoinMany>;
+  return launch(join, dim3(static_cast<unsigned>(items), slices),
                 dim3(kJoinThreads), 0, stream, 1u, a, spread);
 }
 
