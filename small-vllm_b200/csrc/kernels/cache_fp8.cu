@@ -12,11 +12,12 @@
 // keep all of fp32's precision and sincospif never takes its slow path.
 //
 // The bound is memory: per token 4 Hq D + 4 Hk D bytes of bf16 and 2 Hk (D + 1) of cache. Measured on
-// a B200 (us in a graph; bytes at the copy rate): 16/8 heads of 128, 1 token 2.3, 256 tokens 3.5 (0.6),
-// 65536 tokens 146-151 (146); 24/8 heads of 64, 5003 tokens 8.9 (7.2). Small batches are a launch and
-// three trips to memory. What made it fast: positions and slots loaded a token ahead (213 to 152 with
-// the next two), no branch per head (values that are not finite are found at a token's end and the
-// token done again), the norm's weights folded into the rotation once a token, packed fp32 pairs.
+// a B200 (us in a graph; in brackets the bytes at the copy rate): 16/8 heads of 128, 1 token 2.3, 256
+// tokens 3.5 (0.6), 65536 tokens 146-151 (146); 24/8 heads of 64, 5003 tokens 8.9 (7.2). Small batches
+// are a launch and three trips to memory. 65536 tokens took 197 with loads to registers and 209 with
+// the first ring of bulk copies; since then positions and slots are loaded a token ahead, no head has
+// a branch (a token with a value that is not finite is done again at its end), the norm's weights are
+// folded into the rotation once a token, and fp32 values are worked on in pairs.
 //
 // svllm_cache_read_fp8_bf16: the rows of whole requests back in bf16 (exact), as pages in the
 // order of the request: [num_seqs, max_blocks * block_size, Hk, D], zeros behind a request's end. 32
@@ -37,10 +38,11 @@ namespace {
 constexpr int kMaxHalf = 64;  // head_dim 64 or 128
 constexpr int kThreads = 256;
 constexpr int kBulkWarps = 12, kBulkMinWarps = 4;
-constexpr int kBulkStages = 2;  // a third costs small batches more than it gives large ones (T = 5003, 16/8
-                                // of 128: 18.0, 19.6 us; 65536: 151, 147)
-// More passes than so many per SM take the bulk kernel (16/8 heads of 128, us direct and bulk: 256 tokens
-// 3.6, 4.5; 400 5.4, 4.5; 1184 9.1, 5.0; 24/8 of 64: 400 2.6, 3.3; 600 3.6, 3.4; 1184 4.5, 3.5).
+// A third stage takes from middling batches what it gives large ones (us with two and three, 16/8 heads
+// of 128: 5003 tokens 18.0, 19.6; 65536 151.4, 147.1).
+constexpr int kBulkStages = 2;
+// More passes than so many per SM take the bulk kernel (us direct and bulk, 16/8 heads of 128: 256
+// tokens 3.6, 4.5; 400 5.4, 4.5; 1184 9.1, 5.0; 24/8 of 64: 400 2.6, 3.3; 600 3.6, 3.4; 1184 4.5, 3.5).
 constexpr int kDirectPassesPerSm = 16;
 constexpr int64_t kBulkSmem = 210 * 1024;
 constexpr int kReadVecs = 4;  // 16-code vectors a thread of the read-back takes

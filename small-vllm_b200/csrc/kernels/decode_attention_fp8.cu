@@ -38,13 +38,13 @@
 //     which merges through distributed shared memory. One launch.
 //
 // What bounds it, measured on a B200 (16/8 heads of 128, us in a graph): 64 requests of 2064 to 4096
-// rows, 407 MB, 77-79. The warps stream at 6.6 TB/s once they run, 62 us; 2.5 us go by before the
-// first rows are asked for (lengths, then the table, each a trip to memory), 3 between the first and
-// the last warp's end, 4 in the join, 2 between the kernels. One request of 32760 rows: 19.5, of
-// which 10.5 are the stream. Steps of 32 rows take 600 warp instructions, 38 % of the issue slots.
-// Neither more loads in flight (three stages, twelve or fourteen warps, the next load after the
-// products: 79 to 83 us) nor a CTA per share whose warps merge at every item's end (98) did better;
-// registers instead of shared memory for the rows took 168.
+// rows, 407 MB, 77-79. The warps stream at 6.6 TB/s once they run, 62 us; 4.7 us go by until the
+// first rows are there (lengths, table, rows, each a trip to memory after the other), warps end up to
+// 5 apart, and the join takes 4. One request of 32760 rows: 19.5, of which 10.5 are the stream. A
+// step of 32 rows takes 570 warp instructions; 38 % of the issue slots are used. More loads in flight
+// gave nothing (three stages 79.1, twelve warps 77.1-78.9, fourteen 81.5, the next load after the
+// products 80.7); a CTA per share whose warps merge at every item's end took 98, rows loaded to
+// registers instead of shared memory 168.
 #include <cuda_runtime.h>
 
 #include <cfloat>
@@ -73,9 +73,10 @@ constexpr int kMaxSplits = 8;    // CTAs of an item: the portable cluster size
 constexpr int kItemSteps = 4;    // by items up to this many steps of a warp
 constexpr int kJoinThreads = 256;
 // Parts a lane of the join has in flight: few where an item has few parts, which most lanes do not
-// have (us, 1, 2 and 8: 128 requests of 512-1024 rows, 32/8 heads of 64, 3 parts, 29.0, 29.3, 31.0; 24
-// of 2048-4096, 28/4 of 128, 14 parts, 23.3, 23.6, 21.4).
-constexpr int kJoinFew = 2, kJoinMany = 8, kJoinFewParts = 5;
+// have (us, 2 and 8: 148 requests of 512-1024 rows, 16/8 heads of 128, 3 parts, 50.9, 53.1; 64 of
+// 2048-4096, 4 parts, 78.5, 78.8; 48, 5 parts, 62.0, 61.1; 36, 6 parts, 48.4, 47.3; 24, 28/4 heads, 14
+// parts, 23.6, 21.4).
+constexpr int kJoinFew = 2, kJoinMany = 8, kJoinFewParts = 4;
 // The running maximum is moved only when a score passes it by kSlack, so that most steps need one
 // vote instead of a maximum over the warp. Weights reach 2^(kWeightBits + kSlack).
 constexpr float kWeightBits = 6.0f, kSlack = 8.0f;
