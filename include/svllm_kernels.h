@@ -63,7 +63,8 @@ typedef enum svllm_status {
 /* Bits of the device error word. */
 #define SVLLM_DEVERR_BAD_INDEX 1    /* an embedding id outside [0, vocab) (its row is zeroed), a KV
                                        slot past the cache (nothing written), or an index of a
-                                       paged batch that its entry point documents */
+                                       paged batch or a scale of an 8-bit cache that its entry
+                                       point documents */
 #define SVLLM_DEVERR_WAIT_TIMEOUT 2 /* a bulk copy did not land in time: the kernel stopped */
 
 /* Index dtype of positions / token ids. */
@@ -487,8 +488,10 @@ int svllm_rope_cache_fp8_bf16(void* q, const void* k, const void* v, const void*
  * block_size, num_kv_heads, head_dim], row j of request s from slot block_tables[s][j / block_size]
  * * block_size + j % block_size for j < seq_lens[s], zeros behind. Seen as [num_seqs * max_blocks,
  * block_size, ...] the outputs are a paged bf16 cache in which page p of request s is block s *
- * max_blocks + p. k_out and v_out 32-byte aligned, else SVLLM_ERR_UNSUPPORTED. A length outside [0, max_blocks * block_size] is clamped and a table entry
- * outside the cache read as block 0, either with SVLLM_DEVERR_BAD_INDEX.
+ * max_blocks + p. k_out and v_out 32-byte aligned, else SVLLM_ERR_UNSUPPORTED. With
+ * SVLLM_DEVERR_BAD_INDEX: a length outside [0, max_blocks * block_size] is clamped, a table entry
+ * outside the cache read as block 0, and a read row's scale outside [2^-60, 2^60], which the write
+ * above never leaves, taken as the nearest of these.
  */
 int svllm_cache_read_fp8_bf16(void* k_out, void* v_out, const void* k_cache, const void* v_cache,
                               const void* k_scale, const void* v_scale, int64_t num_blocks,
@@ -499,14 +502,14 @@ int svllm_cache_read_fp8_bf16(void* k_out, void* v_out, const void* k_cache, con
 /*
  * Decode attention (svllm_paged_decode_attention_bf16) over the 8-bit cache: out[b, h] =
  * softmax_j(scale * q[b, h] . k_j) v_j over the rows j < seq_lens[b], k_j and v_j codes times
- * scales. Any number of query heads per KV head; q and out 16-byte aligned, a q_token_stride of whole
- * 16 bytes, else SVLLM_ERR_UNSUPPORTED; scale positive and finite, as is scale / ln 2. Products in f16 on exact codes,
- * the softmax numerators rounded to f16 for the second; scores, maxima and sums in fp32. A request
- * of length 0, and a head with no score above -infinity, gives zeros. Lengths and table entries out
- * of range as in svllm_cache_read_fp8_bf16. workspace: at least
+ * scales. Any number of query heads per KV head; q and out 16-byte aligned, a q_token_stride of
+ * whole 16 bytes, else SVLLM_ERR_UNSUPPORTED; scale positive and finite, as is scale / ln 2. Products
+ * in f16 on exact codes, the softmax numerators times V's scales rounded to f16 for the second (those
+ * below 2^-31 of a head's largest may be lost); scores, maxima and sums in fp32. A request of length
+ * 0, and a head with no score above -infinity, gives zeros. Lengths, table entries and scales out of
+ * range as in svllm_cache_read_fp8_bf16. workspace: at least
  * svllm_decode_attention_fp8_workspace_bytes bytes of device memory (NULL where that is 0), 16-byte
- * aligned, any contents;
- * calls that overlap on the GPU must not share it. Results repeat bit for bit.
+ * aligned, any contents; calls that overlap on the GPU must not share it. Results repeat bit for bit.
  */
 int svllm_decode_attention_fp8_bf16(void* out, const void* q, int64_t q_token_stride,
                                     const void* k_cache, const void* v_cache, const void* k_scale,

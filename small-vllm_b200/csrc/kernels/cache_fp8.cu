@@ -373,11 +373,11 @@ __device__ __forceinline__ int64_t position_of(const CacheWriteArgs& a, int64_t 
                       : __ldg(static_cast<const int*>(a.positions) + t);
 }
 
-// A token's slot, negative for "write no cache"; one past the cache raises the error word.
 __device__ __forceinline__ int64_t slot_of(const CacheWriteArgs& a, int64_t t) {
   return __ldg(reinterpret_cast<const long long*>(a.slots) + t);
 }
 
+// A token's slot, negative for "write no cache"; one past the cache raises the error word.
 __device__ __forceinline__ int64_t checked_slot(const CacheWriteArgs& a, int64_t slot) {
   if (slot >= a.num_slots) {
     if (threadIdx.x % kWarpSize == 0) raise_error(a.err, kErrBadIndex);
@@ -729,7 +729,9 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(
   for (int i = 0; i < kReadVecs; ++i) {
     const int64_t v = first + i * kThreads + threadIdx.x;
     if (v >= all) break;
-    const float f = scale_value(scale[i]);
+    const uint32_t used = scale_in_range(scale[i]);
+    if (used != scale[i]) raise_error(a.err, kErrBadIndex);
+    const float f = scale_value(used);
     const uint2 d0 = dequantise4(codes[i].x, f), d1 = dequantise4(codes[i].y, f);
     const uint2 d2 = dequantise4(codes[i].z, f), d3 = dequantise4(codes[i].w, f);
     st_global_v8(out + v * 32, make_uint4(d0.x, d0.y, d1.x, d1.y),

@@ -10,13 +10,14 @@
 // code is an f16 number, so converting costs one instruction for two codes and nothing in
 // precision. The other operands are made to fit f16's range by powers of two: q of each head is
 // scaled so that its largest magnitude lies in [2^14, 2^15) (exact for all elements down to 2^-32
-// of it), and the weights are w_j = 2^(y_j - m + 14) with y_j = x_j + ev_j, x_j the score in base
-// 2 and m the running maximum of y_j, so w_j <= 2^14 and the smallest f16 stands for 2^-38 of the
-// largest weight. The rows' scales thus never touch the codes: 2^ek multiplies a score, ev adds to
+// of it), and the weights are w_j = 2^(y_j - m + 6) with y_j = x_j + ev_j, x_j the score in base 2
+// and m a maximum of the y_j that is moved only when one passes it by 8: w_j <= 2^14, the largest is
+// 2^6 at least, and f16's smallest number, 2^-24, stands for 2^-30 of it or less (a weight below half
+// of that is lost). The rows' scales thus never touch the codes: 2^ek multiplies a score, ev adds to
 // it (in the one rounding of an fma), and the denominator is l = sum_j w_j 2^-ev_j, in fp32. (The
 // weights are taken from y and p from them, not the other way round: at scores so large that x + ev
-// rounds, both then carry the same error, and no weight passes 2^14.) The weights are rounded to
-// f16 (2^-11 of each, an eighth of a bf16 rounding) because the product takes no wider operand.
+// rounds, both then carry the same error, and no weight passes 2^14.) The weights are rounded to f16
+// (2^-11 of each, an eighth of a bf16 rounding) because the product takes no wider operand.
 //
 // Layout. A warp takes steps of 32 cached rows, lane = 4 g + t:
 //   S^T[16 rows x 8 heads] = K[16 x D] . Q^T[D x 8]: lane holds rows g, g + 8 of K, 16 bytes at
@@ -168,6 +169,13 @@ __device__ __forceinline__ uint32_t tile_at(int r, int c) {
     return static_cast<uint32_t>((r >> 1) * 128 + (((r ^ (r >> 2)) & 1) << 6) +
                                  ((c ^ (((r >> 1) & 1) << 1)) << 4));
   }
+}
+
+// The scale bytes of a row's K and V in one word, as they are used.
+__device__ __forceinline__ uint32_t scales_of(const AttnArgs& a, uint32_t k, uint32_t v) {
+  const uint32_t ks = scale_in_range(k), vs = scale_in_range(v);
+  if (ks != k || vs != v) raise_error(a.err, kErrBadIndex);
+  return ks | (vs << 8);
 }
 
 // A request's length, and the steps of its items: one at least, so that a request without rows
@@ -595,7 +603,7 @@ __global__ void __launch_bounds__(kLineWarps * kWarpSize, 1) decode_attention_fp
     uint32_t scales[kHeads];
 #pragma unroll
     for (int i = 0; i < kHeads; ++i) {
-      scales[i] = k_scales[0][i] | (v_scales[0][i] << 8);
+      scales[i] = scales_of(a, k_scales[0][i], v_scales[0][i]);
 #pragma unroll
       for (int n = 0; n + 1 < kStages - 1; ++n) {
         k_scales[n][i] = k_scales[n + 1][i];
@@ -814,7 +822,7 @@ __global__ void __launch_bounds__(kItemWarps * kWarpSize, D == 128 ? 1 : 2) deco
   for (int step = begin; step < steps; step += kItemWarps) {
     cp_async_wait<kStages - 1>();
     __syncwarp();
-    sums.step(ring + stage * Load::kStageBytes, 0, k_scales[0][0] | (v_scales[0][0] << 8),
+    sums.step(ring + stage * Load::kStageBytes, 0, scales_of(a, k_scales[0][0], v_scales[0][0]),
               len - step * kStepRows, q);
 #pragma unroll
     for (int i = 0; i + 1 < kStages; ++i) {

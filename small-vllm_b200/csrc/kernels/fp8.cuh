@@ -34,8 +34,15 @@ __device__ __forceinline__ float exp2_int(int e) {
   return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
 }
 
-// 2^(b - 127) of an e8m0 byte b. The bytes this library writes lie in [67, 187].
+// 2^(b - 127) of an e8m0 byte b in [1, 254].
 __device__ __forceinline__ float scale_value(uint32_t b) { return __uint_as_float(b << 23); }
+
+// A scale byte as it is used: the nearest of those that the writer leaves. Further out, 2^e or what is
+// multiplied with it would leave fp32, and 255 is e8m0's NaN.
+__device__ __forceinline__ uint32_t scale_in_range(uint32_t b) {
+  return min(max(b, static_cast<uint32_t>(kScaleMin + kScaleBias)),
+             static_cast<uint32_t>(kScaleMax + kScaleBias));
+}
 
 // Two values rounded to nearest even and saturated to e4m3 codes, lo in the low byte (a NaN
 // becomes 0x7f).

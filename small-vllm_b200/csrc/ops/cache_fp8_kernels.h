@@ -8,10 +8,10 @@
 namespace svllm::ops {
 
 namespace cpu_impl {
-// Throws for a request whose length passes its table or whose table names a block outside the
-// cache.
-void check_pages(const char* op, const at::Tensor& k_cache, const at::Tensor& block_tables,
-                 const at::Tensor& seq_lens);
+// Throws for a request whose length passes its table, whose table names a block outside the cache, or
+// with a row whose scale lies outside [2^-60, 2^60].
+void check_pages(const char* op, const at::Tensor& k_scale, const at::Tensor& v_scale,
+                 const at::Tensor& block_tables, const at::Tensor& seq_lens);
 void cache_read_fp8(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache,
                     const at::Tensor& v_cache, const at::Tensor& k_scale,
                     const at::Tensor& v_scale, const at::Tensor& block_tables,

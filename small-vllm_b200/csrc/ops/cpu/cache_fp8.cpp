@@ -115,9 +115,10 @@ int64_t rope_cache_fp8(const at::Tensor& q, const at::Tensor& k, const at::Tenso
   return std::count_if(slots, slots + tokens, [&](int64_t slot) { return slot >= num_slots; });
 }
 
-void check_pages(const char* op, const at::Tensor& k_cache, const at::Tensor& block_tables,
-                 const at::Tensor& seq_lens) {
-  const int64_t blocks = k_cache.size(0), bs = k_cache.size(1), width = block_tables.size(1);
+void check_pages(const char* op, const at::Tensor& k_scale, const at::Tensor& v_scale,
+                 const at::Tensor& block_tables, const at::Tensor& seq_lens) {
+  const int64_t blocks = k_scale.size(0), bs = k_scale.size(1), kv_heads = k_scale.size(2);
+  const int64_t width = block_tables.size(1);
   const auto* tables = block_tables.const_data_ptr<int32_t>();
   const auto* seq = seq_lens.const_data_ptr<int32_t>();
   for (int64_t s = 0; s < seq_lens.numel(); ++s) {
@@ -127,6 +128,15 @@ void check_pages(const char* op, const at::Tensor& k_cache, const at::Tensor& bl
       const int64_t block = tables[s * width + p];
       TORCH_CHECK(block >= 0 && block < blocks, op, ": block ", block, " of request ", s,
                   " outside the cache of ", blocks);
+      const int64_t count = std::min(bs, seq[s] - p * bs) * kv_heads;
+      for (const at::Tensor* scale : {&k_scale, &v_scale}) {
+        const auto* e = static_cast<const uint8_t*>(scale->const_data_ptr()) + block * bs * kv_heads;
+        for (int64_t i = 0; i < count; ++i) {
+          TORCH_CHECK(e[i] >= kScaleMin + kScaleBias && e[i] <= kScaleMax + kScaleBias, op,
+                      ": a scale of 2^", int{e[i]} - kScaleBias, " in block ", block,
+                      ", outside [2^", kScaleMin, ", 2^", kScaleMax, "]");
+        }
+      }
     }
   }
 }
@@ -135,7 +145,7 @@ void cache_read_fp8(const at::Tensor& k, const at::Tensor& v, const at::Tensor& 
                     const at::Tensor& v_cache, const at::Tensor& k_scale,
                     const at::Tensor& v_scale, const at::Tensor& block_tables,
                     const at::Tensor& seq_lens) {
-  check_pages("cache_read_fp8", k_cache, block_tables, seq_lens);
+  check_pages("cache_read_fp8", k_scale, v_scale, block_tables, seq_lens);
   const int64_t bs = k_cache.size(1), kv_heads = k_cache.size(2), dim = k_cache.size(3);
   const int64_t width = block_tables.size(1), rows = width * bs;
   const auto* tables = block_tables.const_data_ptr<int32_t>();
@@ -174,7 +184,7 @@ void decode_attention_fp8(const at::Tensor& out, const at::Tensor& q, const at::
                           const at::Tensor& v_cache, const at::Tensor& k_scale,
                           const at::Tensor& v_scale, const at::Tensor& block_tables,
                           const at::Tensor& seq_lens, double scale) {
-  check_pages("decode_attention_fp8", k_cache, block_tables, seq_lens);
+  check_pages("decode_attention_fp8", k_scale, v_scale, block_tables, seq_lens);
   const int64_t requests = q.size(0), heads = q.size(1), dim = q.size(2);
   const int64_t bs = k_cache.size(1), kv_heads = k_cache.size(2), width = block_tables.size(1);
   const auto* tables = block_tables.const_data_ptr<int32_t>();

@@ -15,8 +15,9 @@ namespace svllm::ops {
 //             whole 16 bytes (a view of a qkv projection); caches, scales, block_tables and
 //             seq_lens as cache_read_fp8 takes them; any number of query heads per KV head; scale
 //             positive and finite, head_dim^-0.5 by default; one device.
-// Returns:    A new bf16 tensor [S, heads, head_dim]. Softmax and sums are fp32; on CUDA the
-//             softmax numerators are rounded to f16 for the second product.
+// Returns:    A new bf16 tensor [S, heads, head_dim]. Softmax and sums are fp32; on CUDA the softmax
+//             numerators times V's scales are rounded to f16 for the second product, and those below
+//             2^-31 of a head's largest may be lost there.
 // Throws:     As cache_read_fp8, and on mismatches of q; on CUDA also for a q off 16 bytes.
 at::Tensor decode_attention_fp8(const at::Tensor& q, const at::Tensor& k_cache,
                                 const at::Tensor& v_cache, const at::Tensor& k_scale,

@@ -579,6 +579,66 @@ def test_bad_pages_and_lengths_on_cuda(cuda):
     check_write(c, got, 4, 2, 64, True)
 
 
+def with_scales(caches, rows, byte):
+    """The caches with the scales of the given (block, slot, head) rows of K and of V set."""
+    out = list(caches)
+    for i, at in zip((2, 3), rows):
+        scale = caches[i].view(torch.uint8).clone()
+        scale[at] = byte
+        out[i] = scale.view(E8M0)
+    return out
+
+
+@pytest.mark.parametrize("byte", [0, 66, 188, 254, 255])
+def test_scales_out_of_range_are_refused(byte):
+    """The writer leaves 2^-60 to 2^60, bytes 67 to 187; others among the rows that are read."""
+    lens = [40, 20]
+    tables, total = ref.make_tables(3, lens, 16)
+    caches = ref.make_cache(4, total, 16, 2, 64)
+    q = torch.randn(2, 4, 64, generator=torch.Generator().manual_seed(5)).bfloat16()
+    t = tables.tolist()
+    seen, behind = (t[1][1], 3, 1), (t[1][1], 4, 1)  # rows 19 and 20 of the second request
+    n = torch.tensor(lens, dtype=torch.int32)
+    for rows in [(seen, behind), (behind, seen)]:
+        bad = with_scales(caches, rows, byte)
+        with pytest.raises(RuntimeError, match="scale"):
+            svllm_ops.decode_attention_fp8(q, *bad, tables, n)
+        with pytest.raises(RuntimeError, match="scale"):
+            svllm_ops.cache_read_fp8(*bad, tables, n)
+    unseen = with_scales(caches, (behind, behind), byte)
+    want, bound = ref.attention(q, *caches, tables, lens, 64 ** -0.5)
+    assert ((run_attention("cpu", q, unseen, tables, lens).double() - want).abs() <= bound).all()
+    svllm_ops.cache_read_fp8(*unseen, tables, n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("byte", [0, 66, 188, 254, 255])
+@pytest.mark.parametrize("width", [None, 2000], ids=["by items", "by lines"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_scales_out_of_range_on_cuda(cuda, byte, width, dim):
+    """They raise the error word and count as the nearest in range; a scale behind a request's end is
+    not looked at."""
+    lens = [40, 20]
+    tables, total = ref.make_tables(3, lens, 16, width=width)
+    caches = ref.make_cache(4, total, 16, 2, dim)
+    q = torch.randn(2, 4, dim, generator=torch.Generator().manual_seed(5)).bfloat16()
+    t = tables.tolist()
+    seen, behind = (t[1][1], 3, 1), (t[1][1], 4, 1)
+    n = torch.tensor(lens, dtype=torch.int32)
+    svllm_ops.read_device_error(0, True)
+    for rows, flag in [((seen, behind), 1), ((behind, seen), 1), ((behind, behind), 0)]:
+        bad = with_scales(caches, rows, byte)
+        near = with_scales(caches, rows, min(max(byte, 67), 187))
+        got = run_attention(cuda, q, bad, tables, lens)
+        assert svllm_ops.read_device_error(0, True) == flag
+        assert torch.equal(got, run_attention(cuda, q, near, tables, lens))
+        read = svllm_ops.cache_read_fp8(*(c.to(cuda) for c in bad), tables.to(cuda), n.to(cuda))
+        assert svllm_ops.read_device_error(0, True) == flag
+        want = svllm_ops.cache_read_fp8(*(c.to(cuda) for c in near), tables.to(cuda), n.to(cuda))
+        assert torch.equal(read[0], want[0]) and torch.equal(read[1], want[1])
+        assert svllm_ops.read_device_error(0, True) == 0
+
+
 # ------------------------------------------------------------------------------------ refusals
 
 def test_write_refuses():
