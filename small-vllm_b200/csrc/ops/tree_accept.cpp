@@ -3,6 +3,10 @@
 #include <ATen/ATen.h>
 #include <c10/util/Exception.h>
 
+#include <algorithm>
+#include <functional>
+#include <vector>
+
 #include "ops/common.h"
 #include "ops/tree_accept_kernels.h"
 #include "svllm_kernels.h"
@@ -100,6 +104,7 @@ void tree_commit(const std::vector<at::Tensor>& k_caches, const std::vector<at::
                 "tree_commit: ", k_scales.size(), " K scales and ", v_scales.size(),
                 " V scales for ", k_caches.size(), " layers");
     const at::IntArrayRef rows = first.sizes().slice(0, first.dim() - 1);
+    std::vector<const void*> planes;
     for (const auto* scales : {&k_scales, &v_scales}) {
       for (const at::Tensor& c : *scales) {
         TORCH_CHECK(c.sizes() == rows && c.scalar_type() == at::kFloat8_e8m0fnu &&
@@ -107,8 +112,13 @@ void tree_commit(const std::vector<at::Tensor>& k_caches, const std::vector<at::
                     "tree_commit: scales must be contiguous float8_e8m0fnu ", rows, " on ",
                     first.device(), ", got ", c.scalar_type(), " ", c.sizes(), " on ", c.device());
         (scales == &k_scales ? ks : vs).push_back(c.unsqueeze(-1));
+        planes.push_back(c.const_data_ptr());
       }
     }
+    // before any row moves
+    std::sort(planes.begin(), planes.end(), std::less<const void*>());
+    TORCH_CHECK(std::adjacent_find(planes.begin(), planes.end()) == planes.end(),
+                "tree_commit: invalid argument: scales are given twice");
   }
   const at::Device device = first.device();
   const int64_t requests = num_accepted.numel(), tokens = slot_mapping.numel();

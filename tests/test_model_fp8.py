@@ -153,6 +153,13 @@ def test_accepted_rows_and_scales_move(device):
     with pytest.raises(RuntimeError, match="float8_e8m0fnu"):
         svllm_ops.tree_commit(model.k_cache, model.v_cache, path, accepted, slots, starts,
                               [t.view(torch.uint8) for t in model.k_scale], model.v_scale)
+    # a refused call moves nothing: the codes neither
+    state = [t.view(torch.uint8).clone() for p in planes for t in p]
+    with pytest.raises(RuntimeError, match="given twice"):
+        svllm_ops.tree_commit(model.k_cache, model.v_cache, path, accepted, slots, starts,
+                              model.k_scale, model.k_scale)
+    assert all(torch.equal(t.view(torch.uint8), old)
+               for t, old in zip([t for p in planes for t in p], state))
 
 
 @pytest.mark.gpu
