@@ -73,11 +73,19 @@ constexpr int kPair = 2, kPairSteps = 14;
 constexpr int kMaxSplits = 8;    // CTAs of an item: the portable cluster size
 constexpr int kItemSteps = 4;    // by items up to this many steps of a warp
 constexpr int kJoinThreads = 256;
-// Parts a lane of the join has in flight: few where an item has few parts, which most lanes do not
-// have (us, 2 and 8: 148 requests of 512-1024 rows, 16/8 heads of 128, 3 parts, 50.9, 53.1; 64 of
-// 2048-4096, 4 parts, 78.5, 78.8; 48, 5 parts, 62.0, 61.1; 36, 6 parts, 48.4, 47.3; 24, 28/4 heads, 14
-// parts, 23.6, 21.4).
-constexpr int kJoinFew = 2, kJoinMany = 8, kJoinFewParts = 4;
+// The join of items whose number of parts (of one of middling length) is up to kJoinFewParts takes a
+// thread for four outputs, with kJoinFew parts in flight; with more parts lanes and warps share them.
+// Few parts are bound by the instructions of so many warps, many by the trips to memory (us, few and
+// many: 148 requests of 512-1024 rows, 16/8 heads of 128, 3 parts, 49.0, 50.8; 64 of 1024-2048, 32/4
+// heads, 6 parts, 26.1, 29.2; 28 of 2048-4096, 16/8 heads, 7 parts, 38.0, 38.5; but 20, 9 parts, 30.4,
+// 30.1; 13 of 140-2500, 24/8 heads of 64, 13 parts, 12.7, 9.8).
+constexpr int kJoinFew = 8, kJoinFewParts = 7;
+// Parts a lane has in flight there. At head_dim 128 five are what fits beside a CTA by lines (64
+// registers), so that the join's CTAs wait where they will run (us, five and eight: one request of
+// 32760 rows 18.2, 19.4; 48 of 88-4096, 32/4 heads, 27.9, 28.6; but 24, 28/4 heads, 21.4, 21.2). At 64
+// six do (32 of 2048-4096, 32/8 heads, five, six and eight: 27.8, 27.4, 27.7).
+template <int D>
+constexpr int kJoinMany = D == 128 ? 5 : 6;
 // The running maximum is moved only when a score passes it by kSlack, so that most steps need one
 // vote instead of a maximum over the warp. Weights reach 2^(kWeightBits + kSlack).
 constexpr float kWeightBits = 6.0f, kSlack = 8.0f;
@@ -669,10 +677,10 @@ __global__ void __launch_bounds__(kLineWarps * kWarpSize, 1) decode_attention_fp
 }
 
 // Joins the parts of the items that were cut: blockIdx.x the item, `spread` warps for each 32 of its
-// outputs. A lane takes four dims of every 4 spread-th part, kBatch of them in flight; its
+// outputs. A lane takes four dims of every 4 spread-th part, kJoinMany of them in flight; its
 // fellows' sums come by shuffles, the other warps' through shared memory. The order is fixed by the
 // sizes, so results repeat.
-template <int D, int kHeads, int kBatch>
+template <int D, int kHeads>
 __global__ void __launch_bounds__(kJoinThreads) decode_attention_fp8_join(
     const __grid_constant__ AttnArgs a, int spread) {
   grid_dependency_sync();
@@ -695,11 +703,11 @@ __global__ void __launch_bounds__(kJoinThreads) decode_attention_fp8_join(
   float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float m = -FLT_MAX, l = 0.0f;
   const int step = 4 * spread;
-  for (int p0 = lane / 8 * spread + mate; real && p0 < entry.parts; p0 += step * kBatch) {
-    float2 ml[kBatch];
-    float4 x[kBatch];
+  for (int p0 = lane / 8 * spread + mate; real && p0 < entry.parts; p0 += step * kJoinMany<D>) {
+    float2 ml[kJoinMany<D>];
+    float4 x[kJoinMany<D>];
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
+    for (int i = 0; i < kJoinMany<D>; ++i) {
       const int p = p0 + i * step;
       ml[i] = make_float2(-FLT_MAX, 0.0f);
       x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -714,12 +722,12 @@ __global__ void __launch_bounds__(kJoinThreads) decode_attention_fp8_join(
     }
     float mx = m;
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) mx = fmaxf(mx, ml[i].x);
+    for (int i = 0; i < kJoinMany<D>; ++i) mx = fmaxf(mx, ml[i].x);
     const float f = exp2_approx(m - mx);
     l *= f;
     acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
+    for (int i = 0; i < kJoinMany<D>; ++i) {
       const float w = exp2_approx(ml[i].x - mx);
       l = fmaf(ml[i].y, w, l);
       acc = make_float4(fmaf(x[i].x, w, acc.x), fmaf(x[i].y, w, acc.y), fmaf(x[i].z, w, acc.z),
@@ -766,6 +774,70 @@ __global__ void __launch_bounds__(kJoinThreads) decode_attention_fp8_join(
     *reinterpret_cast<uint2*>(dst) =
         make_uint2(pack_bf16x2(acc.x * r, acc.y * r), pack_bf16x2(acc.z * r, acc.w * r));
   }
+}
+
+// The same where items have few parts: a thread joins four outputs, kJoinFew parts in flight; a CTA
+// takes as many items as fit it, `per_item` threads each.
+template <int D, int kHeads>
+__global__ void __launch_bounds__(kJoinThreads) decode_attention_fp8_join_few(
+    const __grid_constant__ AttnArgs a, int items, int per_item) {
+  grid_dependency_sync();
+  const int in_cta = static_cast<int>(threadIdx.x) / per_item;
+  const int64_t item =
+      static_cast<int64_t>(blockIdx.x) * (static_cast<int>(blockDim.x) / per_item) + in_cta;
+  if (item >= items) return;
+  const JoinEntry entry = a.table[item];
+  if (entry.parts <= 1) return;
+  const int held_heads = min(a.group, kGroup);
+  const int b = static_cast<int>(item) / a.subs;
+  const Heads<kHeads> heads(a, static_cast<int>(item) - b * a.subs);
+  const int within = static_cast<int>(threadIdx.x) - in_cta * per_item;
+  const int row = within / (D / 4), d = within % (D / 4) * 4;
+  const int kv = kHeads == 1 ? 0 : row / held_heads;
+  const int head = row - kv * held_heads;
+  if (kv >= heads.live || head >= heads.count) return;
+  // the first part is the one that begins the item; the others continue it
+  const int begins = kHeads * held_heads, stride = 2 * begins;
+  const int64_t at = static_cast<int64_t>(entry.share) * stride + row;
+  const float2* part_ml = a.part_ml + at;
+  const float* part_acc = a.part_acc + at * D + d;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float m = -FLT_MAX, l = 0.0f;
+  for (int p0 = 0; p0 < entry.parts; p0 += kJoinFew) {
+    float2 ml[kJoinFew];
+    float4 x[kJoinFew];
+#pragma unroll
+    for (int i = 0; i < kJoinFew; ++i) {
+      const int p = min(p0 + i, entry.parts - 1);
+      const int off = p == 0 ? begins : p * stride;
+      ml[i] = part_ml[off];
+      x[i] = *reinterpret_cast<const float4*>(part_acc + static_cast<int64_t>(off) * D);
+    }
+#pragma unroll
+    for (int i = 0; i < kJoinFew; ++i) {  // the last part again: a weight of 0
+      if (p0 + i >= entry.parts) ml[i] = make_float2(-__builtin_huge_valf(), 0.0f);
+    }
+    float mx = m;
+#pragma unroll
+    for (int i = 0; i < kJoinFew; ++i) mx = fmaxf(mx, ml[i].x);
+    const float f = exp2_approx(m - mx);
+    m = mx;
+    l *= f;
+    acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+#pragma unroll
+    for (int i = 0; i < kJoinFew; ++i) {
+      const float w = exp2_approx(ml[i].x - mx);
+      l = fmaf(ml[i].y, w, l);
+      acc = make_float4(fmaf(x[i].x, w, acc.x), fmaf(x[i].y, w, acc.y), fmaf(x[i].z, w, acc.z),
+                        fmaf(x[i].w, w, acc.w));
+    }
+  }
+  const float r = l == 0.0f ? 0.0f : 1.0f / l;
+  uint8_t* dst = static_cast<uint8_t*>(a.out) +
+                 ((static_cast<int64_t>(b) * a.num_heads + heads.first + kv * a.group + head) * D +
+                  d) * 2;
+  *reinterpret_cast<uint2*>(dst) =
+      make_uint2(pack_bf16x2(acc.x * r, acc.y * r), pack_bf16x2(acc.z * r, acc.w * r));
 }
 
 // ------------------------------------------------------------------------------------- by items
@@ -940,15 +1012,21 @@ int launch_lines(const AttnArgs& a, int64_t items, int device, cudaStream_t stre
   const int status =
       launch(kernel, dim3(sms), dim3(kLineWarps * kWarpSize), smem, stream, 1u, a);
   if (status != SVLLM_OK) return status;
+  const int64_t parts = line_shares(device) / items + 2;  // of an item of middling length
+  if (parts <= kJoinFewParts) {
+    const int per_item = kHeads * heads * (D / 4);
+    const int a_cta = kJoinThreads / per_item;
+    return launch(decode_attention_fp8_join_few<D, kHeads>,
+                  dim3(static_cast<unsigned>((items + a_cta - 1) / a_cta)),
+                  dim3(static_cast<unsigned>(a_cta * per_item)), 0, stream, 1u, a,
+                  static_cast<int>(items), per_item);
+  }
   // up to four parts a lane, as far as the warps of a CTA go
-  const int64_t parts = line_shares(device) / items + 2;
   int spread = 1;
   while (spread < kJoinThreads / kWarpSize && parts > 16 * spread) spread *= 2;
   const int runs = kHeads * heads * (D / 32) * spread;
   const unsigned slices = static_cast<unsigned>((runs * kWarpSize + kJoinThreads - 1) / kJoinThreads);
-  const auto join = parts <= kJoinFewParts ? decode_attention_fp8_join<D, kHeads, kJoinFew>
-                                           : decode_attention_fp8_join<D, kHeads, kJoinMany>;
-  return launch(join, dim3(static_cast<unsigned>(items), slices),
+  return launch(decode_attention_fp8_join<D, kHeads>, dim3(static_cast<unsigned>(items), slices),
                 dim3(kJoinThreads), 0, stream, 1u, a, spread);
 }
 

@@ -296,6 +296,12 @@ def test_attention(device, heads, kv_heads, dim, block):
     ([700, 33, 0, 2000] * 4, 27, 3, 64, 16, 2000),
     ([700, 33, 1, 2000] * 4, 3, 1, 64, 12, 9000),
     ([90, 4100], 40, 5, 64, 256, 800),
+    # items of few parts: KV heads in pairs with two groups of query heads each, several items a CTA
+    ([600, 1, 77] * 50, 27, 3, 64, 16, None),
+    ([600, 0, 77] * 50, 9, 3, 64, 16, None),
+    ([900, 30, 2000] * 30, 9, 3, 128, 16, None),
+    ([900, 30, 2000] * 30, 16, 8, 128, 12, None),
+    ([3, 1, 0, 65] * 80, 3, 1, 128, 16, 40),
 ])
 def test_attention_long(cuda, lens, heads, kv_heads, dim, block, width):
     check_attention(cuda, lens, heads, kv_heads, dim, block, width=width)
