@@ -39,10 +39,10 @@
 //     which merges through distributed shared memory. One launch.
 //
 // What bounds it, measured on a B200 (16/8 heads of 128, us in a graph): 64 requests of 2064 to 4096
-// rows, 407 MB, 77-79. The warps stream at 6.6 TB/s once they run, 62 us; 4.7 us go by until the
-// first rows are there (lengths, table, rows, each a trip to memory after the other), warps end up to
-// 5 apart, and the join takes 4. One request of 32760 rows: 19.5, of which 10.5 are the stream. A
-// step of 32 rows takes 570 warp instructions; 38 % of the issue slots are used. More loads in flight
+// rows, 407 MB, 76.7. The warps stream at 6.6 TB/s once they run, 62 us; 4 us go by until the first
+// rows are there (lengths 0.8, the share 0.5, table and rows, each a trip to memory after the other),
+// the last warps end 4 behind the mean, and the join takes 3. One request of 32760 rows: 18.1, of
+// which 10.5 are the stream. A step of 32 rows takes 570 warp instructions; 38 % of the issue slots are used. More loads in flight
 // gave nothing (three stages 79.1, twelve warps 77.1-78.9, fourteen 81.5, the next load after the
 // products 80.7); a CTA per share whose warps merge at every item's end took 98, rows loaded to
 // registers instead of shared memory 168.
