@@ -14,10 +14,15 @@
 // and m a maximum of the y_j that is moved only when one passes it by 8: w_j <= 2^14, the largest is
 // 2^6 at least, and f16's smallest number, 2^-24, stands for 2^-30 of it or less (a weight below half
 // of that is lost). The rows' scales thus never touch the codes: 2^ek multiplies a score, ev adds to
-// it (in the one rounding of an fma), and the denominator is l = sum_j w_j 2^-ev_j, in fp32. (The
-// weights are taken from y and p from them, not the other way round: at scores so large that x + ev
-// rounds, both then carry the same error, and no weight passes 2^14.) The weights are rounded to f16
-// (2^-11 of each, an eighth of a bf16 rounding) because the product takes no wider operand.
+// it (in the one rounding of an fma). The weights are rounded to f16 (2^-11 of each, an eighth of a
+// bf16 rounding) because the product takes no wider operand.
+//
+// The denominator is l = sum_j 2^(d_j - ev_j) with d_j = y_j - m + 6, in fp32. Its terms have an
+// exponential of their own: w_j 2^-ev_j would lose a row whose w_j is below 2^-126, and with scales
+// 120 binades apart such a row may be most of the sum. m lies within 60 of the largest x (and 8 of
+// slack), so the largest term is between 2^-54 and 2^74, and one below 2^-126 less than 2^-72 of it.
+// For the same reason l is moved to another maximum in two steps (half_factor). (x is taken from y,
+// not y from x: at scores so large that x + ev rounds, weight and term then carry the same error.)
 //
 // Layout. A warp takes steps of 32 cached rows, lane = 4 g + t:
 //   S^T[16 rows x 8 heads] = K[16 x D] . Q^T[D x 8]: lane holds rows g, g + 8 of K, 16 bytes at
@@ -128,6 +133,13 @@ struct AttnArgs {
   float scale_log2;
   int* err;
 };
+
+// Half of what moves sums from the maximum m to another: they are multiplied by it twice, so that a
+// denominator, whose terms lie up to 2^60 above and below its numerator's, loses nothing that counts
+// where the whole factor is below fp32's smallest.
+__device__ __forceinline__ float half_factor(float m, float to) {
+  return exp2_approx(0.5f * (m - to));
+}
 
 __device__ __forceinline__ uint32_t transpose8x8_b16(uint32_t x) {
   uint32_t y;
@@ -347,7 +359,7 @@ struct Sums {
     const int g = lane >> 2, t = lane & 3;
     // S^T: lane holds rows g, g + 8 of both tiles x heads 2t, 2t + 1
     float y[2][4];
-    float unscale[2][2];  // 2^-ev
+    float v_exp[2][2];  // ev
     float top[2] = {m[0], m[1]};
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -369,7 +381,7 @@ struct Sums {
         const uint32_t sc = __shfl_sync(0xffffffffu, scales, r);
         const float ks = scale_value(sc & 0xffu);
         const float ev = static_cast<float>(static_cast<int>(sc >> 8) - kScaleBias);
-        unscale[i][e] = scale_value(2 * kScaleBias - (sc >> 8));
+        v_exp[i][e] = ev;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const float v = fmaf(s[2 * e + h], q.x_scale[h] * ks, ev);
@@ -384,9 +396,10 @@ struct Sums {
         top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], off));
         top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], off));
       }
-      const float al[2] = {exp2_approx(m[0] - top[0]), exp2_approx(m[1] - top[1])};
-      l[0] *= al[0];
-      l[1] *= al[1];
+      const float half[2] = {half_factor(m[0], top[0]), half_factor(m[1], top[1])};
+      const float al[2] = {half[0] * half[0], half[1] * half[1]};
+      l[0] = l[0] * half[0] * half[0];
+      l[1] = l[1] * half[1] * half[1];
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) {
 #pragma unroll
@@ -400,8 +413,9 @@ struct Sums {
       float p[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        p[e] = exp2_approx(y[i][e] - m[e & 1] + kWeightBits);
-        l[e & 1] = fmaf(p[e], unscale[i][e >> 1], l[e & 1]);
+        const float d = y[i][e] - m[e & 1] + kWeightBits;
+        p[e] = exp2_approx(d);
+        l[e & 1] += exp2_approx(d - v_exp[i][e >> 1]);
       }
       const uint32_t b0 = transpose8x8_b16(pack_f16x2(p[0], p[1]));  // rows 2t, 2t + 1 of head g
       const uint32_t b1 = transpose8x8_b16(pack_f16x2(p[2], p[3]));  // and + 8
@@ -723,13 +737,13 @@ __global__ void __launch_bounds__(kJoinThreads) decode_attention_fp8_join(
     float mx = m;
 #pragma unroll
     for (int i = 0; i < kJoinMany<D>; ++i) mx = fmaxf(mx, ml[i].x);
-    const float f = exp2_approx(m - mx);
-    l *= f;
+    const float f0 = half_factor(m, mx), f = f0 * f0;
+    l = l * f0 * f0;
     acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
 #pragma unroll
     for (int i = 0; i < kJoinMany<D>; ++i) {
-      const float w = exp2_approx(ml[i].x - mx);
-      l = fmaf(ml[i].y, w, l);
+      const float w0 = half_factor(ml[i].x, mx), w = w0 * w0;
+      l = fmaf(ml[i].y * w0, w0, l);
       acc = make_float4(fmaf(x[i].x, w, acc.x), fmaf(x[i].y, w, acc.y), fmaf(x[i].z, w, acc.z),
                         fmaf(x[i].w, w, acc.w));
     }
@@ -738,9 +752,9 @@ __global__ void __launch_bounds__(kJoinThreads) decode_attention_fp8_join(
 #pragma unroll
   for (int off = 8; off < kWarpSize; off *= 2) {
     const float mx = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-    const float f = exp2_approx(m - mx);
+    const float f0 = half_factor(m, mx), f = f0 * f0;
     m = mx;
-    l *= f;
+    l = l * f0 * f0;
     acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
     l += __shfl_xor_sync(0xffffffffu, l, off);
     acc.x += __shfl_xor_sync(0xffffffffu, acc.x, off);
@@ -759,9 +773,10 @@ __global__ void __launch_bounds__(kJoinThreads) decode_attention_fp8_join(
       const float2 ml = others_ml[w];
       const float4 x = others[w][lane % 8];
       const float mx = fmaxf(m, ml.x);
-      const float f0 = exp2_approx(m - mx), f1 = exp2_approx(ml.x - mx);
+      const float h0 = half_factor(m, mx), h1 = half_factor(ml.x, mx);
+      const float f0 = h0 * h0, f1 = h1 * h1;
       m = mx;
-      l = l * f0 + ml.y * f1;
+      l = l * h0 * h0 + ml.y * h1 * h1;
       acc = make_float4(acc.x * f0 + x.x * f1, acc.y * f0 + x.y * f1, acc.z * f0 + x.z * f1,
                         acc.w * f0 + x.w * f1);
     }
@@ -820,14 +835,14 @@ __global__ void __launch_bounds__(kJoinThreads) decode_attention_fp8_join_few(
     float mx = m;
 #pragma unroll
     for (int i = 0; i < kJoinFew; ++i) mx = fmaxf(mx, ml[i].x);
-    const float f = exp2_approx(m - mx);
+    const float f0 = half_factor(m, mx), f = f0 * f0;
     m = mx;
-    l *= f;
+    l = l * f0 * f0;
     acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
 #pragma unroll
     for (int i = 0; i < kJoinFew; ++i) {
-      const float w = exp2_approx(ml[i].x - mx);
-      l = fmaf(ml[i].y, w, l);
+      const float w0 = half_factor(ml[i].x, mx), w = w0 * w0;
+      l = fmaf(ml[i].y * w0, w0, l);
       acc = make_float4(fmaf(x[i].x, w, acc.x), fmaf(x[i].y, w, acc.y), fmaf(x[i].z, w, acc.z),
                         fmaf(x[i].w, w, acc.w));
     }
@@ -936,9 +951,9 @@ __global__ void __launch_bounds__(kItemWarps * kWarpSize, D == 128 ? 1 : 2) deco
     float o = 0.0f, ls = 0.0f;
 #pragma unroll
     for (int w = 0; w < kItemWarps; ++w) {
-      const float f = exp2_approx(warp_m[w][h] - mx);
-      o = fmaf(accs[w * heads.count * D + idx], f, o);
-      ls = fmaf(warp_l[w][h], f, ls);
+      const float f = half_factor(warp_m[w][h], mx);
+      o = fmaf(accs[w * heads.count * D + idx], f * f, o);
+      ls = fmaf(warp_l[w][h] * f, f, ls);
     }
     if (a.splits == 1) {
       out[idx] = __float2bfloat16_rn(ls == 0.0f ? 0.0f : o / ls);
@@ -974,9 +989,9 @@ __global__ void __launch_bounds__(kItemWarps * kWarpSize, D == 128 ? 1 : 2) deco
     float o = 0.0f, ls = 0.0f;
 #pragma unroll
     for (int r = 0; r < kMaxSplits; ++r) {
-      const float f = exp2_approx(m[r] - mx);
-      o = fmaf(x[r], f, o);
-      ls = fmaf(l[r], f, ls);
+      const float f = half_factor(m[r], mx);
+      o = fmaf(x[r], f * f, o);
+      ls = fmaf(l[r] * f, f, ls);
     }
     out[idx] = __float2bfloat16_rn(ls == 0.0f ? 0.0f : o / ls);
   }

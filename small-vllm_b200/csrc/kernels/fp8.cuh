@@ -6,8 +6,9 @@
 // against max / 448 (the codes keep four significant bits wherever in its binade the maximum
 // lies), and it makes the scaling exact: a value is rounded once, c * 2^e is a bf16 value, and
 // the scale takes one byte, e + 127, the e8m0 encoding. The clamp keeps 2^e, its inverse and the
-// softmax weights times 2^e inside fp32: magnitudes above 448 * 2^60 = 5.2e20 saturate, rows all
-// below 2^-70 become zero.
+// product of the two ends of the range inside fp32: magnitudes above 448 * 2^60 = 5.2e20 saturate,
+// rows all below 2^-70 become zero. (Softmax weights times 2^e are kept inside fp32 by the attention
+// itself, whose maximum is that of their products.)
 #pragma once
 
 #include <cuda_runtime.h>
