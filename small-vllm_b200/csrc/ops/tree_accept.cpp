@@ -98,6 +98,12 @@ void tree_commit(const std::vector<at::Tensor>& k_caches, const std::vector<at::
     }
   }
   const bool scaled = !k_scales.empty() || !v_scales.empty();
+  const bool codes = first.scalar_type() == at::kFloat8_e4m3fn;
+  TORCH_CHECK(scaled || !codes,
+              "tree_commit: float8_e4m3fn caches move with their scales: pass k_scales and v_scales "
+              "(a cache without them moves as bytes, uint8)");
+  TORCH_CHECK(codes || !scaled, "tree_commit: scales are only of float8_e4m3fn caches, got ",
+              first.scalar_type());
   std::vector<at::Tensor> ks, vs;  // as [..., KV heads, 1]
   if (scaled) {
     TORCH_CHECK(k_scales.size() == k_caches.size() && v_scales.size() == v_caches.size(),

@@ -39,7 +39,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> tree_accept(
 //             query_start_loc [S + 1] int32 of the step, no slot in it twice. No two caches share memory;
 //             the same one twice is refused. Of an 8-bit cache (float8_e4m3fn) the scales move too:
 //             k_scales, v_scales one contiguous float8_e8m0fnu [blocks, block_size, KV heads] tensor
-//             per layer, empty for other caches.
+//             per layer, and only of it. Rows of 8-bit values without scales move as bytes (uint8).
 // Throws:     c10::Error on dtype, shape, layout or device mismatches, and on CPU for a path or slot
 //             out of range; on CUDA those raise the device error word and the rows do not move.
 void tree_commit(const std::vector<at::Tensor>& k_caches, const std::vector<at::Tensor>& v_caches,
