@@ -390,7 +390,8 @@ struct Sums {
         }
       }
     }
-    if (__any_sync(0xffffffffu, top[0] > m[0] + kSlack || top[1] > m[1] + kSlack)) {
+    // (differences, as the weights take them: fp32 may round m + kSlack up to the next score)
+    if (__any_sync(0xffffffffu, top[0] - m[0] > kSlack || top[1] - m[1] > kSlack)) {
 #pragma unroll
       for (int off = 4; off < kWarpSize; off *= 2) {
         top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], off));

@@ -123,3 +123,31 @@ def test_scales_spread_over_the_whole_range(device, seed):
     exponents = torch.randint(ref.E_MIN, ref.E_MAX + 1, (n,), generator=g)
     scores = torch.randint(-15, 16, (n,), generator=g).double() * 2.0 ** seed
     check(device, n, 2, 4, 2, 128, None, scores, exponents)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("top", [2, 3])
+def test_scores_whose_steps_pass_the_slack(cuda, dim, top):
+    """Scores of 2^27, where fp32 holds only multiples of 16: a maximum one or two such steps above the
+    running one still moves it, and the row of the largest score has all the weight."""
+    n, base = 64, 2.0 ** 27
+    g = torch.Generator().manual_seed(dim)
+    k = torch.zeros(n, 1, dim, dtype=torch.float64)
+    k[:, 0, 0], k[:, 0, 1] = 128, 1
+    k[n - 1, 0, 1] = top  # in the second step of a warp
+    v = (128 + 256 * torch.rand(n, 1, dim, generator=g)).bfloat16().double()  # scales of 1
+    caches = []
+    for x in (k, v):
+        codes, scale, _ = ref.quantise(x)
+        caches.append((codes.view(4, 16, 1, dim), scale.view(4, 16, 1)))
+    tables = torch.zeros(1, 1000, dtype=torch.int32)
+    tables[0, :4] = torch.arange(4)
+    q = torch.zeros(1, 3, dim, dtype=torch.bfloat16)
+    q[:, :, 0], q[:, :, 1] = base / 128, 16
+    out = svllm_ops.decode_attention_fp8(
+        q.to(cuda), *(t.to(cuda) for t in (caches[0][0], caches[1][0], caches[0][1], caches[1][1])),
+        tables.to(cuda), torch.tensor([n], dtype=torch.int32, device=cuda), LN2).cpu().double()
+    want = ref.values(*caches[1]).view(n, dim)[n - 1].expand(3, dim)
+    # the others weigh 63 * 2^-16 together, their values at most four times this row's
+    assert ((out[0] - want).abs() <= (2.0 ** -8 + 2.0 ** -11 + 4 * 63 * 2.0 ** -16) * want).all()
