@@ -205,6 +205,7 @@ at::Tensor Model::fp8_attention(const at::Tensor& q, int64_t layer, const Attent
     return ops::decode_attention_fp8(q, k_cache_[layer], v_cache_[layer], k_scale_[layer],
                                      v_scale_[layer], tables, lens, std::nullopt);
   }
+  if (q.size(0) == 0) return at::empty(q.sizes(), q.options());  // no token to attend for
   const auto [k, v] = ops::cache_read_fp8(k_cache_[layer], v_cache_[layer], k_scale_[layer],
                                           v_scale_[layer], tables, lens);
   const int64_t pages = tables.numel();
