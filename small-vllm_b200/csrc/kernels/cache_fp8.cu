@@ -561,6 +561,34 @@ __global__ void __launch_bounds__(kBulkWarps * kWarpSize, 1) cache_write_bulk_ke
   }
 }
 
+// The bulk kernel's warps: eight or twelve, as far as their rings fit. An SM takes its tokens in rounds
+// of one a warp, and a round lasts as long as its bytes or as a warp's chain over a token, which is
+// counted in the bytes that pass meanwhile (a pass of k and v costs three of q: maxima and codes; the
+// norms cost a third). The form with the smaller sum is taken. Past kFewTokens an SM the rings stream,
+// which twelve warps do 12-17% slower, so their sum has to be smaller by as much. us with eight and with
+// twelve warps, by the tokens an SM:
+//   6/2 heads of 64, norms:    9: 4.1, 3.1   16: 4.2, 4.6    36: 8.1, 6.1     443: 84.6, 65.4
+//   24/8 of 64:                9: 4.7, 3.8   16: 5.0, 5.7    36: 11.1, 9.5    443: 95.5, 108.0
+//   8/8 of 128, norms:         9: 6.5, 5.3   16: 7.0, 8.2    40: 16.1, 16.7   443: 130.8, 106.0
+//   8/8 of 128:               11: 5.9, 4.8   15: 5.9, 7.2    45: 16.0, 15.5   443: 108.7, 123.9
+//   16/8 of 128, norms:        9: 7.2, 6.0   16: 7.6, 9.3    40: 18.3, 19.9   443: 151.7, 172.1
+//   32/4 of 128, norms (ten):  9: 7.7, 5.7   16: 8.5, 10.3   20: 12.8, 11.9   443: 224.5, 230.8
+// Over 587 such pairs of 26 layouts, 136 of them timed after the rule was set, the choice costs at most
+// 8% against the better of the two.
+int bulk_warps(int64_t per_sm, int64_t bytes, int64_t q_passes, int64_t kv_passes, bool norm,
+               int64_t fit) {
+  if (fit <= 8) return static_cast<int>(fit);
+  constexpr int64_t kChainStart = 40 * 1024, kFewTokens = 64;
+  const int64_t chain = kChainStart + (norm ? 8 : 6) * 1024 * (q_passes + 3 * kv_passes);
+  const auto sum = [&](int64_t warps) {
+    return (per_sm + warps - 1) / warps * (warps * bytes > chain ? warps * bytes : chain);
+  };
+  const int64_t many = fit < kBulkWarps ? fit : kBulkWarps;
+  const bool better =
+      per_sm <= kFewTokens ? sum(many) < sum(8) : 23 * sum(many) < 20 * sum(8);
+  return static_cast<int>(better ? many : 8);
+}
+
 using WriteKernel = void (*)(CacheWriteArgs);
 
 template <int D, bool kNorm>
@@ -573,12 +601,10 @@ int launch_write(const CacheWriteArgs& a, bool aligned, int device, cudaStream_t
   // as many warps as their rings fit (a pass of the last stage may read a pass's bytes past it)
   constexpr int64_t kPassBytes = kHeads * D * 2;
   const int64_t fit = (kBulkSmem - kPassBytes) / (kBulkStages * token_bytes);
-  // Eight warps stream best (16/8 heads of 128, 65536 tokens: 151 us, 172 with twelve), but between
-  // 8 and 40 tokens an SM what counts is the rounds of tokens that a warp takes (24/8 of 64, 5003
-  // tokens: 10.5 us, 8.8 with twelve).
-  const int64_t per_sm = (a.num_tokens + sm_count(device) - 1) / sm_count(device);
-  const int64_t wanted = per_sm > 8 && per_sm <= 40 ? kBulkWarps : 8;
-  const int warps = static_cast<int>(fit < wanted ? fit : wanted);
+  const int64_t kv_passes = (a.num_kv_heads + kHeads - 1) / kHeads;
+  const int warps = bulk_warps((a.num_tokens + sm_count(device) - 1) / sm_count(device),
+                               (4 * int64_t{a.num_heads} + 6 * int64_t{a.num_kv_heads}) * D,
+                               passes - 2 * kv_passes, kv_passes, kNorm, fit);
   if (aligned && a.num_tokens * passes > int64_t{kDirectPassesPerSm} * sm_count(device) &&
       warps >= kBulkMinWarps) {
     const size_t smem = static_cast<size_t>(warps * kBulkStages * token_bytes + kPassBytes);
