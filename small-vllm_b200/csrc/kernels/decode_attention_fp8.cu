@@ -80,11 +80,16 @@ constexpr int kItemSteps = 4;    // by items up to this many steps of a warp
 constexpr int kJoinThreads = 256;
 // The join of items whose number of parts (of one of middling length) is up to kJoinFewParts takes a
 // thread for four outputs, with kJoinFew parts in flight; with more parts lanes and warps share them.
-// Few parts are bound by the instructions of so many warps, many by the trips to memory (us, few and
-// many: 148 requests of 512-1024 rows, 16/8 heads of 128, 3 parts, 49.0, 50.8; 64 of 1024-2048, 32/4
-// heads, 6 parts, 26.1, 29.2; 28 of 2048-4096, 16/8 heads, 7 parts, 38.0, 38.5; but 20, 9 parts, 30.4,
-// 30.1; 13 of 140-2500, 24/8 heads of 64, 13 parts, 12.7, 9.8).
-constexpr int kJoinFew = 8, kJoinFewParts = 7;
+// Few parts are bound by the instructions of so many warps, many by the trips to memory. us with the
+// form for few and for many, requests of 2048-4096 rows (or 1-4096 where marked), by their parts:
+//   heads of 128, 16/8:  5: 53.0, 54.0   7: 37.6, 38.5   8: 31.6, 32.0   9: 29.9, 30.2   10: 27.0, 26.1
+//   32/4:                6: 32.3, 33.0*  7: 36.1, 36.8   8: 27.8, 27.9*  9: 25.1, 24.9*  10: 23.2, 22.8*
+//   heads of 64, 32/8:   4: 49.8, 53.1   5: 45.2, 45.5*  6: 31.4, 32.1   6: 38.8, 37.7*   7: 37.9, 36.9
+//   24/4:                5: 40.5, 41.8*  6: 49.9, 51.8   6: 35.4, 35.7*  7: 32.4, 32.1*  10: 31.5, 30.0
+//   8/8 and 9/3:         4: 48.5, 49.1   5: 42.1, 42.0*  6: 36.7, 34.8*  6: 33.4, 32.4*   7: 36.6, 35.4
+constexpr int kJoinFew = 8;
+template <int D>
+constexpr int kJoinFewParts = D == 128 ? 7 : 5;
 // Parts a lane has in flight there. At head_dim 128 five are what fits beside a CTA by lines (64
 // registers), so that the join's CTAs wait where they will run (us, five and eight: one request of
 // 32760 rows 18.2, 19.4; 48 of 88-4096, 32/4 heads, 27.9, 28.6; but 24, 28/4 heads, 21.4, 21.2). At 64
@@ -1029,7 +1034,7 @@ int launch_lines(const AttnArgs& a, int64_t items, int device, cudaStream_t stre
       launch(kernel, dim3(sms), dim3(kLineWarps * kWarpSize), smem, stream, 1u, a);
   if (status != SVLLM_OK) return status;
   const int64_t parts = line_shares(device) / items + 2;  // of an item of middling length
-  if (parts <= kJoinFewParts) {
+  if (parts <= kJoinFewParts<D>) {
     const int per_item = kHeads * heads * (D / 4);
     const int a_cta = kJoinThreads / per_item;
     return launch(decode_attention_fp8_join_few<D, kHeads>,
