@@ -1,5 +1,6 @@
 // CPU kernels of the 8-bit KV cache's operators on torch's thread pool: the rotary step that
-// quantises as it writes, the read-back, and decode attention. fp32 inside, rounded once.
+// quantises as it writes, the read-back, and decode attention. fp32 inside (the scores' sums in 64
+// bits), rounded once.
 #include <ATen/Parallel.h>
 #include <c10/util/BFloat16.h>
 #include <c10/util/Exception.h>
@@ -195,7 +196,6 @@ void decode_attention_fp8(const at::Tensor& out, const at::Tensor& q, const at::
   const auto* ks = static_cast<const uint8_t*>(k_scale.const_data_ptr());
   const auto* vs = static_cast<const uint8_t*>(v_scale.const_data_ptr());
   auto* op = out.mutable_data_ptr<at::BFloat16>();
-  const float factor = static_cast<float>(scale);
   at::parallel_for(0, requests * heads, 1, [&](int64_t begin, int64_t end) {
     std::vector<float> x, sum(dim);
     for (int64_t u = begin; u < end; ++u) {
@@ -208,11 +208,11 @@ void decode_attention_fp8(const at::Tensor& out, const at::Tensor& q, const at::
       float top = -std::numeric_limits<float>::infinity();
       for (int64_t j = 0; j < seq[s]; ++j) {
         const int64_t row = row_of(j);
-        float dot = 0.0f;
+        double dot = 0.0;  // the largest queries times codes leave fp32, whatever the scale
         for (int64_t d = 0; d < dim; ++d) {
-          dot += static_cast<float>(query[d]) * static_cast<float>(kc[row * dim + d]);
+          dot += static_cast<double>(query[d]) * static_cast<double>(kc[row * dim + d]);
         }
-        x[j] = dot * (factor * scale_value(ks[row]));
+        x[j] = static_cast<float>(dot * scale * scale_value(ks[row]));
         top = std::max(top, x[j]);
       }
       if (std::isinf(top) && top < 0) top = 0.0f;  // every score -infinity, or no row at all

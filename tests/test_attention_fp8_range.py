@@ -11,6 +11,7 @@ import torch
 
 import fp8_reference as ref
 import svllm_ops
+from test_cache_fp8 import check_attention
 
 LN2 = math.log(2.0)  # as the scale: scores in base 2 are q . k
 
@@ -151,3 +152,11 @@ def test_scores_whose_steps_pass_the_slack(cuda, dim, top):
     want = ref.values(*caches[1]).view(n, dim)[n - 1].expand(3, dim)
     # the others weigh 63 * 2^-16 together, their values at most four times this row's
     assert ((out[0] - want).abs() <= (2.0 ** -8 + 2.0 ** -11 + 4 * 63 * 2.0 ** -16) * want).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("power", [-120, 100, 116, 120])
+def test_query_magnitudes(device, power, dim):
+    """Queries anywhere in bf16's range under a scale that brings the scores back."""
+    check_attention(device, [1, 40, 200], 4, 2, dim, 16, spread=0.3, size=2.0 ** power,
+                    scale=2.0 ** (-2 - power))
