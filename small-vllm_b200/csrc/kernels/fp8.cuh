@@ -20,7 +20,6 @@ namespace svllm::k {
 constexpr int kScaleMin = -60;
 constexpr int kScaleMax = 60;
 constexpr int kScaleBias = 127;
-constexpr int kCodeNan = 0x7f;
 
 // The exponent e of a row whose largest magnitude has the given fp32 bits (finite, non-negative).
 // 448 = 1.75 * 2^8, so with max = m * 2^x, m in [1, 2): e = x - 8, one more where m > 1.75.
