@@ -200,7 +200,7 @@ at::Tensor Model::paged_decode_attention(const at::Tensor& q, int64_t layer,
 
 at::Tensor Model::fp8_attention(const at::Tensor& q, int64_t layer, const AttentionMetadata& meta,
                                 const at::Tensor& tables, const at::Tensor& lens,
-                                const at::Tensor& starts) const {
+                                const at::Tensor& starts, const at::Tensor& in_order) const {
   if (meta.decode) {
     return ops::decode_attention_fp8(q, k_cache_[layer], v_cache_[layer], k_scale_[layer],
                                      v_scale_[layer], tables, lens, std::nullopt);
@@ -208,9 +208,7 @@ at::Tensor Model::fp8_attention(const at::Tensor& q, int64_t layer, const Attent
   if (q.size(0) == 0) return at::empty(q.sizes(), q.options());  // no token to attend for
   const auto [k, v] = ops::cache_read_fp8(k_cache_[layer], v_cache_[layer], k_scale_[layer],
                                           v_scale_[layer], tables, lens);
-  const int64_t pages = tables.numel();
-  const auto shape = {pages, block_size_, config_.num_kv_heads, config_.head_dim};
-  const at::Tensor in_order = at::arange(pages, tables.options()).view(tables.sizes());
+  const auto shape = {tables.numel(), block_size_, config_.num_kv_heads, config_.head_dim};
   return ops::tree_attention(q, k.view(shape), v.view(shape), in_order, lens, starts,
                              meta.tree_mask, std::nullopt);
 }
@@ -237,6 +235,11 @@ at::Tensor Model::forward(const at::Tensor& ids, const at::Tensor& positions,
   const AttentionPlan plan =
       paged || meta.tree || fp8 ? AttentionPlan{} : plan_attention(T, meta);
   at::Tensor tables, lens, starts;
+  at::Tensor in_order;  // block tables of the read-back
+  if (fp8 && !meta.decode) {
+    in_order = at::arange(meta.block_tables.numel(), meta.block_tables.options().dtype(at::kInt))
+                   .view(meta.block_tables.sizes());
+  }
   if (meta.tree || fp8) {
     tables = meta.block_tables.to(at::kInt).contiguous();
     lens = meta.seq_lens.to(at::kInt).contiguous();
@@ -273,7 +276,7 @@ at::Tensor Model::forward(const at::Tensor& ids, const at::Tensor& positions,
                       config_.rope_theta, config_.rope_scaling);
     }
     const at::Tensor attn =
-        fp8 ? fp8_attention(q, static_cast<int64_t>(l), meta, tables, lens, starts)
+        fp8 ? fp8_attention(q, static_cast<int64_t>(l), meta, tables, lens, starts, in_order)
                   .view({T, Hq * D})
         : meta.tree ? ops::tree_attention(q, k_cache_[l], v_cache_[l], tables, lens, starts,
                                         meta.tree_mask, std::nullopt)

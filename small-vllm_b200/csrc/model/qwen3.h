@@ -82,7 +82,8 @@ class Model {
   // One verification step: every request feeds a tree (or chain) of drafted tokens, its nodes
   // packed as ops::paged_plan lays them out (its slot_mapping, positions, seq_lens,
   // query_start_loc and tree_mask). Returns the next token after every node, [T] int64: the
-  // targets of ops::tree_accept, which ops::tree_commit follows on k_cache() and v_cache().
+  // targets of ops::tree_accept, which ops::tree_commit follows on k_cache() and v_cache() (and, for
+  // an 8-bit cache, k_scale() and v_scale()).
   at::Tensor verify(const at::Tensor& ids, const at::Tensor& positions,
                     const at::Tensor& slot_mapping, const at::Tensor& block_tables,
                     const at::Tensor& seq_lens, const at::Tensor& query_start_loc,
@@ -121,10 +122,10 @@ class Model {
   at::Tensor paged_decode_attention(const at::Tensor& q, int64_t layer,
                                     const AttentionMetadata& meta) const;
   // Steps over the 8-bit cache. Decode: its attention straight from the codes. Others: the requests'
-  // rows read back in bf16, which are a paged cache in order, and attention over that.
+  // rows read back in bf16, which are a paged cache in the order of in_order, and attention over that.
   at::Tensor fp8_attention(const at::Tensor& q, int64_t layer, const AttentionMetadata& meta,
                            const at::Tensor& tables, const at::Tensor& lens,
-                           const at::Tensor& starts) const;
+                           const at::Tensor& starts, const at::Tensor& in_order) const;
 
   ModelConfig config_;
   at::Tensor embed_;       // [V, H]
