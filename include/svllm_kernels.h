@@ -505,11 +505,12 @@ int svllm_cache_read_fp8_bf16(void* k_out, void* v_out, const void* k_cache, con
  * scales. Any number of query heads per KV head; q and out 16-byte aligned, a q_token_stride of
  * whole 16 bytes, else SVLLM_ERR_UNSUPPORTED; scale positive and finite, as is scale / ln 2. Products
  * in f16 on exact codes, the softmax numerators times V's scales rounded to f16 for the second (those
- * below 2^-31 of a head's largest may be lost); scores, maxima and sums in fp32. A request of length
- * 0, and a head with no score above -infinity, gives zeros. Lengths, table entries and scales out of
- * range as in svllm_cache_read_fp8_bf16. workspace: at least
- * svllm_decode_attention_fp8_workspace_bytes bytes of device memory (NULL where that is 0), 16-byte
- * aligned, any contents; calls that overlap on the GPU must not share it. Results repeat bit for bit.
+ * below 2^-31 of a head's largest may be lost), elements of a query below 2^-32 of its head's largest
+ * off by up to 2^-39 of that; scores, maxima and sums in fp32. A request of length 0, and a head with
+ * no score above -infinity, gives zeros. Lengths, table entries and scales out of range as in
+ * svllm_cache_read_fp8_bf16. workspace: at least svllm_decode_attention_fp8_workspace_bytes bytes of
+ * device memory (NULL where that is 0), 16-byte aligned, any contents; calls that overlap on the GPU
+ * must not share it. Results of the same call repeat bit for bit.
  */
 int svllm_decode_attention_fp8_bf16(void* out, const void* q, int64_t q_token_stride,
                                     const void* k_cache, const void* v_cache, const void* k_scale,

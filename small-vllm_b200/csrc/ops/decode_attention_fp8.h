@@ -17,7 +17,8 @@ namespace svllm::ops {
 //             positive and finite, head_dim^-0.5 by default; one device.
 // Returns:    A new bf16 tensor [S, heads, head_dim]. Softmax and sums are fp32; on CUDA the softmax
 //             numerators times V's scales are rounded to f16 for the second product, and those below
-//             2^-31 of a head's largest may be lost there.
+//             2^-31 of a head's largest may be lost there; elements of a query below 2^-32 of its head's
+//             largest may be off by up to 2^-39 of that.
 // Throws:     As cache_read_fp8, and on mismatches of q; on CUDA also for a q off 16 bytes.
 at::Tensor decode_attention_fp8(const at::Tensor& q, const at::Tensor& k_cache,
                                 const at::Tensor& v_cache, const at::Tensor& k_scale,
