@@ -10,12 +10,12 @@
 // code is an f16 number, so converting costs one instruction for two codes and nothing in
 // precision. The other operands are made to fit f16's range by powers of two: q of each head is
 // scaled so that its largest magnitude lies in [2^14, 2^15) (exact for all elements down to 2^-32
-// of it, the others off by up to 2^-39 of it), and the weights are w_j = 2^(y_j - m + 6) with y_j = x_j + ev_j, x_j the score in base 2
-// and m a maximum of the y_j that is moved only when one passes it by 8: w_j <= 2^14, the largest is
-// 2^6 at least, and f16's smallest number, 2^-24, stands for 2^-30 of it or less (a weight below half
-// of that is lost). The rows' scales thus never touch the codes: 2^ek multiplies a score, ev adds to
-// it (in the one rounding of an fma). The weights are rounded to f16 (2^-11 of each, an eighth of a
-// bf16 rounding) because the product takes no wider operand.
+// of it, the others off by up to 2^-39 of it), and the weights are w_j = 2^(y_j - m + 6) with y_j =
+// x_j + ev_j, x_j the score in base 2 and m a maximum of the y_j that is moved only when one passes it
+// by 8: w_j <= 2^14, the largest is 2^6 at least, and f16's smallest number, 2^-24, stands for 2^-30 of
+// it or less (a weight below half of that is lost). The rows' scales thus never touch the codes: 2^ek
+// multiplies a score, ev adds to it (in the one rounding of an fma). The weights are rounded to f16
+// (2^-11 of each, an eighth of a bf16 rounding) because the product takes no wider operand.
 //
 // The denominator is l = sum_j 2^(d_j - ev_j) with d_j = y_j - m + 6, in fp32. Its terms have an
 // exponential of their own: w_j 2^-ev_j would lose a row whose w_j is below 2^-126, and with scales
@@ -47,10 +47,10 @@
 // rows, 407 MB, 76.5-76.9. The warps stream at 6.6 TB/s once they run, 62 us; 4 us go by until the first
 // rows are there (lengths 0.8, the share 0.5, table and rows, each a trip to memory after the other),
 // the last warps end 4 behind the mean, and the join takes 3. One request of 32760 rows: 18.1, of
-// which 10.5 are the stream. A step of 32 rows takes 577 warp instructions; 39 % of the issue slots are used. More loads in flight
-// gave nothing (three stages 79.1, twelve warps 77.1-78.9, fourteen 81.5, the next load after the
-// products 80.7); a CTA per share whose warps merge at every item's end took 98, rows loaded to
-// registers instead of shared memory 168.
+// which 10.5 are the stream. A step of 32 rows takes 577 warp instructions; 39 % of the issue slots are
+// used. More loads in flight gave nothing (three stages 79.1, twelve warps 77.1-78.9, fourteen 81.5, the
+// next load after the products 80.7); a CTA per share whose warps merge at every item's end took 98,
+// rows loaded to registers instead of shared memory 168.
 #include <cuda_runtime.h>
 
 #include <cfloat>

@@ -34,7 +34,7 @@ def test_many_tokens(cuda, norm, tokens, heads, kv_heads, dim):
 @pytest.mark.gpu
 @pytest.mark.parametrize("heads, kv_heads, dim", [(16, 8, 128), (9, 3, 64)])
 def test_values_that_are_not_finite_stay_in_their_rows(cuda, heads, kv_heads, dim):
-    """V rows with infinities and NaN among many tokens: their codes to the bit, all others as without."""
+    """V rows with infinities and NaN among many tokens: their codes to the bit, the others as without."""
     tokens = 1500
     c = write_case(3, tokens, heads, kv_heads, dim)
     clean = call_write(c, cuda, heads, kv_heads, dim, True)
