@@ -389,7 +389,8 @@ struct Sums {
         v_exp[i][e] = ev;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float v = fmaf(s[2 * e + h], q.x_scale[h] * ks, ev);
+          // (s * ks is exact; the two factors' product may leave fp32 where s is 0)
+          const float v = fmaf(s[2 * e + h] * ks, q.x_scale[h], ev);
           y[i][2 * e + h] = r < live ? v : -__builtin_huge_valf();
           top[h] = fmaxf(top[h], y[i][2 * e + h]);
         }

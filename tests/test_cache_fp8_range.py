@@ -160,3 +160,29 @@ def test_query_magnitudes(device, power, dim):
     """Queries anywhere in bf16's range under a scale that brings the scores back."""
     check_attention(device, [1, 40, 200], 4, 2, dim, 16, spread=0.3, size=2.0 ** power,
                     scale=2.0 ** (-2 - power))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("power", [90, 127])
+def test_large_queries_across_large_keys(device, dim, power):
+    """Scores of exactly 0 between the largest queries and the largest rows of K: the mean of V."""
+    n, block = 70, 16
+    g = torch.Generator().manual_seed(dim)
+    k = (224 + 224 * torch.rand(n + 10, 2, dim, generator=g)).bfloat16().double() * 2.0 ** 60
+    k[:, :, 0] = 0
+    v = (1 + torch.rand(n + 10, 2, dim, generator=g)).bfloat16().double()
+    caches = []
+    for x in (k, v):
+        codes, scale, _ = ref.quantise(x)
+        caches.append((codes.view(5, block, 2, dim), scale.view(5, block, 2)))
+    q = torch.zeros(1, 4, dim, dtype=torch.bfloat16)
+    q[:, :, 0] = 2.0 ** power
+    want = ref.values(*caches[1]).flatten(0, 1)[:n].mean(0).repeat_interleave(2, 0)
+    for width in (5, 2000):
+        tables = torch.zeros(1, width, dtype=torch.int32)
+        tables[0, :5] = torch.arange(5)
+        out = svllm_ops.decode_attention_fp8(
+            q.to(device), *(t.to(device) for t in (caches[0][0], caches[1][0], caches[0][1],
+                                                   caches[1][1])),
+            tables.to(device), torch.tensor([n], dtype=torch.int32, device=device)).cpu().double()
+        assert ((out[0] - want).abs() <= (2.0 ** -8 + 2.0 ** -11 + n * 2.0 ** -23) * want).all()
